@@ -540,6 +540,78 @@ int32_t tf_fp8_linears(const void* x, int64_t x_row_stride, const uint32_t* amax
 int64_t tf_fp8_linears_workspace_bytes(int64_t m, const tf_fp8_mat* mats, int32_t n_mats,
                                        int64_t k);
 
+/* ------------------------------------------- FP8 with a scale per block of 128
+ * Matrices of e4m3 values with one fp32 scale per row and 128 columns
+ * (activations; scale of (row, block) at x_scale[block * x_scale_stride + row])
+ * or per 128 x 128 block (weights; a tf_fp8_mat whose w_scale is not NULL).
+ *
+ * tf_block_quant: s = fl32(max(amax|x|, 1e-12) / 448) per row and 128 columns,
+ * xq = e4m3(fl32(x / s)), rounded to nearest even.  x: bf16 or fp32
+ * [rows, cols], cols a multiple of 8, 16-byte aligned with a row stride that is
+ * a multiple of 8 elements; xq 8-byte aligned with such a stride.  A NaN or inf
+ * makes its block's scale NaN or inf and with it the row's products, no other
+ * row's.
+ *
+ * tf_block_linear: out = bf16(sum over blocks kb of x_scale[m, kb] *
+ * w_scale[n / 128, kb] * (xq w^T over kb) + bias), fp32 accumulation; k a
+ * multiple of 16, any n.  x: bf16 or fp32 (quantised into the workspace; alignment
+ * as above) or e4m3 with x_scale: 16-byte aligned, its row stride a multiple of 16
+ * from the padded width (k up to the next multiple of 128) up and zero bytes
+ * between k and that width.  mat: the weight, 16-byte aligned rows; out
+ * 8-byte aligned.  The result is deterministic.
+ *
+ * tf_gated_mlp: out = h^ Wd^T with h = silu(x Wg^T) * (x Wu^T) in fp32 and h^ its
+ * block-quantised form (qwen3_8/mlp.py:9-54).  gate and up: n = inter
+ * (a multiple of 16) over hidden (a multiple of 16) columns, their out and bias
+ * unused; down: any n over inter columns, with out and optional bias.  x as in
+ * tf_block_linear.
+ *
+ * workspace: device, 16-byte aligned, *_workspace_bytes(...) bytes for the same
+ * sizes and x_dtype on the same device; not shared by calls that overlap in time.
+ */
+int32_t tf_block_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t cols,
+                       int64_t x_row_stride, void* xq, int64_t xq_row_stride, float* x_scale,
+                       int64_t x_scale_stride, tf_stream_t stream);
+
+int64_t tf_block_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t x_dtype);
+
+int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
+                        const float* x_scale, int64_t x_scale_stride, const tf_fp8_mat* mat,
+                        int64_t m, int64_t k, void* workspace, int64_t workspace_bytes,
+                        tf_stream_t stream);
+
+int64_t tf_gated_mlp_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, int64_t n_out,
+                                     int32_t x_dtype);
+
+int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const float* x_scale,
+                     int64_t x_scale_stride, const tf_fp8_mat* gate, const tf_fp8_mat* up,
+                     const tf_fp8_mat* down, int64_t m, int64_t hidden, int64_t inter,
+                     void* workspace, int64_t workspace_bytes, tf_stream_t stream);
+
+/* tf_add_rms_norm: the residual sum and the norms around a block
+ * (qwen3_8/decoder_layer.py:57-81, qwen3_8/rms_norm.py:19-24), per row, in fp32:
+ *   b  = x, or post_weight * x / rms(x) with a post_weight
+ *   r' = residual + residual_scale * gate * b
+ *   y  = weight * r' / rms(r'),   rms(v) = sqrt(mean v^2 + eps)
+ * residual, gate and post_weight may be NULL (0, 1, no norm of x).  r' is stored
+ * to residual_out (NULL: not stored) in the residual's type, or x's without one;
+ * it may be the residual itself.  y (NULL: not computed) is bf16, fp32 or e4m3
+ * with scales as tf_block_quant makes them; it is formed from r' before that is
+ * rounded.  gate: per_column != 0: elements of a row side by side, row stride
+ * 0 or from cols up; else one value per row, gate_row_stride apart.  x, residual,
+ * gate and the weights are bf16 or fp32 each; cols a multiple of 8 up to 16384; rows
+ * 16-byte aligned, strides (elements) multiples of 8.
+ */
+int32_t tf_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_row_stride,
+                        const void* residual, int32_t residual_dtype,
+                        int64_t residual_row_stride, const void* gate, int32_t gate_dtype,
+                        int64_t gate_row_stride, int32_t gate_per_column,
+                        const void* post_weight, int32_t post_weight_dtype, const void* weight,
+                        int32_t weight_dtype, float eps, float residual_scale, int64_t rows,
+                        int64_t cols, void* residual_out, int64_t residual_out_row_stride,
+                        void* y, int32_t y_dtype, int64_t y_row_stride, float* y_scale,
+                        int64_t y_scale_stride, tf_stream_t stream);
+
 /* ------------------------------------------------------------------ Gated DeltaNet decode
  * One-token step of the linear-attention (Gated DeltaNet) layers for a batch
  * whose requests all extend by one token: Qwen3_8LinearAttention.

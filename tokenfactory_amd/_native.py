@@ -6,6 +6,7 @@ raises ``NativeLibraryError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -14,7 +15,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libtf_attn.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 TF_DTYPE_BF16 = 0
 TF_DTYPE_FP8_E4M3 = 1
@@ -171,6 +172,32 @@ SIGNATURES = {
         _i64, _i64, _p, _i64, _p,      # m, k, workspace, workspace_bytes, stream
     ]),
     "tf_fp8_linears_workspace_bytes": (_i64, [_i64, _p, _i32, _i64]),
+    "tf_block_quant": (_i32, [
+        _p, _i32, _i64, _i64, _i64,    # x, x_dtype, rows, cols, x_row_stride
+        _p, _i64, _p, _i64, _p,        # xq, xq_row_stride, x_scale, x_scale_stride, stream
+    ]),
+    "tf_block_linear_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "tf_block_linear": (_i32, [
+        _p, _i32, _i64, _p, _i64,      # x, x_dtype, x_row_stride, x_scale, x_scale_stride
+        _p, _i64, _i64,                # mat, m, k
+        _p, _i64, _p,                  # workspace, workspace_bytes, stream
+    ]),
+    "tf_gated_mlp_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32]),
+    "tf_gated_mlp": (_i32, [
+        _p, _i32, _i64, _p, _i64,      # x, x_dtype, x_row_stride, x_scale, x_scale_stride
+        _p, _p, _p, _i64, _i64, _i64,  # gate, up, down, m, hidden, inter
+        _p, _i64, _p,                  # workspace, workspace_bytes, stream
+    ]),
+    "tf_add_rms_norm": (_i32, [
+        _p, _i32, _i64,                # x, x_dtype, x_row_stride
+        _p, _i32, _i64,                # residual, residual_dtype, residual_row_stride
+        _p, _i32, _i64, _i32,          # gate, gate_dtype, gate_row_stride, gate_per_column
+        _p, _i32, _p, _i32,            # post_weight, its dtype, weight, its dtype
+        _f32, _f32, _i64, _i64,        # eps, residual_scale, rows, cols
+        _p, _i64,                      # residual_out, residual_out_row_stride
+        _p, _i32, _i64, _p, _i64,      # y, y_dtype, y_row_stride, y_scale, y_scale_stride
+        _p,                            # stream
+    ]),
     "tf_gdn_decode": (_i32, [
         _p, _i64, _p, _p, _i64,        # qkv, qkv_row_stride, a, b, ab_row_stride
         _p, _i64,                      # z, z_row_stride
@@ -294,6 +321,15 @@ def current_stream(device) -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context that makes ``device`` the current one (launches go to the current
+    device whatever stream they name); a no-op where it is already."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def plan_device_capacity(total_tokens, batch_size, num_q_heads, num_kv_heads) -> int:

@@ -1,0 +1,108 @@
+"""The residual sum and the norms around a block, in one launch.
+
+A decoder layer adds each block's output to the residual stream and norms the sum
+for the next block (``qwen3_8/decoder_layer.py:57-81``, ``qwen3_8/rms_norm.py:19-24``);
+``add_rms_norm`` does both, with the forms in which models vary that step (a norm
+of the block's output, a gate, a residual multiplier), and hands the result on as
+bf16 / fp32 or quantised for ``block_scaled_linear`` and ``gated_mlp``.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _native
+from .block_fp8 import DTYPES, new_scales, row_stride, rows16
+from .fp8_linear import _ptr, _stream_ptr, on_stream
+
+MAX_COLS = 16384
+_VALUES = (torch.bfloat16, torch.float32)
+
+
+def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
+    if t.dtype not in _VALUES or t.device != like.device or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"add_rms_norm: {name} must be bf16 or fp32 {tuple(shape)} on x's device")
+
+
+def _dtype(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else DTYPES[t.dtype]
+
+
+def _gate_rows(gate: torch.Tensor, shape):
+    """(gate, row stride, per column) of a gate that broadcasts to ``shape``."""
+    g = gate.expand(shape)
+    rows, cols = shape
+    if g.stride(1) == 0:                    # one value per row (or for all of them)
+        return g, (g.stride(0) if rows > 1 else 0), 0
+    if rows == 1 or g.stride(0) == 0:       # one row for all of them
+        return rows16(g[:1]), 0, 1
+    g = rows16(g)
+    return g, g.stride(0), 1
+
+
+def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
+                 weight: Optional[torch.Tensor], eps: float = 1e-6, *,
+                 post_weight: Optional[torch.Tensor] = None,
+                 gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+                 quantize: bool = False, inplace: bool = False, stream=None):
+    """Per row of x, in fp32, with ``rms(v) = sqrt(mean v^2 + eps)``:
+
+        b = x                      (post_weight * x / rms(x) with a post_weight)
+        r = residual + residual_scale * gate * b
+        y = weight * r / rms(r)
+
+    x: bf16 or fp32 ``[rows, cols]``, cols a multiple of 8 up to 16384; residual of
+    the same shape, or None for 0; weight and post_weight ``[cols]``; gate broadcasts
+    to x's shape (``[cols]``, ``[rows, 1]``, ``[rows, cols]``, ...), bf16 or fp32 like
+    every operand.
+
+    Returns ``(y, r)``.  y has x's dtype, or with ``quantize`` is the pair
+    ``(float8_e4m3fn values, fp32 scales)`` of ``quantize_blocks``; it is formed from
+    r before r is rounded to the residual's dtype (x's without a residual).  Without
+    a weight y is None.  ``inplace`` stores r over ``residual``.  Where r is x
+    itself (no residual, gate, scale or post_weight), x is returned as r."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in _VALUES:
+        raise ValueError("add_rms_norm: x must be a 2-D bf16 or fp32 CUDA tensor")
+    rows, cols = x.shape
+    if cols == 0 or cols % 8:
+        raise ValueError(f"add_rms_norm: {cols} columns (a positive multiple of 8)")
+    if cols > MAX_COLS:
+        raise NotImplementedError(f"add_rms_norm: {cols} columns (at most {MAX_COLS})")
+    if quantize and weight is None:
+        raise ValueError("add_rms_norm: quantize needs a weight")
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        if t is not None:
+            _check(name, t, x, (cols,))
+    if residual is not None:
+        _check("residual", residual, x, x.shape)
+    if inplace and (residual is None or rows16(residual) is not residual):
+        raise ValueError("add_rms_norm: in place, residual must be given, with dense 16-byte "
+                         "aligned rows")
+    if gate is not None and (gate.dtype not in _VALUES or gate.device != x.device):
+        raise ValueError("add_rms_norm: gate must be bf16 or fp32 on x's device")
+    scale = float(residual_scale)
+    same = residual is None and gate is None and post_weight is None and scale == 1.0
+    dev = x.device
+    with _native.on_device(dev), on_stream(stream):
+        gp, gs, gcols = (None, 0, 0) if gate is None else _gate_rows(gate, x.shape)
+        xr = rows16(x)
+        rr = None if residual is None else rows16(residual)
+        r = x if same else residual if inplace else torch.empty(
+            (rows, cols), dtype=x.dtype if residual is None else residual.dtype, device=dev)
+        y = ys = None
+        if weight is not None:
+            weight = weight.contiguous()
+            y = torch.empty((rows, cols), device=dev,
+                            dtype=torch.float8_e4m3fn if quantize else x.dtype)
+            ys = new_scales(rows, cols, dev) if quantize else None
+        if post_weight is not None:
+            post_weight = post_weight.contiguous()
+        if rows and not (same and y is None):
+            _native.call("tf_add_rms_norm", _ptr(xr), DTYPES[x.dtype], row_stride(xr), _ptr(rr),
+                         _dtype(rr), 0 if rr is None else row_stride(rr), _ptr(gp), _dtype(gp),
+                         gs, gcols, _ptr(post_weight), _dtype(post_weight), _ptr(weight),
+                         _dtype(weight), float(eps), scale, rows, cols, 0 if same else _ptr(r),
+                         row_stride(r), _ptr(y), _dtype(y), cols, _ptr(ys), rows,
+                         _stream_ptr(stream, dev))
+    return ((y, ys) if quantize else y), r

@@ -1,0 +1,167 @@
+"""FP8 products with a scale for each block of 128 columns of the activations.
+
+``fp8_linear`` quantises activations with one scale per tensor, as the reference's
+linears do (``qwen3_8/fp8_triton.py:127-130``).  Here every row has a scale per
+128 columns, the granularity of the weights' 128 x 128 blocks: a row's result
+depends on that row alone, an outlier costs precision only within its own block,
+and no pass over the whole tensor comes first, so that the producer of the
+activations can write them quantised (``add_rms_norm(..., quantize=True)``).
+
+* ``quantize_blocks(x)`` -> e4m3 rows and their scales
+* ``block_scaled_linear(x, weight, weight_scale_inv, bias)``: the product with a
+  checkpoint's block-FP8 weight (``Fp8Linear.weight`` / ``weight_scale_inv``)
+
+Scales are fp32 ``[rows, ceil(cols / 128)]``, stored with a block's rows side by
+side (``stride(0) == 1``).  There is no non-native path and no gradient.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+from .fp8_linear import _ptr, _stream_ptr, on_stream
+
+BLOCK = 128
+DTYPES = {torch.bfloat16: _native.TF_DTYPE_BF16, torch.float32: _native.TF_DTYPE_FP32,
+          torch.float8_e4m3fn: _native.TF_DTYPE_FP8_E4M3}
+
+
+def blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if the kernels take its rows as they lie (dense columns, rows
+    that do not overlap, 16-byte aligned), else a copy."""
+    unit = 16 if t.element_size() == 1 else 8
+    if (t.stride(1) == 1 and t.data_ptr() % 16 == 0
+            and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """The row stride of ``rows16(t)`` (one row: its width, whatever torch says)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def new_scales(rows: int, cols: int, device) -> torch.Tensor:
+    """Room for the scales of ``rows`` x ``cols`` values, a block's rows side by side."""
+    return torch.empty((blocks(cols), rows), dtype=torch.float32, device=device).t()
+
+
+def quantize_blocks(x: torch.Tensor, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Per row and 128 columns (the last block may be shorter): scale ``s = max(amax
+    |x|, 1e-12) / 448`` in fp32, values ``e4m3(x / s)``, each rounded to nearest
+    even.  x: bf16 or fp32 ``[rows, cols]``, cols a multiple of 8.  Returns
+    float8_e4m3fn ``[rows, cols]`` and fp32 scales ``[rows, ceil(cols / 128)]``.
+    A NaN or infinite value poisons its row's block (scale NaN or inf)."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("quantize_blocks: x must be a 2-D bf16 or fp32 CUDA tensor")
+    rows, cols = x.shape
+    if cols == 0 or cols % 8:
+        raise ValueError(f"quantize_blocks: {cols} columns (a positive multiple of 8)")
+    with _native.on_device(x.device), on_stream(stream):
+        x = rows16(x)
+        xq = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+        scale = new_scales(rows, cols, x.device)
+        _native.call("tf_block_quant", _ptr(x), DTYPES[x.dtype], rows, cols, row_stride(x),
+                     _ptr(xq), cols, _ptr(scale), rows, _stream_ptr(stream, x.device))
+    return xq, scale
+
+
+def check_weight(fn: str, what: str, w: torch.Tensor, scale: torch.Tensor, k: int, device) -> None:
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.device != device:
+        raise ValueError(f"{fn}: {what} must be a 2-D float8_e4m3fn tensor on x's device")
+    n = w.shape[0]
+    if w.shape[1] != k or n == 0:
+        raise ValueError(f"{fn}: {what} {tuple(w.shape)} for inputs of {k}")
+    if w.stride(1) != 1 or w.data_ptr() % 16 or (n > 1 and (w.stride(0) < k or w.stride(0) % 16)):
+        raise ValueError(f"{fn}: {what} rows must be contiguous and 16-byte aligned")
+    if (scale.dtype != torch.float32 or scale.device != device
+            or tuple(scale.shape) != (blocks(n), blocks(k))):
+        raise ValueError(f"{fn}: scales of {what} must be fp32 {(blocks(n), blocks(k))} on x's "
+                         f"device, one per 128 x 128 block")
+
+
+def mat(w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+        out: Optional[torch.Tensor] = None):
+    """A pointer to the ``tf_fp8_mat`` of a checked weight."""
+    n = w.shape[0]
+    return ctypes.byref(_native.Fp8Mat(w.data_ptr(), row_stride(w), scale.data_ptr(),
+                                       scale.stride(0), scale.stride(1), _ptr(bias), n, _ptr(out),
+                                       n))
+
+
+def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: int) -> torch.Tensor:
+    """x as a 2-D tensor of ``k`` columns that the products take."""
+    if not x.is_cuda or x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"{fn}: x {tuple(x.shape)} must be a CUDA tensor of {k} columns")
+    if k % 16:
+        raise NotImplementedError(f"{fn}: {k} columns (a multiple of 16)")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"{fn}: x must be bf16, fp32 or float8_e4m3fn, not {x.dtype}")
+    quantized = x.dtype == torch.float8_e4m3fn
+    if quantized != (x_scale is not None):
+        raise ValueError(f"{fn}: x_scale goes with a float8_e4m3fn x")
+    if not quantized:
+        return x.reshape(-1, k)
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: a quantised x must be 2-D")
+    if (x_scale.dtype != torch.float32 or x_scale.device != x.device
+            or tuple(x_scale.shape) != (x.shape[0], blocks(k))):
+        raise ValueError(f"{fn}: x_scale must be fp32 {(x.shape[0], blocks(k))} on x's device")
+    return x
+
+
+def input_rows(x2d: torch.Tensor, x_scale: Optional[torch.Tensor]):
+    """(x, its row stride, scales, their stride) as the entry points take them;
+    copies what lies otherwise (quantised rows of a width that is not a multiple of
+    128 get zeros behind them)."""
+    if x_scale is None:
+        x2d = rows16(x2d)
+        return x2d, row_stride(x2d), None, 0
+    rows, k = x2d.shape
+    if k % BLOCK:
+        padded = torch.zeros((rows, blocks(k) * BLOCK), dtype=torch.uint8, device=x2d.device)
+        padded[:, :k] = x2d.view(torch.uint8)
+        x2d = padded
+    else:
+        x2d = rows16(x2d)
+    nb = x_scale.shape[1]
+    if not ((rows == 1 or x_scale.stride(0) == 1) and (nb == 1 or x_scale.stride(1) >= rows)):
+        x_scale = x_scale.t().contiguous().t()
+    return x2d, row_stride(x2d), x_scale, rows if nb == 1 else x_scale.stride(1)
+
+
+def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv: torch.Tensor,
+                        bias: Optional[torch.Tensor] = None, *,
+                        x_scale: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """``bf16(sum_kb x_scale[m, kb] * weight_scale_inv[n // 128, kb] * (xq w^T)[m, n] over
+    block kb + bias)``, accumulated in fp32.
+
+    x: bf16 or fp32 ``[..., in]``, quantised here as ``quantize_blocks`` does, or
+    float8_e4m3fn ``[rows, in]`` with its ``x_scale``; weight float8_e4m3fn
+    ``[out, in]`` (in a multiple of 16) with fp32 scales per 128 x 128 block; bias
+    bf16 ``[out]``.  Returns bf16 ``[..., out]``."""
+    fn = "block_scaled_linear"
+    x2d = check_input(fn, x, x_scale, weight.shape[-1])
+    check_weight(fn, "weight", weight, weight_scale_inv, x2d.shape[1], x.device)
+    n, k = weight.shape
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (n,)
+                             or bias.device != x.device or not bias.is_contiguous()):
+        raise ValueError(f"{fn}: bias must be a contiguous bf16 [{n}] on x's device")
+    rows = x2d.shape[0]
+    with _native.on_device(x.device), on_stream(stream):
+        out = torch.empty((rows, n), dtype=torch.bfloat16, device=x.device)
+        if rows:
+            xr, xs, sc, ss = input_rows(x2d, x_scale)
+            nbytes = _native.load().tf_block_linear_workspace_bytes(rows, n, k, DTYPES[x.dtype])
+            ws = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=x.device)
+            _native.call("tf_block_linear", _ptr(xr), DTYPES[x.dtype], xs, _ptr(sc), ss,
+                         mat(weight, weight_scale_inv, bias, out), rows, k, _ptr(ws), nbytes,
+                         _stream_ptr(stream, x.device))
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)

@@ -1,0 +1,851 @@
+// FP8 products with a scale for each block of 128, and the gated feed-forward
+// block built from them.
+//
+// A matrix held in 8 bits is e4m3 values with one fp32 scale per row and 128
+// columns (activations) or per 128 x 128 block (weights):
+//   quantise   s = fl32(max(amax|x|, 1e-12) / 448),  q = e4m3(fl32(x / s))
+//   product    out[m][n] = sum_kb xs[m][kb] ws[n / 128][kb] (xq w^T)[m][n] over block kb
+//   gated MLP  h = silu(x Wg^T) (x Wu^T) in fp32, quantised, times Wd^T
+// The weights are the reference's block-FP8 linears' (qwen3_8/fp8_linear.py:12-212),
+// the block its Qwen3_8MLP (qwen3_8/mlp.py:9-54).  A scale per block instead of
+// one per tensor (fp8_linear.hip) makes a row's result depend on that row alone
+// and needs no pass over the whole tensor before the first value is written, so
+// the quantisation folds into whatever produces the values.
+#include <math.h>
+
+#include <algorithm>
+
+#include "block_quant.h"
+#include "fp8_tile.h"
+#include "tf_common.h"
+#include "tf_internal.h"
+
+namespace tfa {
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------- quantisation
+// One wave: 4 rows x kQuantBlocks blocks; 16 lanes hold a block's 128 columns,
+// 8 each.  All of a lane's loads are issued before the first is used.  Scales
+// are stored [block][row], so the 4 rows of a wave (16 of a workgroup) lie side
+// by side.
+constexpr int kQuantBlocks = 4;
+constexpr int kQuantRows = 4 * (kThreads / kWave);
+
+struct BlockQuantArgs {
+  const uint8_t* x;
+  int64_t xs;              // row stride, elements
+  int64_t rows;
+  int32_t cols, out_cols;  // out_cols: cols, or more to write zeros behind them
+  uint8_t* xq;
+  int64_t qs;
+  float* scale;
+  int64_t ss;              // scale of (row, block) at block * ss + row
+  int32_t col_groups;
+};
+
+template <bool F32>
+__global__ void __launch_bounds__(kThreads) block_quant_kernel(BlockQuantArgs a) {
+  const int64_t rg = blockIdx.x / a.col_groups;
+  const int cg = (int)(blockIdx.x - rg * a.col_groups);
+  const int l = threadIdx.x & 63;
+  const int64_t row = rg * kQuantRows + (threadIdx.x >> 6) * 4 + (l >> 4);
+  if (row >= a.rows) return;
+  const int c0 = cg * kQuantBlocks * kQBlock + 8 * (l & 15);
+  float v[kQuantBlocks][8];
+#pragma unroll
+  for (int b = 0; b < kQuantBlocks; ++b) {
+    const int c = c0 + b * kQBlock;
+    if (c < a.cols) {
+      load8<F32>(a.x, row * a.xs + c, v[b]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[b][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < kQuantBlocks; ++b) {
+    const int c = c0 + b * kQBlock;
+    const float s = block_scale(amax_lanes16(amax_bits8(v[b])));
+    if (c < a.out_cols)
+      *reinterpret_cast<u32x2*>(a.xq + row * a.qs + c) = quant8(v[b], s);
+    if ((l & 15) == 0 && c < a.cols) a.scale[(int64_t)(c / kQBlock) * a.ss + row] = s;
+  }
+}
+
+// ---------------------------------------------------------------- GEMM
+constexpr int kSpread = 3;            // staging instructions issued per row of MFMAs
+constexpr int kGroupM = 8;            // m-tiles per group of the XCD tile order
+constexpr int kMaxSplits = 16;        // split-K factor limit
+
+// As fp8_linear.hip's tile: a workgroup of 2 x WN waves owns 32 MT activation
+// rows x 64 WN weight rows, a wave 16 MT x 64 of them in 4 x MT 16x16 tiles of
+// the transposed product D[n][m].
+template <int MT, int WN, int STAGES>
+struct BlockTile {
+  static constexpr int kThreads = 2 * kWave * WN;
+  static constexpr int kBM = 32 * MT;
+  static constexpr int kBN = 64 * WN;
+  static constexpr int kXBytes = kBM * kKSlice;
+  static constexpr int kWBytes = kBN * kKSlice;
+  static constexpr int kScales = kBM + 2;       // row scales, then two column blocks'
+  static constexpr int kSInst = (kScales + kThreads - 1) / kThreads;
+  static constexpr int kStage = kXBytes + kWBytes + kSInst * kThreads * 4;
+  static constexpr int kRowsPerInst = kThreads / 8;
+  static constexpr int kXInst = kBM / kRowsPerInst;
+  static constexpr int kWInst = kBN / kRowsPerInst;
+  static constexpr int kLoads = kXInst + kWInst + kSInst;   // per thread per slice
+  static constexpr int kAhead = STAGES - 1;
+  static_assert(kBM % kRowsPerInst == 0 && kBN % kRowsPerInst == 0, "staging rows");
+};
+
+struct BlockMat {
+  const uint8_t* w;       // e4m3 [N, K], row stride wrs bytes
+  int64_t wrs;
+  const float* wsc;       // scale of column block n / 128, K block kb at nb * sn + kb * sk
+  int64_t sn, sk;
+  int32_t N, c0;          // columns; first of them among a split's partials
+};
+
+struct BlockGemmArgs {
+  const uint8_t* xq;      // e4m3 [M, 128 KB], zeros behind K, row stride xs bytes
+  int64_t xs;
+  const float* xsc;       // scale of (row, block) at block * xss + row
+  int64_t xss;
+  BlockMat mat[2];        // linear: the weight; gated: gate and up
+  int32_t n_mats, tn1;    // tn1: first n-tile of mat[1] where both are columns of partials
+  int32_t M, KB;
+  int32_t tail;           // bytes of the last K slice that the weights have
+  int32_t tiles_m, tiles, splits, n_cols;
+  float* part;            // split-K: fp32 [splits, M, n_cols]
+  const uint16_t* bias;
+  uint16_t* out;          // bf16 [M, N]
+  int64_t os;
+  uint8_t* hq;            // gated: e4m3 [M, 128 HB], and its scales
+  int64_t hqs;
+  float* hsc;
+  int64_t hss;
+};
+
+__device__ __forceinline__ float silu(float g) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-g * kLog2e));
+}
+
+__device__ __forceinline__ void store_out(const BlockGemmArgs& a, int64_t m, int n, int N,
+                                          f32x4 v) {
+  if (a.bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < N) v[r] += __uint_as_float((uint32_t)a.bias[n + r] << 16);
+  }
+  uint16_t* o = a.out + m * a.os + n;
+  const u32x2 pk = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  if (n + 3 < N && a.os % 4 == 0) {
+    *reinterpret_cast<u32x2*>(o) = pk;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < N) o[r] = (uint16_t)(pk[r >> 1] >> (16 * (r & 1)));
+  }
+}
+
+// GATED: the workgroup's 64 WN = 256 weight rows are 128 rows of the gate and
+// the same 128 of the up projection: of a wave's 64, the first 32 are gate rows
+// and the last 32 the up rows of the same columns, so g and u of one column
+// meet in one lane, and the workgroup holds whole 128-blocks of h.
+template <int MT, int WN, int STAGES, bool GATED>
+__global__ void __launch_bounds__(2 * kWave * WN)
+block_gemm_kernel(BlockGemmArgs a) {
+  using T = BlockTile<MT, WN, STAGES>;
+  static_assert(!GATED || WN == 4, "a gated tile holds one 128-block of h");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[STAGES * T::kStage];
+  const int t = threadIdx.x, w = wave_id(), l = t & 63;
+  const int wm = w / WN, wn = w % WN;
+  const int split = blockIdx.x / a.tiles;
+  int tm_i, tn_i;
+  xcd_tile(blockIdx.x % a.tiles, a.tiles, a.tiles_m, kGroupM, &tm_i, &tn_i);
+  const int second = GATED ? (w >= WN) : (a.n_mats > 1 && tn_i >= a.tn1);
+  const BlockMat mat = a.mat[second];   // gated: the matrix whose rows this wave stages
+  const int m0 = tm_i * T::kBM;
+  const int n0 = GATED ? tn_i * kQBlock : (tn_i - (second ? a.tn1 : 0)) * T::kBN;
+  const int kb0 = (int)((int64_t)a.KB * split / a.splits);
+  const int KB = (int)((int64_t)a.KB * (split + 1) / a.splits) - kb0;
+
+  // Staging as in fp8_linear.hip: thread t moves 16-byte chunk t % 8 of row
+  // kRowsPerInst i + t / 8 (instruction i), fetched from chunk (t % 8) ^ swz(row);
+  // rows past the matrix repeat its last row.  Chunks behind the weights' last
+  // column repeat the slice's first: the activations are zero there.
+  const int srow = t >> 3;
+  const uint32_t cb = 16 * ((t & 7) ^ swz(srow));
+  const uint32_t over = cb >= (uint32_t)a.tail ? cb : 0;
+  const uint8_t* xbase = a.xq + (int64_t)m0 * a.xs;
+  const uint8_t* wbase = mat.w + (int64_t)n0 * mat.wrs;
+  uint32_t xo[T::kXInst], wo[T::kWInst];
+#pragma unroll
+  for (int i = 0; i < T::kXInst; ++i)
+    xo[i] = (uint32_t)min(T::kRowsPerInst * i + srow, a.M - 1 - m0) * (uint32_t)a.xs + cb;
+#pragma unroll
+  for (int i = 0; i < T::kWInst; ++i) {
+    const int r = GATED ? 32 * i + (srow & 31) : T::kRowsPerInst * i + srow;
+    wo[i] = (uint32_t)min(r, mat.N - 1 - n0) * (uint32_t)mat.wrs + cb;
+  }
+  // Scales: element e = i threads + t of a slice's list, the 32 MT rows' and then
+  // those of two column blocks (gated: of gate and up).
+  const uint8_t* sp0[T::kSInst];
+  uint32_t sstep[T::kSInst];
+#pragma unroll
+  for (int i = 0; i < T::kSInst; ++i) {
+    const int e = i * T::kThreads + t;
+    if (e < T::kBM) {
+      sp0[i] = reinterpret_cast<const uint8_t*>(a.xsc + min(m0 + e, a.M - 1));
+      sstep[i] = (uint32_t)a.xss * 4u;
+    } else {
+      const int two = min(e - T::kBM, 1);
+      const BlockMat& sm = GATED ? a.mat[two] : mat;
+      const int nb = GATED ? tn_i : min(n0 / kQBlock + two, (sm.N - 1) / kQBlock);
+      sp0[i] = reinterpret_cast<const uint8_t*>(sm.wsc + nb * sm.sn);
+      sstep[i] = (uint32_t)sm.sk * 4u;
+    }
+  }
+  const uint32_t lds0 = lds_addr(smem);
+
+  auto issue_one = [&](int kb, int st, int idx) {
+    const uint32_t sb = lds0 + st * T::kStage + w * 1024;
+    if (idx < T::kXInst) {
+      dma16(xbase + (int64_t)kb * kKSlice, xo[idx], sb + idx * 16 * T::kThreads);
+    } else if (idx < T::kXInst + T::kWInst) {
+      const int i = idx - T::kXInst;
+      dma16(wbase + (int64_t)kb * kKSlice, wo[i] - (kb == a.KB - 1 ? over : 0u),
+            sb + T::kXBytes + i * 16 * T::kThreads);
+    } else {
+      const int i = idx - T::kXInst - T::kWInst;
+      dma4_at(sp0[i] + (uint64_t)(uint32_t)kb * sstep[i],
+              lds0 + st * T::kStage + T::kXBytes + T::kWBytes + i * 4 * T::kThreads + w * 256);
+    }
+  };
+  auto issue = [&](int kb, int st) {
+#pragma unroll
+    for (int idx = 0; idx < T::kLoads; ++idx) issue_one(kb, st, idx);
+  };
+
+  const int rr = l & 15, g = l >> 4;
+  const int o0 = 16 * ((2 * g) ^ swz(rr)), o1 = 16 * ((2 * g + 1) ^ swz(rr));
+  const int xrow = wm * 16 * MT + rr;   // + 16 tm
+  const int wrow = wn * 64 + rr;        // + 16 tn
+
+  f32x4 acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Slices past the last are never read; their stage is refilled with the last
+  // slice so that every step issues (and waits for) the same loads.
+#pragma unroll
+  for (int i = 0; i < T::kAhead; ++i) issue(kb0 + min(i, KB - 1), i);
+  if constexpr (T::kAhead == 2)
+    vm_wait<T::kLoads>();
+  else
+    vm_wait<0>();
+  __syncthreads();
+
+  // Each MFMA starts from zero; its product is folded into the accumulators
+  // with the row's and the column block's scale, one FMA per element per slice,
+  // between the next row's MFMAs (the last row's during the next slice).
+  f32x4 pl[4];
+  float sl0 = 0.f, sl1 = 0.f;
+#pragma unroll
+  for (int tn = 0; tn < 4; ++tn) pl[tn] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int st = 0;
+  for (int j = 0; j < KB; ++j) {
+    const int knext = kb0 + min(j + T::kAhead, KB - 1), stn = st == 0 ? STAGES - 1 : st - 1;
+    const uint8_t* sp = smem + st * T::kStage;
+    const float* ssp = reinterpret_cast<const float*>(sp + T::kXBytes + T::kWBytes);
+    const float w0 = ssp[T::kBM + (GATED ? 0 : wn >> 1)];
+    const float w1 = GATED ? ssp[T::kBM + 1] : w0;
+    i32x8 wf[4], xf[3];
+    float xr[3];
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn)
+      wf[tn] = frag(sp + T::kXBytes + (wrow + 16 * tn) * kKSlice, o0, o1);
+    xf[0] = frag(sp + xrow * kKSlice, o0, o1);
+    xr[0] = ssp[xrow];
+    if constexpr (MT > 1) {
+      xf[1] = frag(sp + (xrow + 16) * kKSlice, o0, o1);
+      xr[1] = ssp[xrow + 16];
+    }
+    f32x4 p[2][4];
+    float s0 = 0.f, s1 = 0.f;   // scales of row tm - 1
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) {
+#pragma unroll
+      for (int q = 0; q < kSpread; ++q)
+        if (tm * kSpread + q < T::kLoads) issue_one(knext, stn, tm * kSpread + q);
+      if (tm == MT - 1)
+#pragma unroll
+        for (int idx = MT * kSpread; idx < T::kLoads; ++idx) issue_one(knext, stn, idx);
+      if (tm + 2 < MT) {
+        xf[(tm + 2) % 3] = frag(sp + (xrow + 16 * (tm + 2)) * kKSlice, o0, o1);
+        xr[(tm + 2) % 3] = ssp[xrow + 16 * (tm + 2)];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        p[tm & 1][tn] = mfma_fp8(wf[tn], xf[tm % 3]);
+        if (tm > 0)
+          acc[tm - 1][tn] += p[(tm - 1) & 1][tn] * (GATED && tn >= 2 ? s1 : s0);
+        else
+          acc[MT - 1][tn] += pl[tn] * (GATED && tn >= 2 ? sl1 : sl0);
+      }
+      if (tm + 2 < MT) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);   // 3 LDS reads
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // 1 MFMA
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // 4 VALU
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      s0 = xr[tm % 3] * w0;
+      s1 = GATED ? xr[tm % 3] * w1 : s0;
+    }
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) pl[tn] = p[(MT - 1) & 1][tn];
+    sl0 = s0;
+    sl1 = s1;
+    if constexpr (T::kAhead == 2)
+      vm_wait<T::kLoads>();
+    else
+      vm_wait<0>();
+    __syncthreads();
+    st = st == STAGES - 1 ? 0 : st + 1;
+  }
+  vm_wait<0>();   // the refills of the last steps land before the stages are reused
+#pragma unroll
+  for (int tn = 0; tn < 4; ++tn) acc[MT - 1][tn] += pl[tn] * (GATED && tn >= 2 ? sl1 : sl0);
+
+  // Lane holds D[wn 64 + 16 tn + 4 g + r][m0 + wm 16 MT + 16 tm + rr].
+  if constexpr (!GATED) {
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) {
+      const int n = n0 + wn * 64 + 16 * tn + 4 * g;
+      if (n >= mat.N) continue;
+#pragma unroll
+      for (int tm = 0; tm < MT; ++tm) {
+        const int m = m0 + xrow + 16 * tm;
+        if (m >= a.M) continue;
+        if (a.part)   // (n_cols and c0 are multiples of 4: a row's last vector stays in it)
+          *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.M + m) * a.n_cols + mat.c0 + n) =
+              acc[tm][tn];
+        else
+          store_out(a, m, n, mat.N, acc[tm][tn]);
+      }
+    }
+  } else {
+    // h of this lane: columns 32 wn + 16 j + 4 g + r of the block, j = 0, 1.  A
+    // row's amax crosses the four lane groups and the four waves of a row.
+    constexpr int kPitch = kQBlock + 16;   // bytes per row of the output tile
+    uint8_t* tile = smem;
+    uint32_t* amax = reinterpret_cast<uint32_t*>(smem + T::kBM * kPitch);
+    static_assert(T::kBM * (kPitch + 16) <= STAGES * T::kStage, "epilogue fits the stages");
+    __syncthreads();
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) {
+      uint32_t mx = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + 32 * wn + 16 * j + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float h = n + r < mat.N ? silu(acc[tm][j][r]) * acc[tm][2 + j][r] : 0.f;
+          acc[tm][j][r] = h;
+          mx = max(mx, __float_as_uint(h) & 0x7fffffffu);
+        }
+      }
+      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
+      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
+      if (g == 0) amax[4 * (xrow + 16 * tm) + wn] = mx;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) {
+      const int row = xrow + 16 * tm;
+      const u32x4 m4 = ld_s16(amax + 4 * row);
+      const float s = block_scale(max(max(m4[0], m4[1]), max(m4[2], m4[3])));
+      if (wn == 0 && g == 0 && m0 + row < a.M)
+        a.hsc[(int64_t)tn_i * a.hss + m0 + row] = s;
+      const float inv = 1.f / s;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f32x4 h = acc[tm][j];
+        *reinterpret_cast<uint32_t*>(tile + row * kPitch + 32 * wn + 16 * j + 4 * g) =
+            e4m3x4(quotient(h[0], s, inv), quotient(h[1], s, inv), quotient(h[2], s, inv),
+                   quotient(h[3], s, inv));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T::kBM * 8 / T::kThreads; ++i) {
+      const int row = i * (T::kThreads / 8) + (t >> 3), c = 16 * (t & 7);
+      if (m0 + row < a.M)
+        *reinterpret_cast<u32x4*>(a.hq + (m0 + row) * a.hqs + (int64_t)tn_i * kQBlock + c) =
+            ld_s16(tile + row * kPitch + c);
+    }
+  }
+}
+
+// Sum of the splits' partials of four columns, in split order.  Every partial is
+// loaded before the first add, so the loads' latencies overlap.
+__device__ __forceinline__ f32x4 sum_splits(const BlockGemmArgs& a, int64_t e) {
+  const int64_t mn = (int64_t)a.M * a.n_cols;
+  f32x4 p[kMaxSplits];
+#pragma unroll
+  for (int sp = 0; sp < kMaxSplits; ++sp)
+    if (sp < a.splits) p[sp] = *reinterpret_cast<const f32x4*>(a.part + sp * mn + e);
+  f32x4 v = p[0];
+#pragma unroll
+  for (int sp = 1; sp < kMaxSplits; ++sp)
+    if (sp < a.splits) v += p[sp];
+  return v;
+}
+
+// out = bf16(sum of the partials + bias), four columns per thread.
+__global__ void __launch_bounds__(kThreads) block_reduce_kernel(BlockGemmArgs a) {
+  const int64_t e = 4 * ((int64_t)blockIdx.x * kThreads + threadIdx.x);
+  if (e >= (int64_t)a.M * a.n_cols) return;
+  const int64_t m = e / a.n_cols;
+  store_out(a, m, (int)(e - m * a.n_cols), a.mat[0].N, sum_splits(a, e));
+}
+
+// h = silu(g) u from the partials of both projections, quantised: 32 lanes hold
+// a block's 128 columns of one row, four each.
+__global__ void __launch_bounds__(kThreads) gated_finish_kernel(BlockGemmArgs a) {
+  const int hb = (a.mat[0].N + kQBlock - 1) / kQBlock;
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (unit >= (int64_t)a.M * hb) return;   // (all 32 lanes of a unit together)
+  const int64_t m = unit / hb;
+  const int b = (int)(unit - m * hb), c = b * kQBlock + 4 * (threadIdx.x & 31);
+  f32x4 h = {0.f, 0.f, 0.f, 0.f};
+  uint32_t mx = 0;
+  if (c < a.mat[0].N) {   // N is a multiple of 16: four columns in or out together
+    const f32x4 gt = sum_splits(a, m * a.n_cols + c);
+    const f32x4 up = sum_splits(a, m * a.n_cols + a.mat[1].c0 + c);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      h[r] = silu(gt[r]) * up[r];
+      mx = max(mx, __float_as_uint(h[r]) & 0x7fffffffu);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, kWave));
+  const float s = block_scale(mx);
+  if ((threadIdx.x & 31) == 0) a.hsc[b * a.hss + m] = s;
+  *reinterpret_cast<uint32_t*>(a.hq + m * a.hqs + c) = e4m3x4(h[0] / s, h[1] / s, h[2] / s,
+                                                             h[3] / s);
+}
+
+// ---------------------------------------------------------------- plans
+// A tile shape (MT, WN) and its estimated time: a workgroup takes fixed +
+// per_slice x K slices microseconds, workgroups run in rounds of one per CU (two
+// of the small ones share a CU and take 1.5 times as long), a split adds a
+// launch and its partials' way through memory.
+struct Shape {
+  int mt, wn;
+};
+struct ShapeCost {
+  Shape shape;
+  float fixed, per_slice;
+  bool two;        // two workgroups per CU
+};
+constexpr ShapeCost kShapes[] = {{{1, 2}, 3.0f, 0.45f, true},  {{2, 2}, 3.5f, 0.48f, true},
+                                 {{4, 2}, 5.0f, 0.65f, false}, {{8, 2}, 3.0f, 1.10f, false},
+                                 {{6, 4}, 3.0f, 1.62f, false}, {{8, 4}, 3.0f, 1.85f, false}};
+constexpr ShapeCost kGatedShapes[] = {{{2, 4}, 5.0f, 0.75f, false},
+                                      {{4, 4}, 5.0f, 1.10f, false},
+                                      {{6, 4}, 5.0f, 1.62f, false},
+                                      {{8, 4}, 5.0f, 1.85f, false}};
+constexpr float kReduceUs = 3.0f, kPartialBytesPerUs = 5e6f;   // written, then read
+
+struct BlockPlan {
+  Shape shape;
+  int splits;
+  bool fused;      // gated: h leaves the product's kernel quantised
+  float us;
+};
+
+float rounds(const ShapeCost& c, int64_t wgs, int64_t cus) {
+  if (!c.two) return (float)((wgs + cus - 1) / cus);
+  const int64_t full = wgs / (2 * cus), rem = wgs - full * 2 * cus;
+  return 1.5f * (float)full + (rem == 0 ? 0.f : rem <= cus ? 1.f : 1.5f);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// n_mats matrices of n columns each; parts: the result is partials whatever the split.
+BlockPlan plan_linear(int64_t m, int64_t n, int n_mats, int64_t kb, bool parts) {
+  const int64_t cus = device_cu_count();
+  BlockPlan best{kShapes[0].shape, 1, false, INFINITY};
+  for (const ShapeCost& c : kShapes) {
+    const int64_t tiles = ceil_div(m, 32 * c.shape.mt) * ceil_div(n, 64 * c.shape.wn) * n_mats;
+    for (int64_t sp = 1; sp <= kMaxSplits; ++sp) {
+      if (sp > 1 && (kb / sp < 2 || tiles * sp > 2 * cus)) break;
+      const float us =
+          rounds(c, tiles * sp, cus) * (c.fixed + c.per_slice * (float)ceil_div(kb, sp)) +
+          (sp > 1 || parts ? kReduceUs + (float)(sp * m * n * n_mats) * 8.f / kPartialBytesPerUs
+                           : 0.f);
+      if (us < best.us) best = {c.shape, (int)sp, false, us};
+    }
+  }
+  return best;
+}
+
+BlockPlan plan_gated(int64_t m, int64_t inter, int64_t kb) {
+  BlockPlan best = plan_linear(m, inter, 2, kb, true);
+  const int64_t cus = device_cu_count();
+  for (const ShapeCost& c : kGatedShapes) {
+    const int64_t tiles = ceil_div(m, 32 * c.shape.mt) * ceil_div(inter, kQBlock);
+    const float us = rounds(c, tiles, cus) * (c.fixed + c.per_slice * (float)kb);
+    if (us < best.us) best = {c.shape, 1, true, us};
+  }
+  return best;
+}
+
+// fp32 elements of a plan's partials (0: none).
+int64_t part_elems(const BlockPlan& p, int64_t m, int64_t n, int n_mats, bool parts) {
+  return p.fused || (p.splits == 1 && !parts) ? 0 : p.splits * m * round_up(n, 4) * n_mats;
+}
+
+template <int MT, int WN, int STAGES, bool GATED>
+void launch_gemm(BlockGemmArgs a, hipStream_t stream) {
+  using T = BlockTile<MT, WN, STAGES>;
+  a.tiles_m = (int)ceil_div(a.M, T::kBM);
+  a.tn1 = (int)ceil_div(a.mat[0].N, GATED ? kQBlock : T::kBN);
+  a.tiles = a.tiles_m * a.tn1 * (GATED ? 1 : a.n_mats);
+  hipLaunchKernelGGL((block_gemm_kernel<MT, WN, STAGES, GATED>),
+                     dim3((uint32_t)(a.tiles * a.splits)), dim3(T::kThreads), 0, stream, a);
+}
+
+void launch_linear(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
+  a.splits = p.splits;
+  const Shape sh = p.shape;
+  if (sh.mt == 1)
+    launch_gemm<1, 2, 3, false>(a, s);
+  else if (sh.mt == 2)
+    launch_gemm<2, 2, 3, false>(a, s);
+  else if (sh.mt == 4)
+    launch_gemm<4, 2, 3, false>(a, s);
+  else if (sh.wn == 2)
+    launch_gemm<8, 2, 3, false>(a, s);
+  else if (sh.mt == 6)
+    launch_gemm<6, 4, 2, false>(a, s);
+  else
+    launch_gemm<8, 4, 2, false>(a, s);
+}
+
+void launch_fused(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
+  a.splits = 1;
+  if (p.shape.mt == 2)
+    launch_gemm<2, 4, 3, true>(a, s);
+  else if (p.shape.mt == 4)
+    launch_gemm<4, 4, 3, true>(a, s);
+  else if (p.shape.mt == 6)
+    launch_gemm<6, 4, 2, true>(a, s);
+  else
+    launch_gemm<8, 4, 2, true>(a, s);
+}
+
+// ---------------------------------------------------------------- arguments
+constexpr int64_t kMaxDim = 1 << 24;   // columns of a matrix: 32-bit offsets inside a tile
+constexpr int64_t kMaxRows = 1 << 24;
+
+int32_t check_rows(const char* fn, int64_t rows, int64_t cols, int64_t multiple) {
+  if (rows < 0 || cols <= 0 || cols % multiple)
+    return fail(TF_ERR_INVALID, "%s: rows=%lld cols=%lld (cols a positive multiple of %lld)", fn,
+                (long long)rows, (long long)cols, (long long)multiple);
+  if (rows > kMaxRows || cols > kMaxDim)
+    return fail(TF_ERR_UNSUPPORTED, "%s: %lld x %lld is too large", fn, (long long)rows,
+                (long long)cols);
+  return TF_OK;
+}
+
+int32_t quant_setup(const char* fn, const void* x, int32_t x_dtype, int64_t rows, int64_t cols,
+                    int64_t x_row_stride, void* xq, int64_t xq_row_stride, float* x_scale,
+                    int64_t x_scale_stride, int64_t out_cols, BlockQuantArgs* a) {
+  int32_t rc = check_rows(fn, rows, cols, 8);
+  if (rc != TF_OK) return rc;
+  if (x_dtype != TF_DTYPE_BF16 && x_dtype != TF_DTYPE_FP32)
+    return fail(TF_ERR_UNSUPPORTED, "%s: x must be bf16 or fp32 (dtype %d)", fn, x_dtype);
+  if (x_row_stride < cols || x_row_stride % 8 || xq_row_stride < out_cols || xq_row_stride % 8 ||
+      x_scale_stride < rows || x_scale_stride > kMaxRows)
+    return fail(TF_ERR_INVALID, "%s: strides %lld/%lld/%lld (rows multiples of 8; scales from the "
+                "number of rows up)", fn, (long long)x_row_stride, (long long)xq_row_stride,
+                (long long)x_scale_stride);
+  if (rows > 0 && (!x || !xq || !x_scale)) return fail(TF_ERR_INVALID, "%s: null pointer", fn);
+  if (!aligned16(x) || !aligned8(xq) || (reinterpret_cast<uintptr_t>(x_scale) & 3u))
+    return fail(TF_ERR_INVALID, "%s: x 16-byte, xq 8-byte, scales 4-byte aligned", fn);
+  a->x = static_cast<const uint8_t*>(x);
+  a->xs = x_row_stride;
+  a->rows = rows;
+  a->cols = (int32_t)cols;
+  a->out_cols = (int32_t)out_cols;
+  a->xq = static_cast<uint8_t*>(xq);
+  a->qs = xq_row_stride;
+  a->scale = x_scale;
+  a->ss = x_scale_stride;
+  a->col_groups = (int32_t)ceil_div(out_cols, kQuantBlocks * kQBlock);
+  if (ceil_div(rows, kQuantRows) * a->col_groups > INT32_MAX)
+    return fail(TF_ERR_UNSUPPORTED, "%s: too large", fn);
+  return TF_OK;
+}
+
+void launch_quant(const BlockQuantArgs& a, bool f32, hipStream_t s) {
+  const dim3 grid((uint32_t)(ceil_div(a.rows, kQuantRows) * a.col_groups));
+  if (f32)
+    hipLaunchKernelGGL(block_quant_kernel<true>, grid, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(block_quant_kernel<false>, grid, dim3(kThreads), 0, s, a);
+}
+
+// Checks one weight and describes it (out and bias are the caller's).
+int32_t weight_setup(const char* fn, const char* what, const tf_fp8_mat* t, int64_t n, int64_t k,
+                     BlockMat* b) {
+  if (!t) return fail(TF_ERR_INVALID, "%s: no %s", fn, what);
+  if (t->n != n || n <= 0)
+    return fail(TF_ERR_INVALID, "%s: %s has %lld columns, expected %lld", fn, what,
+                (long long)t->n, (long long)n);
+  if (n > kMaxDim) return fail(TF_ERR_UNSUPPORTED, "%s: %s is too large", fn, what);
+  if (!t->w || !t->w_scale) return fail(TF_ERR_INVALID, "%s: %s: null pointer", fn, what);
+  if (!aligned16(t->w) || (reinterpret_cast<uintptr_t>(t->w_scale) & 3u))
+    return fail(TF_ERR_INVALID, "%s: %s 16-byte, its scales 4-byte aligned", fn, what);
+  if (t->w_row_stride < k || t->w_row_stride % 16 || t->w_row_stride > kMaxDim ||
+      t->w_scale_row_stride < 0 || t->w_scale_col_stride < 0 || t->w_scale_col_stride > kMaxDim)
+    return fail(TF_ERR_INVALID, "%s: %s strides %lld/%lld/%lld (rows 16-byte multiples)", fn, what,
+                (long long)t->w_row_stride, (long long)t->w_scale_row_stride,
+                (long long)t->w_scale_col_stride);
+  b->w = static_cast<const uint8_t*>(t->w);
+  b->wrs = t->w_row_stride;
+  b->wsc = t->w_scale;
+  b->sn = t->w_scale_row_stride;
+  b->sk = t->w_scale_col_stride;
+  b->N = (int32_t)n;
+  b->c0 = 0;
+  return TF_OK;
+}
+
+int32_t out_setup(const char* fn, const tf_fp8_mat* t, BlockGemmArgs* a) {
+  if (!t->out) return fail(TF_ERR_INVALID, "%s: null output", fn);
+  if (t->out_row_stride < t->n)
+    return fail(TF_ERR_INVALID, "%s: out row stride %lld for %lld columns", fn,
+                (long long)t->out_row_stride, (long long)t->n);
+  if (!aligned8(t->out) || (reinterpret_cast<uintptr_t>(t->bias) & 1u))
+    return fail(TF_ERR_INVALID, "%s: out must be 8-byte aligned", fn);
+  a->bias = static_cast<const uint16_t*>(t->bias);
+  a->out = static_cast<uint16_t*>(t->out);
+  a->os = t->out_row_stride;
+  return TF_OK;
+}
+
+// Workspace of both products' calls: x quantised (where it comes unquantised),
+// the quantised hidden activations (gated), the partials.
+struct Layout {
+  int64_t xsc, hq, hsc, part, bytes;
+};
+Layout layout(int64_t m, int64_t k, int64_t inter, bool quantized, int64_t parts) {
+  Layout l;
+  l.xsc = quantized ? 0 : round_up(m * round_up(k, kQBlock), 256);
+  l.hq = l.xsc + (quantized ? 0 : round_up(4 * m * ceil_div(k, kQBlock), 256));
+  l.hsc = l.hq + round_up(m * round_up(inter, kQBlock), 256);
+  l.part = l.hsc + round_up(4 * m * ceil_div(inter, kQBlock), 256);
+  l.bytes = l.part + 4 * parts;
+  return l;
+}
+
+// x of a product: quantised rows as they come, or quantised into the workspace.
+int32_t input_setup(const char* fn, const void* x, int32_t x_dtype, int64_t x_row_stride,
+                    const float* x_scale, int64_t x_scale_stride, int64_t m, int64_t k,
+                    uint8_t* ws, const Layout& l, BlockGemmArgs* g, BlockQuantArgs* q) {
+  g->M = (int32_t)m;
+  g->KB = (int32_t)ceil_div(k, kQBlock);
+  g->tail = (int32_t)(k - (int64_t)(g->KB - 1) * kQBlock);
+  if (x_dtype != TF_DTYPE_FP8_E4M3) {
+    float* sc = reinterpret_cast<float*>(ws + l.xsc);
+    const int64_t kp = (int64_t)g->KB * kQBlock;
+    g->xq = ws;
+    g->xs = kp;
+    g->xsc = sc;
+    g->xss = m;
+    return quant_setup(fn, x, x_dtype, m, k, x_row_stride, ws, kp, sc, m, kp, q);
+  }
+  if (!x || !x_scale) return fail(TF_ERR_INVALID, "%s: null pointer", fn);
+  if (!aligned16(x) || (reinterpret_cast<uintptr_t>(x_scale) & 3u))
+    return fail(TF_ERR_INVALID, "%s: x 16-byte, its scales 4-byte aligned", fn);
+  if (x_row_stride < (int64_t)g->KB * kQBlock || x_row_stride % 16 || x_row_stride > kMaxDim ||
+      x_scale_stride < m || x_scale_stride > kMaxRows)
+    return fail(TF_ERR_INVALID, "%s: quantised x strides %lld/%lld (rows a multiple of 16 from "
+                "the padded width up, scales from the number of rows up)", fn,
+                (long long)x_row_stride, (long long)x_scale_stride);
+  g->xq = static_cast<const uint8_t*>(x);
+  g->xs = x_row_stride;
+  g->xsc = x_scale;
+  g->xss = x_scale_stride;
+  return TF_OK;
+}
+
+bool bad_workspace(const void* ws, int64_t bytes, int64_t need) {
+  return need > 0 && (!ws || !aligned16(ws) || bytes < need);
+}
+
+// The product itself: tiles, or partials and their sum.
+void run_linear(BlockGemmArgs g, const BlockPlan& p, float* part, hipStream_t s) {
+  g.n_mats = 1;
+  g.n_cols = (int32_t)round_up(g.mat[0].N, 4);
+  g.part = p.splits > 1 ? part : nullptr;
+  launch_linear(g, p, s);
+  if (!g.part) return;
+  g.splits = p.splits;
+  hipLaunchKernelGGL(block_reduce_kernel,
+                     dim3((uint32_t)ceil_div((int64_t)g.M * g.n_cols / 4, kThreads)),
+                     dim3(kThreads), 0, s, g);
+}
+
+int32_t check_product(const char* fn, int64_t m, int64_t n, int64_t k) {
+  const int32_t rc = check_rows(fn, m, k, 16);
+  if (rc != TF_OK) return rc;
+  if (n <= 0) return fail(TF_ERR_INVALID, "%s: %lld columns", fn, (long long)n);
+  if (n > kMaxDim || ceil_div(m, 32) * ceil_div(n, 64) > INT32_MAX / (2 * kMaxSplits))
+    return fail(TF_ERR_UNSUPPORTED, "%s: %lld x %lld is too large", fn, (long long)m,
+                (long long)n);
+  return TF_OK;
+}
+
+}  // namespace
+}  // namespace tfa
+
+extern "C" {
+
+int32_t tf_block_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t cols,
+                       int64_t x_row_stride, void* xq, int64_t xq_row_stride, float* x_scale,
+                       int64_t x_scale_stride, tf_stream_t stream) {
+  using namespace tfa;
+  clear_error();
+  BlockQuantArgs a;
+  const int32_t rc = quant_setup("block_quant", x, x_dtype, rows, cols, x_row_stride, xq,
+                                 xq_row_stride, x_scale, x_scale_stride, cols, &a);
+  if (rc != TF_OK || rows == 0) return rc;
+  launch_quant(a, x_dtype == TF_DTYPE_FP32, reinterpret_cast<hipStream_t>(stream));
+  return launch_status("tf_block_quant launch");
+}
+
+int64_t tf_block_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t x_dtype) {
+  using namespace tfa;
+  clear_error();
+  const int32_t rc = check_product("block_linear", m, n, k);
+  if (rc != TF_OK) return rc;
+  if (m == 0) return 0;
+  const BlockPlan p = plan_linear(m, n, 1, ceil_div(k, kQBlock), false);
+  return layout(m, k, 0, x_dtype == TF_DTYPE_FP8_E4M3, part_elems(p, m, n, 1, false)).bytes;
+}
+
+int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
+                        const float* x_scale, int64_t x_scale_stride, const tf_fp8_mat* mat,
+                        int64_t m, int64_t k, void* workspace, int64_t workspace_bytes,
+                        tf_stream_t stream) {
+  using namespace tfa;
+  clear_error();
+  if (!mat) return fail(TF_ERR_INVALID, "block_linear: no weight");
+  int32_t rc = check_product("block_linear", m, mat->n, k);
+  if (rc != TF_OK || m == 0) return rc;
+  const int64_t n = mat->n;
+  const BlockPlan p = plan_linear(m, n, 1, ceil_div(k, kQBlock), false);
+  const bool quantized = x_dtype == TF_DTYPE_FP8_E4M3;
+  const Layout l = layout(m, k, 0, quantized, part_elems(p, m, n, 1, false));
+  if (bad_workspace(workspace, workspace_bytes, l.bytes))
+    return fail(TF_ERR_INVALID, "block_linear: workspace of %lld bytes (needs %lld, 16-byte "
+                "aligned)", (long long)workspace_bytes, (long long)l.bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  BlockGemmArgs g{};
+  BlockQuantArgs q;
+  if ((rc = weight_setup("block_linear", "weight", mat, n, k, &g.mat[0])) != TF_OK) return rc;
+  if ((rc = out_setup("block_linear", mat, &g)) != TF_OK) return rc;
+  rc = input_setup("block_linear", x, x_dtype, x_row_stride, x_scale, x_scale_stride, m, k, ws, l,
+                   &g, &q);
+  if (rc != TF_OK) return rc;   // nothing is launched for arguments that any part refuses
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
+  run_linear(g, p, reinterpret_cast<float*>(ws + l.part), s);
+  return launch_status("tf_block_linear launch");
+}
+
+int64_t tf_gated_mlp_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, int64_t n_out,
+                                     int32_t x_dtype) {
+  using namespace tfa;
+  clear_error();
+  int32_t rc = check_product("gated_mlp", m, inter, hidden);
+  if (rc == TF_OK) rc = check_product("gated_mlp", m, n_out, inter);
+  if (rc != TF_OK) return rc;
+  if (m == 0) return 0;
+  const BlockPlan up = plan_gated(m, inter, ceil_div(hidden, kQBlock));
+  const BlockPlan down = plan_linear(m, n_out, 1, ceil_div(inter, kQBlock), false);
+  return layout(m, hidden, inter, x_dtype == TF_DTYPE_FP8_E4M3,
+                std::max(part_elems(up, m, inter, 2, true), part_elems(down, m, n_out, 1, false)))
+      .bytes;
+}
+
+int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const float* x_scale,
+                     int64_t x_scale_stride, const tf_fp8_mat* gate, const tf_fp8_mat* up,
+                     const tf_fp8_mat* down, int64_t m, int64_t hidden, int64_t inter,
+                     void* workspace, int64_t workspace_bytes, tf_stream_t stream) {
+  using namespace tfa;
+  if (!gate || !up || !down) {
+    clear_error();
+    return fail(TF_ERR_INVALID, "gated_mlp: a weight is missing");
+  }
+  const int64_t n_out = down->n;
+  const int64_t need = tf_gated_mlp_workspace_bytes(m, hidden, inter, n_out, x_dtype);
+  if (need < 0) return (int32_t)need;   // (it cleared and set the error)
+  if (m == 0) return TF_OK;
+  if (bad_workspace(workspace, workspace_bytes, need))
+    return fail(TF_ERR_INVALID, "gated_mlp: workspace of %lld bytes (needs %lld, 16-byte aligned)",
+                (long long)workspace_bytes, (long long)need);
+  const BlockPlan pu = plan_gated(m, inter, ceil_div(hidden, kQBlock));
+  const BlockPlan pd = plan_linear(m, n_out, 1, ceil_div(inter, kQBlock), false);
+  const bool quantized = x_dtype == TF_DTYPE_FP8_E4M3;
+  const Layout l = layout(m, hidden, inter, quantized, 0);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* part = reinterpret_cast<float*>(ws + l.part);
+  BlockGemmArgs g{}, d{};
+  BlockQuantArgs q;
+  int32_t rc;
+  if ((rc = weight_setup("gated_mlp", "gate weight", gate, inter, hidden, &g.mat[0])) != TF_OK ||
+      (rc = weight_setup("gated_mlp", "up weight", up, inter, hidden, &g.mat[1])) != TF_OK ||
+      (rc = weight_setup("gated_mlp", "down weight", down, n_out, inter, &d.mat[0])) != TF_OK ||
+      (rc = out_setup("gated_mlp", down, &d)) != TF_OK ||
+      (rc = input_setup("gated_mlp", x, x_dtype, x_row_stride, x_scale, x_scale_stride, m, hidden,
+                        ws, l, &g, &q)) != TF_OK)
+    return rc;
+  d.M = (int32_t)m;
+  d.KB = (int32_t)ceil_div(inter, kQBlock);
+  d.tail = (int32_t)(inter - (int64_t)(d.KB - 1) * kQBlock);
+  d.xq = g.hq = ws + l.hq;
+  d.xs = g.hqs = (int64_t)d.KB * kQBlock;
+  d.xsc = g.hsc = reinterpret_cast<float*>(ws + l.hsc);
+  d.xss = g.hss = m;
+  g.n_mats = 2;
+  g.mat[1].c0 = (int32_t)inter;
+  g.n_cols = (int32_t)(2 * inter);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
+  if (pu.fused) {
+    launch_fused(g, pu, s);
+  } else {
+    g.part = part;
+    launch_linear(g, pu, s);
+    g.splits = pu.splits;
+    hipLaunchKernelGGL(gated_finish_kernel, dim3((uint32_t)ceil_div(m * d.KB, kThreads / 32)),
+                       dim3(kThreads), 0, s, g);
+  }
+  run_linear(d, pd, part, s);
+  return launch_status("tf_gated_mlp launch");
+}
+
+}  // extern "C"

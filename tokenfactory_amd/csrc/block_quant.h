@@ -1,0 +1,75 @@
+// Device side of the block quantisation: e4m3 values with one fp32 scale per 128
+// columns of a row,
+//   s = fl32(max(amax|x|, 1e-12) / 448),  q = e4m3(fl32(x / s)),
+// both roundings as torch's tensor operations make them.  amax travels as the
+// bits of |x|: for them integer order is float order and NaN sorts above inf, so
+// a NaN (or inf) anywhere in a block makes its scale NaN (inf) and with it every
+// product of the block, and no other row's.
+#pragma once
+
+#include "tf_common.h"
+
+namespace tfa {
+
+constexpr int kQBlock = 128;
+
+// Eight consecutive elements (16-byte aligned) of a bf16 or fp32 array.
+template <bool F32>
+__device__ __forceinline__ void load8(const uint8_t* p, int64_t elem, float* v) {
+  if constexpr (F32) {
+    const u32x4 a = ld_g16(p + elem * 4), b = ld_g16(p + elem * 4 + 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = __uint_as_float(a[j]);
+      v[4 + j] = __uint_as_float(b[j]);
+    }
+  } else {
+    const u32x4 a = ld_g16(p + elem * 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = bf16_lo(a[j]);
+      v[2 * j + 1] = bf16_hi(a[j]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t amax_bits8(const float* v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  return m;
+}
+// Maximum over the 16 lanes that hold a block (all of them call it).
+__device__ __forceinline__ uint32_t amax_lanes16(uint32_t m) {
+#pragma unroll
+  for (int d = 8; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, kWave));
+  return m;
+}
+
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+  const uint32_t floor_bits = __float_as_uint(1e-12f);
+  return __uint_as_float(max(amax_bits, floor_bits)) / 448.f;
+}
+
+// fl32(x / s) from inv = fl32(1 / s): one correction step of the approximate
+// quotient by its exact remainder.  Finite x and s only (an inf or NaN scale
+// gives NaN where the division gives 0 or NaN; either poisons the block).
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  const float q = x * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+}
+
+__device__ __forceinline__ float clamp448(float x) {   // NaN stays
+  return x != x ? x : fminf(fmaxf(x, -448.f), 448.f);
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t r =
+      __builtin_amdgcn_cvt_pk_fp8_f32(clamp448(a), clamp448(b), 0u, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(clamp448(c), clamp448(d), r, true);
+}
+__device__ __forceinline__ u32x2 quant8(const float* v, float s) {
+  return u32x2{e4m3x4(v[0] / s, v[1] / s, v[2] / s, v[3] / s),
+               e4m3x4(v[4] / s, v[5] / s, v[6] / s, v[7] / s)};
+}
+
+}  // namespace tfa

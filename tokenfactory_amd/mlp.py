@@ -1,0 +1,92 @@
+"""The gated feed-forward block on block-FP8 weights.
+
+``gated_mlp`` is ``down(silu(gate(x)) * up(x))`` (``qwen3_8/mlp.py:9-54``) with
+activations quantised per row and 128 columns (``block_fp8``): the gate and up
+products share a kernel whose output is the quantised hidden activations, formed
+from the fp32 sums; the down product reads those.
+
+``GatedMLP`` holds the block's weights under the reference's names, as
+``Fp8Linear`` parameters, so a reference layer's state dict loads as is.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from . import _native
+from .block_fp8 import BLOCK, DTYPES, check_input, check_weight, input_rows, mat
+from .fp8_linear import Fp8Linear, _ptr, _stream_ptr, on_stream
+
+
+def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.Tensor,
+              up_weight: torch.Tensor, up_scale_inv: torch.Tensor, down_weight: torch.Tensor,
+              down_scale_inv: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
+              stream=None) -> torch.Tensor:
+    """``bf16(h^ Wd^T)`` with ``h = silu(x^ Wg^T) * (x^ Wu^T)`` in fp32; ``^`` is
+    ``quantize_blocks``' form.
+
+    x: bf16 or fp32 ``[..., hidden]`` or float8_e4m3fn ``[rows, hidden]`` with its
+    ``x_scale``; gate and up weights float8_e4m3fn ``[inter, hidden]``, down
+    ``[out, inter]``, each with fp32 scales per 128 x 128 block; hidden and inter
+    multiples of 16.  Returns bf16 ``[..., out]``."""
+    fn = "gated_mlp"
+    hidden = gate_weight.shape[-1]
+    x2d = check_input(fn, x, x_scale, hidden)
+    dev = x.device
+    check_weight(fn, "gate_weight", gate_weight, gate_scale_inv, hidden, dev)
+    check_weight(fn, "up_weight", up_weight, up_scale_inv, hidden, dev)
+    inter = gate_weight.shape[0]
+    if up_weight.shape[0] != inter:
+        raise ValueError(f"{fn}: {inter} gate and {up_weight.shape[0]} up columns")
+    check_weight(fn, "down_weight", down_weight, down_scale_inv, inter, dev)
+    if inter % 16:
+        raise NotImplementedError(f"{fn}: {inter} hidden activations (a multiple of 16)")
+    rows, n = x2d.shape[0], down_weight.shape[0]
+    with _native.on_device(dev), on_stream(stream):
+        out = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
+        if rows:
+            xr, xs, sc, ss = input_rows(x2d, x_scale)
+            nbytes = _native.load().tf_gated_mlp_workspace_bytes(rows, hidden, inter, n,
+                                                                 DTYPES[x.dtype])
+            ws = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=dev)
+            _native.call("tf_gated_mlp", _ptr(xr), DTYPES[x.dtype], xs, _ptr(sc), ss,
+                         mat(gate_weight, gate_scale_inv), mat(up_weight, up_scale_inv),
+                         mat(down_weight, down_scale_inv, out=out), rows, hidden, inter,
+                         _ptr(ws), nbytes, _stream_ptr(stream, dev))
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
+
+
+class GatedMLP(nn.Module):
+    """One TP rank's share of the gated feed-forward block: ``gate_proj`` and
+    ``up_proj`` ``[intermediate_size / tp, hidden]`` and ``down_proj``, whose partial
+    sums the caller adds over the ranks.  The three ``Fp8Linear``s hold weights and
+    scales; ``forward`` reads them and does not call the modules."""
+
+    def __init__(self, config):
+        super().__init__()
+        q = getattr(config, "quantization_config", None)
+        if not isinstance(q, dict) or q.get("quant_method") != "fp8":
+            raise NotImplementedError("GatedMLP: weights must be block-FP8 (quantization_config "
+                                      "with quant_method fp8)")
+        block = tuple(q.get("weight_block_size", [BLOCK, BLOCK]))
+        if block != (BLOCK, BLOCK):
+            raise NotImplementedError(f"GatedMLP: weight blocks of {block} (128 x 128)")
+        act = getattr(config, "hidden_act", "silu")
+        if act != "silu":
+            raise NotImplementedError(f"GatedMLP: activation {act!r} (silu)")
+        tp = getattr(config, "tp_size", 1)
+        if config.intermediate_size % tp:
+            raise ValueError("intermediate_size must divide by tp_size")
+        inter = config.intermediate_size // tp
+        if inter % 16 or config.hidden_size % 16:
+            raise NotImplementedError(f"GatedMLP: {config.hidden_size} x {inter} (multiples of 16)")
+        self.gate_proj = Fp8Linear(config.hidden_size, inter, block_size=block)
+        self.up_proj = Fp8Linear(config.hidden_size, inter, block_size=block)
+        self.down_proj = Fp8Linear(inter, config.hidden_size, block_size=block)
+
+    def forward(self, x: torch.Tensor, x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+        g, u, d = self.gate_proj, self.up_proj, self.down_proj
+        return gated_mlp(x, g.weight, g.weight_scale_inv, u.weight, u.weight_scale_inv, d.weight,
+                         d.weight_scale_inv, x_scale=x_scale)
