@@ -561,10 +561,10 @@ int64_t tf_fp8_linears_workspace_bytes(int64_t m, const tf_fp8_mat* mats, int32_
  * 8-byte aligned.  The result is deterministic.
  *
  * tf_gated_mlp: out = h^ Wd^T with h = silu(x Wg^T) * (x Wu^T) in fp32 and h^ its
- * block-quantised form (qwen3_8/mlp.py:9-54).  gate and up: n = inter
- * (a multiple of 16) over hidden (a multiple of 16) columns, their out and bias
- * unused; down: any n over inter columns, with out and optional bias.  x as in
- * tf_block_linear.
+ * block-quantised form (qwen3_8/mlp.py:9-54).  mats: a host array of three, read
+ * during the call: gate and up, n = inter (a multiple of 16) over hidden (a
+ * multiple of 16) columns, their out and bias unused; down, any n over inter
+ * columns, with out and optional bias.  x as in tf_block_linear.
  *
  * workspace: device, 16-byte aligned, *_workspace_bytes(...) bytes for the same
  * sizes and x_dtype on the same device; not shared by calls that overlap in time.
@@ -584,9 +584,9 @@ int64_t tf_gated_mlp_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, i
                                      int32_t x_dtype);
 
 int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const float* x_scale,
-                     int64_t x_scale_stride, const tf_fp8_mat* gate, const tf_fp8_mat* up,
-                     const tf_fp8_mat* down, int64_t m, int64_t hidden, int64_t inter,
-                     void* workspace, int64_t workspace_bytes, tf_stream_t stream);
+                     int64_t x_scale_stride, const tf_fp8_mat* mats, int64_t m, int64_t hidden,
+                     int64_t inter, void* workspace, int64_t workspace_bytes,
+                     tf_stream_t stream);
 
 /* tf_add_rms_norm: the residual sum and the norms around a block
  * (qwen3_8/decoder_layer.py:57-81, qwen3_8/rms_norm.py:19-24), per row, in fp32:

@@ -120,23 +120,23 @@ def test_empty_products_touch_nothing():
     lib = _native.load()
     assert lib.tf_block_linear_workspace_bytes(0, 64, 256, BF16) == 0
     assert lib.tf_gated_mlp_workspace_bytes(0, 256, 512, 256, BF16) == 0
-    mats = [ctypes.byref(_mat(n, k)) for n, k in ((512, 256), (512, 256), (256, 512))]
-    assert lib.tf_gated_mlp(None, BF16, 256, None, 0, *mats, 0, 256, 512, None, 0, None) == 0
+    mats = (_native.Fp8Mat * 3)(*[_mat(n, k) for n, k in ((512, 256), (512, 256), (256, 512))])
+    assert lib.tf_gated_mlp(None, BF16, 256, None, 0, mats, 0, 256, 512, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(hidden=250), INVALID), (dict(inter=500), INVALID),
-    (dict(up=(496, 256)), INVALID), (dict(ws_bytes=64), INVALID), (dict(down=None), INVALID),
+    (dict(up=(496, 256)), INVALID), (dict(ws_bytes=64), INVALID), (dict(mats=None), INVALID),
+    (dict(down=(0, 512)), INVALID),
     (dict(x_dtype=9), UNSUPPORTED),
 ])
 def test_mlp_refusals(change, code):
     a = dict(hidden=256, inter=512, up=(512, 256), down=(256, 512), ws_bytes=1 << 30, x_dtype=BF16)
     a.update(change)
-    byref = lambda nk: None if nk is None else ctypes.byref(_mat(*nk))
+    mats = (_native.Fp8Mat * 3)(_mat(512, 256), _mat(*a["up"]), _mat(*a["down"]))
     lib = _native.load()
-    assert lib.tf_gated_mlp(16, a["x_dtype"], 256, None, 0, byref((512, 256)), byref(a["up"]),
-                            byref(a["down"]), 4, a["hidden"], a["inter"], 256, a["ws_bytes"],
-                            None) == code
+    assert lib.tf_gated_mlp(16, a["x_dtype"], 256, None, 0, a.get("mats", mats), 4, a["hidden"],
+                            a["inter"], 256, a["ws_bytes"], None) == code
 
 
 def test_workspaces_cover_the_quantised_rows():

@@ -113,7 +113,8 @@ def check_linear(gpu, m, n, k, bias=False, quantized=False, dtype=torch.bfloat16
 
 # One row to many, tiles cut in every dimension, each tile shape of the plan, split and not.
 @pytest.mark.parametrize("m,n,k", [
-    (1, 64, 16), (1, 1, 48), (1, 5120, 6144), (2, 130, 272), (16, 640, 256), (17, 2592, 5120),
+    (1, 64, 16), (1, 1, 48), (1, 5120, 6144), (1, 40, 17408), (1, 33, 36864), (2, 130, 272),
+    (4, 100, 8192), (5, 77, 9008), (16, 48, 12800), (16, 640, 256), (17, 2592, 5120),
     (33, 129, 128), (48, 5120, 1024), (64, 257, 1040), (65, 512, 384), (100, 2592, 1536),
     (129, 384, 2064), (300, 5120, 640), (700, 513, 400), (1030, 1024, 256), (1900, 12288, 640),
     (2100, 640, 512), (4097, 5120, 256), (8192, 2048, 384)])

@@ -55,7 +55,8 @@ def compare(out, x, host):
 
 # One row to several tiles of rows; widths that end inside a block and a tile.
 @pytest.mark.parametrize("m,hidden,inter", [
-    (1, 16, 16), (1, 256, 1024), (1, 5120, 640), (2, 272, 400), (16, 512, 1040), (17, 1024, 512),
+    (1, 16, 16), (1, 256, 1024), (1, 5120, 640), (1, 512, 8192), (2, 272, 400),
+    (4, 1024, 4112), (7, 512, 8192), (16, 512, 1040), (17, 1024, 512),
     (48, 640, 1152), (64, 384, 272), (65, 256, 2176), (130, 1040, 384), (200, 512, 528),
     (333, 1024, 2176), (520, 256, 640), (1100, 256, 512)])
 @pytest.mark.parametrize("quantized", [False, True])

@@ -185,7 +185,7 @@ SIGNATURES = {
     "tf_gated_mlp_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32]),
     "tf_gated_mlp": (_i32, [
         _p, _i32, _i64, _p, _i64,      # x, x_dtype, x_row_stride, x_scale, x_scale_stride
-        _p, _p, _p, _i64, _i64, _i64,  # gate, up, down, m, hidden, inter
+        _p, _i64, _i64, _i64,          # mats (gate, up, down), m, hidden, inter
         _p, _i64, _p,                  # workspace, workspace_bytes, stream
     ]),
     "tf_add_rms_norm": (_i32, [
@@ -298,7 +298,7 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
 
 def call(name: str, *args) -> int:
     """Calls an int32-status entry point and raises on a negative status."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc < 0:
         msg = lib.tf_attn_last_error().decode(errors="replace")
@@ -323,13 +323,23 @@ def current_stream(device) -> int:
     return _raw_stream(device.index)
 
 
+@contextlib.contextmanager
+def _launching(device, stream):
+    with torch.cuda.device(device), (contextlib.nullcontext() if stream is None
+                                     else torch.cuda.stream(stream)):
+        yield
+
+
 _here = contextlib.nullcontext()
 
 
-def on_device(device):
-    """Context that makes ``device`` the current one (launches go to the current
-    device whatever stream they name); a no-op where it is already."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def launching(device, stream):
+    """Context in which a call on ``device`` allocates and launches: with that device
+    (launches go to the current one, whatever stream they name) and ``stream`` (None:
+    the device's current stream) current.  A no-op where they are already."""
+    if stream is None and torch.cuda.current_device() == device.index:
+        return _here
+    return _launching(device, stream)
 
 
 def plan_device_capacity(total_tokens, batch_size, num_q_heads, num_kv_heads) -> int:

@@ -13,20 +13,15 @@ from typing import Optional
 import torch
 
 from . import _native
-from .block_fp8 import DTYPES, new_scales, row_stride, rows16
-from .fp8_linear import _ptr, _stream_ptr, on_stream
+from .block_fp8 import DTYPES, new_rows, new_scales, row_stride, rows16
 
 MAX_COLS = 16384
 _VALUES = (torch.bfloat16, torch.float32)
 
 
-def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
-    if t.dtype not in _VALUES or t.device != like.device or tuple(t.shape) != tuple(shape):
+def _check(name: str, t: torch.Tensor, shape, device) -> None:
+    if t.dtype not in _VALUES or t.shape != shape or t.device != device:
         raise ValueError(f"add_rms_norm: {name} must be bf16 or fp32 {tuple(shape)} on x's device")
-
-
-def _dtype(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else DTYPES[t.dtype]
 
 
 def _gate_rows(gate: torch.Tensor, shape):
@@ -71,11 +66,13 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
         raise NotImplementedError(f"add_rms_norm: {cols} columns (at most {MAX_COLS})")
     if quantize and weight is None:
         raise ValueError("add_rms_norm: quantize needs a weight")
-    for name, t in (("weight", weight), ("post_weight", post_weight)):
-        if t is not None:
-            _check(name, t, x, (cols,))
+    dev = x.device
+    if weight is not None:
+        _check("weight", weight, (cols,), dev)
+    if post_weight is not None:
+        _check("post_weight", post_weight, (cols,), dev)
     if residual is not None:
-        _check("residual", residual, x, x.shape)
+        _check("residual", residual, x.shape, dev)
     if inplace and (residual is None or rows16(residual) is not residual):
         raise ValueError("add_rms_norm: in place, residual must be given, with dense 16-byte "
                          "aligned rows")
@@ -83,26 +80,36 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
         raise ValueError("add_rms_norm: gate must be bf16 or fp32 on x's device")
     scale = float(residual_scale)
     same = residual is None and gate is None and post_weight is None and scale == 1.0
-    dev = x.device
-    with _native.on_device(dev), on_stream(stream):
-        gp, gs, gcols = (None, 0, 0) if gate is None else _gate_rows(gate, x.shape)
-        xr = rows16(x)
-        rr = None if residual is None else rows16(residual)
-        r = x if same else residual if inplace else torch.empty(
-            (rows, cols), dtype=x.dtype if residual is None else residual.dtype, device=dev)
+    xt = rt = DTYPES[x.dtype]
+    yt = DTYPES[torch.float8_e4m3fn] if quantize else xt
+    with _native.launching(dev, stream):
+        xr, rp, rs, r = rows16(x), 0, 0, x
+        if residual is not None:
+            rr, rt = rows16(residual), DTYPES[residual.dtype]
+            rp, rs = rr.data_ptr(), row_stride(rr)
+        if inplace:
+            r = residual
+        elif not same:
+            r = new_rows(rows, cols, x.dtype if residual is None else residual.dtype, dev)
+        gp = gs = gt = gcols = wp = wt = pp = pt = yp = sp = 0
+        if gate is not None:
+            g, gs, gcols = _gate_rows(gate, x.shape)
+            gp, gt = g.data_ptr(), DTYPES[g.dtype]
+        if post_weight is not None:
+            post_weight = post_weight.contiguous()
+            pp, pt = post_weight.data_ptr(), DTYPES[post_weight.dtype]
         y = ys = None
         if weight is not None:
             weight = weight.contiguous()
-            y = torch.empty((rows, cols), device=dev,
-                            dtype=torch.float8_e4m3fn if quantize else x.dtype)
-            ys = new_scales(rows, cols, dev) if quantize else None
-        if post_weight is not None:
-            post_weight = post_weight.contiguous()
+            wp, wt = weight.data_ptr(), DTYPES[weight.dtype]
+            y = new_rows(rows, cols, torch.float8_e4m3fn if quantize else x.dtype, dev)
+            yp = y.data_ptr()
+            if quantize:
+                ys = new_scales(rows, cols, dev)
+                sp = ys.data_ptr()
         if rows and not (same and y is None):
-            _native.call("tf_add_rms_norm", _ptr(xr), DTYPES[x.dtype], row_stride(xr), _ptr(rr),
-                         _dtype(rr), 0 if rr is None else row_stride(rr), _ptr(gp), _dtype(gp),
-                         gs, gcols, _ptr(post_weight), _dtype(post_weight), _ptr(weight),
-                         _dtype(weight), float(eps), scale, rows, cols, 0 if same else _ptr(r),
-                         row_stride(r), _ptr(y), _dtype(y), cols, _ptr(ys), rows,
-                         _stream_ptr(stream, dev))
+            _native.call("tf_add_rms_norm", xr.data_ptr(), xt, row_stride(xr), rp, rt, rs, gp, gt,
+                         gs, gcols, pp, pt, wp, wt, eps, scale, rows, cols,
+                         0 if same else r.data_ptr(), row_stride(r), yp, yt, cols, sp, rows,
+                         _native.current_stream(dev))
     return ((y, ys) if quantize else y), r

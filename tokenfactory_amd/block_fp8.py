@@ -16,13 +16,12 @@ side (``stride(0) == 1``).  There is no non-native path and no gradient.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import _native
-from .fp8_linear import _ptr, _stream_ptr, on_stream
+from .fp8_linear import _ptr
 
 BLOCK = 128
 DTYPES = {torch.bfloat16: _native.TF_DTYPE_BF16, torch.float32: _native.TF_DTYPE_FP32,
@@ -36,9 +35,11 @@ def blocks(n: int) -> int:
 def rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if the kernels take its rows as they lie (dense columns, rows
     that do not overlap, 16-byte aligned), else a copy."""
-    unit = 16 if t.element_size() == 1 else 8
-    if (t.stride(1) == 1 and t.data_ptr() % 16 == 0
-            and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0))):
+    unit = 16 if t.dtype == torch.float8_e4m3fn else 8
+    rows, cols = t.shape
+    if t.data_ptr() % 16 == 0 and (
+            t.is_contiguous() and (rows == 1 or cols % unit == 0)
+            or t.stride(1) == 1 and (rows == 1 or (t.stride(0) >= cols and t.stride(0) % unit == 0))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -48,9 +49,14 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def new_rows(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def new_scales(rows: int, cols: int, device) -> torch.Tensor:
     """Room for the scales of ``rows`` x ``cols`` values, a block's rows side by side."""
-    return torch.empty((blocks(cols), rows), dtype=torch.float32, device=device).t()
+    return torch.empty_strided((rows, blocks(cols)), (1, rows), dtype=torch.float32,
+                               device=device)
 
 
 def quantize_blocks(x: torch.Tensor, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -64,36 +70,35 @@ def quantize_blocks(x: torch.Tensor, stream=None) -> Tuple[torch.Tensor, torch.T
     rows, cols = x.shape
     if cols == 0 or cols % 8:
         raise ValueError(f"quantize_blocks: {cols} columns (a positive multiple of 8)")
-    with _native.on_device(x.device), on_stream(stream):
+    dev = x.device
+    with _native.launching(dev, stream):
         x = rows16(x)
-        xq = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = new_scales(rows, cols, x.device)
-        _native.call("tf_block_quant", _ptr(x), DTYPES[x.dtype], rows, cols, row_stride(x),
-                     _ptr(xq), cols, _ptr(scale), rows, _stream_ptr(stream, x.device))
+        xq = new_rows(rows, cols, torch.float8_e4m3fn, dev)
+        scale = new_scales(rows, cols, dev)
+        _native.call("tf_block_quant", x.data_ptr(), DTYPES[x.dtype], rows, cols, row_stride(x),
+                     xq.data_ptr(), cols, scale.data_ptr(), rows, _native.current_stream(dev))
     return xq, scale
 
 
 def check_weight(fn: str, what: str, w: torch.Tensor, scale: torch.Tensor, k: int, device) -> None:
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.device != device:
-        raise ValueError(f"{fn}: {what} must be a 2-D float8_e4m3fn tensor on x's device")
-    n = w.shape[0]
-    if w.shape[1] != k or n == 0:
-        raise ValueError(f"{fn}: {what} {tuple(w.shape)} for inputs of {k}")
-    if w.stride(1) != 1 or w.data_ptr() % 16 or (n > 1 and (w.stride(0) < k or w.stride(0) % 16)):
+    n = w.shape[0] if w.dim() == 2 else 0
+    if w.dtype != torch.float8_e4m3fn or n == 0 or w.shape[1] != k or w.device != device:
+        raise ValueError(f"{fn}: {what} must be float8_e4m3fn [out, {k}] on x's device, not "
+                         f"{w.dtype} {tuple(w.shape)}")
+    if rows16(w) is not w:
         raise ValueError(f"{fn}: {what} rows must be contiguous and 16-byte aligned")
-    if (scale.dtype != torch.float32 or scale.device != device
-            or tuple(scale.shape) != (blocks(n), blocks(k))):
+    if (scale.dtype != torch.float32 or scale.shape != (blocks(n), blocks(k))
+            or scale.device != device):
         raise ValueError(f"{fn}: scales of {what} must be fp32 {(blocks(n), blocks(k))} on x's "
                          f"device, one per 128 x 128 block")
 
 
 def mat(w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
-        out: Optional[torch.Tensor] = None):
-    """A pointer to the ``tf_fp8_mat`` of a checked weight."""
+        out: Optional[torch.Tensor] = None) -> tuple:
+    """The fields of the ``tf_fp8_mat`` of a checked weight."""
     n = w.shape[0]
-    return ctypes.byref(_native.Fp8Mat(w.data_ptr(), row_stride(w), scale.data_ptr(),
-                                       scale.stride(0), scale.stride(1), _ptr(bias), n, _ptr(out),
-                                       n))
+    sn, sk = scale.stride()
+    return (w.data_ptr(), row_stride(w), scale.data_ptr(), sn, sk, _ptr(bias), n, _ptr(out), n)
 
 
 def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: int) -> torch.Tensor:
@@ -137,6 +142,12 @@ def input_rows(x2d: torch.Tensor, x_scale: Optional[torch.Tensor]):
     return x2d, row_stride(x2d), x_scale, rows if nb == 1 else x_scale.stride(1)
 
 
+def workspace(name: str, device, *sizes):
+    """(scratch or None, bytes) that entry point ``name`` asks for."""
+    nbytes = _native.call(name, *sizes)
+    return (torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+
 def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv: torch.Tensor,
                         bias: Optional[torch.Tensor] = None, *,
                         x_scale: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
@@ -155,13 +166,13 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv:
                              or bias.device != x.device or not bias.is_contiguous()):
         raise ValueError(f"{fn}: bias must be a contiguous bf16 [{n}] on x's device")
     rows = x2d.shape[0]
-    with _native.on_device(x.device), on_stream(stream):
-        out = torch.empty((rows, n), dtype=torch.bfloat16, device=x.device)
+    dev, dtype = x.device, DTYPES[x.dtype]
+    with _native.launching(dev, stream):
+        out = new_rows(rows, n, torch.bfloat16, dev)
         if rows:
             xr, xs, sc, ss = input_rows(x2d, x_scale)
-            nbytes = _native.load().tf_block_linear_workspace_bytes(rows, n, k, DTYPES[x.dtype])
-            ws = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=x.device)
-            _native.call("tf_block_linear", _ptr(xr), DTYPES[x.dtype], xs, _ptr(sc), ss,
-                         mat(weight, weight_scale_inv, bias, out), rows, k, _ptr(ws), nbytes,
-                         _stream_ptr(stream, x.device))
+            ws, nbytes = workspace("tf_block_linear_workspace_bytes", dev, rows, n, k, dtype)
+            mats = (_native.Fp8Mat * 1)(mat(weight, weight_scale_inv, bias, out))
+            _native.call("tf_block_linear", xr.data_ptr(), dtype, xs, _ptr(sc), ss, mats, rows, k,
+                         _ptr(ws), nbytes, _native.current_stream(dev))
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)

@@ -443,6 +443,224 @@ __global__ void __launch_bounds__(kThreads) gated_finish_kernel(BlockGemmArgs a)
                                                              h[3] / s);
 }
 
+// ---------------------------------------------------------------- few rows
+// Products of at most 16 rows: bound by the weights' way from memory, which one
+// launch has to ask for at once.  A workgroup of 8 waves owns 16 columns (gated:
+// of both projections); the waves take the K slices in turn, load them into
+// registers a few slices ahead, and add their sums through LDS at the end, in
+// wave order.  A load covers whole 128-byte lines (8 lanes a row; 16 rows of 64
+// bytes read the same matrix at 3.4 TB/s instead of 5.1), so the operands, which
+// want a lane per row, pass through LDS of the wave's own.  They are widened to
+// bf16, exactly: the bf16 MFMA adds in fp32, where the fp8 one cuts each product
+// 13 bits below the largest of its eight, and there is time for it.
+// XK: x is e4m3 rows with scales (kXRows), or bf16 / fp32 rows that every
+// workgroup quantises into LDS while its first weights are on their way: no
+// launch of its own, free while the blocks are few and all workgroups run at once
+// (1 row of 6144 times 5120 columns 11.1 us against 11.4 for quantised rows alone;
+// the 1088 workgroups of 5120 x 2 x 17408 lost 13 us, a launch takes 4).
+// Gated: h = silu(g) u is written in fp32; the next product quantises it.
+enum { kXRows = 0, kXBf16 = 1, kXF32 = 2 };
+constexpr int kRowsMax = 16;
+constexpr int kRowsWaves = 8;
+
+struct RowsArgs {
+  const uint8_t* x;       // rows, stride xs elements
+  int64_t xs;
+  const float* xsc;       // e4m3 rows: scale of (row, block) at block * xss + row
+  int64_t xss;
+  BlockMat mat[2];
+  int32_t M, K, KB, tail;
+  const uint16_t* bias;
+  uint16_t* out;          // bf16 [M, N]
+  int64_t os;
+  float* h;               // gated: [M, N]
+};
+
+// Row pitch of x in LDS (bytes) and the LDS that M rows take with their scales.
+__host__ __device__ constexpr int64_t rows_pitch(int64_t kb) { return kb * kQBlock + 16; }
+__host__ __device__ constexpr int64_t rows_lds(int64_t m, int64_t kb) {
+  return m * (rows_pitch(kb) + 4 * kb);
+}
+
+struct RowsSlice {        // one K slice of 16 weight rows (and of x), as loaded
+  u32x4 w[2][2], x[2];
+  float ws[2], xs;
+};
+
+template <bool GATED, int XK>
+__global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsArgs a) {
+  constexpr int kMats = GATED ? 2 : 1;
+  constexpr int kTiles = kMats + (XK == kXRows);          // 2 KB of LDS each, per wave
+  constexpr int kDepth = GATED ? 2 : 4;   // (128 VGPRs: two workgroups per CU)
+  static_assert(!GATED || XK == kXRows, "a gated product's x comes quantised");
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[kRowsWaves][kTiles][16 * kKSlice];
+  extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
+  const int t = threadIdx.x, w = wave_id(), l = t & 63, rr = l & 15, g = l >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int row = min(rr, a.M - 1);
+  const int64_t pitch = rows_pitch(a.KB);
+  float* xscale = reinterpret_cast<float*>(xlds + a.M * pitch);
+
+  // Loads: lane l has chunk l % 8 of row l / 8, and of row l / 8 + 8.
+  const int lr = l >> 3, lc = 16 * (l & 7);
+  const uint8_t* wp[kMats][2];
+  const uint8_t* wsp[kMats];
+#pragma unroll
+  for (int i = 0; i < kMats; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      wp[i][h] = a.mat[i].w + (int64_t)min(n0 + lr + 8 * h, a.mat[i].N - 1) * a.mat[i].wrs;
+    wsp[i] = reinterpret_cast<const uint8_t*>(a.mat[i].wsc + (n0 / kQBlock) * a.mat[i].sn);
+  }
+  const uint8_t* xp[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) xp[h] = a.x + min(lr + 8 * h, a.M - 1) * a.xs + lc;
+  const int n_slices = (a.KB - w + kRowsWaves - 1) / kRowsWaves;   // of this wave
+
+  auto load = [&](RowsSlice& s, int i) {
+    const int kb = w + i * kRowsWaves;
+    const int64_t k = (int64_t)kb * kQBlock;
+    // chunks behind the weights' last column: the slice's first (x is zero there)
+    const int c = kb == a.KB - 1 && lc >= a.tail ? 0 : lc;
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s.w[m][h] = ld_nt16(wp[m][h] + k + c);
+      s.ws[m] = *reinterpret_cast<const float*>(wsp[m] + (int64_t)kb * a.mat[m].sk * 4);
+    }
+    if constexpr (XK == kXRows) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s.x[h] = ld_g16(xp[h] + k);
+      s.xs = a.xsc[kb * a.xss + row];
+    }
+  };
+  // A tile in LDS: row r's chunk c at chunk c ^ swz(r), so that neither the rows'
+  // writes nor the operands' reads (16 rows of a chunk) meet in a bank.
+  const int put0 = lr * kKSlice + (lc ^ (16 * swz(lr)));
+  const int put1 = (lr + 8) * kKSlice + (lc ^ (16 * swz(lr + 8)));
+  const int get0 = rr * kKSlice + 16 * (g ^ swz(rr)), get1 = rr * kKSlice + 16 * ((g + 4) ^ swz(rr));
+  f32x4 acc[kMats];
+#pragma unroll
+  for (int m = 0; m < kMats; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](const RowsSlice& s, int i) {
+    const int kb = w + i * kRowsWaves;
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+      st_s16(tiles[w][m] + put0, s.w[m][0]);
+      st_s16(tiles[w][m] + put1, s.w[m][1]);
+    }
+    if constexpr (XK == kXRows) {
+      st_s16(tiles[w][kMats] + put0, s.x[0]);
+      st_s16(tiles[w][kMats] + put1, s.x[1]);
+    }
+    wave_lds_sync();
+    // Operands: lane l has chunks l / 16 and l / 16 + 4 of row l % 16, of both sides.
+    u32x4 wf[kMats][2], xf[2];
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+      wf[m][0] = ld_s16(tiles[w][m] + get0);
+      wf[m][1] = ld_s16(tiles[w][m] + get1);
+    }
+    float xs;
+    if constexpr (XK == kXRows) {
+      xf[0] = ld_s16(tiles[w][kMats] + get0);
+      xf[1] = ld_s16(tiles[w][kMats] + get1);
+      xs = s.xs;
+    } else {
+      const uint8_t* p = xlds + row * pitch + kb * kQBlock + 16 * g;
+      xf[0] = ld_s16(p);
+      xf[1] = ld_s16(p + 64);
+      xs = xscale[row * a.KB + kb];
+    }
+    wave_lds_sync();   // (before the next slice's writes)
+    f32x4 p[kMats];
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) p[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = q >> 1, d = 2 * (q & 1);
+      const u32x4 xb = e4m3x8_to_bf16x8(xf[c][d], xf[c][d + 1]);
+#pragma unroll
+      for (int m = 0; m < kMats; ++m)
+        p[m] = mfma_16x16x32(e4m3x8_to_bf16x8(wf[m][c][d], wf[m][c][d + 1]), xb, p[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) acc[m] += p[m] * (xs * s.ws[m]);
+  };
+
+  RowsSlice ring[kDepth];
+#pragma unroll
+  for (int j = 0; j < kDepth; ++j)
+    if (j < n_slices) load(ring[j], j);
+  if constexpr (XK != kXRows) {
+    // 16 lanes quantise a block, four blocks' loads in flight
+    constexpr int kAtOnce = 4;
+    const int units = a.M * a.KB;
+    for (int u0 = t >> 4; u0 < units; u0 += kAtOnce * kRowsWaves * 4) {
+      float v[kAtOnce][8];
+#pragma unroll
+      for (int b = 0; b < kAtOnce; ++b) {
+        const int u = u0 + b * kRowsWaves * 4, m = u / a.KB, c = (u - m * a.KB) * kQBlock + 8 * rr;
+        if (u < units && c < a.K) {
+          load8<XK == kXF32>(a.x, m * a.xs + c, v[b]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[b][j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kAtOnce; ++b) {
+        const int u = u0 + b * kRowsWaves * 4, m = u / a.KB, kb = u - m * a.KB;
+        if (u >= units) break;   // (16 lanes together)
+        const float s = block_scale(amax_lanes16(amax_bits8(v[b])));
+        *reinterpret_cast<u32x2*>(xlds + m * pitch + kb * kQBlock + 8 * rr) = quant8(v[b], s);
+        if (rr == 0) xscale[m * a.KB + kb] = s;
+      }
+    }
+    __syncthreads();
+  }
+  int i = 0;
+  for (; i + 2 * kDepth <= n_slices; i += kDepth) {
+#pragma unroll
+    for (int j = 0; j < kDepth; ++j) {
+      use(ring[j], i + j);
+      load(ring[j], i + kDepth + j);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kDepth; ++j) {
+    if (i + j < n_slices) use(ring[j], i + j);
+    if (i + kDepth + j < n_slices) load(ring[j], i + kDepth + j);
+  }
+#pragma unroll
+  for (int j = 0; j < kDepth; ++j)
+    if (i + kDepth + j < n_slices) use(ring[j], i + kDepth + j);
+
+  // Lane holds D[4 g + r][rr]: row rr, columns 4 g + r.  A wave's sums take its own
+  // tiles' place.
+#pragma unroll
+  for (int m = 0; m < kMats; ++m)
+    *reinterpret_cast<f32x4*>(&tiles[w][m][4 * (16 * rr + 4 * g)]) = acc[m];
+  __syncthreads();
+  if (t >= 256) return;
+  const int m = t >> 4, n = n0 + (t & 15);
+  float sum[kMats];
+#pragma unroll
+  for (int q = 0; q < kMats; ++q) {
+    sum[q] = 0.f;
+#pragma unroll
+    for (int v = 0; v < kRowsWaves; ++v)
+      sum[q] += *reinterpret_cast<const float*>(&tiles[v][q][4 * t]);
+  }
+  if (m >= a.M || n >= a.mat[0].N) return;
+  if constexpr (GATED) {
+    a.h[(int64_t)m * a.mat[0].N + n] = silu(sum[0]) * sum[1];
+  } else {
+    if (a.bias) sum[0] += __uint_as_float((uint32_t)a.bias[n] << 16);
+    a.out[(int64_t)m * a.os + n] = (uint16_t)(pack_bf16(sum[0], 0.f) & 0xffffu);
+  }
+}
+
 // ---------------------------------------------------------------- plans
 // A tile shape (MT, WN) and its estimated time: a workgroup takes fixed +
 // per_slice x K slices microseconds, workgroups run in rounds of one per CU (two
@@ -554,6 +772,30 @@ void launch_fused(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
     launch_gemm<8, 4, 2, true>(a, s);
 }
 
+// Whether a product of M rows runs on the kernel of few rows, and whether that
+// quantises its x itself: at most two rows (4 rows of 6144 times 5120 columns: 17.9 us,
+// 12.6 and a launch of 4 from quantised rows), of a length whose e4m3 values fit
+// beside the tiles of two workgroups, in workgroups that all run at once (two per CU).
+constexpr int64_t kRowsOwn = 2, kRowsLds = 40 << 10;
+bool few_rows(int64_t m) { return m <= kRowsMax; }
+bool rows_quantise(int64_t m, int64_t n, int64_t kb) {
+  return m <= kRowsOwn && rows_lds(m, kb) <= kRowsLds &&
+         ceil_div(n, 16) <= 2 * device_cu_count();
+}
+
+void launch_rows(const RowsArgs& a, int xk, hipStream_t s) {
+  const dim3 grid((uint32_t)ceil_div(a.mat[0].N, 16)), block(kRowsWaves * kWave);
+  const size_t lds = xk == kXRows ? 0 : (size_t)rows_lds(a.M, a.KB);
+  if (xk == kXRows && a.h)
+    hipLaunchKernelGGL((block_rows_kernel<true, kXRows>), grid, block, lds, s, a);
+  else if (xk == kXRows)
+    hipLaunchKernelGGL((block_rows_kernel<false, kXRows>), grid, block, lds, s, a);
+  else if (xk == kXBf16)
+    hipLaunchKernelGGL((block_rows_kernel<false, kXBf16>), grid, block, lds, s, a);
+  else
+    hipLaunchKernelGGL((block_rows_kernel<false, kXF32>), grid, block, lds, s, a);
+}
+
 // ---------------------------------------------------------------- arguments
 constexpr int64_t kMaxDim = 1 << 24;   // columns of a matrix: 32-bit offsets inside a tile
 constexpr int64_t kMaxRows = 1 << 24;
@@ -609,7 +851,6 @@ void launch_quant(const BlockQuantArgs& a, bool f32, hipStream_t s) {
 // Checks one weight and describes it (out and bias are the caller's).
 int32_t weight_setup(const char* fn, const char* what, const tf_fp8_mat* t, int64_t n, int64_t k,
                      BlockMat* b) {
-  if (!t) return fail(TF_ERR_INVALID, "%s: no %s", fn, what);
   if (t->n != n || n <= 0)
     return fail(TF_ERR_INVALID, "%s: %s has %lld columns, expected %lld", fn, what,
                 (long long)t->n, (long long)n);
@@ -695,6 +936,25 @@ bool bad_workspace(const void* ws, int64_t bytes, int64_t need) {
   return need > 0 && (!ws || !aligned16(ws) || bytes < need);
 }
 
+// The product of few rows; xk: of g.xq, or of the rows that q describes.
+RowsArgs rows_args(const BlockGemmArgs& g, int64_t k, int xk, const BlockQuantArgs& q) {
+  RowsArgs r{};
+  r.x = xk == kXRows ? g.xq : q.x;
+  r.xs = xk == kXRows ? g.xs : q.xs;
+  r.xsc = g.xsc;
+  r.xss = g.xss;
+  r.mat[0] = g.mat[0];
+  r.mat[1] = g.mat[1];
+  r.M = g.M;
+  r.K = (int32_t)k;
+  r.KB = g.KB;
+  r.tail = g.tail;
+  r.bias = g.bias;
+  r.out = g.out;
+  r.os = g.os;
+  return r;
+}
+
 // The product itself: tiles, or partials and their sum.
 void run_linear(BlockGemmArgs g, const BlockPlan& p, float* part, hipStream_t s) {
   g.n_mats = 1;
@@ -706,6 +966,25 @@ void run_linear(BlockGemmArgs g, const BlockPlan& p, float* part, hipStream_t s)
   hipLaunchKernelGGL(block_reduce_kernel,
                      dim3((uint32_t)ceil_div((int64_t)g.M * g.n_cols / 4, kThreads)),
                      dim3(kThreads), 0, s, g);
+}
+
+// Quantises the x of g's one product in a launch of its own unless the kernel of few
+// rows does it; says what that kernel's x is.
+int quantize_input(bool f32, const BlockGemmArgs& g, const BlockQuantArgs& q, hipStream_t s) {
+  if (rows_quantise(g.M, g.mat[0].N, g.KB)) return f32 ? kXF32 : kXBf16;
+  launch_quant(q, f32, s);
+  return kXRows;
+}
+
+// fp32 elements of partials that a product, or the first half of a gated block (its
+// unquantised h, where that leaves the kernel), needs.
+int64_t linear_parts(int64_t m, int64_t n, int64_t k) {
+  if (few_rows(m)) return 0;
+  return part_elems(plan_linear(m, n, 1, ceil_div(k, kQBlock), false), m, n, 1, false);
+}
+int64_t gated_parts(int64_t m, int64_t inter, int64_t hidden) {
+  if (few_rows(m)) return m * inter;
+  return part_elems(plan_gated(m, inter, ceil_div(hidden, kQBlock)), m, inter, 2, true);
 }
 
 int32_t check_product(const char* fn, int64_t m, int64_t n, int64_t k) {
@@ -742,8 +1021,7 @@ int64_t tf_block_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t
   const int32_t rc = check_product("block_linear", m, n, k);
   if (rc != TF_OK) return rc;
   if (m == 0) return 0;
-  const BlockPlan p = plan_linear(m, n, 1, ceil_div(k, kQBlock), false);
-  return layout(m, k, 0, x_dtype == TF_DTYPE_FP8_E4M3, part_elems(p, m, n, 1, false)).bytes;
+  return layout(m, k, 0, x_dtype == TF_DTYPE_FP8_E4M3, linear_parts(m, n, k)).bytes;
 }
 
 int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
@@ -756,9 +1034,8 @@ int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
   int32_t rc = check_product("block_linear", m, mat->n, k);
   if (rc != TF_OK || m == 0) return rc;
   const int64_t n = mat->n;
-  const BlockPlan p = plan_linear(m, n, 1, ceil_div(k, kQBlock), false);
   const bool quantized = x_dtype == TF_DTYPE_FP8_E4M3;
-  const Layout l = layout(m, k, 0, quantized, part_elems(p, m, n, 1, false));
+  const Layout l = layout(m, k, 0, quantized, linear_parts(m, n, k));
   if (bad_workspace(workspace, workspace_bytes, l.bytes))
     return fail(TF_ERR_INVALID, "block_linear: workspace of %lld bytes (needs %lld, 16-byte "
                 "aligned)", (long long)workspace_bytes, (long long)l.bytes);
@@ -771,8 +1048,11 @@ int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
                    &g, &q);
   if (rc != TF_OK) return rc;   // nothing is launched for arguments that any part refuses
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
-  run_linear(g, p, reinterpret_cast<float*>(ws + l.part), s);
+  const int xk = quantized ? kXRows : quantize_input(x_dtype == TF_DTYPE_FP32, g, q, s);
+  if (few_rows(m))
+    launch_rows(rows_args(g, k, xk, q), xk, s);
+  else
+    run_linear(g, plan_linear(m, n, 1, g.KB, false), reinterpret_cast<float*>(ws + l.part), s);
   return launch_status("tf_block_linear launch");
 }
 
@@ -784,22 +1064,21 @@ int64_t tf_gated_mlp_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, i
   if (rc == TF_OK) rc = check_product("gated_mlp", m, n_out, inter);
   if (rc != TF_OK) return rc;
   if (m == 0) return 0;
-  const BlockPlan up = plan_gated(m, inter, ceil_div(hidden, kQBlock));
-  const BlockPlan down = plan_linear(m, n_out, 1, ceil_div(inter, kQBlock), false);
   return layout(m, hidden, inter, x_dtype == TF_DTYPE_FP8_E4M3,
-                std::max(part_elems(up, m, inter, 2, true), part_elems(down, m, n_out, 1, false)))
+                std::max(gated_parts(m, inter, hidden), linear_parts(m, n_out, inter)))
       .bytes;
 }
 
 int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const float* x_scale,
-                     int64_t x_scale_stride, const tf_fp8_mat* gate, const tf_fp8_mat* up,
-                     const tf_fp8_mat* down, int64_t m, int64_t hidden, int64_t inter,
-                     void* workspace, int64_t workspace_bytes, tf_stream_t stream) {
+                     int64_t x_scale_stride, const tf_fp8_mat* mats, int64_t m, int64_t hidden,
+                     int64_t inter, void* workspace, int64_t workspace_bytes,
+                     tf_stream_t stream) {
   using namespace tfa;
-  if (!gate || !up || !down) {
+  if (!mats) {
     clear_error();
-    return fail(TF_ERR_INVALID, "gated_mlp: a weight is missing");
+    return fail(TF_ERR_INVALID, "gated_mlp: no weights");
   }
+  const tf_fp8_mat *gate = mats, *up = mats + 1, *down = mats + 2;
   const int64_t n_out = down->n;
   const int64_t need = tf_gated_mlp_workspace_bytes(m, hidden, inter, n_out, x_dtype);
   if (need < 0) return (int32_t)need;   // (it cleared and set the error)
@@ -807,8 +1086,6 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
   if (bad_workspace(workspace, workspace_bytes, need))
     return fail(TF_ERR_INVALID, "gated_mlp: workspace of %lld bytes (needs %lld, 16-byte aligned)",
                 (long long)workspace_bytes, (long long)need);
-  const BlockPlan pu = plan_gated(m, inter, ceil_div(hidden, kQBlock));
-  const BlockPlan pd = plan_linear(m, n_out, 1, ceil_div(inter, kQBlock), false);
   const bool quantized = x_dtype == TF_DTYPE_FP8_E4M3;
   const Layout l = layout(m, hidden, inter, quantized, 0);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -835,6 +1112,18 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
   g.n_cols = (int32_t)(2 * inter);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
+  if (few_rows(m)) {
+    RowsArgs r = rows_args(g, hidden, kXRows, q);
+    r.h = part;
+    launch_rows(r, kXRows, s);
+    rc = quant_setup("gated_mlp", part, TF_DTYPE_FP32, m, inter, inter, ws + l.hq, d.xs,
+                     g.hsc, m, d.xs, &q);
+    if (rc != TF_OK) return rc;
+    const int xk = quantize_input(true, d, q, s);
+    launch_rows(rows_args(d, inter, xk, q), xk, s);
+    return launch_status("tf_gated_mlp launch");
+  }
+  const BlockPlan pu = plan_gated(m, inter, g.KB);
   if (pu.fused) {
     launch_fused(g, pu, s);
   } else {
@@ -844,7 +1133,7 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
     hipLaunchKernelGGL(gated_finish_kernel, dim3((uint32_t)ceil_div(m * d.KB, kThreads / 32)),
                        dim3(kThreads), 0, s, g);
   }
-  run_linear(d, pd, part, s);
+  run_linear(d, plan_linear(m, n_out, 1, d.KB, false), part, s);
   return launch_status("tf_gated_mlp launch");
 }
 

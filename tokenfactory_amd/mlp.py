@@ -16,8 +16,9 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .block_fp8 import BLOCK, DTYPES, check_input, check_weight, input_rows, mat
-from .fp8_linear import Fp8Linear, _ptr, _stream_ptr, on_stream
+from .block_fp8 import (BLOCK, DTYPES, check_input, check_weight, input_rows, mat, new_rows,
+                        workspace)
+from .fp8_linear import Fp8Linear, _ptr
 
 
 def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.Tensor,
@@ -44,17 +45,18 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
     if inter % 16:
         raise NotImplementedError(f"{fn}: {inter} hidden activations (a multiple of 16)")
     rows, n = x2d.shape[0], down_weight.shape[0]
-    with _native.on_device(dev), on_stream(stream):
-        out = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
+    dtype = DTYPES[x.dtype]
+    with _native.launching(dev, stream):
+        out = new_rows(rows, n, torch.bfloat16, dev)
         if rows:
             xr, xs, sc, ss = input_rows(x2d, x_scale)
-            nbytes = _native.load().tf_gated_mlp_workspace_bytes(rows, hidden, inter, n,
-                                                                 DTYPES[x.dtype])
-            ws = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=dev)
-            _native.call("tf_gated_mlp", _ptr(xr), DTYPES[x.dtype], xs, _ptr(sc), ss,
-                         mat(gate_weight, gate_scale_inv), mat(up_weight, up_scale_inv),
-                         mat(down_weight, down_scale_inv, out=out), rows, hidden, inter,
-                         _ptr(ws), nbytes, _stream_ptr(stream, dev))
+            ws, nbytes = workspace("tf_gated_mlp_workspace_bytes", dev, rows, hidden, inter, n,
+                                   dtype)
+            mats = (_native.Fp8Mat * 3)(mat(gate_weight, gate_scale_inv),
+                                        mat(up_weight, up_scale_inv),
+                                        mat(down_weight, down_scale_inv, out=out))
+            _native.call("tf_gated_mlp", xr.data_ptr(), dtype, xs, _ptr(sc), ss, mats, rows, hidden,
+                         inter, ws.data_ptr(), nbytes, _native.current_stream(dev))
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
 
 
