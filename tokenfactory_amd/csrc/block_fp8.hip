@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) block_quant_kernel(BlockQuantArgs a)
 }
 
 // ---------------------------------------------------------------- GEMM
-constexpr int kSpread = 3;            // staging instructions issued per row of MFMAs
+constexpr int kSpread = 2, kAtStep = 4;   // staging instructions per row of MFMAs; see below
 constexpr int kGroupM = 8;            // m-tiles per group of the XCD tile order
 constexpr int kMaxSplits = 16;        // split-K factor limit
 
@@ -96,7 +96,6 @@ struct BlockTile {
   static constexpr int kXInst = kBM / kRowsPerInst;
   static constexpr int kWInst = kBN / kRowsPerInst;
   static constexpr int kLoads = kXInst + kWInst + kSInst;   // per thread per slice
-  static constexpr int kAhead = STAGES - 1;
   static_assert(kBM % kRowsPerInst == 0 && kBN % kRowsPerInst == 0, "staging rows");
 };
 
@@ -216,17 +215,21 @@ block_gemm_kernel(BlockGemmArgs a) {
       dma16(xbase + (int64_t)kb * kKSlice, xo[idx], sb + idx * 16 * T::kThreads);
     } else if (idx < T::kXInst + T::kWInst) {
       const int i = idx - T::kXInst;
-      dma16(wbase + (int64_t)kb * kKSlice, wo[i] - (kb == a.KB - 1 ? over : 0u),
-            sb + T::kXBytes + i * 16 * T::kThreads);
+      dma16(wbase + (int64_t)kb * kKSlice, wo[i], sb + T::kXBytes + i * 16 * T::kThreads);
     } else {
       const int i = idx - T::kXInst - T::kWInst;
       dma4_at(sp0[i] + (uint64_t)(uint32_t)kb * sstep[i],
               lds0 + st * T::kStage + T::kXBytes + T::kWBytes + i * 4 * T::kThreads + w * 256);
     }
   };
-  auto issue = [&](int kb, int st) {
+  // Before slice kb is staged: from the last on, chunks that the weights lack.
+  bool cut = false;
+  auto enter = [&](int kb) {
+    if (kb == a.KB - 1 && !cut) {
+      cut = true;
 #pragma unroll
-    for (int idx = 0; idx < T::kLoads; ++idx) issue_one(kb, st, idx);
+      for (int i = 0; i < T::kWInst; ++i) wo[i] -= over;
+    }
   };
 
   const int rr = l & 15, g = l >> 4;
@@ -240,88 +243,115 @@ block_gemm_kernel(BlockGemmArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Slices past the last are never read; their stage is refilled with the last
+  // A slice's loads start at the step that frees its stage: kAtStep of x there,
+  // kSpread per row after it (5120 x 2 x 17408 columns at 8192 rows: 1217 us; all three a
+  // row from the next slice on 1273, two barriers a slice to free the weights' part
+  // of a stage sooner 1231).
+  constexpr int kInLast = MT > 1 ? (kAtStep < T::kXInst ? kAtStep : T::kXInst) : T::kLoads;
+  int kfill;
+  // Slices past the last are never used; their stage is refilled with the last
   // slice so that every step issues (and waits for) the same loads.
 #pragma unroll
-  for (int i = 0; i < T::kAhead; ++i) issue(kb0 + min(i, KB - 1), i);
-  if constexpr (T::kAhead == 2)
-    vm_wait<T::kLoads>();
-  else
-    vm_wait<0>();
+  for (int i = 0; i < STAGES; ++i) {
+    kfill = kb0 + min(i, KB - 1);
+    if (i < STAGES - 1 || MT == 1) enter(kfill);
+#pragma unroll
+    for (int idx = 0; idx < (i < STAGES - 1 ? T::kLoads : kInLast); ++idx) issue_one(kfill, i, idx);
+  }
+  vm_wait<(STAGES - 2) * T::kLoads + kInLast>();
   __syncthreads();
 
-  // Each MFMA starts from zero; its product is folded into the accumulators
-  // with the row's and the column block's scale, one FMA per element per slice,
-  // between the next row's MFMAs (the last row's during the next slice).
-  f32x4 pl[4];
-  float sl0 = 0.f, sl1 = 0.f;
+  // A slice is MT rows of four MFMAs.  Each MFMA starts from zero; its product is
+  // folded into the accumulators with the row's and the column block's scale, one
+  // FMA per element, between the next row's MFMAs (the last row's during the next
+  // slice).  A row's operand is read one row ahead, and the step to the next slice
+  // is taken before the last row: by then every wave has read all of this slice,
+  // and the next one's weights are read each behind the last MFMA that uses their
+  // registers, so that no wave starts a slice by waiting for twelve reads.
+  i32x8 wf[4], xf[2];
+  f32x4 p[2][4];
+  float xr[2], w0, w1, s0 = 0.f, s1 = 0.f;   // s0, s1: scales of the row before
 #pragma unroll
-  for (int tn = 0; tn < 4; ++tn) pl[tn] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int tn = 0; tn < 4; ++tn) p[0][tn] = p[1][tn] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto scales_of = [&](int st) {
+    return reinterpret_cast<const float*>(smem + st * T::kStage + T::kXBytes + T::kWBytes);
+  };
+  auto read_x = [&](int st, int tm, int slot) {
+    xf[slot] = frag(smem + st * T::kStage + (xrow + 16 * tm) * kKSlice, o0, o1);
+    xr[slot] = scales_of(st)[xrow + 16 * tm];
+  };
+  auto read_w = [&](int st, int tn) {
+    wf[tn] = frag(smem + st * T::kStage + T::kXBytes + (wrow + 16 * tn) * kKSlice, o0, o1);
+  };
+  auto read_ws = [&](int st) {
+    w0 = scales_of(st)[T::kBM + (GATED ? 0 : wn >> 1)];
+    w1 = GATED ? scales_of(st)[T::kBM + 1] : w0;
+  };
+  read_x(0, 0, 0);
+#pragma unroll
+  for (int tn = 0; tn < 4; ++tn) read_w(0, tn);
+  read_ws(0);
   int st = 0;
   for (int j = 0; j < KB; ++j) {
-    const int knext = kb0 + min(j + T::kAhead, KB - 1), stn = st == 0 ? STAGES - 1 : st - 1;
-    const uint8_t* sp = smem + st * T::kStage;
-    const float* ssp = reinterpret_cast<const float*>(sp + T::kXBytes + T::kWBytes);
-    const float w0 = ssp[T::kBM + (GATED ? 0 : wn >> 1)];
-    const float w1 = GATED ? ssp[T::kBM + 1] : w0;
-    i32x8 wf[4], xf[3];
-    float xr[3];
-#pragma unroll
-    for (int tn = 0; tn < 4; ++tn)
-      wf[tn] = frag(sp + T::kXBytes + (wrow + 16 * tn) * kKSlice, o0, o1);
-    xf[0] = frag(sp + xrow * kKSlice, o0, o1);
-    xr[0] = ssp[xrow];
-    if constexpr (MT > 1) {
-      xf[1] = frag(sp + (xrow + 16) * kKSlice, o0, o1);
-      xr[1] = ssp[xrow + 16];
-    }
-    f32x4 p[2][4];
-    float s0 = 0.f, s1 = 0.f;   // scales of row tm - 1
+    const int st1 = st == STAGES - 1 ? 0 : st + 1;   // the next slice's stage
+    if constexpr (MT > 1) enter(kfill);
 #pragma unroll
     for (int tm = 0; tm < MT; ++tm) {
+      // The stage of the slice before is free: slice j - 1 + STAGES goes there.
+      if (tm < MT - 1) {
+        const int from = kInLast + tm * kSpread;
+        const int to = tm == MT - 2 ? T::kLoads : min(from + kSpread, T::kLoads);
 #pragma unroll
-      for (int q = 0; q < kSpread; ++q)
-        if (tm * kSpread + q < T::kLoads) issue_one(knext, stn, tm * kSpread + q);
-      if (tm == MT - 1)
+        for (int idx = from; idx < to; ++idx)
+          issue_one(kfill, st == 0 ? STAGES - 1 : st - 1, idx);
+      }
+      const float c0 = xr[tm & 1] * w0, c1 = GATED ? xr[tm & 1] * w1 : c0;
+      if (tm == MT - 1) {
+        vm_wait<(STAGES - 2) * T::kLoads>();
+        __syncthreads();
+        kfill = kb0 + min(j + STAGES, KB - 1);
+        if constexpr (MT == 1) enter(kfill);
 #pragma unroll
-        for (int idx = MT * kSpread; idx < T::kLoads; ++idx) issue_one(knext, stn, idx);
-      if (tm + 2 < MT) {
-        xf[(tm + 2) % 3] = frag(sp + (xrow + 16 * (tm + 2)) * kKSlice, o0, o1);
-        xr[(tm + 2) % 3] = ssp[xrow + 16 * (tm + 2)];
+        for (int q = 0; q < kInLast; ++q) issue_one(kfill, st, q);
+        read_x(st1, 0, MT & 1);
+        read_ws(st1);
+      } else {
+        read_x(st, tm + 1, (tm + 1) & 1);
       }
       __builtin_amdgcn_sched_barrier(0);
+      // products of the row before: of this slice, or the last one's
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn) {
-        p[tm & 1][tn] = mfma_fp8(wf[tn], xf[tm % 3]);
-        if (tm > 0)
-          acc[tm - 1][tn] += p[(tm - 1) & 1][tn] * (GATED && tn >= 2 ? s1 : s0);
-        else
-          acc[MT - 1][tn] += pl[tn] * (GATED && tn >= 2 ? sl1 : sl0);
+        const int back = tm > 0 ? tm - 1 : MT - 1;
+        f32x4 q = p[back & 1][tn];
+        p[tm & 1][tn] = mfma_fp8(wf[tn], xf[tm & 1]);
+        if (tm == MT - 1) read_w(st1, tn);
+        acc[back][tn] += q * (GATED && tn >= 2 ? s1 : s0);
       }
-      if (tm + 2 < MT) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);   // 3 LDS reads
+      if (tm == MT - 1)
+        __builtin_amdgcn_sched_group_barrier(0x100, GATED ? 5 : 4, 0);   // LDS reads
+      else
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // 1 MFMA
+        if (tm == MT - 1) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // 4 VALU
       }
       __builtin_amdgcn_sched_barrier(0);
-      s0 = xr[tm % 3] * w0;
-      s1 = GATED ? xr[tm % 3] * w1 : s0;
+      s0 = c0;
+      s1 = c1;
     }
-#pragma unroll
-    for (int tn = 0; tn < 4; ++tn) pl[tn] = p[(MT - 1) & 1][tn];
-    sl0 = s0;
-    sl1 = s1;
-    if constexpr (T::kAhead == 2)
-      vm_wait<T::kLoads>();
-    else
-      vm_wait<0>();
-    __syncthreads();
-    st = st == STAGES - 1 ? 0 : st + 1;
+    if constexpr (MT & 1) {   // (an even MT has read it into the first slot)
+      xf[0] = xf[1];
+      xr[0] = xr[1];
+    }
+    st = st1;
   }
   vm_wait<0>();   // the refills of the last steps land before the stages are reused
 #pragma unroll
-  for (int tn = 0; tn < 4; ++tn) acc[MT - 1][tn] += pl[tn] * (GATED && tn >= 2 ? sl1 : sl0);
+  for (int tn = 0; tn < 4; ++tn)
+    acc[MT - 1][tn] += p[(MT - 1) & 1][tn] * (GATED && tn >= 2 ? s1 : s0);
 
   // Lane holds D[wn 64 + 16 tn + 4 g + r][m0 + wm 16 MT + 16 tm + rr].
   if constexpr (!GATED) {
@@ -665,7 +695,12 @@ __global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsA
 // A tile shape (MT, WN) and its estimated time: a workgroup takes fixed +
 // per_slice x K slices microseconds, workgroups run in rounds of one per CU (two
 // of the small ones share a CU and take 1.5 times as long), a split adds a
-// launch and its partials' way through memory.
+// launch and its partials' way through memory.  Fitted to a sweep of every shape
+// and 1 to 16 splits over 24 numbers of rows from 17 to 8192 at six products (640
+// to 12288 columns, K 2176 to 17408) and four gated ones: the choice is within
+// 10 % of the sweep's best everywhere and 0.3 % on average.  What the rarer shapes
+// are for: without 192 rows x 128 columns 333 x 5120 x 12288 takes 49.9 us for 37.6,
+// without 128 x 256 1500 x 5120 x 17408 149.8 for 131.7.
 struct Shape {
   int mt, wn;
 };
@@ -674,14 +709,15 @@ struct ShapeCost {
   float fixed, per_slice;
   bool two;        // two workgroups per CU
 };
-constexpr ShapeCost kShapes[] = {{{1, 2}, 3.0f, 0.45f, true},  {{2, 2}, 3.5f, 0.48f, true},
-                                 {{4, 2}, 5.0f, 0.65f, false}, {{8, 2}, 3.0f, 1.10f, false},
-                                 {{6, 4}, 3.0f, 1.62f, false}, {{8, 4}, 3.0f, 1.85f, false}};
-constexpr ShapeCost kGatedShapes[] = {{{2, 4}, 5.0f, 0.75f, false},
-                                      {{4, 4}, 5.0f, 1.10f, false},
-                                      {{6, 4}, 5.0f, 1.62f, false},
-                                      {{8, 4}, 5.0f, 1.85f, false}};
-constexpr float kReduceUs = 3.0f, kPartialBytesPerUs = 5e6f;   // written, then read
+constexpr ShapeCost kShapes[] = {{{1, 2}, 2.48f, 0.470f, true},  {{2, 2}, 2.80f, 0.493f, true},
+                                 {{4, 2}, 3.15f, 0.708f, false}, {{6, 2}, 2.28f, 0.888f, false},
+                                 {{4, 4}, 1.45f, 0.938f, false}, {{6, 4}, 1.79f, 1.374f, false},
+                                 {{8, 4}, 2.96f, 1.550f, false}};
+constexpr ShapeCost kGatedShapes[] = {{{2, 4}, 3.04f, 0.750f, false},
+                                      {{4, 4}, 4.39f, 1.090f, false},
+                                      {{6, 4}, 1.93f, 1.572f, false},
+                                      {{8, 4}, 4.67f, 1.771f, false}};
+constexpr float kReduceUs = 2.8f, kPartialBytesPerUs = 2.8e6f;   // written, then read
 
 struct BlockPlan {
   Shape shape;
@@ -750,10 +786,12 @@ void launch_linear(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
     launch_gemm<1, 2, 3, false>(a, s);
   else if (sh.mt == 2)
     launch_gemm<2, 2, 3, false>(a, s);
-  else if (sh.mt == 4)
+  else if (sh.mt == 4 && sh.wn == 2)
     launch_gemm<4, 2, 3, false>(a, s);
-  else if (sh.wn == 2)
-    launch_gemm<8, 2, 3, false>(a, s);
+  else if (sh.mt == 6 && sh.wn == 2)
+    launch_gemm<6, 2, 3, false>(a, s);
+  else if (sh.mt == 4)
+    launch_gemm<4, 4, 3, false>(a, s);
   else if (sh.mt == 6)
     launch_gemm<6, 4, 2, false>(a, s);
   else
