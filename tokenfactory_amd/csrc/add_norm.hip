@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) add_norm_kernel(AddNormArgs
     if (a.y_dtype == DT_FP8_E4M3) {   // (the 16 lanes of a block take this path together)
       const float s = block_scale(amax_lanes16(amax_bits8(y)));
       if (col[i] < a.cols) {
-        *reinterpret_cast<u32x2*>(a.y + row * a.ys + col[i]) = quant8(y, s);
+        *reinterpret_cast<u32x2*>(a.y + row * a.ys + col[i]) = quant8(y, block_div(s));
         if (col[i] % kQBlock == 0) a.ysc[(int64_t)(col[i] / kQBlock) * a.yss + row] = s;
       }
     } else if (col[i] < a.cols) {

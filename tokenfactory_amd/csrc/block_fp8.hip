@@ -26,12 +26,12 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------- quantisation
-// One wave: 4 rows x kQuantBlocks blocks; 16 lanes hold a block's 128 columns,
-// 8 each.  All of a lane's loads are issued before the first is used.  Scales
-// are stored [block][row], so the 4 rows of a wave (16 of a workgroup) lie side
-// by side.
-constexpr int kQuantBlocks = 4;
-constexpr int kQuantRows = 4 * (kThreads / kWave);
+// One wave: kQuantRows rows x 4 blocks of 128 columns, a row's 512 at a time; 16
+// lanes hold a block's columns, 8 each.  All of a lane's loads are issued before
+// the first is used.  Scales are stored [block][row].
+constexpr int kQuantCols = 4 * kQBlock;
+constexpr int kQuantRows = 4;
+constexpr int kQuantWgRows = kQuantRows * (kThreads / kWave);
 
 struct BlockQuantArgs {
   const uint8_t* x;
@@ -50,26 +50,25 @@ __global__ void __launch_bounds__(kThreads) block_quant_kernel(BlockQuantArgs a)
   const int64_t rg = blockIdx.x / a.col_groups;
   const int cg = (int)(blockIdx.x - rg * a.col_groups);
   const int l = threadIdx.x & 63;
-  const int64_t row = rg * kQuantRows + (threadIdx.x >> 6) * 4 + (l >> 4);
-  if (row >= a.rows) return;
-  const int c0 = cg * kQuantBlocks * kQBlock + 8 * (l & 15);
-  float v[kQuantBlocks][8];
+  const int64_t row0 = rg * kQuantWgRows + wave_id() * kQuantRows;
+  const int c = cg * kQuantCols + 8 * l;
+  float v[kQuantRows][8];
 #pragma unroll
-  for (int b = 0; b < kQuantBlocks; ++b) {
-    const int c = c0 + b * kQBlock;
-    if (c < a.cols) {
-      load8<F32>(a.x, row * a.xs + c, v[b]);
+  for (int r = 0; r < kQuantRows; ++r) {
+    if (row0 + r < a.rows && c < a.cols) {
+      load8<F32>(a.x, (row0 + r) * a.xs + c, v[r]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[b][j] = 0.f;
+      for (int j = 0; j < 8; ++j) v[r][j] = 0.f;
     }
   }
 #pragma unroll
-  for (int b = 0; b < kQuantBlocks; ++b) {
-    const int c = c0 + b * kQBlock;
-    const float s = block_scale(amax_lanes16(amax_bits8(v[b])));
+  for (int r = 0; r < kQuantRows; ++r) {
+    const int64_t row = row0 + r;
+    if (row >= a.rows) break;   // (a wave's rows are its own)
+    const float s = block_scale(amax_lanes16(amax_bits8(v[r])));
     if (c < a.out_cols)
-      *reinterpret_cast<u32x2*>(a.xq + row * a.qs + c) = quant8(v[b], s);
+      *reinterpret_cast<u32x2*>(a.xq + row * a.qs + c) = quant8(v[r], block_div(s));
     if ((l & 15) == 0 && c < a.cols) a.scale[(int64_t)(c / kQBlock) * a.ss + row] = s;
   }
 }
@@ -403,13 +402,12 @@ block_gemm_kernel(BlockGemmArgs a) {
       const float s = block_scale(max(max(m4[0], m4[1]), max(m4[2], m4[3])));
       if (wn == 0 && g == 0 && m0 + row < a.M)
         a.hsc[(int64_t)tn_i * a.hss + m0 + row] = s;
-      const float inv = 1.f / s;
+      const BlockDiv d = block_div(s);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const f32x4 h = acc[tm][j];
         *reinterpret_cast<uint32_t*>(tile + row * kPitch + 32 * wn + 16 * j + 4 * g) =
-            e4m3x4(quotient(h[0], s, inv), quotient(h[1], s, inv), quotient(h[2], s, inv),
-                   quotient(h[3], s, inv));
+            quant4(h[0], h[1], h[2], h[3], d);
       }
     }
     __syncthreads();
@@ -469,8 +467,8 @@ __global__ void __launch_bounds__(kThreads) gated_finish_kernel(BlockGemmArgs a)
   for (int d = 16; d >= 1; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, kWave));
   const float s = block_scale(mx);
   if ((threadIdx.x & 31) == 0) a.hsc[b * a.hss + m] = s;
-  *reinterpret_cast<uint32_t*>(a.hq + m * a.hqs + c) = e4m3x4(h[0] / s, h[1] / s, h[2] / s,
-                                                             h[3] / s);
+  *reinterpret_cast<uint32_t*>(a.hq + m * a.hqs + c) =
+      quant4(h[0], h[1], h[2], h[3], block_div(s));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -643,7 +641,7 @@ __global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsA
         const int u = u0 + b * kRowsWaves * 4, m = u / a.KB, kb = u - m * a.KB;
         if (u >= units) break;   // (16 lanes together)
         const float s = block_scale(amax_lanes16(amax_bits8(v[b])));
-        *reinterpret_cast<u32x2*>(xlds + m * pitch + kb * kQBlock + 8 * rr) = quant8(v[b], s);
+        *reinterpret_cast<u32x2*>(xlds + m * pitch + kb * kQBlock + 8 * rr) = quant8(v[b], block_div(s));
         if (rr == 0) xscale[m * a.KB + kb] = s;
       }
     }
@@ -872,14 +870,14 @@ int32_t quant_setup(const char* fn, const void* x, int32_t x_dtype, int64_t rows
   a->qs = xq_row_stride;
   a->scale = x_scale;
   a->ss = x_scale_stride;
-  a->col_groups = (int32_t)ceil_div(out_cols, kQuantBlocks * kQBlock);
-  if (ceil_div(rows, kQuantRows) * a->col_groups > INT32_MAX)
+  a->col_groups = (int32_t)ceil_div(out_cols, kQuantCols);
+  if (ceil_div(rows, kQuantWgRows) * a->col_groups > INT32_MAX)
     return fail(TF_ERR_UNSUPPORTED, "%s: too large", fn);
   return TF_OK;
 }
 
 void launch_quant(const BlockQuantArgs& a, bool f32, hipStream_t s) {
-  const dim3 grid((uint32_t)(ceil_div(a.rows, kQuantRows) * a.col_groups));
+  const dim3 grid((uint32_t)(ceil_div(a.rows, kQuantWgRows) * a.col_groups));
   if (f32)
     hipLaunchKernelGGL(block_quant_kernel<true>, grid, dim3(kThreads), 0, s, a);
   else
