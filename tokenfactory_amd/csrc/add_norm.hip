@@ -14,7 +14,6 @@
 // HBM-bound: a row is read once into registers and written once.  A workgroup
 // owns a row, a thread NV groups of 8 columns, one wave-wide and one LDS step per
 // sum; 16 neighbouring lanes hold the 128 columns of a scale.
-#include <algorithm>
 
 #include "block_quant.h"
 #include "tf_common.h"
@@ -86,21 +85,29 @@ __device__ __forceinline__ void store8(uint8_t* p, int64_t elem, int f32, const 
   }
 }
 
-// Sum over the workgroup; every thread gets the same bits.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
+// Sum over the workgroup, in 64 bits from the waves' sums on (a value next to a
+// border of e4m3 moves by a step for an error in the last bits); every thread gets
+// the same bits.
+__device__ __forceinline__ double block_sum(float v, float* red) {
+  v = sum_lanes16(v);
+  v += __shfl_xor(v, 16, kWave);
+  v += __shfl_xor(v, 32, kWave);
   const int n = blockDim.x / kWave;
   if (n == 1) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = red[0];
-  for (int i = 1; i < n; ++i) v += red[i];
-  return v;
+  double s = red[0];
+  for (int i = 1; i < n; ++i) s += red[i];
+  return s;
+}
+
+// 1 / rms of a row from its sum of squares.
+__device__ __forceinline__ float inverse_rms(double sum, const AddNormArgs& a) {
+  return 1.f / sqrtf((float)(sum / a.cols + a.eps));
 }
 
 template <int NV>
-__global__ void __launch_bounds__(kMaxWaves * kWave) add_norm_kernel(AddNormArgs a) {
+__global__ void __launch_bounds__(kMaxWaves * kWave, NV == 1 ? 8 : 4) add_norm_kernel(AddNormArgs a) {
   __shared__ float red[2][kMaxWaves];
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x;
@@ -137,7 +144,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) add_norm_kernel(AddNormArgs
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-    const float rstd = 1.f / sqrtf(block_sum(ss, red[0]) / (float)a.cols + a.eps);
+    const float rstd = inverse_rms(block_sum(ss, red[0]), a);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (col[i] >= a.cols) continue;
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) add_norm_kernel(AddNormArgs
     if (a.res_out) store8(a.res_out, row * a.ros + col[i], a.ro_f32, v[i]);
   }
   if (!a.y) return;
-  const float rstd = 1.f / sqrtf(block_sum(ss, red[1]) / (float)a.cols + a.eps);
+  const float rstd = inverse_rms(block_sum(ss, red[1]), a);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

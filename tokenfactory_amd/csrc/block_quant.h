@@ -39,11 +39,26 @@ __device__ __forceinline__ uint32_t amax_bits8(const float* v) {
   for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
   return m;
 }
+// v of another of the 16 lanes of a row (a DPP control), without a way through LDS.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+}
+// The steps of a reduction over 16 lanes: lanes 1 and 2 away, then the mirrored lane
+// of 8 and of 16, whose group's value by then is the same in all its lanes.
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppMirror8 = 0x141, kDppMirror16 = 0x140;
 // Maximum over the 16 lanes that hold a block (all of them call it).
 __device__ __forceinline__ uint32_t amax_lanes16(uint32_t m) {
-#pragma unroll
-  for (int d = 8; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, kWave));
-  return m;
+  m = max(m, (uint32_t)dpp<kDppXor1>((int)m));
+  m = max(m, (uint32_t)dpp<kDppXor2>((int)m));
+  m = max(m, (uint32_t)dpp<kDppMirror8>((int)m));
+  return max(m, (uint32_t)dpp<kDppMirror16>((int)m));
+}
+__device__ __forceinline__ float sum_lanes16(float v) {
+  v += __int_as_float(dpp<kDppXor1>(__float_as_int(v)));
+  v += __int_as_float(dpp<kDppXor2>(__float_as_int(v)));
+  v += __int_as_float(dpp<kDppMirror8>(__float_as_int(v)));
+  return v + __int_as_float(dpp<kDppMirror16>(__float_as_int(v)));
 }
 
 __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
