@@ -123,6 +123,12 @@ def test_linear(gpu, m, n, k, quantized):
     check_linear(gpu, m, n, k, bias=n % 3 == 0, quantized=quantized)
 
 
+# More tiles than CUs, the last of them split along K (256 whole of 264, 512 of 539).
+@pytest.mark.parametrize("m,n,k", [(1300, 6139, 4096), (1290, 12300, 4000)])
+def test_last_round_of_tiles_split(gpu, m, n, k):
+    check_linear(gpu, m, n, k, bias=True, quantized=True)
+
+
 def test_linear_fp32_input_and_leading_dims(gpu):
     check_linear(gpu, 23, 200, 400, dtype=torch.float32)
     x = make_x(24, 400, 5).to(gpu)

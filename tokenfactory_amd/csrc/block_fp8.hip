@@ -103,20 +103,26 @@ struct BlockMat {
   int64_t wrs;
   const float* wsc;       // scale of column block n / 128, K block kb at nb * sn + kb * sk
   int64_t sn, sk;
-  int32_t N, c0;          // columns; first of them among a split's partials
+  int32_t N;
 };
 
+// Output tiles [0, full) are computed whole, by a workgroup each; the rest, which
+// would leave CUs idle, by `splits` workgroups each over parts of K, whose fp32
+// partial tiles a second kernel adds in split order (the result does not depend on
+// timing).  Gate and up products that leave the kernel unfused (n_mats == 2) are all
+// partials: their tiles are those of both matrices side by side.
 struct BlockGemmArgs {
   const uint8_t* xq;      // e4m3 [M, 128 KB], zeros behind K, row stride xs bytes
   int64_t xs;
   const float* xsc;       // scale of (row, block) at block * xss + row
   int64_t xss;
   BlockMat mat[2];        // linear: the weight; gated: gate and up
-  int32_t n_mats, tn1;    // tn1: first n-tile of mat[1] where both are columns of partials
+  int32_t n_mats, tn1;    // tn1: first n-tile of mat[1] where n_mats is 2
   int32_t M, KB;
   int32_t tail;           // bytes of the last K slice that the weights have
-  int32_t tiles_m, tiles, splits, n_cols;
-  float* part;            // split-K: fp32 [splits, M, n_cols]
+  int32_t tiles_m, tiles, full, splits;
+  int32_t bm, bn;         // rows and (weight) rows of a tile
+  float* part;            // fp32 [tiles - full][splits][bm][bn]
   const uint16_t* bias;
   uint16_t* out;          // bf16 [M, N]
   int64_t os;
@@ -168,15 +174,26 @@ block_gemm_kernel(BlockGemmArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[STAGES * T::kStage];
   const int t = threadIdx.x, w = wave_id(), l = t & 63;
   const int wm = w / WN, wn = w % WN;
-  const int split = blockIdx.x / a.tiles;
+  const bool whole = GATED || (int)blockIdx.x < a.full;
+  int lin, split = 0, slot = 0;
+  if (whole) {
+    lin = xcd_order(blockIdx.x, a.full);
+  } else {
+    const int i = blockIdx.x - a.full, rest = a.tiles - a.full;
+    split = i / rest;
+    const int o = xcd_order(i - split * rest, rest);
+    lin = a.full + o;
+    slot = o * a.splits + split;
+  }
   int tm_i, tn_i;
-  xcd_tile(blockIdx.x % a.tiles, a.tiles, a.tiles_m, kGroupM, &tm_i, &tn_i);
+  tile_at(lin, a.tiles, a.tiles_m, kGroupM, &tm_i, &tn_i);
   const int second = GATED ? (w >= WN) : (a.n_mats > 1 && tn_i >= a.tn1);
   const BlockMat mat = a.mat[second];   // gated: the matrix whose rows this wave stages
   const int m0 = tm_i * T::kBM;
   const int n0 = GATED ? tn_i * kQBlock : (tn_i - (second ? a.tn1 : 0)) * T::kBN;
-  const int kb0 = (int)((int64_t)a.KB * split / a.splits);
-  const int KB = (int)((int64_t)a.KB * (split + 1) / a.splits) - kb0;
+  const int parts = whole ? 1 : a.splits;
+  const int kb0 = (int)((int64_t)a.KB * split / parts);
+  const int KB = (int)((int64_t)a.KB * (split + 1) / parts) - kb0;
 
   // Staging as in fp8_linear.hip: thread t moves 16-byte chunk t % 8 of row
   // kRowsPerInst i + t / 8 (instruction i), fetched from chunk (t % 8) ^ swz(row);
@@ -373,6 +390,18 @@ block_gemm_kernel(BlockGemmArgs a) {
     acc[MT - 1][tn] += p[(MT - 1) & 1][tn] * (GATED && tn >= 2 ? s1 : s0);
 
   // Lane holds D[wn 64 + 16 tn + 4 g + r][m0 + wm 16 MT + 16 tm + rr].
+  if (!whole) {   // (never where gated)
+    float* part = a.part + (int64_t)slot * T::kBM * T::kBN + wn * 64 + 4 * g;
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) {
+      const int row = xrow + 16 * tm;
+      if (m0 + row >= a.M) continue;
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+        *reinterpret_cast<f32x4*>(part + row * T::kBN + 16 * tn) = acc[tm][tn];
+    }
+    return;
+  }
   if constexpr (!GATED) {
 #pragma unroll
     for (int tn = 0; tn < 4; ++tn) {
@@ -381,12 +410,7 @@ block_gemm_kernel(BlockGemmArgs a) {
 #pragma unroll
       for (int tm = 0; tm < MT; ++tm) {
         const int m = m0 + xrow + 16 * tm;
-        if (m >= a.M) continue;
-        if (a.part)   // (n_cols and c0 are multiples of 4: a row's last vector stays in it)
-          *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.M + m) * a.n_cols + mat.c0 + n) =
-              acc[tm][tn];
-        else
-          store_out(a, m, n, mat.N, acc[tm][tn]);
+        if (m < a.M) store_out(a, m, n, mat.N, acc[tm][tn]);
       }
     }
   } else {
@@ -443,48 +467,59 @@ block_gemm_kernel(BlockGemmArgs a) {
 
 // Sum of the splits' partials of four columns, in split order.  Every partial is
 // loaded before the first add, so the loads' latencies overlap.
-__device__ __forceinline__ f32x4 sum_splits(const BlockGemmArgs& a, int64_t e) {
-  const int64_t mn = (int64_t)a.M * a.n_cols;
-  f32x4 p[kMaxSplits];
+__device__ __forceinline__ f32x4 sum_splits(const BlockGemmArgs& a, const float* p) {
+  const int64_t step = (int64_t)a.bm * a.bn;
+  f32x4 v[kMaxSplits];
 #pragma unroll
   for (int sp = 0; sp < kMaxSplits; ++sp)
-    if (sp < a.splits) p[sp] = *reinterpret_cast<const f32x4*>(a.part + sp * mn + e);
-  f32x4 v = p[0];
+    if (sp < a.splits) v[sp] = *reinterpret_cast<const f32x4*>(p + sp * step);
 #pragma unroll
   for (int sp = 1; sp < kMaxSplits; ++sp)
-    if (sp < a.splits) v += p[sp];
-  return v;
+    if (sp < a.splits) v[0] += v[sp];
+  return v[0];
 }
 
-// out = bf16(sum of the partials + bias), four columns per thread.
+// The split tiles of a product (blockIdx.y): out = bf16(sum of the partials + bias),
+// four columns per thread, rows in order.
 __global__ void __launch_bounds__(kThreads) block_reduce_kernel(BlockGemmArgs a) {
-  const int64_t e = 4 * ((int64_t)blockIdx.x * kThreads + threadIdx.x);
-  if (e >= (int64_t)a.M * a.n_cols) return;
-  const int64_t m = e / a.n_cols;
-  store_out(a, m, (int)(e - m * a.n_cols), a.mat[0].N, sum_splits(a, e));
+  const int o = blockIdx.y;
+  int tm, tn;
+  tile_at(a.full + o, a.tiles, a.tiles_m, kGroupM, &tm, &tn);
+  const int quads = a.bn == 256 ? 6 : 5;   // log2(bn / 4)
+  const int in = blockIdx.x * kThreads + threadIdx.x;
+  const int row = in >> quads, col = 4 * (in & ((1 << quads) - 1));
+  const int64_t m = (int64_t)tm * a.bm + row;
+  const int n = tn * a.bn + col;
+  if (m >= a.M || n >= a.mat[0].N) return;
+  const float* p = a.part + ((int64_t)o * a.splits * a.bm + row) * a.bn + col;
+  store_out(a, m, n, a.mat[0].N, sum_splits(a, p));
 }
 
-// h = silu(g) u from the partials of both projections, quantised: 32 lanes hold
-// a block's 128 columns of one row, four each.
+// h = silu(g) u from the partials of both projections, quantised: 32 lanes hold a
+// block's 128 columns of one row, four each.
 __global__ void __launch_bounds__(kThreads) gated_finish_kernel(BlockGemmArgs a) {
   const int hb = (a.mat[0].N + kQBlock - 1) / kQBlock;
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (unit >= (int64_t)a.M * hb) return;   // (all 32 lanes of a unit together)
-  const int64_t m = unit / hb;
-  const int b = (int)(unit - m * hb), c = b * kQBlock + 4 * (threadIdx.x & 31);
+  const int m = (int)(unit / hb), b = (int)(unit - (int64_t)m * hb);
+  const int c = b * kQBlock + 4 * (threadIdx.x & 31);
   f32x4 h = {0.f, 0.f, 0.f, 0.f};
   uint32_t mx = 0;
   if (c < a.mat[0].N) {   // N is a multiple of 16: four columns in or out together
-    const f32x4 gt = sum_splits(a, m * a.n_cols + c);
-    const f32x4 up = sum_splits(a, m * a.n_cols + a.mat[1].c0 + c);
+    const int tm = m / a.bm, tn = c / a.bn;
+    const int og = tile_index(tm, tn, a.tiles, a.tiles_m, kGroupM);
+    const int ou = tile_index(tm, a.tn1 + tn, a.tiles, a.tiles_m, kGroupM);
+    const float* p = a.part + (int64_t)(m - tm * a.bm) * a.bn + c - tn * a.bn;
+    const int64_t step = (int64_t)a.splits * a.bm * a.bn;
+    const f32x4 gt = sum_splits(a, p + og * step), up = sum_splits(a, p + ou * step);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       h[r] = silu(gt[r]) * up[r];
       mx = max(mx, __float_as_uint(h[r]) & 0x7fffffffu);
     }
   }
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, kWave));
+  mx = amax_lanes16(mx);
+  mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
   const float s = block_scale(mx);
   if ((threadIdx.x & 31) == 0) a.hsc[b * a.hss + m] = s;
   *reinterpret_cast<uint32_t*>(a.hq + m * a.hqs + c) =
@@ -718,7 +753,10 @@ __global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsA
 // to 12288 columns, K 2176 to 17408) and four gated ones: the choice is within
 // 10 % of the sweep's best everywhere and 0.3 % on average.  What the rarer shapes
 // are for: without 192 rows x 128 columns 333 x 5120 x 12288 takes 49.9 us for 37.6,
-// without 128 x 256 1500 x 5120 x 17408 149.8 for 131.7.
+// without 128 x 256 1500 x 5120 x 17408 149.8 for 131.7.  A split is taken of the
+// tiles behind the last full round only: with every tile whole 4096 x 5120 x 17408
+// takes 357 us for 318 (256 tiles whole, 64 by 4 workgroups each), 1300 x 12288 x
+// 4096 100 for 91.
 struct Shape {
   int mt, wn;
 };
@@ -739,8 +777,9 @@ constexpr float kReduceUs = 2.8f, kPartialBytesPerUs = 2.8e6f;   // written, the
 
 struct BlockPlan {
   Shape shape;
-  int splits;
-  bool fused;      // gated: h leaves the product's kernel quantised
+  int full, splits;   // tiles computed whole; workgroups per tile of the others
+  int64_t part;       // fp32 elements of partials
+  bool fused;         // gated: h leaves the product's kernel quantised
   float us;
 };
 
@@ -763,20 +802,25 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 constexpr int64_t kWideRows = 64;
 bool wide_gated(int64_t m) { return m <= kWideRows; }
 
-// n_mats matrices of n columns each; parts: the result is partials whatever the split.
+// n_mats matrices of n columns each; parts: every tile leaves as partials, split or not.
 BlockPlan plan_linear(int64_t m, int64_t n, int n_mats, int64_t kb, bool parts) {
   const int64_t cus = device_cu_count();
-  BlockPlan best{kShapes[0].shape, 1, false, INFINITY};
+  BlockPlan best{kShapes[0].shape, 0, 1, 0, false, INFINITY};
   for (const ShapeCost& c : kShapes) {
     if (n_mats == 2 && wide_gated(m) && c.shape.mt > 2) continue;   // (no wide form)
-    const int64_t tiles = ceil_div(m, 32 * c.shape.mt) * ceil_div(n, 64 * c.shape.wn) * n_mats;
+    const int64_t bm = 32 * c.shape.mt, bn = 64 * c.shape.wn;
+    const int64_t tiles = ceil_div(m, bm) * ceil_div(n, bn) * n_mats;
+    const int64_t round = c.two ? 2 * cus : cus;
+    const float filled = (float)(m * n * n_mats) / (float)(tiles * bm * bn);
     for (int64_t sp = 1; sp <= kMaxSplits; ++sp) {
-      if (sp > 1 && (kb / sp < 2 || tiles * sp > 2 * cus)) break;
-      const float us =
-          rounds(c, tiles * sp, cus) * (c.fixed + c.per_slice * (float)ceil_div(kb, sp)) +
-          (sp > 1 || parts ? kReduceUs + (float)(sp * m * n * n_mats) * 8.f / kPartialBytesPerUs
-                           : 0.f);
-      if (us < best.us) best = {c.shape, (int)sp, false, us};
+      const int64_t full = parts ? 0 : sp == 1 ? tiles : tiles / round * round;
+      const int64_t rest = tiles - full;   // split, or partials
+      if (sp > 1 && (kb / sp < 2 || rest == 0 || rest * sp > 2 * cus)) break;
+      float us = rounds(c, full, cus) * (c.fixed + c.per_slice * (float)kb);
+      if (rest > 0)
+        us += rounds(c, rest * sp, cus) * (c.fixed + c.per_slice * (float)ceil_div(kb, sp)) +
+              kReduceUs + filled * (float)(rest * sp * bm * bn) * 8.f / kPartialBytesPerUs;
+      if (us < best.us) best = {c.shape, (int)full, (int)sp, rest * sp * bm * bn, false, us};
     }
   }
   return best;
@@ -789,57 +833,67 @@ BlockPlan plan_gated(int64_t m, int64_t inter, int64_t kb) {
     if (wide_gated(m) && c.shape.mt > 2) continue;
     const int64_t tiles = ceil_div(m, 32 * c.shape.mt) * ceil_div(inter, kQBlock);
     const float us = rounds(c, tiles, cus) * (c.fixed + c.per_slice * (float)kb);
-    if (us < best.us) best = {c.shape, 1, true, us};
+    if (us < best.us) best = {c.shape, (int)tiles, 1, 0, true, us};
   }
   return best;
-}
-
-// fp32 elements of a plan's partials (0: none).
-int64_t part_elems(const BlockPlan& p, int64_t m, int64_t n, int n_mats, bool parts) {
-  return p.fused || (p.splits == 1 && !parts) ? 0 : p.splits * m * round_up(n, 4) * n_mats;
 }
 
 template <int MT, int WN, int STAGES, bool GATED, bool WIDE = false>
 void launch_gemm(BlockGemmArgs a, hipStream_t stream) {
   using T = BlockTile<MT, WN, STAGES>;
+  a.bm = T::kBM;
+  a.bn = T::kBN;
   a.tiles_m = (int)ceil_div(a.M, T::kBM);
   a.tn1 = (int)ceil_div(a.mat[0].N, GATED ? kQBlock : T::kBN);
   a.tiles = a.tiles_m * a.tn1 * (GATED ? 1 : a.n_mats);
+  const int rest = a.tiles - a.full;
   hipLaunchKernelGGL((block_gemm_kernel<MT, WN, STAGES, GATED, WIDE>),
-                     dim3((uint32_t)(a.tiles * a.splits)), dim3(T::kThreads), 0, stream, a);
+                     dim3((uint32_t)(a.full + rest * a.splits)), dim3(T::kThreads), 0, stream, a);
+  if (rest == 0) return;
+  if (a.n_mats == 2)
+    hipLaunchKernelGGL(gated_finish_kernel,
+                       dim3((uint32_t)ceil_div(a.M * ceil_div(a.mat[0].N, kQBlock),
+                                               kThreads / 32)),
+                       dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL(block_reduce_kernel,
+                       dim3(T::kBM * T::kBN / 4 / kThreads, (uint32_t)rest), dim3(kThreads), 0,
+                       stream, a);
 }
 
-// The tiles of a product, or with two matrices of gate and up as partials.
-void launch_linear(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
+// The tiles of a product, or with two matrices of a gated one, and the kernel that
+// finishes the partials where there are any.
+void launch_tiles(BlockGemmArgs a, const BlockPlan& p, int n_mats, float* part, hipStream_t s) {
+  a.n_mats = n_mats;
+  a.full = p.full;
   a.splits = p.splits;
+  a.part = part;
   const Shape sh = p.shape;
-  const bool wide = a.n_mats == 2 && wide_gated(a.M);
-  if (sh.mt == 1)
+  const bool wide = n_mats == 2 && wide_gated(a.M);
+  if (p.fused) {
+    if (sh.mt == 2)
+      wide ? launch_gemm<2, 4, 3, true, true>(a, s) : launch_gemm<2, 4, 3, true>(a, s);
+    else if (sh.mt == 4)
+      launch_gemm<4, 4, 3, true>(a, s);
+    else if (sh.mt == 6)
+      launch_gemm<6, 4, 2, true>(a, s);
+    else
+      launch_gemm<8, 4, 2, true>(a, s);
+  } else if (sh.mt == 1) {
     wide ? launch_gemm<1, 2, 3, false, true>(a, s) : launch_gemm<1, 2, 3, false>(a, s);
-  else if (sh.mt == 2)
+  } else if (sh.mt == 2) {
     wide ? launch_gemm<2, 2, 3, false, true>(a, s) : launch_gemm<2, 2, 3, false>(a, s);
-  else if (sh.mt == 4 && sh.wn == 2)
+  } else if (sh.mt == 4 && sh.wn == 2) {
     launch_gemm<4, 2, 3, false>(a, s);
-  else if (sh.mt == 6 && sh.wn == 2)
+  } else if (sh.mt == 6 && sh.wn == 2) {
     launch_gemm<6, 2, 3, false>(a, s);
-  else if (sh.mt == 4)
+  } else if (sh.mt == 4) {
     launch_gemm<4, 4, 3, false>(a, s);
-  else if (sh.mt == 6)
+  } else if (sh.mt == 6) {
     launch_gemm<6, 4, 2, false>(a, s);
-  else
+  } else {
     launch_gemm<8, 4, 2, false>(a, s);
-}
-
-void launch_fused(BlockGemmArgs a, const BlockPlan& p, hipStream_t s) {
-  a.splits = 1;
-  if (p.shape.mt == 2)
-    wide_gated(a.M) ? launch_gemm<2, 4, 3, true, true>(a, s) : launch_gemm<2, 4, 3, true>(a, s);
-  else if (p.shape.mt == 4)
-    launch_gemm<4, 4, 3, true>(a, s);
-  else if (p.shape.mt == 6)
-    launch_gemm<6, 4, 2, true>(a, s);
-  else
-    launch_gemm<8, 4, 2, true>(a, s);
+  }
 }
 
 // Whether a product of M rows runs on the kernel of few rows, and whether that
@@ -939,7 +993,6 @@ int32_t weight_setup(const char* fn, const char* what, const tf_fp8_mat* t, int6
   b->sn = t->w_scale_row_stride;
   b->sk = t->w_scale_col_stride;
   b->N = (int32_t)n;
-  b->c0 = 0;
   return TF_OK;
 }
 
@@ -1025,19 +1078,6 @@ RowsArgs rows_args(const BlockGemmArgs& g, int64_t k, int xk, const BlockQuantAr
   return r;
 }
 
-// The product itself: tiles, or partials and their sum.
-void run_linear(BlockGemmArgs g, const BlockPlan& p, float* part, hipStream_t s) {
-  g.n_mats = 1;
-  g.n_cols = (int32_t)round_up(g.mat[0].N, 4);
-  g.part = p.splits > 1 ? part : nullptr;
-  launch_linear(g, p, s);
-  if (!g.part) return;
-  g.splits = p.splits;
-  hipLaunchKernelGGL(block_reduce_kernel,
-                     dim3((uint32_t)ceil_div((int64_t)g.M * g.n_cols / 4, kThreads)),
-                     dim3(kThreads), 0, s, g);
-}
-
 // Quantises the x of g's one product in a launch of its own unless the kernel of few
 // rows does it; says what that kernel's x is.
 int quantize_input(bool f32, const BlockGemmArgs& g, const BlockQuantArgs& q, hipStream_t s) {
@@ -1046,15 +1086,13 @@ int quantize_input(bool f32, const BlockGemmArgs& g, const BlockQuantArgs& q, hi
   return kXRows;
 }
 
-// fp32 elements of partials that a product, or the first half of a gated block (its
-// unquantised h, where that leaves the kernel), needs.
+// fp32 elements that a product, or the first half of a gated block (partials, or the
+// unquantised h of the kernel of few rows), passes through the workspace.
 int64_t linear_parts(int64_t m, int64_t n, int64_t k) {
-  if (few_rows(m)) return 0;
-  return part_elems(plan_linear(m, n, 1, ceil_div(k, kQBlock), false), m, n, 1, false);
+  return few_rows(m) ? 0 : plan_linear(m, n, 1, ceil_div(k, kQBlock), false).part;
 }
 int64_t gated_parts(int64_t m, int64_t inter, int64_t hidden) {
-  if (few_rows(m)) return m * inter;
-  return part_elems(plan_gated(m, inter, ceil_div(hidden, kQBlock)), m, inter, 2, true);
+  return few_rows(m) ? m * inter : plan_gated(m, inter, ceil_div(hidden, kQBlock)).part;
 }
 
 int32_t check_product(const char* fn, int64_t m, int64_t n, int64_t k) {
@@ -1122,7 +1160,7 @@ int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
   if (few_rows(m))
     launch_rows(rows_args(g, k, xk, q), xk, s);
   else
-    run_linear(g, plan_linear(m, n, 1, g.KB, false), reinterpret_cast<float*>(ws + l.part), s);
+    launch_tiles(g, plan_linear(m, n, 1, g.KB, false), 1, reinterpret_cast<float*>(ws + l.part), s);
   return launch_status("tf_block_linear launch");
 }
 
@@ -1177,9 +1215,6 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
   d.xs = g.hqs = (int64_t)d.KB * kQBlock;
   d.xsc = g.hsc = reinterpret_cast<float*>(ws + l.hsc);
   d.xss = g.hss = m;
-  g.n_mats = 2;
-  g.mat[1].c0 = (int32_t)inter;
-  g.n_cols = (int32_t)(2 * inter);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
   if (few_rows(m)) {
@@ -1193,17 +1228,8 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
     launch_rows(rows_args(d, inter, xk, q), xk, s);
     return launch_status("tf_gated_mlp launch");
   }
-  const BlockPlan pu = plan_gated(m, inter, g.KB);
-  if (pu.fused) {
-    launch_fused(g, pu, s);
-  } else {
-    g.part = part;
-    launch_linear(g, pu, s);
-    g.splits = pu.splits;
-    hipLaunchKernelGGL(gated_finish_kernel, dim3((uint32_t)ceil_div(m * d.KB, kThreads / 32)),
-                       dim3(kThreads), 0, s, g);
-  }
-  run_linear(d, plan_linear(m, n_out, 1, d.KB, false), part, s);
+  launch_tiles(g, plan_gated(m, inter, g.KB), 2, part, s);
+  launch_tiles(d, plan_linear(m, n_out, 1, d.KB, false), 1, part, s);
   return launch_status("tf_gated_mlp launch");
 }
 

@@ -72,16 +72,27 @@ __device__ __forceinline__ f32x4 mfma_fp8(const i32x8& w, const i32x8& x) {
 // 4 n-tiles for 32 CUs) whose X and W slices its L2 serves once to all of
 // them.  Under split-K (grid = splits x T) the same permutation is applied to
 // each split's tiles.
-__device__ __forceinline__ void xcd_tile(int b, int tiles, int tiles_m, int gm_max, int* tm,
-                                         int* tn) {
+__device__ __forceinline__ int xcd_order(int b, int tiles) {
   const int x = b & 7, i = b >> 3, q = tiles >> 3, r = tiles & 7;
-  const int lin = x * q + min(x, r) + i;
+  return x * q + min(x, r) + i;
+}
+__device__ __forceinline__ void tile_at(int lin, int tiles, int tiles_m, int gm_max, int* tm,
+                                        int* tn) {
   const int tiles_n = tiles / tiles_m;
   const int group = gm_max * tiles_n;
   const int gid = lin / group, in = lin - gid * group;
   const int gm = min(tiles_m - gid * gm_max, gm_max);
   *tm = gid * gm_max + in % gm;
   *tn = in / gm;
+}
+// The place of a tile in that order.
+__device__ __forceinline__ int tile_index(int tm, int tn, int tiles, int tiles_m, int gm_max) {
+  const int gid = tm / gm_max, gm = min(tiles_m - gid * gm_max, gm_max);
+  return gid * gm_max * (tiles / tiles_m) + tn * gm + tm - gid * gm_max;
+}
+__device__ __forceinline__ void xcd_tile(int b, int tiles, int tiles_m, int gm_max, int* tm,
+                                         int* tn) {
+  tile_at(xcd_order(b, tiles), tiles, tiles_m, gm_max, tm, tn);
 }
 
 }  // namespace tfa
