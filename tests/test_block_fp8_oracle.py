@@ -1,6 +1,7 @@
 """The block-scaled FP8 oracle against closed forms, and the refusals of the operators'
 entry points (CPU only: nothing is launched)."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -8,6 +9,7 @@ import torch
 from oracle import block_fp8 as ob
 from tokenfactory_amd import (GatedMLP, _native, add_rms_norm, block_scaled_linear, gated_mlp,
                               quantize_blocks)
+from tokenfactory_amd.add_norm import _clash
 
 INVALID, UNSUPPORTED = _native.TF_ERR_INVALID, _native.TF_ERR_UNSUPPORTED
 BF16, FP8, FP32 = _native.TF_DTYPE_BF16, _native.TF_DTYPE_FP8_E4M3, _native.TF_DTYPE_FP32
@@ -219,3 +221,33 @@ def test_module_holds_the_reference_parameters():
 def test_module_refusals(change):
     with pytest.raises(NotImplementedError):
         GatedMLP(type("C", (_Config,), change)())
+
+
+def test_more_than_a_launch_holds_is_refused():
+    """2^32 threads: a thread per 8 columns (norm, quantisation), 128 per 32 x 64 outputs."""
+    lib = _native.load()
+    assert _norm(rows=1 << 22, cols=8192, xs=8192, rs=8192, ros=8192, ys=8192) == UNSUPPORTED
+    assert lib.tf_block_quant(16, BF16, 1 << 24, 1 << 20, 1 << 20, 16, 1 << 20, 16, 1 << 24,
+                              None) == UNSUPPORTED
+    assert lib.tf_block_linear_workspace_bytes(1 << 20, 1 << 17, 256, BF16) == UNSUPPORTED
+    assert lib.tf_gated_mlp_workspace_bytes(1 << 20, 256, 1 << 17, 256, BF16) == UNSUPPORTED
+
+
+def test_a_stream_of_another_device_is_refused():
+    stream = types.SimpleNamespace(device=torch.device("cuda", 1))
+    with pytest.raises(ValueError):
+        with _native.launching(torch.device("cuda", 0), stream):
+            pass
+
+
+def test_operands_that_an_in_place_sum_would_overwrite():
+    buf = torch.zeros((8, 64), dtype=torch.bfloat16)
+    r = buf[1:5, 16:32]
+    same = buf[1:5, 16:32]
+    other = torch.zeros_like(r)
+    assert not any(_clash(r, t) for t in (None, same, other, other[0], other[:, :1]))
+    # other columns of the same rows, in either order, and rows before or after
+    assert not any(_clash(r, t) for t in (buf[1:5, 32:48], buf[1:5, :16], buf[0:1, 16:32], buf[5]))
+    for t in (buf[2:6, 16:32], buf[0:4, 16:32], buf[1:5, 24:40], buf[1:5, 8:24], buf[2, 16:32],
+              buf[1:5, 16:17], r.view(torch.uint8)[:, :16], buf[0:8:2, 16:32], buf[1:2, 16:32]):
+        assert _clash(r, t)

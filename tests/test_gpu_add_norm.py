@@ -177,3 +177,31 @@ def test_refusals(gpu):
         add_rms_norm(torch.zeros((1, 16392), device=gpu), None, torch.ones(16392, device=gpu))
     with pytest.raises(RuntimeError):
         add_rms_norm(x, None, w, gate=torch.ones((3, 1), device=gpu))
+
+
+def test_in_place_refuses_operands_that_it_would_overwrite(gpu):
+    x, w = make_x(4, 256, 1).to(gpu), weights(256, 2, torch.bfloat16).to(gpu)
+    buf = make_x(6, 512, 3).to(gpu)
+    r = buf[:4, :256]
+    for kw in (dict(x=buf[1:5, :256]), dict(gate=buf[0, :256]), dict(gate=r[:, :1]),
+               dict(post_weight=buf[1, :256]), dict(weight=buf[2, :256])):
+        a = dict(x=x, weight=w)
+        a.update(kw)
+        keep = buf.clone()
+        with pytest.raises(ValueError):
+            add_rms_norm(a.pop("x"), r, a.pop("weight"), EPS, inplace=True, **a)
+        assert torch.equal(buf, keep)
+    gate = buf[:4, 256:]                     # other columns of the same rows
+    want = add_rms_norm(x, r, w, EPS, gate=gate)
+    got = add_rms_norm(x, r, w, EPS, gate=gate, inplace=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(r, want[1])
+
+
+def test_weights_that_lie_unaligned(gpu):
+    x = make_x(5, 264, 1).to(gpu)
+    flat = weights(600, 2).to(gpu)
+    for off in (1, 3, 265):
+        w, p = flat[off:off + 264], flat[off + 2:off + 266]
+        want = add_rms_norm(x, x, w.clone(), EPS, post_weight=p.clone())
+        got = add_rms_norm(x, x, w, EPS, post_weight=p)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -256,3 +256,23 @@ def test_scales_far_apart_do_not_lose_small_blocks(gpu):
     # one rounding of e4m3: 2^-4 of a normal value (and of the block's largest / 448 below)
     assert float(rel.max()) <= 2 ** -4 and float(small.max()) <= 2 ** -4
     assert not math.isnan(float(small.max()))
+
+
+def test_a_copy_of_the_rows_is_made_on_the_calls_stream(gpu):
+    """Leading dims that no view flattens: the copy must not run on the current stream,
+    which the given one does not wait for."""
+    w, ws = (t.to(gpu) for t in make_weight(128, 256, 30))
+    base = make_x(64 * 256, 32, 31).to(gpu).view(64, 256, 32)
+    x = base.transpose(1, 2)                       # [64, 32, 256]
+    want = block_scaled_linear(x.reshape(-1, 256), w, ws).view(64, 32, 128)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    big = torch.zeros(1 << 28, device=gpu)
+    for _ in range(40):                            # keeps the current stream busy meanwhile
+        big.add_(1.0)
+    got = block_scaled_linear(x, w, ws, stream=s)
+    with torch.cuda.stream(s):
+        same = torch.equal(got, want)              # (waits for the call's stream only)
+    assert same
+    with pytest.raises(ValueError):
+        block_scaled_linear(x[..., :0], w[:, :0], ws[:, :0])

@@ -325,6 +325,8 @@ def current_stream(device) -> int:
 
 @contextlib.contextmanager
 def _launching(device, stream):
+    if stream is not None and stream.device != device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {device}")
     with torch.cuda.device(device), (contextlib.nullcontext() if stream is None
                                      else torch.cuda.stream(stream)):
         yield

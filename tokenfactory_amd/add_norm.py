@@ -24,6 +24,38 @@ def _check(name: str, t: torch.Tensor, shape, device) -> None:
         raise ValueError(f"add_rms_norm: {name} must be bf16 or fp32 {tuple(shape)} on x's device")
 
 
+def _vector(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if it lies dense and 16-byte aligned, else a copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from the first to behind the last element."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _clash(r: torch.Tensor, t: Optional[torch.Tensor]) -> bool:
+    """Whether rows written over ``r`` may change what another row or thread reads of
+    ``t``: they share memory and are not the very same elements (those are read by the
+    thread that writes them) or other columns of the same rows."""
+    if t is None or t.numel() == 0 or r.numel() == 0:
+        return False
+    off = t.data_ptr() - r.data_ptr()
+    if off >= _extent(r) or -off >= _extent(t):
+        return False
+    if t.shape != r.shape:
+        return True
+    if t.stride() == r.stride() and t.dtype == r.dtype and off == 0:
+        return False
+    size = r.element_size()
+    row, width = r.stride(0) * size, r.shape[1] * size
+    if t.stride(1) == 1 and t.stride(0) * t.element_size() == row:
+        return not (off % row >= width and off % row + t.shape[1] * t.element_size() <= row)
+    return True
+
+
 def _gate_rows(gate: torch.Tensor, shape):
     """(gate, row stride, per column) of a gate that broadcasts to ``shape``."""
     g = gate.expand(shape)
@@ -76,6 +108,9 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     if inplace and (residual is None or rows16(residual) is not residual):
         raise ValueError("add_rms_norm: in place, residual must be given, with dense 16-byte "
                          "aligned rows")
+    if inplace and any(_clash(residual, t) for t in (x, gate, weight, post_weight)):
+        raise ValueError("add_rms_norm: in place, residual must not share memory with another "
+                         "operand (x or a gate of its shape may be residual itself)")
     if gate is not None and (gate.dtype not in _VALUES or gate.device != x.device):
         raise ValueError("add_rms_norm: gate must be bf16 or fp32 on x's device")
     scale = float(residual_scale)
@@ -96,11 +131,11 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
             g, gs, gcols = _gate_rows(gate, x.shape)
             gp, gt = g.data_ptr(), DTYPES[g.dtype]
         if post_weight is not None:
-            post_weight = post_weight.contiguous()
+            post_weight = _vector(post_weight)
             pp, pt = post_weight.data_ptr(), DTYPES[post_weight.dtype]
         y = ys = None
         if weight is not None:
-            weight = weight.contiguous()
+            weight = _vector(weight)
             wp, wt = weight.data_ptr(), DTYPES[weight.dtype]
             y = new_rows(rows, cols, torch.float8_e4m3fn if quantize else x.dtype, dev)
             yp = y.data_ptr()

@@ -101,10 +101,12 @@ def mat(w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = Non
     return (w.data_ptr(), row_stride(w), scale.data_ptr(), sn, sk, _ptr(bias), n, _ptr(out), n)
 
 
-def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: int) -> torch.Tensor:
-    """x as a 2-D tensor of ``k`` columns that the products take."""
+def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: int) -> int:
+    """The rows of an x of ``k`` columns that the products take."""
     if not x.is_cuda or x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"{fn}: x {tuple(x.shape)} must be a CUDA tensor of {k} columns")
+    if k == 0:
+        raise ValueError(f"{fn}: no columns")
     if k % 16:
         raise NotImplementedError(f"{fn}: {k} columns (a multiple of 16)")
     if x.dtype not in DTYPES:
@@ -113,29 +115,28 @@ def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: in
     if quantized != (x_scale is not None):
         raise ValueError(f"{fn}: x_scale goes with a float8_e4m3fn x")
     if not quantized:
-        return x.reshape(-1, k)
+        return x.numel() // k
     if x.dim() != 2:
         raise ValueError(f"{fn}: a quantised x must be 2-D")
     if (x_scale.dtype != torch.float32 or x_scale.device != x.device
             or tuple(x_scale.shape) != (x.shape[0], blocks(k))):
         raise ValueError(f"{fn}: x_scale must be fp32 {(x.shape[0], blocks(k))} on x's device")
-    return x
+    return x.shape[0]
 
 
-def input_rows(x2d: torch.Tensor, x_scale: Optional[torch.Tensor]):
-    """(x, its row stride, scales, their stride) as the entry points take them;
+def input_rows(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
+    """(x's rows, their stride, scales, their stride) as the entry points take them;
     copies what lies otherwise (quantised rows of a width that is not a multiple of
-    128 get zeros behind them)."""
+    128 get zeros behind them), on the stream that is current."""
     if x_scale is None:
-        x2d = rows16(x2d)
+        x2d = rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
         return x2d, row_stride(x2d), None, 0
-    rows, k = x2d.shape
+    rows, k = x.shape
     if k % BLOCK:
-        padded = torch.zeros((rows, blocks(k) * BLOCK), dtype=torch.uint8, device=x2d.device)
-        padded[:, :k] = x2d.view(torch.uint8)
-        x2d = padded
+        x2d = torch.zeros((rows, blocks(k) * BLOCK), dtype=torch.uint8, device=x.device)
+        x2d[:, :k] = x.view(torch.uint8)
     else:
-        x2d = rows16(x2d)
+        x2d = rows16(x)
     nb = x_scale.shape[1]
     if not ((rows == 1 or x_scale.stride(0) == 1) and (nb == 1 or x_scale.stride(1) >= rows)):
         x_scale = x_scale.t().contiguous().t()
@@ -159,18 +160,17 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv:
     ``[out, in]`` (in a multiple of 16) with fp32 scales per 128 x 128 block; bias
     bf16 ``[out]``.  Returns bf16 ``[..., out]``."""
     fn = "block_scaled_linear"
-    x2d = check_input(fn, x, x_scale, weight.shape[-1])
-    check_weight(fn, "weight", weight, weight_scale_inv, x2d.shape[1], x.device)
+    rows = check_input(fn, x, x_scale, weight.shape[-1])
+    check_weight(fn, "weight", weight, weight_scale_inv, x.shape[-1], x.device)
     n, k = weight.shape
     if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (n,)
                              or bias.device != x.device or not bias.is_contiguous()):
         raise ValueError(f"{fn}: bias must be a contiguous bf16 [{n}] on x's device")
-    rows = x2d.shape[0]
     dev, dtype = x.device, DTYPES[x.dtype]
     with _native.launching(dev, stream):
         out = new_rows(rows, n, torch.bfloat16, dev)
         if rows:
-            xr, xs, sc, ss = input_rows(x2d, x_scale)
+            xr, xs, sc, ss = input_rows(x, x_scale)
             ws, nbytes = workspace("tf_block_linear_workspace_bytes", dev, rows, n, k, dtype)
             mats = (_native.Fp8Mat * 1)(mat(weight, weight_scale_inv, bias, out))
             _native.call("tf_block_linear", xr.data_ptr(), dtype, xs, _ptr(sc), ss, mats, rows, k,

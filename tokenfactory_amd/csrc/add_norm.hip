@@ -296,6 +296,9 @@ extern "C" int32_t tf_add_rms_norm(
   const int64_t chunks = cols / 8;
   const int nv = chunks > kWave * kMaxWaves ? 2 : 1;
   const int threads = (int)((chunks + (int64_t)nv * kWave - 1) / ((int64_t)nv * kWave)) * kWave;
+  if (rows * threads > UINT32_MAX)   // (of one launch)
+    return fail(TF_ERR_UNSUPPORTED, "add_rms_norm: %lld x %lld is too large", (long long)rows,
+                (long long)cols);
   const dim3 grid((uint32_t)rows), block(threads);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (nv == 1)

@@ -959,7 +959,7 @@ int32_t quant_setup(const char* fn, const void* x, int32_t x_dtype, int64_t rows
   a->scale = x_scale;
   a->ss = x_scale_stride;
   a->col_groups = (int32_t)ceil_div(out_cols, kQuantCols);
-  if (ceil_div(rows, kQuantWgRows) * a->col_groups > INT32_MAX)
+  if (ceil_div(rows, kQuantWgRows) * a->col_groups > UINT32_MAX / kThreads)   // (of one launch)
     return fail(TF_ERR_UNSUPPORTED, "%s: too large", fn);
   return TF_OK;
 }
@@ -1099,7 +1099,8 @@ int32_t check_product(const char* fn, int64_t m, int64_t n, int64_t k) {
   const int32_t rc = check_rows(fn, m, k, 16);
   if (rc != TF_OK) return rc;
   if (n <= 0) return fail(TF_ERR_INVALID, "%s: %lld columns", fn, (long long)n);
-  if (n > kMaxDim || ceil_div(m, 32) * ceil_div(n, 64) > INT32_MAX / (2 * kMaxSplits))
+  // a launch has 2^32 threads: 128 for 32 x 64 outputs where tiles are smallest
+  if (n > kMaxDim || ceil_div(m, 32) * ceil_div(n, 64) > UINT32_MAX / 128)
     return fail(TF_ERR_UNSUPPORTED, "%s: %lld x %lld is too large", fn, (long long)m,
                 (long long)n);
   return TF_OK;

@@ -34,7 +34,7 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
     multiples of 16.  Returns bf16 ``[..., out]``."""
     fn = "gated_mlp"
     hidden = gate_weight.shape[-1]
-    x2d = check_input(fn, x, x_scale, hidden)
+    rows = check_input(fn, x, x_scale, hidden)
     dev = x.device
     check_weight(fn, "gate_weight", gate_weight, gate_scale_inv, hidden, dev)
     check_weight(fn, "up_weight", up_weight, up_scale_inv, hidden, dev)
@@ -44,12 +44,12 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
     check_weight(fn, "down_weight", down_weight, down_scale_inv, inter, dev)
     if inter % 16:
         raise NotImplementedError(f"{fn}: {inter} hidden activations (a multiple of 16)")
-    rows, n = x2d.shape[0], down_weight.shape[0]
+    n = down_weight.shape[0]
     dtype = DTYPES[x.dtype]
     with _native.launching(dev, stream):
         out = new_rows(rows, n, torch.bfloat16, dev)
         if rows:
-            xr, xs, sc, ss = input_rows(x2d, x_scale)
+            xr, xs, sc, ss = input_rows(x, x_scale)
             ws, nbytes = workspace("tf_gated_mlp_workspace_bytes", dev, rows, hidden, inter, n,
                                    dtype)
             mats = (_native.Fp8Mat * 3)(mat(gate_weight, gate_scale_inv),
