@@ -13,7 +13,11 @@
 //
 // HBM-bound: a row is read once into registers and written once.  A workgroup
 // owns a row, a thread NV groups of 8 columns, one wave-wide and one LDS step per
-// sum; 16 neighbouring lanes hold the 128 columns of a scale.
+// sum; 16 neighbouring lanes hold the 128 columns of a scale.  8192 x 5120 bf16 with
+// a residual, quantised: 66 us = 4.5 TB/s (a copy of its 294 MB takes 57); rows kept
+// in flight by a workgroup for the next one, rows in order per XCD and non-temporal
+// accesses took 72 to 82.  777 x 2560 with an fp32 residual, post norm and gate: 8.1;
+// 48 x 5120: 4.2, a launch and two dependent sums.
 
 #include "block_quant.h"
 #include "tf_common.h"
