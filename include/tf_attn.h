@@ -556,9 +556,9 @@ int64_t tf_fp8_linears_workspace_bytes(int64_t m, const tf_fp8_mat* mats, int32_
  * w_scale[n / 128, kb] * (xq w^T over kb) + bias), fp32 accumulation; k a
  * multiple of 16, any n.  x: bf16 or fp32 (quantised into the workspace; alignment
  * as above) or e4m3 with x_scale: 16-byte aligned, its row stride a multiple of 16
- * from the padded width (k up to the next multiple of 128) up and zero bytes
- * between k and that width.  mat: the weight, 16-byte aligned rows; out
- * 8-byte aligned.  The result is deterministic.
+ * from k up (where k is no multiple of 128, more than 16 rows are copied into the
+ * workspace).  mat: the weight, 16-byte aligned rows; out 8-byte aligned.  The result
+ * is deterministic.
  *
  * tf_gated_mlp: out = h^ Wd^T with h = silu(x Wg^T) * (x Wu^T) in fp32 and h^ its
  * block-quantised form (qwen3_8/mlp.py:9-54).  mats: a host array of three, read

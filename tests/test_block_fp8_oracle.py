@@ -109,7 +109,7 @@ def _linear(m=4, k=256, n=64, x=16, x_dtype=BF16, xs=256, sc=None, ss=0, ws=256,
     (dict(ws_bytes=100), INVALID),
     (dict(x_dtype=FP8, sc=None, ss=4), INVALID),  # quantised without scales
     (dict(x_dtype=FP8, sc=16, ss=3), INVALID),
-    (dict(x_dtype=FP8, sc=16, ss=4, k=208, xs=208), INVALID),   # rows end before the padded width
+    (dict(x_dtype=FP8, sc=16, ss=4, k=208, xs=192), INVALID),   # rows overlap
     (dict(m=1 << 23, n=1 << 23), UNSUPPORTED),
 ])
 def test_linear_refusals(kw, code):
@@ -147,7 +147,8 @@ def test_workspaces_cover_the_quantised_rows():
         kp, kb = -(-k // 128) * 128, -(-k // 128)
         own = lib.tf_block_linear_workspace_bytes(m, 640, k, BF16)
         given = lib.tf_block_linear_workspace_bytes(m, 640, k, FP8)
-        assert own - given >= m * kp + 4 * m * kb and given >= 0
+        padded = m * kp if k % 128 and m > 16 else 0     # a copy with zeros behind its rows
+        assert own >= given + 4 * m * kb + m * kp - padded and given >= padded
         assert lib.tf_gated_mlp_workspace_bytes(m, k, 640, k, FP8) >= m * 640 + 4 * m * 5
     assert lib.tf_block_linear_workspace_bytes(4, 64, 100, BF16) == INVALID
     assert lib.tf_gated_mlp_workspace_bytes(4, 128, 100, 128, BF16) == INVALID

@@ -276,3 +276,18 @@ def test_a_copy_of_the_rows_is_made_on_the_calls_stream(gpu):
     assert same
     with pytest.raises(ValueError):
         block_scaled_linear(x[..., :0], w[:, :0], ws[:, :0])
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+def test_nothing_behind_quantised_rows_is_used(gpu, m):
+    """Rows of a width that ends inside a block, in a wider buffer of NaNs."""
+    k = 1040
+    q, s = ob.quantize(make_x(m, k, 40))
+    w, ws = (t.to(gpu) for t in make_weight(192, k, 41))
+    want = block_scaled_linear(q.to(gpu), w, ws, x_scale=s.to(gpu))
+    buf = torch.full((m, k + 240), 0x7F, dtype=torch.uint8, device=gpu)
+    rows = buf[:, :k]
+    rows.copy_(q.view(torch.uint8))
+    got = block_scaled_linear(rows.view(torch.float8_e4m3fn), w, ws, x_scale=s.to(gpu))
+    assert torch.equal(got, want)
+    assert bool((buf[:, k:] == 0x7F).all())

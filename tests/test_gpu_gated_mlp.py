@@ -152,3 +152,14 @@ def test_module_loads_a_reference_layer(gpu):
     with pytest.raises(ValueError):
         gated_mlp(x, *[t for lin in (mlp.gate_proj, mlp.down_proj, mlp.down_proj)
                        for t in (lin.weight, lin.weight_scale_inv)])
+
+
+@pytest.mark.parametrize("m", [4, 30, 300])
+def test_nothing_behind_quantised_rows_is_used(gpu, m):
+    q, s = ob.quantize(make_x(m, 400, 50))
+    _, dev = make_mlp(400, 272, 96, 51, gpu)
+    want = gated_mlp(q.to(gpu), *dev, x_scale=s.to(gpu))
+    buf = torch.full((m, 640), 0x7F, dtype=torch.uint8, device=gpu)
+    rows = buf[:, 16:416]
+    rows.copy_(q.view(torch.uint8))
+    assert torch.equal(gated_mlp(rows.view(torch.float8_e4m3fn), *dev, x_scale=s.to(gpu)), want)

@@ -126,18 +126,11 @@ def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: in
 
 def input_rows(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
     """(x's rows, their stride, scales, their stride) as the entry points take them;
-    copies what lies otherwise (quantised rows of a width that is not a multiple of
-    128 get zeros behind them), on the stream that is current."""
+    copies what lies otherwise, on the stream that is current."""
+    x2d = rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     if x_scale is None:
-        x2d = rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
         return x2d, row_stride(x2d), None, 0
-    rows, k = x.shape
-    if k % BLOCK:
-        x2d = torch.zeros((rows, blocks(k) * BLOCK), dtype=torch.uint8, device=x.device)
-        x2d[:, :k] = x.view(torch.uint8)
-    else:
-        x2d = rows16(x)
-    nb = x_scale.shape[1]
+    rows, nb = x_scale.shape
     if not ((rows == 1 or x_scale.stride(0) == 1) and (nb == 1 or x_scale.stride(1) >= rows)):
         x_scale = x_scale.t().contiguous().t()
     return x2d, row_stride(x2d), x_scale, rows if nb == 1 else x_scale.stride(1)

@@ -74,6 +74,18 @@ __global__ void __launch_bounds__(kThreads) block_quant_kernel(BlockQuantArgs a)
   }
 }
 
+// Quantised rows whose last block is short, with zeros behind them (a.x and a.xq in
+// bytes, a.cols a multiple of 16): what the tiles stage.  16 bytes a thread.
+__global__ void __launch_bounds__(kThreads) block_pad_kernel(BlockQuantArgs a) {
+  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int per = a.out_cols / 16;
+  const int64_t row = e / per;
+  if (row >= a.rows) return;
+  const int c = 16 * (int)(e - row * per);
+  *reinterpret_cast<u32x4*>(a.xq + row * a.qs + c) =
+      c < a.cols ? ld_g16(a.x + row * a.xs + c) : u32x4{0u, 0u, 0u, 0u};
+}
+
 // ---------------------------------------------------------------- GEMM
 constexpr int kSpread = 2, kAtStep = 4;   // staging instructions per row of MFMAs; see below
 constexpr int kGroupM = 8;            // m-tiles per group of the XCD tile order
@@ -118,7 +130,8 @@ struct BlockMat {
 // timing).  Gate and up products that leave the kernel unfused (n_mats == 2) are all
 // partials: their tiles are those of both matrices side by side.
 struct BlockGemmArgs {
-  const uint8_t* xq;      // e4m3 [M, 128 KB], zeros behind K, row stride xs bytes
+  const uint8_t* xq;      // e4m3 [M, 128 KB], zeros behind K, row stride xs bytes (few
+                          // rows: [M, K], nothing is read behind K)
   int64_t xs;
   const float* xsc;       // scale of (row, block) at block * xss + row
   int64_t xss;
@@ -604,14 +617,15 @@ __global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsA
   }
   const uint8_t* xp[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) xp[h] = a.x + min(lr + 8 * h, a.M - 1) * a.xs + lc;
+  for (int h = 0; h < 2; ++h) xp[h] = a.x + min(lr + 8 * h, a.M - 1) * a.xs;
   const int n_slices = (a.KB - w + kRowsWaves - 1) / kRowsWaves;   // of this wave
 
   auto load = [&](RowsSlice& s, int i) {
     const int kb = w + i * kRowsWaves;
     const int64_t k = (int64_t)kb * kQBlock;
-    // chunks behind the weights' last column: the slice's first (x is zero there)
-    const int c = kb == a.KB - 1 && lc >= a.tail ? 0 : lc;
+    // chunks behind the last column: the slice's first, times zeros for x
+    const bool gone = kb == a.KB - 1 && lc >= a.tail;
+    const int c = gone ? 0 : lc;
 #pragma unroll
     for (int m = 0; m < kMats; ++m) {
 #pragma unroll
@@ -620,7 +634,10 @@ __global__ void __launch_bounds__(kRowsWaves * kWave, 4) block_rows_kernel(RowsA
     }
     if constexpr (XK == kXRows) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s.x[h] = ld_g16(xp[h] + k);
+      for (int h = 0; h < 2; ++h) {
+        s.x[h] = ld_g16(xp[h] + k + c);
+        if (gone) s.x[h] = u32x4{0u, 0u, 0u, 0u};
+      }
       s.xs = a.xsc[kb * a.xss + row];
     }
   };
@@ -1021,9 +1038,12 @@ int32_t out_setup(const char* fn, const tf_fp8_mat* t, BlockGemmArgs* a) {
 struct Layout {
   int64_t xsc, hq, hsc, part, bytes;
 };
+// Whether a product copies its quantised x to have zeros behind a short last block.
+bool pads(int64_t m, int64_t k) { return k % kQBlock != 0 && !few_rows(m); }
+
 Layout layout(int64_t m, int64_t k, int64_t inter, bool quantized, int64_t parts) {
   Layout l;
-  l.xsc = quantized ? 0 : round_up(m * round_up(k, kQBlock), 256);
+  l.xsc = quantized && !pads(m, k) ? 0 : round_up(m * round_up(k, kQBlock), 256);
   l.hq = l.xsc + (quantized ? 0 : round_up(4 * m * ceil_div(k, kQBlock), 256));
   l.hsc = l.hq + round_up(m * round_up(inter, kQBlock), 256);
   l.part = l.hsc + round_up(4 * m * ceil_div(inter, kQBlock), 256);
@@ -1031,7 +1051,8 @@ Layout layout(int64_t m, int64_t k, int64_t inter, bool quantized, int64_t parts
   return l;
 }
 
-// x of a product: quantised rows as they come, or quantised into the workspace.
+// x of a product: quantised rows as they come or padded into the workspace, or
+// others quantised into it.
 int32_t input_setup(const char* fn, const void* x, int32_t x_dtype, int64_t x_row_stride,
                     const float* x_scale, int64_t x_scale_stride, int64_t m, int64_t k,
                     uint8_t* ws, const Layout& l, BlockGemmArgs* g, BlockQuantArgs* q) {
@@ -1050,16 +1071,33 @@ int32_t input_setup(const char* fn, const void* x, int32_t x_dtype, int64_t x_ro
   if (!x || !x_scale) return fail(TF_ERR_INVALID, "%s: null pointer", fn);
   if (!aligned16(x) || (reinterpret_cast<uintptr_t>(x_scale) & 3u))
     return fail(TF_ERR_INVALID, "%s: x 16-byte, its scales 4-byte aligned", fn);
-  if (x_row_stride < (int64_t)g->KB * kQBlock || x_row_stride % 16 || x_row_stride > kMaxDim ||
-      x_scale_stride < m || x_scale_stride > kMaxRows)
+  if (x_row_stride < k || x_row_stride % 16 || x_row_stride > kMaxDim || x_scale_stride < m ||
+      x_scale_stride > kMaxRows)
     return fail(TF_ERR_INVALID, "%s: quantised x strides %lld/%lld (rows a multiple of 16 from "
-                "the padded width up, scales from the number of rows up)", fn,
-                (long long)x_row_stride, (long long)x_scale_stride);
+                "their width up, scales from the number of rows up)", fn, (long long)x_row_stride,
+                (long long)x_scale_stride);
   g->xq = static_cast<const uint8_t*>(x);
   g->xs = x_row_stride;
   g->xsc = x_scale;
   g->xss = x_scale_stride;
+  if (pads(m, k)) {
+    q->x = g->xq;
+    q->xs = x_row_stride;
+    q->rows = m;
+    q->cols = (int32_t)k;
+    q->out_cols = g->KB * kQBlock;
+    q->xq = ws;
+    q->qs = q->out_cols;
+    g->xq = ws;
+    g->xs = q->qs;
+  }
   return TF_OK;
+}
+
+void launch_pad(const BlockQuantArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(block_pad_kernel,
+                     dim3((uint32_t)ceil_div(a.rows * (a.out_cols / 16), kThreads)),
+                     dim3(kThreads), 0, s, a);
 }
 
 bool bad_workspace(const void* ws, int64_t bytes, int64_t need) {
@@ -1085,9 +1123,15 @@ RowsArgs rows_args(const BlockGemmArgs& g, int64_t k, int xk, const BlockQuantAr
   return r;
 }
 
-// Quantises the x of g's one product in a launch of its own unless the kernel of few
-// rows does it; says what that kernel's x is.
-int quantize_input(bool f32, const BlockGemmArgs& g, const BlockQuantArgs& q, hipStream_t s) {
+// Makes the x of g's one product in a launch of its own unless it comes quantised or the
+// kernel of few rows quantises it; says what that kernel's x is.
+int prepare_input(int32_t dtype, int64_t k, const BlockGemmArgs& g, const BlockQuantArgs& q,
+                  hipStream_t s) {
+  if (dtype == TF_DTYPE_FP8_E4M3) {
+    if (pads(g.M, k)) launch_pad(q, s);
+    return kXRows;
+  }
+  const bool f32 = dtype == TF_DTYPE_FP32;
   if (rows_quantise(g.M, g.mat[0].N, g.KB)) return f32 ? kXF32 : kXBf16;
   launch_quant(q, f32, s);
   return kXRows;
@@ -1164,7 +1208,7 @@ int32_t tf_block_linear(const void* x, int32_t x_dtype, int64_t x_row_stride,
                    &g, &q);
   if (rc != TF_OK) return rc;   // nothing is launched for arguments that any part refuses
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int xk = quantized ? kXRows : quantize_input(x_dtype == TF_DTYPE_FP32, g, q, s);
+  const int xk = prepare_input(x_dtype, k, g, q, s);
   if (few_rows(m))
     launch_rows(rows_args(g, k, xk, q), xk, s);
   else
@@ -1224,7 +1268,10 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
   d.xsc = g.hsc = reinterpret_cast<float*>(ws + l.hsc);
   d.xss = g.hss = m;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (!quantized) launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
+  if (!quantized)
+    launch_quant(q, x_dtype == TF_DTYPE_FP32, s);
+  else if (pads(m, hidden))
+    launch_pad(q, s);
   if (few_rows(m)) {
     RowsArgs r = rows_args(g, hidden, kXRows, q);
     r.h = part;
@@ -1232,7 +1279,7 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
     rc = quant_setup("gated_mlp", part, TF_DTYPE_FP32, m, inter, inter, ws + l.hq, d.xs,
                      g.hsc, m, d.xs, &q);
     if (rc != TF_OK) return rc;
-    const int xk = quantize_input(true, d, q, s);
+    const int xk = prepare_input(TF_DTYPE_FP32, inter, d, q, s);
     launch_rows(rows_args(d, inter, xk, q), xk, s);
     return launch_status("tf_gated_mlp launch");
   }
