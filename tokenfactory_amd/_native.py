@@ -312,6 +312,7 @@ def call(name: str, *args) -> int:
 
 # (private to torch; a build without it pays for the Stream object)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def current_stream(device) -> int:
@@ -339,7 +340,7 @@ def launching(device, stream):
     """Context in which a call on ``device`` allocates and launches: with that device
     (launches go to the current one, whatever stream they name) and ``stream`` (None:
     the device's current stream) current.  A no-op where they are already."""
-    if stream is None and torch.cuda.current_device() == device.index:
+    if stream is None and _current_device() == device.index:
         return _here
     return _launching(device, stream)
 

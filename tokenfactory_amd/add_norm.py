@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .block_fp8 import DTYPES, new_rows, new_scales, row_stride, rows16
+from .block_fp8 import DTYPES, new_rows, new_scales, rows16
 
 MAX_COLS = 16384
 _VALUES = (torch.bfloat16, torch.float32)
@@ -63,9 +63,8 @@ def _gate_rows(gate: torch.Tensor, shape):
     if g.stride(1) == 0:                    # one value per row (or for all of them)
         return g, (g.stride(0) if rows > 1 else 0), 0
     if rows == 1 or g.stride(0) == 0:       # one row for all of them
-        return rows16(g[:1]), 0, 1
-    g = rows16(g)
-    return g, g.stride(0), 1
+        return rows16(g[:1])[0], 0, 1
+    return *rows16(g), 1
 
 
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
@@ -105,7 +104,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
         _check("post_weight", post_weight, (cols,), dev)
     if residual is not None:
         _check("residual", residual, x.shape, dev)
-    if inplace and (residual is None or rows16(residual) is not residual):
+    if inplace and (residual is None or rows16(residual)[0] is not residual):
         raise ValueError("add_rms_norm: in place, residual must be given, with dense 16-byte "
                          "aligned rows")
     if inplace and any(_clash(residual, t) for t in (x, gate, weight, post_weight)):
@@ -118,12 +117,13 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     xt = rt = DTYPES[x.dtype]
     yt = DTYPES[torch.float8_e4m3fn] if quantize else xt
     with _native.launching(dev, stream):
-        xr, rp, rs, r = rows16(x), 0, 0, x
+        xr, xs = rows16(x)
+        rp, rs, r, ros = 0, 0, x, cols
         if residual is not None:
-            rr, rt = rows16(residual), DTYPES[residual.dtype]
-            rp, rs = rr.data_ptr(), row_stride(rr)
+            rr, rs = rows16(residual)
+            rp, rt = rr.data_ptr(), DTYPES[residual.dtype]
         if inplace:
-            r = residual
+            r, ros = residual, rs
         elif not same:
             r = new_rows(rows, cols, x.dtype if residual is None else residual.dtype, dev)
         gp = gs = gt = gcols = wp = wt = pp = pt = yp = sp = 0
@@ -143,8 +143,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
                 ys = new_scales(rows, cols, dev)
                 sp = ys.data_ptr()
         if rows and not (same and y is None):
-            _native.call("tf_add_rms_norm", xr.data_ptr(), xt, row_stride(xr), rp, rt, rs, gp, gt,
-                         gs, gcols, pp, pt, wp, wt, eps, scale, rows, cols,
-                         0 if same else r.data_ptr(), row_stride(r), yp, yt, cols, sp, rows,
-                         _native.current_stream(dev))
+            _native.call("tf_add_rms_norm", xr.data_ptr(), xt, xs, rp, rt, rs, gp, gt, gs, gcols,
+                         pp, pt, wp, wt, eps, scale, rows, cols, 0 if same else r.data_ptr(), ros,
+                         yp, yt, cols, sp, rows, _native.current_stream(dev))
     return ((y, ys) if quantize else y), r

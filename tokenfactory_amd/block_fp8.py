@@ -32,21 +32,20 @@ def blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself if the kernels take its rows as they lie (dense columns, rows
-    that do not overlap, 16-byte aligned), else a copy."""
-    unit = 16 if t.dtype == torch.float8_e4m3fn else 8
+def rows16(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(rows, their stride): ``t`` itself if the kernels take its rows as they lie
+    (dense columns, rows that do not overlap, 16-byte aligned), else a copy; the stride
+    of one row is its width, whatever torch says.  Widths are multiples of 8, or 16 of
+    e4m3 values."""
     rows, cols = t.shape
-    if t.data_ptr() % 16 == 0 and (
-            t.is_contiguous() and (rows == 1 or cols % unit == 0)
-            or t.stride(1) == 1 and (rows == 1 or (t.stride(0) >= cols and t.stride(0) % unit == 0))):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def row_stride(t: torch.Tensor) -> int:
-    """The row stride of ``rows16(t)`` (one row: its width, whatever torch says)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t, cols
+        if t.stride(1) == 1:
+            stride = t.stride(0) if rows > 1 else cols
+            if stride >= cols and stride % (16 if t.dtype == torch.float8_e4m3fn else 8) == 0:
+                return t, stride
+    return t.clone(memory_format=torch.contiguous_format), cols
 
 
 def new_rows(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
@@ -72,33 +71,30 @@ def quantize_blocks(x: torch.Tensor, stream=None) -> Tuple[torch.Tensor, torch.T
         raise ValueError(f"quantize_blocks: {cols} columns (a positive multiple of 8)")
     dev = x.device
     with _native.launching(dev, stream):
-        x = rows16(x)
+        x, stride = rows16(x)
         xq = new_rows(rows, cols, torch.float8_e4m3fn, dev)
         scale = new_scales(rows, cols, dev)
-        _native.call("tf_block_quant", x.data_ptr(), DTYPES[x.dtype], rows, cols, row_stride(x),
+        _native.call("tf_block_quant", x.data_ptr(), DTYPES[x.dtype], rows, cols, stride,
                      xq.data_ptr(), cols, scale.data_ptr(), rows, _native.current_stream(dev))
     return xq, scale
 
 
-def check_weight(fn: str, what: str, w: torch.Tensor, scale: torch.Tensor, k: int, device) -> None:
+def check_weight(fn: str, what: str, w: torch.Tensor, scale: torch.Tensor, k: int, device) -> tuple:
+    """The fields of the ``tf_fp8_mat`` of a weight up to its bias."""
     n = w.shape[0] if w.dim() == 2 else 0
     if w.dtype != torch.float8_e4m3fn or n == 0 or w.shape[1] != k or w.device != device:
         raise ValueError(f"{fn}: {what} must be float8_e4m3fn [out, {k}] on x's device, not "
                          f"{w.dtype} {tuple(w.shape)}")
-    if rows16(w) is not w:
+    ptr = w.data_ptr()
+    stride = k if w.is_contiguous() or n == 1 else w.stride(0)
+    if ptr % 16 or stride % 16 or stride < k or w.stride(1) != 1:
         raise ValueError(f"{fn}: {what} rows must be contiguous and 16-byte aligned")
-    if (scale.dtype != torch.float32 or scale.shape != (blocks(n), blocks(k))
-            or scale.device != device):
-        raise ValueError(f"{fn}: scales of {what} must be fp32 {(blocks(n), blocks(k))} on x's "
-                         f"device, one per 128 x 128 block")
-
-
-def mat(w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
-        out: Optional[torch.Tensor] = None) -> tuple:
-    """The fields of the ``tf_fp8_mat`` of a checked weight."""
-    n = w.shape[0]
+    shape = (-(-n // BLOCK), -(-k // BLOCK))
+    if scale.dtype != torch.float32 or scale.shape != shape or scale.device != device:
+        raise ValueError(f"{fn}: scales of {what} must be fp32 {shape} on x's device, one per "
+                         f"128 x 128 block")
     sn, sk = scale.stride()
-    return (w.data_ptr(), row_stride(w), scale.data_ptr(), sn, sk, _ptr(bias), n, _ptr(out), n)
+    return ptr, stride, scale.data_ptr(), sn, sk
 
 
 def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: int) -> int:
@@ -127,19 +123,23 @@ def check_input(fn: str, x: torch.Tensor, x_scale: Optional[torch.Tensor], k: in
 def input_rows(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
     """(x's rows, their stride, scales, their stride) as the entry points take them;
     copies what lies otherwise, on the stream that is current."""
-    x2d = rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    x2d, stride = rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     if x_scale is None:
-        return x2d, row_stride(x2d), None, 0
+        return x2d, stride, None, 0
     rows, nb = x_scale.shape
-    if not ((rows == 1 or x_scale.stride(0) == 1) and (nb == 1 or x_scale.stride(1) >= rows)):
-        x_scale = x_scale.t().contiguous().t()
-    return x2d, row_stride(x2d), x_scale, rows if nb == 1 else x_scale.stride(1)
+    s0, s1 = x_scale.stride()
+    if not ((rows == 1 or s0 == 1) and (nb == 1 or s1 >= rows)):
+        x_scale, s1 = x_scale.t().contiguous().t(), rows
+    return x2d, stride, x_scale, rows if nb == 1 else s1
 
 
 def workspace(name: str, device, *sizes):
     """(scratch or None, bytes) that entry point ``name`` asks for."""
     nbytes = _native.call(name, *sizes)
     return (torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+
+_OneMat = _native.Fp8Mat * 1
 
 
 def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv: torch.Tensor,
@@ -154,18 +154,18 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv:
     bf16 ``[out]``.  Returns bf16 ``[..., out]``."""
     fn = "block_scaled_linear"
     rows = check_input(fn, x, x_scale, weight.shape[-1])
-    check_weight(fn, "weight", weight, weight_scale_inv, x.shape[-1], x.device)
+    dev, dtype = x.device, DTYPES[x.dtype]
+    mat = check_weight(fn, "weight", weight, weight_scale_inv, x.shape[-1], dev)
     n, k = weight.shape
     if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (n,)
-                             or bias.device != x.device or not bias.is_contiguous()):
+                             or bias.device != dev or not bias.is_contiguous()):
         raise ValueError(f"{fn}: bias must be a contiguous bf16 [{n}] on x's device")
-    dev, dtype = x.device, DTYPES[x.dtype]
     with _native.launching(dev, stream):
         out = new_rows(rows, n, torch.bfloat16, dev)
         if rows:
             xr, xs, sc, ss = input_rows(x, x_scale)
             ws, nbytes = workspace("tf_block_linear_workspace_bytes", dev, rows, n, k, dtype)
-            mats = (_native.Fp8Mat * 1)(mat(weight, weight_scale_inv, bias, out))
-            _native.call("tf_block_linear", xr.data_ptr(), dtype, xs, _ptr(sc), ss, mats, rows, k,
-                         _ptr(ws), nbytes, _native.current_stream(dev))
+            _native.call("tf_block_linear", xr.data_ptr(), dtype, xs, _ptr(sc), ss,
+                         _OneMat((*mat, _ptr(bias), n, out.data_ptr(), n)), rows, k, _ptr(ws),
+                         nbytes, _native.current_stream(dev))
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)

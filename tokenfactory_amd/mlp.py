@@ -16,9 +16,12 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .block_fp8 import (BLOCK, DTYPES, check_input, check_weight, input_rows, mat, new_rows,
+from .block_fp8 import (BLOCK, DTYPES, check_input, check_weight, input_rows, new_rows,
                         workspace)
 from .fp8_linear import Fp8Linear, _ptr
+
+
+_GateUpDown = _native.Fp8Mat * 3
 
 
 def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.Tensor,
@@ -36,12 +39,12 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
     hidden = gate_weight.shape[-1]
     rows = check_input(fn, x, x_scale, hidden)
     dev = x.device
-    check_weight(fn, "gate_weight", gate_weight, gate_scale_inv, hidden, dev)
-    check_weight(fn, "up_weight", up_weight, up_scale_inv, hidden, dev)
+    gate = check_weight(fn, "gate_weight", gate_weight, gate_scale_inv, hidden, dev)
+    up = check_weight(fn, "up_weight", up_weight, up_scale_inv, hidden, dev)
     inter = gate_weight.shape[0]
     if up_weight.shape[0] != inter:
         raise ValueError(f"{fn}: {inter} gate and {up_weight.shape[0]} up columns")
-    check_weight(fn, "down_weight", down_weight, down_scale_inv, inter, dev)
+    down = check_weight(fn, "down_weight", down_weight, down_scale_inv, inter, dev)
     if inter % 16:
         raise NotImplementedError(f"{fn}: {inter} hidden activations (a multiple of 16)")
     n = down_weight.shape[0]
@@ -52,9 +55,8 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
             xr, xs, sc, ss = input_rows(x, x_scale)
             ws, nbytes = workspace("tf_gated_mlp_workspace_bytes", dev, rows, hidden, inter, n,
                                    dtype)
-            mats = (_native.Fp8Mat * 3)(mat(gate_weight, gate_scale_inv),
-                                        mat(up_weight, up_scale_inv),
-                                        mat(down_weight, down_scale_inv, out=out))
+            mats = _GateUpDown((*gate, None, inter, None, inter), (*up, None, inter, None, inter),
+                               (*down, None, n, out.data_ptr(), n))
             _native.call("tf_gated_mlp", xr.data_ptr(), dtype, xs, _ptr(sc), ss, mats, rows, hidden,
                          inter, ws.data_ptr(), nbytes, _native.current_stream(dev))
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
