@@ -149,3 +149,28 @@ def test_two_threads_on_streams_of_their_own(gpu):
     for t in threads:
         t.join()
     assert not errors and not bad
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows behind 2^31 elements and 2^32 bytes of inputs, results and scratch."""
+    base, rows = make_x(64, 8192, 70), 64 * 4400
+    print(f"[large] {rows} x 8192", flush=True)
+    x = base.to(gpu).repeat(rows // 64, 1)
+    ends = torch.tensor([0, 1, rows // 2 + 3, rows - 2, rows - 1])
+    want_x = base[ends % 64]
+    q, s = quantize_blocks(x)
+    wq, wsc = ob.quantize(want_x)
+    assert torch.equal(q.view(torch.uint8)[ends.to(gpu)].cpu(), wq.view(torch.uint8))
+    assert torch.equal(s[ends.to(gpu)].cpu(), wsc)
+    w = norm_test.weights(8192, 71)
+    y, r = add_rms_norm(x, x, w.to(gpu), EPS)
+    norm_test.compare(y[ends.to(gpu)], r[ends.to(gpu)], want_x, want_x, w, None, None, 1.0, False)
+    del y, r
+    w, ws = make_weight(8200, 8192, 72)         # out: 2.3e9 elements
+    out = block_scaled_linear(q, w.to(gpu), ws.to(gpu), x_scale=s)
+    linear_close(out[ends.to(gpu)], ob.dequantize(wq, wsc), w, ws)
+    del out, q, s
+    host, dev = mlp_test.make_mlp(256, 8208, 128, 73, gpu)
+    out = gated_mlp(x[:, :256], *dev)           # hidden activations: 2.3e9 bytes
+    mlp_test.compare(out[ends.to(gpu)].double().cpu(), ob.dequantize(*ob.quantize(want_x[:, :256])),
+                     host)
