@@ -136,7 +136,9 @@ def input_rows(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
 def workspace(name: str, device, *sizes):
     """(scratch or None, bytes) that entry point ``name`` asks for."""
     nbytes = _native.call(name, *sizes)
-    return (torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None), nbytes
+    if not nbytes:
+        return None, 0
+    return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device), nbytes
 
 
 _OneMat = _native.Fp8Mat * 1
