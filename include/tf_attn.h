@@ -595,7 +595,8 @@ int32_t tf_gated_mlp(const void* x, int32_t x_dtype, int64_t x_row_stride, const
  *   y  = weight * r' / rms(r'),   rms(v) = sqrt(mean v^2 + eps)
  * residual, gate and post_weight may be NULL (0, 1, no norm of x).  r' is stored
  * to residual_out (NULL: not stored) in the residual's type, or x's without one;
- * it may be the residual itself.  y (NULL: not computed) is bf16, fp32 or e4m3
+ * it may be the residual itself, but no other operand's memory unless x or a gate per
+ * element is that same matrix.  y (NULL: not computed) is bf16, fp32 or e4m3
  * with scales as tf_block_quant makes them; it is formed from r' before that is
  * rounded.  gate: per_column != 0: elements of a row side by side, row stride
  * 0 or from cols up; else one value per row, gate_row_stride apart.  x, residual,

@@ -86,7 +86,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     Returns ``(y, r)``.  y has x's dtype, or with ``quantize`` is the pair
     ``(float8_e4m3fn values, fp32 scales)`` of ``quantize_blocks``; it is formed from
     r before r is rounded to the residual's dtype (x's without a residual).  Without
-    a weight y is None.  ``inplace`` stores r over ``residual``.  Where r is x
+    a weight y is None.  ``inplace`` stores r over ``residual``, which must not share
+    memory with another operand (x or a gate of its shape may be it).  Where r is x
     itself (no residual, gate, scale or post_weight), x is returned as r."""
     if x.dim() != 2 or not x.is_cuda or x.dtype not in _VALUES:
         raise ValueError("add_rms_norm: x must be a 2-D bf16 or fp32 CUDA tensor")
