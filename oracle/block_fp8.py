@@ -18,7 +18,7 @@ def blocks(x: torch.Tensor) -> torch.Tensor:
     """[rows, cols] -> [rows, blocks, 128] with zeros behind the last column."""
     rows, cols = x.shape
     n = -(-cols // BLOCK)
-    out = torch.zeros((rows, n * BLOCK), dtype=x.dtype)
+    out = x.new_zeros((rows, n * BLOCK))
     out[:, :cols] = x
     return out.view(rows, n, BLOCK)
 

@@ -111,7 +111,7 @@ def check_linear(gpu, m, n, k, bias=False, quantized=False, dtype=torch.bfloat16
     return out
 
 
-# One row to many, tiles cut in every dimension, each tile shape of the plan, split and not.
+# One row to many, tiles cut in every dimension (every tile shape: test_gpu_block_tiles.py).
 @pytest.mark.parametrize("m,n,k", [
     (1, 64, 16), (1, 1, 48), (1, 5120, 6144), (1, 40, 17408), (1, 33, 36864), (2, 130, 272),
     (4, 100, 8192), (5, 77, 9008), (16, 48, 12800), (16, 640, 256), (17, 2592, 5120),
