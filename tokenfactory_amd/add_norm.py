@@ -88,7 +88,9 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     r before r is rounded to the residual's dtype (x's without a residual).  Without
     a weight y is None.  ``inplace`` stores r over ``residual``, which must not share
     memory with another operand (x or a gate of its shape may be it).  Where r is x
-    itself (no residual, gate, scale or post_weight), x is returned as r."""
+    itself (no residual, gate, scale or post_weight), x is returned as r.  No gradients:
+    operands that ask for one are refused while autograd records."""
+    _native.refuse_gradients("add_rms_norm", x, residual, weight, post_weight, gate)
     if x.dim() != 2 or not x.is_cuda or x.dtype not in _VALUES:
         raise ValueError("add_rms_norm: x must be a 2-D bf16 or fp32 CUDA tensor")
     rows, cols = x.shape
@@ -147,4 +149,6 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
             _native.call("tf_add_rms_norm", xr.data_ptr(), xt, xs, rp, rt, rs, gp, gt, gs, gcols,
                          pp, pt, wp, wt, eps, scale, rows, cols, 0 if same else r.data_ptr(), ros,
                          yp, yt, cols, sp, rows, _native.current_stream(dev))
+    if inplace:
+        torch.autograd.graph.increment_version(residual)   # (written behind autograd's back)
     return ((y, ys) if quantize else y), r

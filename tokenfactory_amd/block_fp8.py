@@ -12,7 +12,8 @@ activations can write them quantised (``add_rms_norm(..., quantize=True)``).
   checkpoint's block-FP8 weight (``Fp8Linear.weight`` / ``weight_scale_inv``)
 
 Scales are fp32 ``[rows, ceil(cols / 128)]``, stored with a block's rows side by
-side (``stride(0) == 1``).  There is no non-native path and no gradient.
+side (``stride(0) == 1``).  There is no non-native path and no gradient: operands that
+ask for one are refused while autograd records.
 """
 from __future__ import annotations
 
@@ -64,6 +65,7 @@ def quantize_blocks(x: torch.Tensor, stream=None) -> Tuple[torch.Tensor, torch.T
     even.  x: bf16 or fp32 ``[rows, cols]``, cols a multiple of 8.  Returns
     float8_e4m3fn ``[rows, cols]`` and fp32 scales ``[rows, ceil(cols / 128)]``.
     A NaN or infinite value poisons its row's block (scale NaN or inf)."""
+    _native.refuse_gradients("quantize_blocks", x)
     if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("quantize_blocks: x must be a 2-D bf16 or fp32 CUDA tensor")
     rows, cols = x.shape
@@ -155,6 +157,7 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv:
     ``[out, in]`` (in a multiple of 16) with fp32 scales per 128 x 128 block; bias
     bf16 ``[out]``.  Returns bf16 ``[..., out]``."""
     fn = "block_scaled_linear"
+    _native.refuse_gradients(fn, x, x_scale, weight, weight_scale_inv, bias)
     rows = check_input(fn, x, x_scale, weight.shape[-1])
     dev, dtype = x.device, DTYPES[x.dtype]
     mat = check_weight(fn, "weight", weight, weight_scale_inv, x.shape[-1], dev)

@@ -34,8 +34,10 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
     x: bf16 or fp32 ``[..., hidden]`` or float8_e4m3fn ``[rows, hidden]`` with its
     ``x_scale``; gate and up weights float8_e4m3fn ``[inter, hidden]``, down
     ``[out, inter]``, each with fp32 scales per 128 x 128 block; hidden and inter
-    multiples of 16.  Returns bf16 ``[..., out]``."""
+    multiples of 16.  Returns bf16 ``[..., out]``; no gradients."""
     fn = "gated_mlp"
+    _native.refuse_gradients(fn, x, x_scale, gate_weight, gate_scale_inv, up_weight, up_scale_inv,
+                             down_weight, down_scale_inv)
     hidden = gate_weight.shape[-1]
     rows = check_input(fn, x, x_scale, hidden)
     dev = x.device
