@@ -65,9 +65,9 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
 
 
 class GatedMLP(nn.Module):
-    """One TP rank's share of the gated feed-forward block: ``gate_proj`` and
-    ``up_proj`` ``[intermediate_size / tp, hidden]`` and ``down_proj``, whose partial
-    sums the caller adds over the ranks.  The three ``Fp8Linear``s hold weights and
+    """One TP rank's share of the gated feed-forward block (whole blocks of 128 columns):
+    ``gate_proj`` and ``up_proj`` ``[intermediate_size / tp, hidden]`` and ``down_proj``,
+    whose partial sums the caller adds over the ranks.  The three ``Fp8Linear``s hold weights and
     scales; ``forward`` reads them and does not call the modules."""
 
     def __init__(self, config):
@@ -86,6 +86,9 @@ class GatedMLP(nn.Module):
         if config.intermediate_size % tp:
             raise ValueError("intermediate_size must divide by tp_size")
         inter = config.intermediate_size // tp
+        if tp > 1 and inter % BLOCK:   # (no rows of the checkpoint's scales are the share's)
+            raise NotImplementedError(f"GatedMLP: {inter} columns a rank cut a block of {BLOCK} "
+                                      "columns that share a scale")
         if inter % 16 or config.hidden_size % 16:
             raise NotImplementedError(f"GatedMLP: {config.hidden_size} x {inter} (multiples of 16)")
         self.gate_proj = Fp8Linear(config.hidden_size, inter, block_size=block)
