@@ -1,7 +1,9 @@
 """What ``GatedMLP`` takes as its configuration and projections (CPU only)."""
 import pytest
+import torch
+import torch.nn as nn
 
-from tokenfactory_amd import GatedMLP
+from tokenfactory_amd import Fp8Linear, GatedMLP
 
 
 class Config:
@@ -25,3 +27,39 @@ def test_whole_blocks_and_unshared_widths_are_taken():
     assert GatedMLP(config(tp_size=8)).down_proj.weight.shape == (256, 2176)
     assert GatedMLP(config(intermediate_size=1088)).up_proj.weight.shape == (1088, 256)
     assert GatedMLP(config(intermediate_size=1088, tp_size=1)).up_proj.weight.shape == (1088, 256)
+
+
+def altered(mlp, how):
+    proj = mlp.up_proj
+    if how == "hook":
+        proj.register_forward_hook(lambda m, i, o: o)
+    elif how == "pre-hook":
+        proj.register_forward_pre_hook(lambda m, i: i)
+    elif how == "forward":
+        proj.forward = lambda x: x
+    elif how == "subclass":
+        mlp.up_proj = type("Adapted", (Fp8Linear,), {})(256, 512)
+    elif how == "other module":
+        mlp.up_proj = nn.Linear(256, 512, bias=False)
+    elif how == "bias":
+        mlp.up_proj = Fp8Linear(256, 512, bias=True)
+    elif how == "blocks":
+        mlp.up_proj = Fp8Linear(256, 512, block_size=(64, 64))
+    return mlp
+
+
+@pytest.mark.parametrize("how", ["hook", "pre-hook", "forward", "subclass", "other module", "bias",
+                                 "blocks"])
+def test_a_projection_that_does_more_is_not_passed_by(how):
+    """The block reads the weights and calls no module."""
+    mlp = altered(GatedMLP(config(intermediate_size=512)), how)
+    with pytest.raises(NotImplementedError, match="up_proj"):
+        mlp(torch.zeros((2, 256), dtype=torch.bfloat16))
+
+
+def test_plain_projections_are_read():
+    mlp = GatedMLP(config(intermediate_size=512))
+    handle = mlp.gate_proj.register_forward_hook(lambda m, i, o: o)
+    handle.remove()
+    with pytest.raises(ValueError):     # (the tensors lie on the CPU)
+        mlp(torch.zeros((2, 256), dtype=torch.bfloat16))

@@ -18,7 +18,7 @@ import torch.nn as nn
 from . import _native
 from .block_fp8 import (BLOCK, DTYPES, check_input, check_weight, input_rows, new_rows,
                         workspace)
-from .fp8_linear import Fp8Linear, _ptr
+from .fp8_linear import Fp8Linear, _ptr, _unaltered
 
 
 _GateUpDown = _native.Fp8Mat * 3
@@ -67,8 +67,9 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, gate_scale_inv: torch.
 class GatedMLP(nn.Module):
     """One TP rank's share of the gated feed-forward block (whole blocks of 128 columns):
     ``gate_proj`` and ``up_proj`` ``[intermediate_size / tp, hidden]`` and ``down_proj``,
-    whose partial sums the caller adds over the ranks.  The three ``Fp8Linear``s hold weights and
-    scales; ``forward`` reads them and does not call the modules."""
+    whose partial sums the caller adds over the ranks.  The three ``Fp8Linear``s hold
+    weights and scales; ``forward`` reads them and does not call the modules, so that
+    one that is more than that (a subclass, a hook, a bias) is refused."""
 
     def __init__(self, config):
         super().__init__()
@@ -96,6 +97,12 @@ class GatedMLP(nn.Module):
         self.down_proj = Fp8Linear(inter, config.hidden_size, block_size=block)
 
     def forward(self, x: torch.Tensor, x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
-        g, u, d = self.gate_proj, self.up_proj, self.down_proj
-        return gated_mlp(x, g.weight, g.weight_scale_inv, u.weight, u.weight_scale_inv, d.weight,
-                         d.weight_scale_inv, x_scale=x_scale)
+        weights = []
+        for name in ("gate_proj", "up_proj", "down_proj"):
+            lin = self._modules[name]
+            if not _unaltered(lin, Fp8Linear) or lin.bias is not None \
+                    or (lin.block_h, lin.block_w) != (BLOCK, BLOCK):
+                raise NotImplementedError(f"GatedMLP: {name} must be a plain Fp8Linear of 128 x 128 "
+                                          "blocks without a bias: its call is passed by")
+            weights += lin.weight, lin.weight_scale_inv
+        return gated_mlp(x, *weights, x_scale=x_scale)
