@@ -987,6 +987,8 @@ int32_t input_setup(const char* fn, const void* x, int32_t x_dtype, int64_t x_ro
   g->xsc = x_scale;
   g->xss = x_scale_stride;
   if (pads(m, k)) {
+    if (m * (g->KB * kQBlock / 16) > UINT32_MAX)   // (threads of one launch)
+      return fail(TF_ERR_UNSUPPORTED, "%s: too large", fn);
     q->x = g->xq;
     q->xs = x_row_stride;
     q->rows = m;
