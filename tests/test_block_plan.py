@@ -97,3 +97,14 @@ def test_plans_are_launches(plan, cus):
             assert full == 0
         elif splits == 1:
             assert full == tiles
+
+
+def test_partials_that_no_launch_finishes_are_not_planned(plan):
+    """A launch has 2^32 threads, gated_finish_kernel 32 of them per row and block."""
+    rng = random.Random(3)
+    log = lambda a, b: int(round(math.exp(rng.uniform(math.log(a), math.log(b)))))
+    for m, n, k in [(8460377, 18144, 269168), (1 << 20, 20480, 65536)] + [
+            (log(1 << 19, 1 << 24), 16 * log(64, 4096), 16 * log(1024, 1 << 16))
+            for _ in range(20000)]:
+        fused = plan(m, n, k, True)[4]
+        assert fused or m * -(-n // 128) * 32 < 1 << 32, (m, n, k)

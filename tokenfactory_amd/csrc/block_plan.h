@@ -93,6 +93,8 @@ inline BlockPlan plan_linear(int64_t m, int64_t n, int n_mats, int64_t kb, bool 
 
 inline BlockPlan plan_gated(int64_t m, int64_t inter, int64_t kb, int64_t cus) {
   BlockPlan best = plan_linear(m, inter, 2, kb, true, cus);
+  // (a launch has 2^32 threads; the one that finishes partials 32 per row and block)
+  if (m * ceil_div(inter, kGatedCols) * 32 > UINT32_MAX) best.us = INFINITY;
   for (const ShapeCost& c : kGatedShapes) {
     if (wide_gated(m) && c.shape.mt > 2) continue;
     const int64_t tiles = ceil_div(m, 32 * c.shape.mt) * ceil_div(inter, kGatedCols);
