@@ -8,7 +8,7 @@
 //   gated MLP  h = silu(x Wg^T) (x Wu^T) in fp32, quantised, times Wd^T
 // The weights are the reference's block-FP8 linears' (qwen3_8/fp8_linear.py:12-212),
 // the block its Qwen3_8MLP (qwen3_8/mlp.py:9-54).  A scale per block instead of
-// one per tensor (fp8_linear.hip) makes a row's result depend on that row alone
+// one per tensor (fp8_linear.hip) keeps a row's result free of the other rows' values
 // and needs no pass over the whole tensor before the first value is written, so
 // the quantisation folds into whatever produces the values.
 #include <algorithm>
