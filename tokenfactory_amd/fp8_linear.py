@@ -384,9 +384,21 @@ class Fp8Linear(nn.Module):
         full = full[: self.out_features, : self.in_features]
         return (self.weight.to(torch.float32) * full).to(target_dtype)
 
-    def forward(self, x: torch.Tensor, x_amax: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, x_amax: Optional[torch.Tensor] = None,
+                x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x_amax``: optional max ``|x|`` from x's producer (see
-        ``quantize_activations``); the result does not change."""
+        ``quantize_activations``); the result does not change.  ``x_scale``: x is
+        float8_e4m3fn with a scale per row and 128 columns (``quantize_blocks``,
+        ``add_rms_norm(..., quantize=True)``), multiplied by ``block_scaled_linear``."""
+        if x_scale is not None:
+            if x_amax is not None:
+                raise ValueError("Fp8Linear: an amax goes with an x that is not quantised")
+            if (self.block_h, self.block_w) != (128, 128):
+                raise NotImplementedError(f"Fp8Linear: quantised x and weight blocks of "
+                                          f"{self.block_h} x {self.block_w} (128 x 128)")
+            from .block_fp8 import block_scaled_linear   # (it imports this module)
+            return block_scaled_linear(x, self.weight, self.weight_scale_inv, self.bias,
+                                       x_scale=x_scale)
         return block_fp8_linear(x, self.weight, self.weight_scale_inv, self.bias,
                                 self.block_h, self.block_w, x_amax=x_amax)
 
