@@ -348,9 +348,11 @@ def launching(device, stream):
 def refuse_gradients(fn: str, *tensors) -> None:
     """For entry points that record no gradients: raises where autograd would record
     one of an operand (None: absent)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{fn} records no gradients: call it under torch.no_grad() or "
-                                  "with detached operands")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{fn} records no gradients: call it under "
+                                          "torch.no_grad() or with detached operands")
 
 
 def plan_device_capacity(total_tokens, batch_size, num_q_heads, num_kv_heads) -> int:
