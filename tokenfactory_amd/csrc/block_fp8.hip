@@ -92,11 +92,12 @@ constexpr int kGroupM = 8;            // m-tiles per group of the XCD tile order
 // As fp8_linear.hip's tile: a workgroup of 2 x WN waves owns 32 MT activation
 // rows x 64 WN weight rows, a wave 16 MT x 64 of them in 4 x MT 16x16 tiles of
 // the transposed product D[n][m].  Large products (8192 rows times 5120 x 2 x 17408:
-// 1240 us = 2.36 PFLOP/s) have the MFMA busy 58 % of the time at the 1.9 GHz that
-// the power allows: MFMA and fold alone take 763 us, with the operands' way from LDS
-// 985, the staging alone 955 (81 % of its requests hit L2).  Small ones are bound by
-// the 36 to 60 GB/s that a CU's loads into LDS bring in, whatever their depth: 48
-// rows 48.7 us for 178 MB of weights, 3.7 TB/s on the 136 CUs that have a tile.
+// 1265 us in a kernel trace = 2.31 PFLOP/s) have the MFMA busy 58 % of the time at the
+// 1.9 GHz that the power allows: of an earlier build's 1273 us MFMA and fold alone took
+// 763, with the operands' way from LDS 985, the staging alone 955 (81 % of its requests
+// hit L2).  Small ones are bound by the 36 to 60 GB/s that a CU's loads into LDS bring
+// in, whatever their depth: 48 rows 48.7 us for 178 MB of weights, 3.7 TB/s on the 136
+// CUs that have a tile.
 template <int MT, int WN, int STAGES>
 struct BlockTile {
   static constexpr int kThreads = 2 * kWave * WN;
@@ -286,9 +287,9 @@ block_gemm_kernel(BlockGemmArgs a) {
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // A slice's loads start at the step that frees its stage: kAtStep of x there,
-  // kSpread per row after it (5120 x 2 x 17408 columns at 8192 rows: 1217 us; all three a
-  // row from the next slice on 1273, two barriers a slice to free the weights' part
-  // of a stage sooner 1231).
+  // kSpread per row after it (5120 x 2 x 17408 columns at 8192 rows, timed beside each
+  // other: 1217 us; all three a row from the next slice on 1273, two barriers a slice to
+  // free the weights' part of a stage sooner 1231).
   constexpr int kInLast = MT > 1 ? (kAtStep < T::kXInst ? kAtStep : T::kXInst) : T::kLoads;
   int kfill;
   // Slices past the last are never used; their stage is refilled with the last

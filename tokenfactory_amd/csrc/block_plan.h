@@ -12,9 +12,11 @@ namespace tfa {
 // of the small ones share a CU and take 1.5 times as long), a split adds a
 // launch and its partials' way through memory.  Fitted to a sweep of every shape
 // and 1 to 16 splits over 24 numbers of rows from 17 to 8192 at six products (640
-// to 12288 columns, K 2176 to 17408) and four gated ones: the choice is within
-// 10 % of the sweep's best everywhere and 0.3 % on average.  What the rarer shapes
-// are for: without 192 rows x 128 columns 333 x 5120 x 12288 takes 49.9 us for 37.6,
+// to 12288 columns, K 2176 to 17408) and four gated ones; with the present kernels
+// the same sweep finds the choice 1.3 % behind the best of 144 products on average and
+// 13 % at most (3000 x 5120 x 2592: 57.4 us for 50.8), 0.2 % and 8 % for 96 gated
+// ones.  The estimates only rank the shapes: the wide forms take longer than theirs
+// (48 x 5120 x 2 x 17408 33 us, measured 48).  What the rarer shapes are for: without 192 rows x 128 columns 333 x 5120 x 12288 takes 49.9 us for 37.6,
 // without 128 x 256 1500 x 5120 x 17408 149.8 for 131.7.  A split is taken of the
 // tiles behind the last full round only: with every tile whole 4096 x 5120 x 17408
 // takes 357 us for 318 (256 tiles whole, 64 by 4 workgroups each), 1300 x 12288 x
@@ -60,9 +62,10 @@ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // 13 bits below the largest of its eight (1.5e-5 of a sum of Gaussian values, 1e-4
 // where a few channels are large), which rounding h to e4m3 turns into whole steps
 // of the values next to a border: the block's output is 0.23 % off instead of 0.17 %
-// (the bf16 rounding alone), single rows 0.4 %.  Up to 64 rows the staging takes
-// as long as the wider MFMAs (48 rows of 5120 x 17408: 72 us both ways; 24.0 and
-// 25.2 for 2176 columns); at 200 rows of 2048 x 5120 they would cost 5 of 29 us.
+// (the bf16 rounding alone), single rows 0.4 %.  Up to 64 rows the staging hides most
+// of the wider MFMAs (block of 5120 x 17408 at 48 rows 76.3 us for 74.0, at 64 78.1 for
+// 76.3; of 5120 x 2176 at 48 25.5 for 23.2); at 200 rows of 2048 x 5120 they would cost
+// 5 of 29 us.
 constexpr int64_t kWideRows = 64;
 inline bool wide_gated(int64_t m) { return m <= kWideRows; }
 
