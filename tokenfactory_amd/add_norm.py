@@ -47,8 +47,11 @@ def _clash(r: torch.Tensor, t: Optional[torch.Tensor]) -> bool:
         return False
     if t.shape != r.shape:
         return True
-    if t.stride() == r.stride() and t.dtype == r.dtype and off == 0:
+    strides = zip(t.shape, t.stride(), r.stride())     # (a single row's says nothing)
+    if off == 0 and t.dtype == r.dtype and all(n == 1 or a == b for n, a, b in strides):
         return False
+    if t.shape[0] == 1:
+        return True
     size = r.element_size()
     row, width = r.stride(0) * size, r.shape[1] * size
     if t.stride(1) == 1 and t.stride(0) * t.element_size() == row:
