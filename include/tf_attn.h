@@ -572,7 +572,8 @@ int64_t tf_fp8_linears_workspace_bytes(int64_t m, const tf_fp8_mat* mats, int32_
  * tf_gated_mlp: out = h^ Wd^T with h = silu(x Wg^T) * (x Wu^T) in fp32 and h^ its
  * block-quantised form (qwen3_8/mlp.py:9-54).  Where the fp8 MFMA adds gate and up (above
  * 64 rows), its cut moves values of h next to a border of e4m3 by a step: the output is
- * some 0.23 % off its formula in the norm where rounding it to bf16 alone is 0.17 %.
+ * some 0.23 % off its formula in the norm where rounding it to bf16 alone is 0.17 %
+ * (0.36 % was seen where a few channels of x are far larger than the rest).
  * mats: a host array of three, read during the call: gate and up, n = inter (a
  * multiple of 16) over hidden (a multiple of 16) columns, their out and bias unused;
  * down, any n over inter columns, with out and optional bias.  x as in tf_block_linear.

@@ -64,8 +64,8 @@ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // of the values next to a border: the block's output is 0.23 % off instead of 0.17 %
 // (the bf16 rounding alone), single rows 0.4 %.  Up to 64 rows the staging hides most
 // of the wider MFMAs (block of 5120 x 17408 at 48 rows 76.3 us for 74.0, at 64 78.1 for
-// 76.3; of 5120 x 2176 at 48 25.5 for 23.2); at 200 rows of 2048 x 5120 they would cost
-// 5 of 29 us.
+// 76.3; of 5120 x 2176 at 48 25.5 for 23.2).  Above, they would take 112 us for 84 at 65
+// rows of 5120 x 17408, 37 for 31 at 200 of 5120 x 2176.
 constexpr int64_t kWideRows = 64;
 inline bool wide_gated(int64_t m) { return m <= kWideRows; }
 
