@@ -63,3 +63,12 @@ def test_plain_projections_are_read():
     handle.remove()
     with pytest.raises(ValueError):     # (the tensors lie on the CPU)
         mlp(torch.zeros((2, 256), dtype=torch.bfloat16))
+
+
+def test_a_loaders_parameter_class_is_read():
+    """A weight is read where it lies, whatever class of parameter holds it."""
+    mlp = GatedMLP(config(intermediate_size=512))
+    loaded = type("Loaded", (nn.Parameter,), {})
+    mlp.up_proj.weight = loaded(mlp.up_proj.weight.data, requires_grad=False)
+    with pytest.raises(ValueError):     # (the tensors lie on the CPU)
+        mlp(torch.zeros((2, 256), dtype=torch.bfloat16))

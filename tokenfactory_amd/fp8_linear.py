@@ -239,18 +239,18 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor,
 
 
 def _unaltered(linear, kind) -> bool:
-    """Whether ``linear`` itself is ``kind`` and no more (no subclass of the module or of
-    its weight, replaced forward or hook of its own)."""
+    """Whether ``linear`` itself is ``kind`` and no more (no subclass, replaced forward or
+    hook of its own)."""
     return (type(linear) is kind and "forward" not in linear.__dict__
-            and type(linear._parameters.get("weight")) is nn.Parameter
             and not (linear._forward_hooks or linear._forward_pre_hooks
                      or linear._backward_hooks or linear._backward_pre_hooks))
 
 
 def _plain(linear, kind) -> bool:
     """Whether calling ``linear`` runs ``kind.forward`` on plain tensors and nothing
-    else."""
-    return _unaltered(linear, kind) and not nn.modules.module._has_any_global_hook()
+    else (no subclass of its weight, no global hook)."""
+    return (_unaltered(linear, kind) and type(linear._parameters.get("weight")) is nn.Parameter
+            and not nn.modules.module._has_any_global_hook())
 
 
 # Elements of x up to which the gate projections share a launch.  Above, the
