@@ -68,6 +68,6 @@ def test_autograd_sees_a_residual_summed_in_place(gpu):
     x = torch.ones((4, 256), dtype=torch.bfloat16, device=gpu)
     with torch.no_grad():
         _, r = add_rms_norm(x, residual, None, inplace=True)
-    assert r is residual and float(residual[0, 0]) == 3.0
+    assert r is residual and float(residual.detach()[0, 0]) == 3.0
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
