@@ -298,6 +298,37 @@ int32_t tf_attn_rows(
     void* workspace, int64_t workspace_bytes, int32_t num_workgroups, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
 
+/* tf_attn_shared: attention over parts of contexts, joined (a step whose requests
+ * share prefixes: their keys are read once for all of them).
+ * items: device int32 [n_items][8] = {b, tok0, n_tok, row0, k0, k1, pfx, pfx_tok},
+ * 16-byte aligned, at most 2048: rows row0 .. row0 + 16 row_groups - 1 of the n_tok * G
+ * rows (row = t * G + h) of the tokens at tokens[tok0] over keys [k0, k1) of request
+ * b's table row; k1 < 0: up to the last key that its rows see.  The first n_shared
+ * items are shared parts, whose tokens may be of any requests; the others are the
+ * requests' own, one request's tokens each, and say which output rows there are:
+ * pfx = the first item of the shared part of that request (-1: none; its items follow
+ * each other, row0 a multiple of 16 row_groups), pfx_tok = where the request's tokens
+ * start among that part's.  b = -1 is padding.
+ * tokens: device int32 [..][4] = {q row, request, tokens of the request that follow, 0}:
+ * a token sees keys up to seq_lens[request] - 1 - that many.
+ * slot_rows: the most rows that any item uses.  The other arguments are
+ * tf_attn_decode's; rows that see no key are zeros.  Workspace:
+ * tf_attn_shared_workspace_bytes of the same sizes, 16-byte aligned; calls that overlap
+ * in time must not share it. */
+int64_t tf_attn_shared_workspace_bytes(int32_t n_items, int32_t row_groups, int32_t slot_rows,
+                                       int32_t num_q_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t kv_dtype);
+
+int32_t tf_attn_shared(
+    const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+    int64_t pool_slots, int32_t kv_dtype, const float* k_scale, const float* v_scale,
+    const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
+    const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* items,
+    int32_t n_items, int32_t n_shared, const int32_t* tokens, int32_t row_groups,
+    int32_t slot_rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
+    int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
+
 /* tf_attn_plan_blocks: the row blocks of a step, built on the device from its
  * work list and decode items (of either planner, padding included): the decode
  * items, and the requests of at most max_rows rows (ext * G), become blocks of 16

@@ -8,6 +8,8 @@ Public surface (the reference's names and contracts, see each module):
   ``_slot_based_attention`` signatures
 * ``slot_based_attention`` / ``write_kv`` / ``gather_kv`` /
   ``qk_norm_rope_kv_write`` - the kernels' Python entry points
+* ``shared_prefix_attention`` / ``SharedPrefixes`` - attention of a step whose requests
+  share prefixes, read once per group
 * ``LinearAttention`` / ``gdn_decode_step`` - Gated DeltaNet decode step
   (``qwen3_8/linear_attention.py``)
 * ``Fp8Linear`` / ``block_fp8_linear`` - block-FP8 linear (``qwen3_8/fp8_linear.py``,
@@ -21,6 +23,7 @@ Public surface (the reference's names and contracts, see each module):
 from .forward_batch import ForwardBatch
 from .attention import gather_kv, qk_norm_rope_kv_write, slot_based_attention, write_kv
 from .kv_pool import FullAttnKVPool
+from .shared_prefix import SharedPrefixes, shared_prefix_attention
 from .fp8_linear import Fp8Linear, block_fp8_linear
 from .full_attention import FullAttention
 from .linear_attention import LinearAttention, gdn_decode_step
@@ -35,6 +38,7 @@ __all__ = [
     "FullAttention",
     "GatedMLP",
     "LinearAttention",
+    "SharedPrefixes",
     "add_rms_norm",
     "block_fp8_linear",
     "block_scaled_linear",
@@ -43,6 +47,7 @@ __all__ = [
     "gather_kv",
     "qk_norm_rope_kv_write",
     "quantize_blocks",
+    "shared_prefix_attention",
     "slot_based_attention",
     "write_kv",
 ]

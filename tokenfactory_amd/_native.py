@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libtf_attn.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 TF_DTYPE_BF16 = 0
 TF_DTYPE_FP8_E4M3 = 1
@@ -115,6 +115,20 @@ SIGNATURES = {
         _p, _p,
     ]),
     "tf_attn_extend_split_workspace_bytes": (_i64, []),
+    "tf_attn_shared_workspace_bytes": (_i64, [_i32] * 7),
+    "tf_attn_shared": (_i32, [
+        _p, _i64,
+        _p, _p, _i64, _i32, _p, _p,
+        _p, _i64, _i64, _i64,
+        _p, _p,                        # req_pool_indices, seq_lens
+        _p, _i32, _i32, _p,            # items, n_items, n_shared, tokens
+        _i32, _i32,                    # row_groups, slot_rows
+        _i32, _i32, _i32, _f32,
+        _p, _i64,
+        _p, _i64,                      # workspace, workspace_bytes
+        _p, _i64, _i64,
+        _p, _p,
+    ]),
     "tf_attn_plan_decode_items": (_i32, [_p, _i32, _p, _p, _i32]),
     "tf_req_to_token_sync": (_i32, [
         _p, _i64, _i64, _i64,          # req_to_token, rtt_rows, rtt_row_stride, rtt_cols

@@ -463,6 +463,41 @@ def _check_inputs(q, k_buf, v_buf, batch):
                          f"{rtt.shape[1]}")
 
 
+def _pool_scales(q, kv_dtype: int, k_scale, v_scale):
+    """The scales as the entry points take them (None for a bf16 pool)."""
+    if kv_dtype != _native.TF_DTYPE_FP8_E4M3:
+        return None, None
+    if k_scale is None or v_scale is None:
+        raise ValueError("an fp8 KV pool needs k_scale and v_scale")
+    return tuple(s.to(device=q.device, dtype=torch.float32).reshape(1).contiguous()
+                 for s in (k_scale, v_scale))
+
+
+def _output(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 \
+            or out.stride(1) != q.shape[2]:
+        raise ValueError("out must match q's shape/dtype with dense heads and dims")
+    return out
+
+
+def _epilogue(q, gate, out_amax) -> tuple:
+    """The entry points' trailing arguments: gate, its strides, out_amax."""
+    if gate is not None and (
+            gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != q.device
+            or gate.stride(2) != 1 or gate.stride(0) % 8 or gate.stride(1) % 8
+            or gate.data_ptr() % 16):
+        raise ValueError("gate must be a bf16 [T, Hq, D] view on q's device with "
+                         "contiguous dims, strides in multiples of 8 and a 16-byte "
+                         "aligned start")
+    if out_amax is not None and (out_amax.dtype != torch.int32 or out_amax.numel() != 1
+                                 or out_amax.device != q.device):
+        raise ValueError("out_amax must be a 1-element int32 tensor on q's device")
+    strides = (0, 0) if gate is None else (gate.stride(0), gate.stride(1))
+    return (_ptr(gate), *strides, _ptr(out_amax))
+
+
 class _DevPtr:
     """A raw device address posing as a tensor for ``_ptr``."""
 
@@ -516,40 +551,16 @@ class SlotAttentionCall:
         if scaling is None:
             scaling = head_dim ** -0.5
         kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
-        if kv_dtype == _native.TF_DTYPE_FP8_E4M3:
-            if k_scale is None or v_scale is None:
-                raise ValueError("an fp8 KV pool needs k_scale and v_scale")
-            with on_stream(stream):   # conversions run, and live, where they are read
-                k_scale = k_scale.to(device=q.device, dtype=torch.float32).reshape(1).contiguous()
-                v_scale = v_scale.to(device=q.device, dtype=torch.float32).reshape(1).contiguous()
-        else:
-            k_scale = v_scale = None
+        with on_stream(stream):   # conversions run, and live, where they are read
+            k_scale, v_scale = _pool_scales(q, kv_dtype, k_scale, v_scale)
         if q.stride(2) != 1 or q.stride(1) != head_dim:
             with on_stream(stream):
                 q = q.contiguous()
-        if out is None:
-            out = torch.empty((n_tok, n_q, head_dim), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 \
-                or out.stride(1) != head_dim:
-            raise ValueError("out must match q's shape/dtype with dense heads and dims")
-
-        if gate is not None:
-            if gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != q.device \
-                    or gate.stride(2) != 1 or gate.stride(0) % 8 or gate.stride(1) % 8 \
-                    or gate.data_ptr() % 16:
-                raise ValueError("gate must be a bf16 [T, Hq, D] view on q's device with "
-                                 "contiguous dims, strides in multiples of 8 and a 16-byte "
-                                 "aligned start")
-            self._epilogue_args = (gate.data_ptr(), gate.stride(0), gate.stride(1))
-        else:
-            self._epilogue_args = (None, 0, 0)
-        self.gate = gate
-        if out_amax is not None and (out_amax.dtype != torch.int32 or out_amax.numel() != 1
-                                     or out_amax.device != q.device):
-            raise ValueError("out_amax must be a 1-element int32 tensor on q's device")
-        self.out_amax = out_amax
+        out = _output(q, out)
         # the launches' trailing arguments: gate, its strides, out_amax
-        self._epilogue_args = self._epilogue_args + (_ptr(out_amax),)
+        self._epilogue_args = _epilogue(q, gate, out_amax)
+        self.gate = gate
+        self.out_amax = out_amax
 
         bsz = batch.batch_size
         ext_lens = [int(e) for e in batch.extend_lens]

@@ -1,0 +1,531 @@
+// Attention over parts of contexts, joined: steps whose requests share a prefix
+// (tf_attn_shared), its keys read once for all of them.
+//
+// The softmax over a row's keys splits at any key: with m_i, l_i and o_i the maximum,
+// the sum of 2^(s - m_i) and the sum of 2^(s - m_i) V over part i,
+//   m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m) / l.
+// Part items are (query tokens, keys [k0, k1) of one request's table row): a group's
+// shared keys are an item with the tokens of all of its requests, the keys behind them
+// one item per request, or several where it has more rows than a unit.  Every item
+// leaves fp32 partials, which part_merge_kernel joins.
+//
+// part_stream_kernel is the decode kernel's scheme (decode.hip: persistent workgroups
+// that own equal shares of the tiles of all units, unit = (item, kv head)), with the
+// tokens of an item looked up in a list, since a group's requests lie anywhere in the
+// batch.  Bound by HBM as that kernel: a key's K and V rows are read by one unit per 16
+// or 32 query rows.
+#include <math.h>
+
+#include "attn_row.h"
+#include "prefix_attn.h"
+#include "stream_tile.h"
+#include "tf_common.h"
+#include "tf_internal.h"
+
+namespace tfa {
+namespace {
+
+// The context length of a request, clamped to its table row.
+__device__ __forceinline__ int context_len(const PartArgs& a, int b) {
+  const int64_t len = min(a.seq_lens[b], a.rtt_cols);
+  return len > 0 ? (int)len : 0;
+}
+
+// Keys that token t of an item sees, counted from key 0.
+__device__ __forceinline__ int token_seen(const PartArgs& a, const PartTok& t) {
+  return context_len(a, t.b) - t.back;
+}
+
+// Keys of an item: a shared part's own bounds (a row of a shorter context masks what
+// lies behind it), else up to the last key that its last row sees.
+template <class C>
+__device__ __forceinline__ int part_keys(const PartArgs& a, const PartItem& it) {
+  if (it.b < 0) return 0;
+  int end;
+  if (it.k1 >= 0) {
+    end = min((int64_t)it.k1, a.rtt_cols);
+  } else {
+    const int last = min(it.row0 + C::kRows, it.n_tok * a.group) - 1;
+    end = token_seen(a, a.toks[it.tok0 + last / a.group]);
+  }
+  return max(0, end - it.k0);
+}
+
+template <class C>
+__global__ void __launch_bounds__(kWaves * kWave, C::NG == 1 || C::DP == 128 ? 2 : 1)
+part_stream_kernel(PartArgs a) {
+  __shared__ DecodeSmem<C> sm;
+  const int D = C::OTHER ? a.head_dim : C::DP;
+  const int row_bytes = C::FP8 ? D : 2 * D;
+  const int n_chunks = row_bytes / 16;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = wave_id();
+  const int g = lane >> 4;
+  const int n = lane & 15;
+
+  item_prefix(a.n_items, [&](int i) {
+    return (part_keys<C>(a, a.items[i]) + kTile - 1) / kTile;
+  }, sm.ipre, sm.wsum);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.n_items; i += kWaves * kWave) a.ipre[i] = sm.ipre[i];
+  const int64_t N = (int64_t)a.hkv * sm.ipre[a.n_items];
+  const int P = (int)min<int64_t>(a.n_blocks, N);   // (owners of a unit are consecutive)
+  if ((int)blockIdx.x >= P) return;
+  const int64_t x_end = (int64_t)(blockIdx.x + 1) * N / P;
+  int64_t x = (int64_t)blockIdx.x * N / P;
+
+  const float sl2 = a.scale_log2 * (C::FP8 ? a.k_scale[0] : 1.f);
+  const int64_t slot_bytes = (int64_t)a.hkv * row_bytes;
+
+  int item = 0;   // the first whose tiles reach x
+  {
+    int lo = 0, hi = a.n_items - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)a.hkv * sm.ipre[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    item = lo;
+  }
+
+  while (x < x_end) {
+    // ---- the segment: unit (item, hk), tiles [t0, t1)
+    while ((int64_t)a.hkv * sm.ipre[item + 1] <= x) ++item;
+    const int Ti = sm.ipre[item + 1] - sm.ipre[item];
+    const int64_t r = x - (int64_t)a.hkv * sm.ipre[item];
+    const int hk = (int)(r / Ti);
+    const int t0 = (int)(r - (int64_t)hk * Ti);
+    const int t1 = (int)min<int64_t>(Ti, t0 + (x_end - x));
+    x += t1 - t0;
+
+    const PartItem im = a.items[item];
+    const int L = part_keys<C>(a, im);
+    const int n_rows = im.n_tok * a.group - im.row0;       // of kRows
+    const int n_groups = min((n_rows + 15) / 16, C::NG);
+    const int64_t row = clamp_i64(a.rpi[im.b], 0, a.rtt_rows - 1);
+    const int64_t* rtt = a.rtt + row * a.rtt_stride + im.k0;
+    const uint8_t* kbase = a.k_pool + (int64_t)hk * row_bytes;
+    const uint8_t* vbase = a.v_pool + (int64_t)hk * row_bytes;
+    // Row n of group q: its token and head, and how many of the part's keys it sees.
+    auto row_of = [&](int q, int& qrow, int& hq, int& seen) {
+      const int rho = im.row0 + min(16 * q + n, n_rows - 1);
+      const int t = rho / a.group;
+      const PartTok tok = a.toks[im.tok0 + t];
+      qrow = tok.qrow;
+      hq = hk * a.group + rho - t * a.group;
+      seen = token_seen(a, tok) - im.k0;
+      return 16 * q + n < n_rows;
+    };
+    int seen[C::NG];
+#pragma unroll
+    for (int q = 0; q < C::NG; ++q) {
+      int qrow, hq;
+      row_of(q, qrow, hq, seen[q]);
+    }
+
+    WaveState<C> st;
+    reset_state<C>(st);
+    for (int sub = t0; sub < t1; sub += kMaxChunk / kTile) {
+      const int c0 = sub * kTile;
+      const int n_loc = min(L, min(t1, sub + kMaxChunk / kTile) * kTile) - c0;
+      const int n_tiles = (n_loc + kTile - 1) / kTile;
+      // ---- the slot ids (and, once per segment, the Q^T fragments)
+      __syncthreads();
+      for (int i = tid; i < n_loc; i += kWaves * kWave)
+        sm.u.loop.slots[i] = (int32_t)pool_row(rtt[c0 + i], a.pool_slots, false);
+      if (sub == t0) {
+#pragma unroll
+        for (int q = 0; q < C::NG; ++q) {
+          if (w != q % kWaves || q >= n_groups) continue;
+          int qrow, hq, s;
+          const bool ok = row_of(q, qrow, hq, s);
+          const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+          for (int kk = 0; kk < C::kSteps; ++kk) {
+            const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
+            sm.qfrag[q][kk][lane] =
+                ok && (!C::OTHER || d0 < D) ? ld_g16(qp + d0) : u32x4{0u, 0u, 0u, 0u};
+          }
+        }
+      }
+      __syncthreads();
+
+      // ---- this wave's tiles, loads a tile ahead (see decode_kernel)
+      int it = w;
+      if (it < n_tiles) {
+        u32x4 qf[C::kSteps];
+        if (C::NG == 1) {
+#pragma unroll
+          for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.qfrag[0][kk][lane];
+        }
+        KBuf<C> kb;
+        VBuf<C> vb;
+        const int32_t* slots = sm.u.loop.slots;
+        u32x4* ks = sm.u.loop.kstage[w];
+        auto scores = [&](int it, u32x2 (&pt)[C::NG], u32x2 (&pl)[C::NG][2]) {
+          u32x4 kf[C::kSteps];
+          k_frags<C>(ks, g, n, kf);
+#pragma unroll
+          for (int q = 0; q < C::NG; ++q) {
+            if (C::NG > 1) {
+              if (q >= n_groups) break;
+#pragma unroll
+              for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.qfrag[q][kk][lane];
+            }
+            const int lim = min(n_loc, seen[q] - c0);
+            pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q],
+                                  [](const float (&)[4]) {});
+          }
+        };
+        u32x2 pt[C::NG], pl[C::NG][2];
+        issue_rows<C>(kb.k, slots, it, n_loc, g, n, kbase, slot_bytes, n_chunks);
+        issue_rows<C>(vb.v, slots, it, n_loc, g, n, vbase, slot_bytes, n_chunks);
+        for (; it + kWaves < n_tiles; it += kWaves) {
+          stage_k<C>(kb, ks, g, n);
+          __builtin_amdgcn_sched_barrier(0);
+          issue_rows<C>(kb.k, slots, it + kWaves, n_loc, g, n, kbase, slot_bytes, n_chunks);
+          __builtin_amdgcn_sched_barrier(0);
+          scores(it, pt, pl);
+          pv<C>(vb, pt, pl, st, n_groups);
+          __builtin_amdgcn_sched_barrier(0);
+          issue_rows<C>(vb.v, slots, it + kWaves, n_loc, g, n, vbase, slot_bytes, n_chunks);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        stage_k<C>(kb, ks, g, n);
+        scores(it, pt, pl);
+        pv<C>(vb, pt, pl, st, n_groups);
+      }
+    }
+
+#pragma unroll
+    for (int q = 0; q < C::NG; ++q) {
+      st.l[q] += __shfl_xor(st.l[q], 16, kWave);
+      st.l[q] += __shfl_xor(st.l[q], 32, kWave);
+    }
+    block_merge<C>(sm.u.merge, w, lane, st, n_groups);
+    if (w != 0) continue;
+    // Partials of (workgroup, unit), a row's dims side by side.  Lane (g, n) holds of
+    // row n the dims 128 s + 32 g + 8 r + e (bf16: accumulator 8 s + e) or 64 g + 16 r
+    // + e (fp8), four neighbours per store.
+    const int64_t slot = (int64_t)blockIdx.x + (int64_t)item * a.hkv + hk;
+#pragma unroll
+    for (int q = 0; q < C::NG; ++q) {
+      if (16 * q + n >= n_rows) continue;
+      const int64_t pr = slot * a.slot_rows + 16 * q + n;
+      float* po = a.part_o + pr * C::DP;
+#pragma unroll
+      for (int i = 0; i < C::kAcc; i += 4)
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr)
+          *reinterpret_cast<f32x4*>(po + (C::FP8 ? 64 * g + 16 * rr + i
+                                                 : 128 * (i >> 3) + 32 * g + 8 * rr + (i & 7))) =
+              f32x4{st.acc[q][i][rr], st.acc[q][i + 1][rr], st.acc[q][i + 2][rr],
+                    st.acc[q][i + 3][rr]};
+      if (g == 0) a.part_ml[pr] = float2{st.m[q], st.l[q]};
+    }
+  }
+}
+
+// Joins the parts of every row: WPR waves per row take its partials in turn, kAhead of
+// them in flight per wave, lane l dims 4 l .. 4 l + 3.  Bound by the latency of those
+// reads (and by their bytes where a prefix is cut into many pieces).  A row whose sum
+// is not finite is done again over the keys it sees: an MFMA multiplies V rows that a
+// row does not see by zero, which is NaN for an infinite or NaN value there.
+// A row without a visible key is zeros.
+constexpr int kMergeWaves = 8;
+constexpr int kAhead = 8;
+
+// Owners of a streamed unit's partials: slots first .. first + count - 1.
+struct Owners {
+  int64_t first;
+  int count;
+};
+__device__ __forceinline__ Owners unit_owners(const PartArgs& a, int item, int hk) {
+  const int before = a.ipre[item], Ti = a.ipre[item + 1] - before, total = a.ipre[a.n_items];
+  if (Ti == 0) return Owners{0, 0};
+  const int64_t N = (int64_t)a.hkv * total;
+  const int64_t p = (int64_t)a.hkv * before + (int64_t)hk * Ti;
+  const int P = (int)min<int64_t>(a.n_blocks, N);
+  const int b0 = owner_of(p, N, P);
+  return Owners{b0 + (int64_t)item * a.hkv + hk, owner_of(p + Ti - 1, N, P) - b0 + 1};
+}
+
+template <int DP, bool FP8, int WPR>
+__global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArgs a) {
+  constexpr int kRows = kMergeWaves / WPR;   // rows of the unit side by side
+  __shared__ f32x4 so[kMergeWaves][kWave];
+  __shared__ float sm_m[kMergeWaves], sm_l[kMergeWaves];
+  const int lane = threadIdx.x & 63;
+  const int w = wave_id();
+  const int item = a.own0 + (int)(blockIdx.x / a.hkv);
+  const int hk = (int)(blockIdx.x % a.hkv);
+  const PartItem im = a.items[item];
+  const int n = (int)blockIdx.y * kRows + w / WPR;     // the wave's row of the unit
+  const int n_rows = im.b < 0 ? 0 : min(im.n_tok * a.group - im.row0, a.unit_rows);
+  if ((int)blockIdx.y * kRows >= n_rows) return;
+  bool write = n < n_rows;
+
+  const int rho = im.row0 + min(n, n_rows - 1);
+  const int t = rho / a.group;
+  const PartTok tok = a.toks[im.tok0 + t];
+  const int hq = hk * a.group + rho - t * a.group;
+  const int D = a.head_dim;
+  const bool lane_in = 4 * lane < DP, lane_out = 4 * lane < D;
+  u32x2 gv = {0u, 0u};
+  if (write && a.gate && lane_out)
+    gv = ld_g8(a.gate + (int64_t)tok.qrow * a.gate_stride + (int64_t)hq * a.gate_hstride +
+               4 * lane);
+
+  // Partials: the request's own part, then the shared one's.
+  const Owners own = unit_owners(a, item, hk);
+  Owners pre{0, 0};
+  int pre_row = 0;
+  if (im.pfx >= 0) {
+    const int rp = (im.pfx_tok + t) * a.group + rho - t * a.group;
+    pre = unit_owners(a, im.pfx + rp / a.unit_rows, hk);
+    pre_row = rp % a.unit_rows;
+  }
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int parts = write ? own.count + pre.count : 0;
+  for (int k0 = w % WPR; k0 < parts; k0 += WPR * kAhead) {
+    f32x4 o[kAhead];
+    float2 ml[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = min(k0 + WPR * k, parts - 1);
+      const int64_t pr = i < own.count ? (own.first + i) * a.slot_rows + n
+                                       : (pre.first + i - own.count) * a.slot_rows + pre_row;
+      ml[k] = a.part_ml[pr];
+      o[k] = lane_in ? reinterpret_cast<const f32x4*>(a.part_o + pr * DP)[lane]
+                     : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k0 + WPR * k >= parts) ml[k] = float2{-INFINITY, 0.f};   // a repeat of the last one
+      mn = fmaxf(mn, ml[k].x);
+    }
+    // (NaN rows have a maximum of -inf and a NaN sum: the sum goes through)
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float a1 = fast_exp2(m - ref);
+    acc *= a1;
+    l *= a1;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float a2 = fast_exp2(ml[k].x - ref);
+      if (k0 + WPR * k < parts) acc += o[k] * a2;
+      l += ml[k].y * a2;
+    }
+    m = mn;
+  }
+  if (WPR > 1) {
+    so[w][lane] = acc;
+    if (lane == 0) {
+      sm_m[w] = m;
+      sm_l[w] = l;
+    }
+    __syncthreads();
+    if (w % WPR) write = false;   // the row's first wave goes on alone
+    if (write) {
+#pragma unroll
+      for (int k = 1; k < WPR; ++k) {
+        const float m2 = sm_m[w + k], l2 = sm_l[w + k];
+        const float mn = fmaxf(m, m2);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float a1 = fast_exp2(m - ref), a2 = fast_exp2(m2 - ref);
+        acc = acc * a1 + so[w + k][lane] * a2;
+        l = l * a1 + l2 * a2;
+        m = mn;
+      }
+    }
+  }
+
+  uint32_t om = 0;
+  const float vscale = FP8 ? a.v_scale[0] : 1.f;
+  __bf16* orow = a.out + (int64_t)tok.qrow * a.out_stride + (int64_t)hq * D;
+  if (write && __ballot(not_finite(acc))) {
+    const int row_bytes = FP8 ? D : 2 * D;
+    const int seen = token_seen(a, tok);
+    RowState rs;
+    attend_row<FP8>(rs, a.q + (int64_t)tok.qrow * a.q_stride + (int64_t)hq * D,
+                    reinterpret_cast<uint32_t*>(&so[w][0]), D,
+                    a.rtt + clamp_i64(a.rpi[im.b], 0, a.rtt_rows - 1) * a.rtt_stride, 0, seen,
+                    a.pool_slots, false, a.k_pool + (int64_t)hk * row_bytes,
+                    a.v_pool + (int64_t)hk * row_bytes, (int64_t)a.hkv * row_bytes,
+                    a.scale_log2 * (FP8 ? a.k_scale[0] : 1.f), lane);
+    om = write_row(rs, seen > 0 ? vscale / rs.l : 0.f, D, orow,
+                   a.gate ? a.gate + (int64_t)tok.qrow * a.gate_stride +
+                                (int64_t)hq * a.gate_hstride
+                          : nullptr,
+                   lane);
+    write = false;
+  }
+  if (write && lane_out) {
+    const float inv = l > 0.f || l != l ? vscale / l : 0.f;
+    u32x2 o = {pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+    if (a.gate) {
+      o[0] = gate_pair(o[0], gv[0]);
+      o[1] = gate_pair(o[1], gv[1]);
+    }
+    om = max(max(o[0] & 0x7fffu, (o[0] >> 16) & 0x7fffu),
+             max(o[1] & 0x7fffu, (o[1] >> 16) & 0x7fffu));
+    *reinterpret_cast<u32x2*>(orow + 4 * lane) = o;
+  }
+  amax_commit(a.amax, om);
+}
+
+// Kernel shape and workspace of a call.
+struct PartPlan {
+  bool fp8, narrow, other;
+  int32_t unit_rows;    // 16 or 32
+  int32_t n_blocks;     // persistent workgroups
+  int64_t ipre_bytes, ml_bytes, o_bytes;
+  int64_t total() const { return ipre_bytes + ml_bytes + o_bytes; }
+};
+
+int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t slot_rows,
+                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
+                   PartPlan* p) {
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
+    return fail(TF_ERR_INVALID, "%s: num_q_heads=%d not a multiple of num_kv_heads=%d", fn,
+                num_q_heads, num_kv_heads);
+  if (kv_dtype != TF_DTYPE_BF16 && kv_dtype != TF_DTYPE_FP8_E4M3)
+    return fail(TF_ERR_UNSUPPORTED, "%s: kv_dtype=%d", fn, kv_dtype);
+  p->fp8 = kv_dtype == TF_DTYPE_FP8_E4M3;
+  if (head_dim < 8 || head_dim > 256 || head_dim % (p->fp8 ? 16 : 8))
+    return fail(TF_ERR_UNSUPPORTED,
+                "%s: head_dim=%d (a multiple of 8, for fp8 pools of 16, up to 256)", fn, head_dim);
+  if (n_items < 0 || (row_groups != 1 && row_groups != 2) || slot_rows < 1 ||
+      slot_rows > 16 * row_groups)
+    return fail(TF_ERR_INVALID, "%s: n_items=%d row_groups=%d slot_rows=%d", fn, n_items,
+                row_groups, slot_rows);
+  if (n_items > kMaxItems)
+    return fail(TF_ERR_UNSUPPORTED, "%s: %d parts in one call (at most %d)", fn, n_items,
+                kMaxItems);
+  p->other = head_dim != 256;
+  p->narrow = head_dim <= 128 && !p->fp8;
+  p->unit_rows = 16 * row_groups;
+  p->n_blocks = device_cu_count() * (p->narrow ? 2 : 1);
+  const int64_t rows = (p->n_blocks + (int64_t)n_items * num_kv_heads) * slot_rows;
+  p->ipre_bytes = ((int64_t)(n_items + 1) * 4 + 255) / 256 * 256;
+  p->ml_bytes = (rows * 8 + 255) / 256 * 256;
+  p->o_bytes = rows * (p->narrow ? 128 : 256) * 4;
+  return TF_OK;
+}
+
+template <class C>
+void launch_stream(const PartArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((part_stream_kernel<C>), dim3((unsigned)a.n_blocks), dim3(kWaves * kWave), 0,
+                     s, a);
+}
+
+template <int NG>
+void launch_stream_groups(const PartArgs& a, const PartPlan& p, hipStream_t s) {
+  if (p.narrow) return launch_stream<Cfg<128, false, NG, true, true>>(a, s);
+  if (p.other && p.fp8) return launch_stream<Cfg<256, true, NG, true, true>>(a, s);
+  if (p.other) return launch_stream<Cfg<256, false, NG, true, true>>(a, s);
+  if (p.fp8) return launch_stream<Cfg<256, true, NG, false, true>>(a, s);
+  return launch_stream<Cfg<256, false, NG, false, true>>(a, s);
+}
+
+template <int WPR>
+void launch_merge(const PartArgs& a, const PartPlan& p, int n_own, int rows, hipStream_t s) {
+  const dim3 grid((unsigned)(n_own * a.hkv),
+                  (unsigned)((rows + kMergeWaves / WPR - 1) / (kMergeWaves / WPR)));
+  const dim3 block(kMergeWaves * kWave);
+  if (p.narrow)
+    hipLaunchKernelGGL((part_merge_kernel<128, false, WPR>), grid, block, 0, s, a);
+  else if (p.fp8)
+    hipLaunchKernelGGL((part_merge_kernel<256, true, WPR>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((part_merge_kernel<256, false, WPR>), grid, block, 0, s, a);
+}
+
+}  // namespace
+}  // namespace tfa
+
+extern "C" int64_t tf_attn_shared_workspace_bytes(int32_t n_items, int32_t row_groups,
+                                                  int32_t slot_rows, int32_t num_q_heads,
+                                                  int32_t num_kv_heads, int32_t head_dim,
+                                                  int32_t kv_dtype) {
+  using namespace tfa;
+  clear_error();
+  PartPlan p;
+  const int rc = make_part_plan("shared", n_items, row_groups, slot_rows, num_q_heads,
+                                num_kv_heads, head_dim, kv_dtype, &p);
+  return rc != TF_OK ? rc : p.total();
+}
+
+extern "C" int32_t tf_attn_shared(
+    const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+    int64_t pool_slots, int32_t kv_dtype, const float* k_scale, const float* v_scale,
+    const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
+    const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* items,
+    int32_t n_items, int32_t n_shared, const int32_t* tokens, int32_t row_groups,
+    int32_t slot_rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
+    int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream) {
+  using namespace tfa;
+  clear_error();
+  PartPlan p;
+  int rc = make_part_plan("shared", n_items, row_groups, slot_rows, num_q_heads, num_kv_heads,
+                          head_dim, kv_dtype, &p);
+  if (rc != TF_OK) return rc;
+  if (n_shared < 0 || n_shared > n_items)
+    return fail(TF_ERR_INVALID, "shared: %d of %d parts are shared", n_shared, n_items);
+  if (n_items == n_shared) return TF_OK;
+  rc = check_slot_call("shared", q, q_row_stride, k_pool, v_pool, pool_slots, kv_dtype, k_scale,
+                       v_scale, req_to_token, rtt_rows, rtt_row_stride, rtt_cols,
+                       req_pool_indices, seq_lens, 0, num_q_heads, head_dim, out, out_row_stride,
+                       gate, gate_row_stride, gate_head_stride, workspace, workspace_bytes,
+                       p.total());
+  if (rc != TF_OK) return rc;
+  if (!items || !tokens || !aligned16(items) || !aligned16(tokens))
+    return fail(TF_ERR_INVALID, "shared: items and tokens must be 16-byte aligned");
+  PartArgs a = {};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_stride = q_row_stride;
+  a.k_pool = static_cast<const uint8_t*>(k_pool);
+  a.v_pool = static_cast<const uint8_t*>(v_pool);
+  a.pool_slots = pool_slots;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.rtt = req_to_token;
+  a.rtt_rows = rtt_rows;
+  a.rtt_stride = rtt_row_stride;
+  a.rtt_cols = rtt_cols;
+  a.rpi = req_pool_indices;
+  a.seq_lens = seq_lens;
+  a.items = reinterpret_cast<const PartItem*>(items);
+  a.toks = reinterpret_cast<const PartTok*>(tokens);
+  a.n_items = n_items;
+  a.own0 = n_shared;
+  a.unit_rows = p.unit_rows;
+  a.slot_rows = slot_rows;
+  a.hkv = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.head_dim = head_dim;
+  a.n_blocks = p.n_blocks;
+  a.scale_log2 = scale * kLog2e;
+  a.out = static_cast<__bf16*>(out);
+  a.out_stride = out_row_stride;
+  a.gate = static_cast<const __bf16*>(gate);
+  a.gate_stride = gate_row_stride;
+  a.gate_hstride = gate_head_stride;
+  a.amax = out_amax;
+  char* ws = static_cast<char*>(workspace);
+  a.ipre = reinterpret_cast<int32_t*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ipre_bytes);
+  a.part_o = reinterpret_cast<float*>(ws + p.ipre_bytes + p.ml_bytes);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (row_groups == 1)
+    launch_stream_groups<1>(a, p, s);
+  else
+    launch_stream_groups<2>(a, p, s);
+  rc = launch_status("tf_attn_shared stream launch");
+  if (rc != TF_OK) return rc;
+  launch_merge<4>(a, p, n_items - n_shared, slot_rows, s);
+  return launch_status("tf_attn_shared merge launch");
+}

@@ -20,6 +20,16 @@ int device_cu_count();
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
+// The checks that the entry points of the streaming kernels share.
+int check_slot_call(const char* fn, const void* q, int64_t q_row_stride, const void* k_pool,
+                    const void* v_pool, int64_t pool_slots, int32_t kv_dtype, const float* k_scale,
+                    const float* v_scale, const int64_t* req_to_token, int64_t rtt_rows,
+                    int64_t rtt_row_stride, int64_t rtt_cols, const int64_t* req_pool_indices,
+                    const int64_t* seq_lens, int32_t seq_len_override, int32_t num_q_heads,
+                    int32_t head_dim, const void* out, int64_t out_row_stride, const void* gate,
+                    int64_t gate_row_stride, int64_t gate_head_stride, const void* workspace,
+                    int64_t workspace_bytes, int64_t need_bytes);
+
 // A block of query rows of one request for the streaming kernel (decode.hip):
 // rows row0 .. of the request's ext * G rows (row = t * G + h), q row of its
 // first token.  b < 0: padding.

@@ -1,0 +1,224 @@
+"""Attention of a step whose requests share prefixes.
+
+Requests that hit the same radix-cache node hold the same slots in front
+(``engine/scheduler.py:187-224``): samples of one prompt, a batch behind one system
+prompt, branches of a conversation.  ``slot_based_attention`` reads every request's
+whole context; ``shared_prefix_attention`` reads a group's shared keys and values once
+for all of its requests, and each request's own behind them, and joins the two by their
+softmax statistics.  Same inputs, output and semantics otherwise.
+
+``SharedPrefixes`` names the groups of a step.  It keeps the step's work lists on the
+device, so that the layers of a model share them, as ``ForwardBatch`` carries those of
+``slot_based_attention``.  There is no non-native path and no gradient.
+"""
+from __future__ import annotations
+
+import threading
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _native
+from .attention import (SHORT_ROWS, _KV_DTYPES, _check_inputs, _epilogue, _output, _plan_event,
+                        _pool_scales, _upload, _ws_lock, slot_based_attention)
+from .block_fp8 import workspace
+from .planning import plan_extend
+
+MAX_PARTS = 2048          # parts of contexts in one launch
+_captured: List[object] = []   # lists that captured graphs read
+
+
+class SharedPrefixes:
+    """The groups of a step: ``(members, length)`` each, members batch indices of
+    requests whose table rows hold the same slots in their first ``length`` entries.  A
+    request is in one group at most.  The lengths may exceed what a request sees (its
+    rows mask the rest), so that one object serves a step's layers and, while the
+    extend lengths stay the same, later steps too; ``seq_lens`` are read at launch.
+
+    A graph may capture calls once an eager call with the same layout has run (it
+    uploads the lists); lists that a graph reads stay allocated."""
+
+    def __init__(self, groups: Iterable[Tuple[Sequence[int], int]]):
+        self.groups: List[Tuple[List[int], int]] = []
+        seen: set = set()
+        for members, length in groups:
+            members, length = [int(b) for b in members], int(length)
+            if length < 0 or length > 0x7fffffff or any(b < 0 for b in members):
+                raise ValueError(f"shared prefix of {length} tokens for requests {members[:8]}")
+            if len(set(members)) != len(members) or seen.intersection(members):
+                raise ValueError("a request appears twice in the groups")
+            seen.update(members)
+            if length and len(members) > 1:   # (nothing is shared otherwise)
+                self.groups.append((members, length))
+        self._last = max(seen, default=-1)
+        self._lock = threading.Lock()
+        self._plans: Dict[tuple, _Plan] = {}
+
+    def _plan(self, batch, ext_lens, n_q, n_kv, head_dim, device) -> "_Plan":
+        if self._last >= batch.batch_size:
+            raise ValueError(f"request {self._last} of a batch of {batch.batch_size}")
+        width = batch.req_to_token.shape[1]
+        if any(n > width for _, n in self.groups):
+            raise ValueError(f"a shared prefix exceeds req_to_token's width {width}")
+        key = (device.index, tuple(ext_lens), n_q, n_kv, head_dim)
+        with self._lock:
+            plan = self._plans.get(key)
+            if plan is None:
+                plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device)
+            return plan
+
+
+class _Plan:
+    """The device lists of one step layout: parts of contexts, their tokens, and the
+    extend kernel's entries of long prompts, which share nothing (MFMA-bound)."""
+
+    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device):
+        group = n_q // n_kv
+        self.device = device
+        long_ = {b for b, e in enumerate(ext_lens) if head_dim == 256 and e * group > SHORT_ROWS}
+        starts = np.concatenate([[0], np.cumsum(ext_lens)])
+        groups = [([b for b in m if b not in long_], n) for m, n in groups]
+        groups = [(m, n) for m, n in groups if len(m) > 1]
+        self.shares = bool(groups)
+        rows_of = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
+        rows_of += [e * group for b, e in enumerate(ext_lens) if b not in long_]
+        self.row_groups = 2 if rows_of and max(rows_of) > 16 else 1
+        unit = 16 * self.row_groups
+
+        items, tokens = [], []
+        front = {}   # request -> (its shared part's first item, its first token there, keys)
+
+        def add(b, toks, k0, k1, pfx=-1, pfx_tok=0):
+            tok0 = len(tokens)
+            tokens.extend(toks)
+            for row0 in range(0, len(toks) * group, unit):
+                items.append((b, tok0, len(toks), row0, k0, k1, pfx, pfx_tok))
+
+        def request_tokens(b):
+            return [(starts[b] + t, b, ext_lens[b] - 1 - t, 0) for t in range(ext_lens[b])]
+
+        for members, length in groups:
+            first, at = len(items), 0
+            toks = []
+            for b in members:
+                front[b] = (first, len(toks), length)
+                toks += request_tokens(b)
+            add(members[0], toks, 0, length)
+        self.n_shared = len(items)
+        for b in range(len(ext_lens)):
+            if b not in long_:
+                pfx, pfx_tok, k0 = front.get(b, (-1, 0, 0))
+                add(b, request_tokens(b), k0, -1, pfx, pfx_tok)
+        self.n_items = len(items)
+        self.slot_rows = min(unit, max(rows_of, default=1))
+        work = np.zeros((0, 8), dtype=np.int32)
+        if long_:
+            work = plan_extend(ext_lens, n_q, n_kv, decode_to_decode_kernel=True)
+            work = work[np.isin(work[:, 0], list(long_))]
+        self.n_work = len(work)
+        self._host = np.concatenate([
+            np.asarray(items, dtype=np.int32).reshape(-1), work.reshape(-1),
+            np.asarray(tokens, dtype=np.int32).reshape(-1)])
+        self._lock = threading.Lock()
+        self._lists: Optional[torch.Tensor] = None
+        self._users: set = set()
+        self._event = None
+        self._uploaded_on = 0
+        self._kept = False
+
+    def lists(self) -> Tuple[int, int, int]:
+        """Addresses of (items, work, tokens) for launches on the current stream."""
+        stream = torch.cuda.current_stream(self.device)
+        capturing = torch.cuda.is_current_stream_capturing()
+        with self._lock:
+            if self._lists is None:
+                if capturing:
+                    raise RuntimeError("shared prefixes cannot be planned in a graph capture: "
+                                       "run the call once before it")
+                self._lists = _upload(self._host, self.device, stream)
+                self._uploaded_on = stream.cuda_stream
+                self._users.add(stream.cuda_stream)
+                with _ws_lock:
+                    self._event = _plan_event(self.device, stream)
+                    self._event.record(stream)
+            elif stream.cuda_stream not in self._users:
+                if not capturing:   # (torch waits for the device before it captures)
+                    self._users.add(stream.cuda_stream)
+                    self._lists.record_stream(stream)
+                    stream.wait_event(self._event)
+            if capturing and not self._kept:
+                self._kept = True
+                _captured.append(self._lists)
+            base = self._lists.data_ptr()
+        return base, base + 32 * self.n_items, base + 32 * (self.n_items + self.n_work)
+
+
+def shared_prefix_attention(
+    q: torch.Tensor,
+    layer_k_buffer: torch.Tensor,
+    layer_v_buffer: torch.Tensor,
+    batch,
+    shared: SharedPrefixes,
+    *,
+    scaling: Optional[float] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+    out_amax: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> torch.Tensor:
+    """``slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch)`` for a batch
+    whose ``shared`` groups' keys and values are read once per group; the first member's
+    table row is the one read.  Arguments and result as there (sums are joined in another
+    order, so bf16 results may differ in the last bit).
+
+    Steps in which nothing is shared run ``slot_based_attention`` itself: no group of two
+    requests with few new tokens (prompts of more than 64 rows, new tokens x query heads
+    per kv head, are bound by their products at head_dim 256, not by their keys' bytes),
+    an fp8 pool whose head_dim is not a multiple of 16, or more than 2048 parts."""
+    fn = "shared_prefix_attention"
+    _native.refuse_gradients(fn, q, layer_k_buffer, layer_v_buffer, gate)
+    _check_inputs(q, layer_k_buffer, layer_v_buffer, batch)
+    n_tok, n_q, head_dim = q.shape
+    n_slots, n_kv, _ = layer_k_buffer.shape
+    if n_q % n_kv:
+        raise ValueError(f"num_q_heads {n_q} is not a multiple of num_kv_heads {n_kv}")
+    ext_lens = [int(e) for e in batch.extend_lens]
+    if len(ext_lens) != batch.batch_size or sum(ext_lens) != n_tok or min(ext_lens, default=1) < 1:
+        raise ValueError(f"extend_lens {ext_lens[:8]}... do not match "
+                         f"batch_size={batch.batch_size}, T={n_tok}")
+    kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
+    plan = shared._plan(batch, ext_lens, n_q, n_kv, head_dim, q.device)
+    with _native.launching(q.device, stream):
+        if not plan.shares or plan.n_items > MAX_PARTS \
+                or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
+            return slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, scaling=scaling,
+                                        k_scale=k_scale, v_scale=v_scale, out=out, gate=gate,
+                                        out_amax=out_amax)
+        scaling = head_dim ** -0.5 if scaling is None else float(scaling)
+        k_scale, v_scale = _pool_scales(q, kv_dtype, k_scale, v_scale)
+        if q.stride(2) != 1 or q.stride(1) != head_dim:
+            q = q.contiguous()
+        out = _output(q, out)
+        epilogue = _epilogue(q, gate, out_amax)
+        items, work, tokens = plan.lists()
+        handle = _native.current_stream(q.device)
+        rtt = batch.req_to_token
+        pool = (layer_k_buffer.data_ptr(), layer_v_buffer.data_ptr(), n_slots, kv_dtype,
+                None if k_scale is None else k_scale.data_ptr(),
+                None if v_scale is None else v_scale.data_ptr(),
+                rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
+                batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
+        ws, nbytes = workspace("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
+                               plan.row_groups, plan.slot_rows, n_q, n_kv, head_dim, kv_dtype)
+        if plan.n_work:
+            _native.call("tf_attn_extend", q.data_ptr(), q.stride(0), *pool, 0, work, plan.n_work,
+                         n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), *epilogue,
+                         handle)
+        _native.call("tf_attn_shared", q.data_ptr(), q.stride(0), *pool, items, plan.n_items,
+                     plan.n_shared, tokens, plan.row_groups, plan.slot_rows, n_q, n_kv, head_dim,
+                     scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
+                     handle)
+    return out
