@@ -329,6 +329,29 @@ int32_t tf_attn_shared(
     void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
 
+/* tf_attn_weights: scores[req_pool_indices[b], k] += (add 0: =) the softmax weights that
+ * request b's last min(window, extend_lens[b]) new tokens give key k, summed in fp32 over
+ * those tokens and all query heads, for k < seq_lens[b] (each a table row of its own;
+ * scores behind that stay).  A token sees keys up to its own position, as in
+ * tf_attn_extend.  q: the q_rows new tokens' rows, request after request; extend_lens: device
+ * int64 [batch_size], NULL: one new token each (q row b, window 1).  max_len: the keys per
+ * request that the workspace holds (longer contexts end there).  Only K is read;
+ * head_dim: a multiple of 8 up to 256.  scores: fp32, scores_row_stride >= rtt_cols.
+ * Workspace: tf_attn_weights_workspace_bytes of the same sizes (window 1 without
+ * extend_lens), 16-byte aligned; calls that overlap in time must not share it. */
+int64_t tf_attn_weights_workspace_bytes(int32_t batch_size, int32_t window, int32_t max_len,
+                                        int32_t num_q_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int32_t kv_dtype);
+
+int32_t tf_attn_weights(
+    const void* q, int64_t q_row_stride, int64_t q_rows, const void* k_pool, int64_t pool_slots,
+    int32_t kv_dtype, const float* k_scale, const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride,
+    int64_t rtt_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+    int32_t seq_len_override, const int64_t* extend_lens, int32_t batch_size, int32_t window,
+    int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    float* scores, int64_t scores_row_stride, int32_t add, void* workspace,
+    int64_t workspace_bytes, tf_stream_t stream);
+
 /* tf_attn_plan_blocks: the row blocks of a step, built on the device from its
  * work list and decode items (of either planner, padding included): the decode
  * items, and the requests of at most max_rows rows (ext * G), become blocks of 16

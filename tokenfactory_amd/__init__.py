@@ -10,6 +10,7 @@ Public surface (the reference's names and contracts, see each module):
   ``qk_norm_rope_kv_write`` - the kernels' Python entry points
 * ``shared_prefix_attention`` / ``SharedPrefixes`` - attention of a step whose requests
   share prefixes, read once per group
+* ``scored_attention`` - attention that sums up the weight every cached token gets
 * ``LinearAttention`` / ``gdn_decode_step`` - Gated DeltaNet decode step
   (``qwen3_8/linear_attention.py``)
 * ``Fp8Linear`` / ``block_fp8_linear`` - block-FP8 linear (``qwen3_8/fp8_linear.py``,
@@ -23,6 +24,7 @@ Public surface (the reference's names and contracts, see each module):
 from .forward_batch import ForwardBatch
 from .attention import gather_kv, qk_norm_rope_kv_write, slot_based_attention, write_kv
 from .kv_pool import FullAttnKVPool
+from .scored_attention import scored_attention
 from .shared_prefix import SharedPrefixes, shared_prefix_attention
 from .fp8_linear import Fp8Linear, block_fp8_linear
 from .full_attention import FullAttention
@@ -47,6 +49,7 @@ __all__ = [
     "gather_kv",
     "qk_norm_rope_kv_write",
     "quantize_blocks",
+    "scored_attention",
     "shared_prefix_attention",
     "slot_based_attention",
     "write_kv",

@@ -129,6 +129,17 @@ SIGNATURES = {
         _p, _i64, _i64,
         _p, _p,
     ]),
+    "tf_attn_weights_workspace_bytes": (_i64, [_i32] * 7),
+    "tf_attn_weights": (_i32, [
+        _p, _i64, _i64,                # q, q_row_stride, q_rows
+        _p, _i64, _i32, _p,            # k_pool, pool_slots, kv_dtype, k_scale
+        _p, _i64, _i64, _i64,          # req_to_token, rtt_rows, rtt_row_stride, rtt_cols
+        _p, _p, _i32, _p,              # req_pool_indices, seq_lens, its override, extend_lens
+        _i32, _i32, _i32,              # batch_size, window, max_len
+        _i32, _i32, _i32, _f32,        # num_q_heads, num_kv_heads, head_dim, scale
+        _p, _i64, _i32,                # scores, scores_row_stride, add
+        _p, _i64, _p,                  # workspace, workspace_bytes, stream
+    ]),
     "tf_attn_plan_decode_items": (_i32, [_p, _i32, _p, _p, _i32]),
     "tf_req_to_token_sync": (_i32, [
         _p, _i64, _i64, _i64,          # req_to_token, rtt_rows, rtt_row_stride, rtt_cols

@@ -1,0 +1,99 @@
+"""Attention that also sums up how much every cached token is looked at.
+
+``scored_attention`` is ``slot_based_attention`` with one more result: per request and
+cached position, the softmax weight that the step's last ``window`` new tokens give it,
+summed over them and over all query heads.  ``scores`` has ``req_to_token``'s layout
+(``[max_reqs, max_context_len]``, a position's score beside its slot) and is shared by
+the model's full-attention layers, whose weights add up in it, as the layers share the
+slots; ``evict_tokens`` reads it.  There is no non-native path and no gradient.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _native
+from .attention import _KV_DTYPES, _check_inputs, _pool_scales, slot_based_attention
+from .block_fp8 import workspace
+from .fp8_linear import _ptr
+
+
+def check_scores(fn: str, scores: torch.Tensor, table: torch.Tensor) -> None:
+    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.device != table.device \
+            or scores.shape[0] < table.shape[0] or scores.shape[1] < table.shape[1] \
+            or scores.stride(1) != 1 or (scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]):
+        raise ValueError(f"{fn}: scores must be fp32 with req_to_token's rows and columns "
+                         f"{tuple(table.shape)}, on its device, row-major")
+
+
+def scored_attention(
+    q: torch.Tensor,
+    layer_k_buffer: torch.Tensor,
+    layer_v_buffer: torch.Tensor,
+    batch,
+    scores: torch.Tensor,
+    *,
+    window: int = 32,
+    add: bool = True,
+    scaling: Optional[float] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+    out_amax: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> torch.Tensor:
+    """``slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, ...)``, and
+    ``scores[req_pool_indices[b], k] += w[b, k]`` for ``k < seq_lens[b]``, w the fp32 sum
+    over the request's last ``min(window, extend_len)`` new tokens and all heads of
+    their softmax weights (``add`` False: ``= w``, for a request's first step or scores of
+    the last step alone).  Positions behind a request's length stay as they are.  A table
+    row stands for one request of the batch at most.
+
+    A captured call follows ``seq_lens`` (and ``extend_lens_tensor``) in place up to
+    ``req_to_token``'s width; an eager one covers ``batch.max_seq_len`` keys, as the
+    batch promises."""
+    fn = "scored_attention"
+    _native.refuse_gradients(fn, q, layer_k_buffer, layer_v_buffer, gate, scores)
+    _check_inputs(q, layer_k_buffer, layer_v_buffer, batch)
+    check_scores(fn, scores, batch.req_to_token)
+    if window < 1:
+        raise ValueError(f"{fn}: window {window}")
+    rows = batch.req_pool_indices_list
+    if rows is not None and len(set(rows)) != len(rows):
+        raise ValueError(f"{fn}: a request row appears twice in one batch")
+    n_tok, n_q, head_dim = q.shape
+    n_slots, n_kv, _ = layer_k_buffer.shape
+    bsz, device = batch.batch_size, q.device
+    kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
+    longest = max((int(e) for e in batch.extend_lens), default=1)
+    ext_t = batch.extend_lens_tensor
+    if longest > 1 and (ext_t is None or ext_t.device != device or ext_t.dtype != torch.long
+                        or ext_t.numel() != bsz or not ext_t.is_contiguous()):
+        raise ValueError(f"{fn}: batch.extend_lens_tensor must be contiguous int64 [batch_size] "
+                         "on q's device")
+    with _native.launching(device, stream):
+        k_scale, v_scale = _pool_scales(q, kv_dtype, k_scale, v_scale)
+        if q.stride(2) != 1 or q.stride(1) != head_dim:
+            q = q.contiguous()
+        out = slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, scaling=scaling,
+                                   k_scale=k_scale, v_scale=v_scale, out=out, gate=gate,
+                                   out_amax=out_amax)
+        if n_tok == 0:
+            return out
+        rtt = batch.req_to_token
+        span = (rtt.shape[1] if torch.cuda.is_current_stream_capturing()
+                else max(1, int(batch.max_seq_len)))
+        window = min(int(window), longest)
+        ws, nbytes = workspace("tf_attn_weights_workspace_bytes", device, bsz, window, span, n_q,
+                               n_kv, head_dim, kv_dtype)
+        _native.call("tf_attn_weights", q.data_ptr(), q.stride(0), n_tok,
+                     layer_k_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale), rtt.data_ptr(), rtt.shape[0],
+                     rtt.stride(0), rtt.shape[1], batch.req_pool_indices.data_ptr(),
+                     batch.seq_lens.data_ptr(), int(batch.max_seq_len) if bsz == 1 else 0,
+                     _ptr(ext_t) if longest > 1 else None, bsz, window, span, n_q, n_kv, head_dim,
+                     head_dim ** -0.5 if scaling is None else float(scaling), scores.data_ptr(),
+                     scores.stride(0), int(bool(add)), ws.data_ptr(), nbytes,
+                     _native.current_stream(device))
+    return out
