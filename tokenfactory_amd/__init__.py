@@ -11,6 +11,7 @@ Public surface (the reference's names and contracts, see each module):
 * ``shared_prefix_attention`` / ``SharedPrefixes`` - attention of a step whose requests
   share prefixes, read once per group
 * ``scored_attention`` - attention that sums up the weight every cached token gets
+* ``evict_tokens`` - drops the cached tokens of the least weight
 * ``LinearAttention`` / ``gdn_decode_step`` - Gated DeltaNet decode step
   (``qwen3_8/linear_attention.py``)
 * ``Fp8Linear`` / ``block_fp8_linear`` - block-FP8 linear (``qwen3_8/fp8_linear.py``,
@@ -24,6 +25,7 @@ Public surface (the reference's names and contracts, see each module):
 from .forward_batch import ForwardBatch
 from .attention import gather_kv, qk_norm_rope_kv_write, slot_based_attention, write_kv
 from .kv_pool import FullAttnKVPool
+from .evict import evict_tokens
 from .scored_attention import scored_attention
 from .shared_prefix import SharedPrefixes, shared_prefix_attention
 from .fp8_linear import Fp8Linear, block_fp8_linear
@@ -44,6 +46,7 @@ __all__ = [
     "add_rms_norm",
     "block_fp8_linear",
     "block_scaled_linear",
+    "evict_tokens",
     "gated_mlp",
     "gdn_decode_step",
     "gather_kv",
