@@ -5,7 +5,7 @@ import torch
 
 from tests.helpers import small_case
 from tokenfactory_amd import SharedPrefixes, shared_prefix_attention
-from tokenfactory_amd.shared_prefix import _Plan
+from tokenfactory_amd.shared_prefix import MIN_STEPS, _Plan, cut_units
 
 
 @pytest.mark.parametrize("groups", [[([0, 0], 5)], [([0, 1], 5), ([1, 2], 5)], [([0, -1], 5)],
@@ -37,34 +37,64 @@ def test_groups_must_fit_the_batch():
         SharedPrefixes([([0, 1], 400)])._plan(wl.batch, [1, 1], 4, 1, 64, dev)
 
 
+def lists(plan):
+    """(items, work, pieces, tokens, units) of a plan's host copy."""
+    cuts = [at // 4 for at in plan._offsets] + [len(plan._host)]
+    parts = [plan._host[a:b] for a, b in zip(cuts, cuts[1:])]
+    return [x.reshape(-1, n) for x, n in zip(parts, (8, 8, 8, 4, 2))]
+
+
+EXT = [1, 4, 2, 1, 70, 1] + [1] * 60
+GROUPS = [([0, 1, 5] + list(range(6, 60)), 1000), ([2, 4, 62], 50)]
+
+
 @pytest.mark.parametrize("head_dim", [256, 128])
 def test_plan_covers_every_row_and_key_once(head_dim):
-    """Each output row has one own part; own and shared parts meet at the shared length;
-    a row's place in the shared part names the same token."""
-    ext = [1, 4, 2, 1, 70, 1]
-    groups = [([0, 1, 5], 100), ([2, 4], 50)]
-    group = 6
-    plan = _Plan(groups, ext, 24, 4, head_dim, torch.device("cpu"))
+    """Each output row has one own part; own and shared parts meet at the shared length; a
+    row's place in the shared part names the same token; pieces cover a unit's keys."""
+    group, n_kv = 6, 4
+    plan = _Plan(GROUPS, EXT, 24, n_kv, head_dim, torch.device("cpu"), 64)
     long_ = {4} if head_dim == 256 else set()
-    items = plan._host[:8 * plan.n_items].reshape(-1, 8)
-    toks = plan._host[8 * (plan.n_items + plan.n_work):].reshape(-1, 4)
+    items, work, pieces, toks, units = lists(plan)
     unit = 16 * plan.row_groups
-    starts = np.concatenate([[0], np.cumsum(ext)])
+    starts = np.concatenate([[0], np.cumsum(EXT)])
     rows = set()
     for b, tok0, n, row0, k0, k1, pfx, pfx_tok in items[plan.n_shared:]:
         assert k1 == -1 and row0 % unit == 0
-        shares = [length for m, length in groups if b in m and len(set(m) - long_) > 1]
+        shares = [length for m, length in GROUPS if b in m and len(set(m) - long_) > 1]
         assert k0 == (shares[0] if shares else 0) and (pfx >= 0) == bool(shares)
         for rho in range(row0, min(row0 + unit, n * group)):
             t = rho // group
-            assert toks[tok0 + t].tolist() == [starts[b] + t, b, ext[b] - 1 - t, 0]
+            assert toks[tok0 + t].tolist() == [starts[b] + t, b, EXT[b] - 1 - t, 0]
             rows.add((b, rho))
-            if pfx >= 0:
-                rp = (pfx_tok + t) * group + rho % group
+            if pfx < 0:
+                continue
+            rp = (pfx_tok + t) * group + rho % group
+            if head_dim != 256:
                 front = items[pfx + rp // unit]
                 assert front[3] == rp // unit * unit and front[4] == 0 and front[5] == k0
                 assert toks[front[1] + pfx_tok + t].tolist() == toks[tok0 + t].tolist()
                 assert rp < front[2] * group
-    assert rows == {(b, r) for b, e in enumerate(ext) if b not in long_ for r in range(e * group)}
-    work = plan._host[8 * plan.n_items:8 * (plan.n_items + plan.n_work)].reshape(-1, 8)
+                continue
+            for hk in range(n_kv):
+                slot, n_parts = units[pfx + rp // 256 * n_kv + hk]
+                cut = pieces[slot:slot + n_parts]
+                assert (cut[:, 1] == hk).all() and (cut[:, 2] == rp // 256 * 256).all()
+                assert cut[:, 7].tolist() == list(range(slot + 1, slot + n_parts + 1))
+                assert cut[0, 5] == 0 and cut[-1, 6] == k0
+                assert (cut[1:, 5] == cut[:-1, 6]).all() and (cut[:, 5] < cut[:, 6]).all()
+                for _, _, _, front, n_front, *_ in cut:
+                    assert toks[front + pfx_tok + t].tolist() == toks[tok0 + t].tolist()
+                    assert rp < n_front * group
+    assert rows == {(b, r) for b, e in enumerate(EXT) if b not in long_ for r in range(e * group)}
     assert set(work[:, 0].tolist()) == long_
+    assert (len(pieces) > 0) == (head_dim == 256) and len(pieces) <= 64
+
+
+@pytest.mark.parametrize("steps,cus", [([256] * 8, 256), ([1024] * 24, 256), ([1], 256),
+                                       ([1, 500, 3], 16), ([100] * 300, 256), ([8] * 31, 256)])
+def test_cuts(steps, cus):
+    cuts = cut_units(steps, cus)
+    assert len(cuts) == len(steps)
+    assert sum(cuts) <= max(cus, len(steps))
+    assert all(1 <= c <= max(1, -(-s // MIN_STEPS)) for c, s in zip(cuts, steps))

@@ -44,6 +44,7 @@
 
 #include <type_traits>
 
+#include "prefix_attn.h"
 #include "tf_common.h"
 #include "tf_internal.h"
 
@@ -400,11 +401,16 @@ __device__ __forceinline__ bool softmax_tile(const f32x16& s, Row& row, float sl
 // no key a row sees, and any score raises it.
 constexpr float kNoKeys = -1e30f;
 
-// kSplit: the work list may hold pieces of entries (an instance of its own: as
-// one kernel, large prefills took 0.4 % and mixed steps 2 % longer).
-template <bool FP8, bool kSplit>
+// What the work list holds: whole entries; pieces of entries too (an instance of its
+// own: as one kernel, large prefills took 0.4 % and mixed steps 2 % longer); or pieces of
+// shared prefixes, whose rows are of the tokens that the entry lists (prefix_attn.hip).
+enum : int { kWhole = 0, kPieces = 1, kPrefix = 2 };
+
+template <bool FP8, int kList>
 __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   __shared__ Smem<FP8> sm;
+  constexpr bool kSplit = kList != kWhole;
+  constexpr bool kShared = kList == kPrefix;
   constexpr int kKS = kStagesOf<FP8>, kVS = kVStagesOf<FP8>;
 
   const int tid = threadIdx.x;
@@ -427,9 +433,11 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   // The tiles come from the lengths at planning, the keys from the lengths now:
   // the last piece (the next entry of the list starts at tile 0) takes every key
   // from its first one on, and a piece left without keys writes empty partials.
+  // (A piece of a prefix: keys [wk[5], wk[6]); q_start is its first token's entry.)
   const int part = kSplit ? wk[7] : 0;
-  const int key0 = part ? kBN * wk[5] : 0;
-  int64_t len = a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b];
+  const int key0 = kShared ? wk[5] : part ? kBN * wk[5] : 0;
+  int64_t len = kShared ? (int64_t)wk[6]
+                        : a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b];
   if (len > a.rtt_cols) len = a.rtt_cols;
   const int L = (int)len - key0;
   const int P = L - ext;
@@ -442,15 +450,19 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   // This lane's row; padding lanes compute a valid duplicate row and never
   // write it.
   const int rho_c = min(row0 + kRowsPerWave * w + n, rows_total - 1);
-  const int limit = P + rho_c / G;   // last visible key
+  int limit = P + rho_c / G;   // last visible key
+  if constexpr (kShared) {
+    const PartTok tok = a.toks[q_start + rho_c / G];
+    limit = (int)min<int64_t>(L, min(a.seq_lens[tok.b], a.rtt_cols) - tok.back - key0) - 1;
+  }
 
   // Keys [0, kend) are needed by the item; keys below w_full are visible to
   // every row of this wave. Every wave runs all n_tiles tiles (keys past a
   // row's limit are masked; key 0 is visible to every row, so each row's max
   // is finite after tile 0).
   const int blk_last_row = min(row0 + kExtendItemRows, rows_total) - 1;
-  const int keys = min(L, P + blk_last_row / G + 1);
-  const bool inner = kSplit && part && blockIdx.x + 1 < gridDim.x && wk[8 + 5] > 0;
+  const int keys = kShared ? L : min(L, P + blk_last_row / G + 1);
+  const bool inner = kList == kPieces && part && blockIdx.x + 1 < gridDim.x && wk[8 + 5] > 0;
   const int kend = inner ? min(keys, kBN * (wk[6] - wk[5])) : keys;
   if (L <= 0 || kend <= 0) {
     if (kSplit && part && tid < kExtendItemRows)
@@ -461,7 +473,15 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   const int n_tiles = (kend + kBN - 1) / kBN;
   const int last = n_tiles - 1;
   const int w_first = row0 + kRowsPerWave * w;
-  const int w_full = w_first < rows_total ? P + w_first / G + 1 : 0;
+  int w_full = w_first < rows_total ? P + w_first / G + 1 : 0;
+  if constexpr (kShared) {
+    w_full = limit + 1;
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) w_full = min(w_full, __shfl_xor(w_full, m, kWave));
+    w_full = __builtin_amdgcn_readfirstlane(w_full);
+  }
+  // Waves without rows only stage (few requests share a prefix as a rule).
+  const bool idle = kShared && w_first >= rows_total;
 
   // fp8 pools: scores and outputs are computed from the e4m3 values and
   // scaled by k_scale / v_scale (folded into the exponent scale and 1 / l).
@@ -534,7 +554,8 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
       const int r = 2 * i + g;
       const int rho = min(row0 + kRowsPerWave * w + r, rows_total - 1);
       const int t = rho / G, h = rho - t * G;
-      qv[i] = ld_g16(a.q + (int64_t)(q_start + t) * a.q_stride + (int64_t)(hk * G + h) * kD + 8 * n);
+      const int64_t qrow = kShared ? a.toks[q_start + t].qrow : q_start + t;
+      qv[i] = ld_g16(a.q + qrow * a.q_stride + (int64_t)(hk * G + h) * kD + 8 * n);
     }
     slot_issue(rtt, 0, kend, w, lane, sm.slots);
 #pragma unroll
@@ -626,7 +647,25 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   constexpr bool kTail = !FP8;
   const int n_stage = kTail ? max(n_tiles - kAhead, 0) : n_tiles;
 
-  if (w < kLeadWaves) {
+  if (idle) {
+    for (int j = 0; j < n_tiles; ++j) {
+      const bool staged = j < n_stage;
+      if (staged) {
+        slot_chunk(j);
+        stage_for(j);
+        const auto ids = st.fetch();
+#pragma unroll
+        for (int p = 0; p < 2; ++p) st.issue_part(ids, p);
+      }
+      if (staged) {
+        widen(j + 1, Unstaged{});
+        step_end(Staged{});
+      } else {
+        widen(j + 1, Staged{});
+        step_end(Unstaged{});
+      }
+    }
+  } else if (w < kLeadWaves) {
     auto lead_step = [&](int j, auto staged) {
       constexpr bool kS = decltype(staged)::value;
       if constexpr (kS) {
@@ -681,7 +720,21 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
     // fp32 partials in the accumulators' own order (1 KB per store), each
     // row's reference maximum (log2 units) and sum.
     const float l = row.l + __shfl_xor(row.l, 32, kWave);
-    if (w_first < rows_total) {
+    if constexpr (kShared) {   // a row's dims side by side, for the merge by rows
+      const int ln = opaque(lane);
+      const int n = ln & 31, g = ln >> 5;
+      const int64_t pr = (int64_t)(wk[7] - 1) * kExtendItemRows + kRowsPerWave * w + n;
+      if (wk[2] + kRowsPerWave * w + n < wk[4] * a.group) {
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq)
+            *reinterpret_cast<f32x4*>(a.part_o + pr * kD + 32 * mt + 8 * rq + 4 * g) =
+                f32x4{acc[mt][4 * rq], acc[mt][4 * rq + 1], acc[mt][4 * rq + 2],
+                      acc[mt][4 * rq + 3]};
+        if (g == 0) reinterpret_cast<float2*>(a.part_ml)[pr] = float2{row.moff, l};
+      }
+    } else if (w_first < rows_total) {
       f32x4* po = reinterpret_cast<f32x4*>(a.part_o) +
                   ((int64_t)(part - 1) * kWaves + w) * 32 * kWave + lane;
 #pragma unroll
@@ -833,6 +886,17 @@ int64_t part_ml_bytes(int64_t n) { return n * kExtendItemRows * 2 * 4; }
 int64_t part_bytes(int64_t n) { return part_ml_bytes(n) + n * kExtendItemRows * kD * 4; }
 
 }  // namespace
+
+int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, bool fp8, hipStream_t s) {
+  if (fp8)
+    hipLaunchKernelGGL((extend_mfma_kernel<true, kPrefix>), dim3((unsigned)n_pieces),
+                       dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((extend_mfma_kernel<false, kPrefix>), dim3((unsigned)n_pieces),
+                       dim3(kThreads), 0, s, a);
+  return launch_status("tf_attn_shared prefix launch");
+}
+
 }  // namespace tfa
 
 namespace {
@@ -946,7 +1010,7 @@ int32_t extend_launch(const void* q, int64_t q_row_stride, const void* k_pool,
       out_row_stride < (int64_t)num_q_heads * head_dim)
     return fail(TF_ERR_INVALID, "extend: row stride smaller than num_q_heads*head_dim");
 
-  ExtendArgs a;
+  ExtendArgs a = {};
   a.q = static_cast<const __bf16*>(q);
   a.q_stride = q_row_stride;
   a.k_pool = static_cast<const uint8_t*>(k_pool);
@@ -1009,13 +1073,13 @@ int32_t extend_launch(const void* q, int64_t q_row_stride, const void* k_pool,
   const bool fp8 = kv_dtype == TF_DTYPE_FP8_E4M3;
   const dim3 items((unsigned)n_work), block(kThreads);
   if (merges && fp8)
-    hipLaunchKernelGGL((extend_mfma_kernel<true, true>), items, block, 0, s, a);
+    hipLaunchKernelGGL((extend_mfma_kernel<true, kPieces>), items, block, 0, s, a);
   else if (merges)
-    hipLaunchKernelGGL((extend_mfma_kernel<false, true>), items, block, 0, s, a);
+    hipLaunchKernelGGL((extend_mfma_kernel<false, kPieces>), items, block, 0, s, a);
   else if (fp8)
-    hipLaunchKernelGGL((extend_mfma_kernel<true, false>), items, block, 0, s, a);
+    hipLaunchKernelGGL((extend_mfma_kernel<true, kWhole>), items, block, 0, s, a);
   else
-    hipLaunchKernelGGL((extend_mfma_kernel<false, false>), items, block, 0, s, a);
+    hipLaunchKernelGGL((extend_mfma_kernel<false, kWhole>), items, block, 0, s, a);
   const int rc = launch_status("tf_attn_extend launch");
   if (rc != TF_OK || n_merges == 0) return rc;
   const dim3 grid((unsigned)n_merges, kWaves);

@@ -8,8 +8,9 @@ namespace tfa {
 
 // Query rows row0 .. of the n_tok tokens at tokens[tok0] (row = t * G + head of the kv
 // head's group) over keys [k0, k1) of request b's table row; k1 < 0: up to what the
-// rows see.  pfx: of a request's own part, the first item of the shared part before it
-// (-1: none), and pfx_tok where the request's tokens start among that part's.
+// rows see.  pfx: of a request's own part, the shared part before it (-1: none): its
+// first item, or its first unit in PartArgs::units; pfx_tok: where the request's tokens
+// start among that part's.
 struct PartItem {
   int32_t b, tok0, n_tok, row0, k0, k1, pfx, pfx_tok;
 };
@@ -46,6 +47,11 @@ struct PartArgs {
   int32_t* ipre;           // prefix of the items' tiles, for the merge
   float2* part_ml;         // partials of (workgroup + unit) slots
   float* part_o;
+  // Shared parts that the extend kernel took in pieces (NULL: they are items): unit
+  // pfx + (row / 256) * hkv + kv head is {first slot, slots}.
+  const int2* units;
+  const float2* piece_ml;  // [slot][256], [slot][256][256]
+  const float* piece_o;
 };
 
 }  // namespace tfa

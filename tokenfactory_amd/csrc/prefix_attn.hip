@@ -9,6 +9,9 @@
 // one item per request, or several where it has more rows than a unit.  Every item
 // leaves fp32 partials, which part_merge_kernel joins.
 //
+// At head_dim 256 the shared parts go through the extend kernel's MFMA tiles instead
+// (extend.hip, kPrefix), cut over their keys so that every CU has a piece.
+//
 // part_stream_kernel is the decode kernel's scheme (decode.hip: persistent workgroups
 // that own equal shares of the tiles of all units, unit = (item, kv head)), with the
 // tokens of an item looked up in a list, since a group's requests lie anywhere in the
@@ -280,11 +283,21 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
   // Partials: the request's own part, then the shared one's.
   const Owners own = unit_owners(a, item, hk);
   Owners pre{0, 0};
-  int pre_row = 0;
+  const float2* pre_ml = a.part_ml;   // of row `pre_row` of slot pre.first, and on
+  const float* pre_o = a.part_o;
+  int pre_rows = a.slot_rows, pre_row = 0;
   if (im.pfx >= 0) {
     const int rp = (im.pfx_tok + t) * a.group + rho - t * a.group;
-    pre = unit_owners(a, im.pfx + rp / a.unit_rows, hk);
-    pre_row = rp % a.unit_rows;
+    if (a.units) {
+      const int2 u = a.units[im.pfx + rp / kExtendItemRows * a.hkv + hk];
+      pre = Owners{u.x, u.y};
+      pre_ml = a.piece_ml;
+      pre_o = a.piece_o;
+      pre_rows = kExtendItemRows;
+    } else {
+      pre = unit_owners(a, im.pfx + rp / a.unit_rows, hk);
+    }
+    pre_row = rp % (a.units ? kExtendItemRows : a.unit_rows);
   }
   float m = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -295,10 +308,11 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int i = min(k0 + WPR * k, parts - 1);
-      const int64_t pr = i < own.count ? (own.first + i) * a.slot_rows + n
-                                       : (pre.first + i - own.count) * a.slot_rows + pre_row;
-      ml[k] = a.part_ml[pr];
-      o[k] = lane_in ? reinterpret_cast<const f32x4*>(a.part_o + pr * DP)[lane]
+      const bool mine = i < own.count;
+      const int64_t pr = mine ? (own.first + i) * a.slot_rows + n
+                              : (pre.first + i - own.count) * pre_rows + pre_row;
+      ml[k] = (mine ? a.part_ml : pre_ml)[pr];
+      o[k] = lane_in ? reinterpret_cast<const f32x4*>((mine ? a.part_o : pre_o) + pr * DP)[lane]
                      : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     float mn = m;
@@ -315,7 +329,8 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const float a2 = fast_exp2(ml[k].x - ref);
-      if (k0 + WPR * k < parts) acc += o[k] * a2;
+      // (a part without a key for the row may not have written its O)
+      if (k0 + WPR * k < parts && ml[k].y != 0.f) acc += o[k] * a2;
       l += ml[k].y * a2;
     }
     m = mn;
@@ -381,12 +396,14 @@ struct PartPlan {
   bool fp8, narrow, other;
   int32_t unit_rows;    // 16 or 32
   int32_t n_blocks;     // persistent workgroups
-  int64_t ipre_bytes, ml_bytes, o_bytes;
-  int64_t total() const { return ipre_bytes + ml_bytes + o_bytes; }
+  int64_t ipre_bytes, ml_bytes, o_bytes, piece_ml_bytes, piece_o_bytes;
+  int64_t total() const {
+    return ipre_bytes + ml_bytes + o_bytes + piece_ml_bytes + piece_o_bytes;
+  }
 };
 
 int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t slot_rows,
-                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
+                   int32_t n_pieces, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
                    PartPlan* p) {
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
     return fail(TF_ERR_INVALID, "%s: num_q_heads=%d not a multiple of num_kv_heads=%d", fn,
@@ -404,6 +421,8 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   if (n_items > kMaxItems)
     return fail(TF_ERR_UNSUPPORTED, "%s: %d parts in one call (at most %d)", fn, n_items,
                 kMaxItems);
+  if (n_pieces < 0 || (n_pieces && head_dim != 256))
+    return fail(TF_ERR_INVALID, "%s: n_pieces=%d at head_dim=%d", fn, n_pieces, head_dim);
   p->other = head_dim != 256;
   p->narrow = head_dim <= 128 && !p->fp8;
   p->unit_rows = 16 * row_groups;
@@ -412,6 +431,8 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   p->ipre_bytes = ((int64_t)(n_items + 1) * 4 + 255) / 256 * 256;
   p->ml_bytes = (rows * 8 + 255) / 256 * 256;
   p->o_bytes = rows * (p->narrow ? 128 : 256) * 4;
+  p->piece_ml_bytes = (int64_t)n_pieces * kExtendItemRows * 8;
+  p->piece_o_bytes = (int64_t)n_pieces * kExtendItemRows * 256 * 4;
   return TF_OK;
 }
 
@@ -447,13 +468,13 @@ void launch_merge(const PartArgs& a, const PartPlan& p, int n_own, int rows, hip
 }  // namespace tfa
 
 extern "C" int64_t tf_attn_shared_workspace_bytes(int32_t n_items, int32_t row_groups,
-                                                  int32_t slot_rows, int32_t num_q_heads,
-                                                  int32_t num_kv_heads, int32_t head_dim,
-                                                  int32_t kv_dtype) {
+                                                  int32_t slot_rows, int32_t n_pieces,
+                                                  int32_t num_q_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim, int32_t kv_dtype) {
   using namespace tfa;
   clear_error();
   PartPlan p;
-  const int rc = make_part_plan("shared", n_items, row_groups, slot_rows, num_q_heads,
+  const int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, num_q_heads,
                                 num_kv_heads, head_dim, kv_dtype, &p);
   return rc != TF_OK ? rc : p.total();
 }
@@ -464,17 +485,19 @@ extern "C" int32_t tf_attn_shared(
     const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
     const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* items,
     int32_t n_items, int32_t n_shared, const int32_t* tokens, int32_t row_groups,
-    int32_t slot_rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    int32_t slot_rows, const int32_t* pieces, int32_t n_pieces, const int32_t* units,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
     void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream) {
   using namespace tfa;
   clear_error();
   PartPlan p;
-  int rc = make_part_plan("shared", n_items, row_groups, slot_rows, num_q_heads, num_kv_heads,
-                          head_dim, kv_dtype, &p);
+  int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, num_q_heads,
+                          num_kv_heads, head_dim, kv_dtype, &p);
   if (rc != TF_OK) return rc;
-  if (n_shared < 0 || n_shared > n_items)
-    return fail(TF_ERR_INVALID, "shared: %d of %d parts are shared", n_shared, n_items);
+  if (n_shared < 0 || n_shared > n_items || (n_shared && n_pieces))
+    return fail(TF_ERR_INVALID, "shared: %d of %d parts are shared, and %d pieces", n_shared,
+                n_items, n_pieces);
   if (n_items == n_shared) return TF_OK;
   rc = check_slot_call("shared", q, q_row_stride, k_pool, v_pool, pool_slots, kv_dtype, k_scale,
                        v_scale, req_to_token, rtt_rows, rtt_row_stride, rtt_cols,
@@ -484,6 +507,8 @@ extern "C" int32_t tf_attn_shared(
   if (rc != TF_OK) return rc;
   if (!items || !tokens || !aligned16(items) || !aligned16(tokens))
     return fail(TF_ERR_INVALID, "shared: items and tokens must be 16-byte aligned");
+  if (n_pieces && (!pieces || !units || !aligned16(pieces) || !aligned8(units)))
+    return fail(TF_ERR_INVALID, "shared: pieces and units must be 16- and 8-byte aligned");
   PartArgs a = {};
   a.q = static_cast<const __bf16*>(q);
   a.q_stride = q_row_stride;
@@ -520,6 +545,35 @@ extern "C" int32_t tf_attn_shared(
   a.part_ml = reinterpret_cast<float2*>(ws + p.ipre_bytes);
   a.part_o = reinterpret_cast<float*>(ws + p.ipre_bytes + p.ml_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (n_pieces) {
+    a.units = reinterpret_cast<const int2*>(units);
+    char* at = ws + p.ipre_bytes + p.ml_bytes + p.o_bytes;
+    a.piece_ml = reinterpret_cast<float2*>(at);
+    a.piece_o = reinterpret_cast<float*>(at + p.piece_ml_bytes);
+    ExtendArgs e = {};
+    e.q = a.q;
+    e.q_stride = a.q_stride;
+    e.k_pool = a.k_pool;
+    e.v_pool = a.v_pool;
+    e.pool_slots = a.pool_slots;
+    e.k_scale = a.k_scale;
+    e.v_scale = a.v_scale;
+    e.rtt = a.rtt;
+    e.rtt_rows = a.rtt_rows;
+    e.rtt_stride = a.rtt_stride;
+    e.rtt_cols = a.rtt_cols;
+    e.rpi = a.rpi;
+    e.seq_lens = a.seq_lens;
+    e.work = pieces;
+    e.hkv = a.hkv;
+    e.group = a.group;
+    e.scale_log2 = a.scale_log2;
+    e.part_ml = reinterpret_cast<float*>(at);
+    e.part_o = reinterpret_cast<float*>(at + p.piece_ml_bytes);
+    e.toks = a.toks;
+    rc = launch_prefix_pieces(e, n_pieces, p.fp8, s);
+    if (rc != TF_OK) return rc;
+  }
   if (row_groups == 1)
     launch_stream_groups<1>(a, p, s);
   else

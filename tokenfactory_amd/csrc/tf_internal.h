@@ -58,6 +58,7 @@ void plan_units(int32_t n_items, int32_t num_kv_heads, int32_t n_hgroups, int32_
 // Extend kernel arguments (validated by tf_attn_extend).  Work items cover
 // kExtendItemRows flattened (token, q-head-of-group) rows each.
 constexpr int kExtendItemRows = 256;
+struct PartTok;
 struct ExtendArgs {
   const __bf16* q;
   int64_t q_stride;
@@ -81,7 +82,12 @@ struct ExtendArgs {
   uint32_t* amax;                 // optional: raised to max |out| (bf16 bits)
   float* part_o;                  // split entries: fp32 partials (work[7] - 1 = slot)
   float* part_ml;
+  const PartTok* toks;            // pieces of shared prefixes: the tokens of their rows
 };
+// The extend kernel over pieces of shared prefixes (head_dim 256): work entries {b, kv
+// head, row0, first token, tokens, first key, end key, slot + 1}, b's table row read for
+// all of them; partials [slot][256 rows][256], as prefix_attn.hip merges them.
+int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, bool fp8, hipStream_t s);
 
 // Slot attention for head dims other than 256 (attn_generic.hip): one wave per
 // query row.  work != NULL: the rows of n_rows extend work entries; else the

@@ -20,10 +20,10 @@ import numpy as np
 import torch
 
 from . import _native
-from .attention import (SHORT_ROWS, _KV_DTYPES, _check_inputs, _epilogue, _output, _plan_event,
-                        _pool_scales, _upload, _ws_lock, slot_based_attention)
+from .attention import (SHORT_ROWS, _KV_DTYPES, _check_inputs, _cu_count, _epilogue, _output,
+                        _plan_event, _pool_scales, _upload, _ws_lock, slot_based_attention)
 from .block_fp8 import workspace
-from .planning import plan_extend
+from .planning import EXTEND_TILE_ROWS, plan_extend
 
 MAX_PARTS = 2048          # parts of contexts in one launch
 _captured: List[object] = []   # lists that captured graphs read
@@ -65,61 +65,97 @@ class SharedPrefixes:
         with self._lock:
             plan = self._plans.get(key)
             if plan is None:
-                plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device)
+                plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device,
+                                                _cu_count(device))
             return plan
 
 
-class _Plan:
-    """The device lists of one step layout: parts of contexts, their tokens, and the
-    extend kernel's entries of long prompts, which share nothing (MFMA-bound)."""
+KEYS_PER_STEP = 32   # of the extend kernel
+MIN_STEPS = 8        # of a piece of a prefix
 
-    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device):
+
+def cut_units(steps: Sequence[int], cus: int) -> List[int]:
+    """Pieces per unit, steps[i] steps of keys long: the shortest pieces of which there are
+    no more than CUs (a piece more would be a round more), of MIN_STEPS at least."""
+    lo, hi = MIN_STEPS, max([MIN_STEPS, *steps])
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if sum(-(-s // mid) for s in steps) <= cus:
+            hi = mid
+        else:
+            lo = mid + 1
+    return [max(1, -(-s // lo)) for s in steps]
+
+
+class _Plan:
+    """The device lists of one step layout: parts of contexts and their tokens; at head_dim
+    256 the pieces of the shared ones; and the extend kernel's entries of long prompts,
+    which share nothing (MFMA-bound)."""
+
+    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus):
         group = n_q // n_kv
         self.device = device
-        long_ = {b for b, e in enumerate(ext_lens) if head_dim == 256 and e * group > SHORT_ROWS}
-        starts = np.concatenate([[0], np.cumsum(ext_lens)])
+        mfma = head_dim == 256
+        long_ = {b for b, e in enumerate(ext_lens) if mfma and e * group > SHORT_ROWS}
+        starts = [0, *np.cumsum(ext_lens).tolist()]
         groups = [([b for b in m if b not in long_], n) for m, n in groups]
         groups = [(m, n) for m, n in groups if len(m) > 1]
         self.shares = bool(groups)
-        rows_of = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
-        rows_of += [e * group for b, e in enumerate(ext_lens) if b not in long_]
-        self.row_groups = 2 if rows_of and max(rows_of) > 16 else 1
+        shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
+        rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
+        if not mfma:
+            rows += shared_rows
+        self.row_groups = 2 if max(rows, default=1) > 16 else 1
         unit = 16 * self.row_groups
+        self.slot_rows = min(unit, max(rows, default=1))
 
-        items, tokens = [], []
-        front = {}   # request -> (its shared part's first item, its first token there, keys)
+        items, tokens, pieces, units = [], [], [], []
+        front = {}   # request -> (its shared part, its first token there, keys)
 
-        def add(b, toks, k0, k1, pfx=-1, pfx_tok=0):
+        def add(b, tok0, n, k0, k1, pfx=-1, pfx_tok=0):
+            for row0 in range(0, n * group, unit):
+                items.append((b, tok0, n, row0, k0, k1, pfx, pfx_tok))
+
+        def add_tokens(b):
+            at = len(tokens)
+            tokens.extend((starts[b] + t, b, ext_lens[b] - 1 - t, 0) for t in range(ext_lens[b]))
+            return at
+
+        n_blocks = [-(-r // EXTEND_TILE_ROWS) for r in shared_rows]
+        cuts = cut_units([-(-n // KEYS_PER_STEP) for (_, n), k in zip(groups, n_blocks)
+                          for _ in range(k * n_kv)], cus) if mfma else []
+        for (members, length), blocks in zip(groups, n_blocks):
             tok0 = len(tokens)
-            tokens.extend(toks)
-            for row0 in range(0, len(toks) * group, unit):
-                items.append((b, tok0, len(toks), row0, k0, k1, pfx, pfx_tok))
-
-        def request_tokens(b):
-            return [(starts[b] + t, b, ext_lens[b] - 1 - t, 0) for t in range(ext_lens[b])]
-
-        for members, length in groups:
-            first, at = len(items), 0
-            toks = []
             for b in members:
-                front[b] = (first, len(toks), length)
-                toks += request_tokens(b)
-            add(members[0], toks, 0, length)
+                front[b] = (len(units) if mfma else len(items), add_tokens(b) - tok0, length)
+            n = len(tokens) - tok0
+            if not mfma:
+                add(members[0], tok0, n, 0, length)
+                continue
+            steps = -(-length // KEYS_PER_STEP)
+            for block in range(blocks):
+                for hk in range(n_kv):
+                    parts = cuts[len(units)]
+                    units.append((len(pieces), parts))
+                    for i in range(parts):
+                        k0, k1 = (KEYS_PER_STEP * (steps * x // parts) for x in (i, i + 1))
+                        pieces.append((members[0], hk, EXTEND_TILE_ROWS * block, tok0, n, k0,
+                                       min(k1, length), len(pieces) + 1))
         self.n_shared = len(items)
         for b in range(len(ext_lens)):
             if b not in long_:
                 pfx, pfx_tok, k0 = front.get(b, (-1, 0, 0))
-                add(b, request_tokens(b), k0, -1, pfx, pfx_tok)
+                add(b, add_tokens(b), ext_lens[b], k0, -1, pfx, pfx_tok)
         self.n_items = len(items)
-        self.slot_rows = min(unit, max(rows_of, default=1))
         work = np.zeros((0, 8), dtype=np.int32)
         if long_:
             work = plan_extend(ext_lens, n_q, n_kv, decode_to_decode_kernel=True)
             work = work[np.isin(work[:, 0], list(long_))]
-        self.n_work = len(work)
-        self._host = np.concatenate([
-            np.asarray(items, dtype=np.int32).reshape(-1), work.reshape(-1),
-            np.asarray(tokens, dtype=np.int32).reshape(-1)])
+        self.n_work, self.n_pieces = len(work), len(pieces)
+        parts = [np.asarray(x, dtype=np.int32).reshape(-1)
+                 for x in (items, work, pieces, tokens, units)]
+        self._offsets = np.cumsum([0] + [4 * len(x) for x in parts])[:5].tolist()
+        self._host = np.concatenate(parts)
         self._lock = threading.Lock()
         self._lists: Optional[torch.Tensor] = None
         self._users: set = set()
@@ -127,8 +163,9 @@ class _Plan:
         self._uploaded_on = 0
         self._kept = False
 
-    def lists(self) -> Tuple[int, int, int]:
-        """Addresses of (items, work, tokens) for launches on the current stream."""
+    def lists(self) -> List[int]:
+        """Addresses of (items, work, pieces, tokens, units) for launches on the current
+        stream."""
         stream = torch.cuda.current_stream(self.device)
         capturing = torch.cuda.is_current_stream_capturing()
         with self._lock:
@@ -151,7 +188,7 @@ class _Plan:
                 self._kept = True
                 _captured.append(self._lists)
             base = self._lists.data_ptr()
-        return base, base + 32 * self.n_items, base + 32 * (self.n_items + self.n_work)
+        return [base + at for at in self._offsets]
 
 
 def shared_prefix_attention(
@@ -203,7 +240,7 @@ def shared_prefix_attention(
             q = q.contiguous()
         out = _output(q, out)
         epilogue = _epilogue(q, gate, out_amax)
-        items, work, tokens = plan.lists()
+        items, work, pieces, tokens, units = plan.lists()
         handle = _native.current_stream(q.device)
         rtt = batch.req_to_token
         pool = (layer_k_buffer.data_ptr(), layer_v_buffer.data_ptr(), n_slots, kv_dtype,
@@ -212,13 +249,14 @@ def shared_prefix_attention(
                 rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
                 batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
         ws, nbytes = workspace("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
-                               plan.row_groups, plan.slot_rows, n_q, n_kv, head_dim, kv_dtype)
+                               plan.row_groups, plan.slot_rows, plan.n_pieces, n_q, n_kv,
+                               head_dim, kv_dtype)
         if plan.n_work:
             _native.call("tf_attn_extend", q.data_ptr(), q.stride(0), *pool, 0, work, plan.n_work,
                          n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), *epilogue,
                          handle)
         _native.call("tf_attn_shared", q.data_ptr(), q.stride(0), *pool, items, plan.n_items,
-                     plan.n_shared, tokens, plan.row_groups, plan.slot_rows, n_q, n_kv, head_dim,
-                     scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
+                     plan.n_shared, tokens, plan.row_groups, plan.slot_rows, pieces,
+                     plan.n_pieces, units, n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
                      handle)
     return out
