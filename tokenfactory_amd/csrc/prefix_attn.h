@@ -37,15 +37,16 @@ struct PartArgs {
   int32_t n_items, own0;
   int32_t unit_rows;       // query rows of a unit
   int32_t slot_rows;       // of them that any unit uses: rows of a partial slot
-  int32_t hkv, group, head_dim, n_blocks;
+  int32_t hkv, group, head_dim;
+  int32_t n_workers;       // waves that stream the items
   float scale_log2;
   __bf16* out;
   int64_t out_stride;
   const __bf16* gate;
   int64_t gate_stride, gate_hstride;
   uint32_t* amax;
-  int32_t* ipre;           // prefix of the items' tiles, for the merge
-  float2* part_ml;         // partials of (workgroup + unit) slots
+  int32_t* ipre;           // prefix of the items' spans, for the merge
+  float2* part_ml;         // partials of (worker + unit) slots
   float* part_o;
   // Shared parts that the extend kernel took in pieces (NULL: they are items): unit
   // pfx + (row / 256) * hkv + kv head is {first slot, slots}.

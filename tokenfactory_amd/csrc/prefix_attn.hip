@@ -12,11 +12,13 @@
 // At head_dim 256 the shared parts go through the extend kernel's MFMA tiles instead
 // (extend.hip, kPrefix), cut over their keys so that every CU has a piece.
 //
-// part_stream_kernel is the decode kernel's scheme (decode.hip: persistent workgroups
-// that own equal shares of the tiles of all units, unit = (item, kv head)), with the
-// tokens of an item looked up in a list, since a group's requests lie anywhere in the
-// batch.  Bound by HBM as that kernel: a key's K and V rows are read by one unit per 16
-// or 32 query rows.
+// part_stream_kernel does the decode kernel's tile work (decode.hip) with waves that
+// work alone: a persistent wave owns an equal share of all units' tiles (unit = (item, kv
+// head)), and what it finds of a unit is a partial of its own.  With a unit's start
+// counted as 8 tiles this is what short and ragged contexts need: 64 requests of 1 to
+// 1024 keys (139 MB) take 30 us, 45 in the decode kernel, whose workgroups join their
+// waves at the end of every unit; 64 of 4096 keys 165 us (6.5 TB/s) and 168.  Bound by
+// HBM, or by the latency of a unit's first loads where contexts are short.
 #include <math.h>
 
 #include "attn_row.h"
@@ -54,10 +56,29 @@ __device__ __forceinline__ int part_keys(const PartArgs& a, const PartItem& it) 
   return max(0, end - it.k0);
 }
 
+// What a unit costs beside its tiles (its slot ids, queries and partials), in tiles.
+constexpr int kUnitTiles = 8;
+constexpr int kHalfTiles = 8;                    // a wave stages slot ids for 8 tiles ahead,
+constexpr int kHalf = kHalfTiles * kTile;        // in two halves by turns
+
+// Positions of an item's units: its tiles behind kUnitTiles positions without work.
+__device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUnitTiles : 0; }
+
+template <class C>
+struct StreamSmem {
+  struct {
+    int32_t slots[2 * kHalf];
+    u32x4 kstage[kTile * C::kChunks];          // see stage_k
+    u32x4 qfrag[C::NG][C::kSteps][kWave];
+  } wave[kWaves];
+  int32_t ipre[kMaxItems + 1];                 // exclusive prefix of the items' spans
+  int32_t wsum[kWaves];
+};
+
 template <class C>
 __global__ void __launch_bounds__(kWaves * kWave, C::NG == 1 || C::DP == 128 ? 2 : 1)
 part_stream_kernel(PartArgs a) {
-  __shared__ DecodeSmem<C> sm;
+  __shared__ StreamSmem<C> sm;
   const int D = C::OTHER ? a.head_dim : C::DP;
   const int row_bytes = C::FP8 ? D : 2 * D;
   const int n_chunks = row_bytes / 16;
@@ -68,21 +89,30 @@ part_stream_kernel(PartArgs a) {
   const int g = lane >> 4;
   const int n = lane & 15;
 
-  item_prefix(a.n_items, [&](int i) {
-    return (part_keys<C>(a, a.items[i]) + kTile - 1) / kTile;
-  }, sm.ipre, sm.wsum);
+  // (every item by a thread of its own first: three loads in a row each)
+  int32_t* spans = reinterpret_cast<int32_t*>(&sm.wave[0]);
+  static_assert(sizeof(sm.wave) >= 4 * kMaxItems, "spans of the items");
+  for (int i = tid; i < a.n_items; i += kWaves * kWave)
+    spans[i] = unit_span((part_keys<C>(a, a.items[i]) + kTile - 1) / kTile);
+  __syncthreads();
+  item_prefix(a.n_items, [&](int i) { return spans[i]; }, sm.ipre, sm.wsum);
   if (blockIdx.x == 0)
     for (int i = tid; i <= a.n_items; i += kWaves * kWave) a.ipre[i] = sm.ipre[i];
+  // Every wave is a worker of its own: what a unit costs in front of its tiles (loads in
+  // a row) is then hidden by the other waves of the CU, and nothing is joined here.
   const int64_t N = (int64_t)a.hkv * sm.ipre[a.n_items];
-  const int P = (int)min<int64_t>(a.n_blocks, N);   // (owners of a unit are consecutive)
-  if ((int)blockIdx.x >= P) return;
-  const int64_t x_end = (int64_t)(blockIdx.x + 1) * N / P;
-  int64_t x = (int64_t)blockIdx.x * N / P;
+  const int P = (int)min<int64_t>(a.n_workers, N);   // (owners of a unit are consecutive)
+  const int me = blockIdx.x * kWaves + w;
+  if (me >= P) return;
+  const int64_t x_end = (int64_t)(me + 1) * N / P;
+  int64_t x = (int64_t)me * N / P;
 
   const float sl2 = a.scale_log2 * (C::FP8 ? a.k_scale[0] : 1.f);
   const int64_t slot_bytes = (int64_t)a.hkv * row_bytes;
+  int32_t* const slots = sm.wave[w].slots;
+  u32x4* const ks = sm.wave[w].kstage;
 
-  int item = 0;   // the first whose tiles reach x
+  int item = 0;   // the first whose units reach x
   {
     int lo = 0, hi = a.n_items - 1;
     while (lo < hi) {
@@ -95,12 +125,14 @@ part_stream_kernel(PartArgs a) {
   while (x < x_end) {
     // ---- the segment: unit (item, hk), tiles [t0, t1)
     while ((int64_t)a.hkv * sm.ipre[item + 1] <= x) ++item;
-    const int Ti = sm.ipre[item + 1] - sm.ipre[item];
+    const int span = sm.ipre[item + 1] - sm.ipre[item];
     const int64_t r = x - (int64_t)a.hkv * sm.ipre[item];
-    const int hk = (int)(r / Ti);
-    const int t0 = (int)(r - (int64_t)hk * Ti);
-    const int t1 = (int)min<int64_t>(Ti, t0 + (x_end - x));
-    x += t1 - t0;
+    const int hk = (int)(r / span);
+    const int v0 = (int)(r - (int64_t)hk * span);
+    const int v1 = (int)min<int64_t>(span, v0 + (x_end - x));
+    x += v1 - v0;
+    const int t0 = max(0, v0 - kUnitTiles), t1 = v1 - kUnitTiles;
+    if (t0 >= t1) continue;
 
     const PartItem im = a.items[item];
     const int L = part_keys<C>(a, im);
@@ -120,98 +152,107 @@ part_stream_kernel(PartArgs a) {
       seen = token_seen(a, tok) - im.k0;
       return 16 * q + n < n_rows;
     };
+    u32x4 qf[C::kSteps];
     int seen[C::NG];
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
       int qrow, hq;
-      row_of(q, qrow, hq, seen[q]);
+      const bool ok = row_of(q, qrow, hq, seen[q]);
+      const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+      for (int kk = 0; kk < C::kSteps; ++kk) {
+        const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
+        qf[kk] = ok && (!C::OTHER || d0 < D) ? ld_g16(qp + d0) : u32x4{0u, 0u, 0u, 0u};
+      }
+      if (C::NG > 1) {   // (one group's stay in registers)
+#pragma unroll
+        for (int kk = 0; kk < C::kSteps; ++kk) sm.wave[w].qfrag[q][kk][lane] = qf[kk];
+      }
     }
 
     WaveState<C> st;
     reset_state<C>(st);
-    for (int sub = t0; sub < t1; sub += kMaxChunk / kTile) {
-      const int c0 = sub * kTile;
-      const int n_loc = min(L, min(t1, sub + kMaxChunk / kTile) * kTile) - c0;
-      const int n_tiles = (n_loc + kTile - 1) / kTile;
-      // ---- the slot ids (and, once per segment, the Q^T fragments)
-      __syncthreads();
-      for (int i = tid; i < n_loc; i += kWaves * kWave)
-        sm.u.loop.slots[i] = (int32_t)pool_row(rtt[c0 + i], a.pool_slots, false);
-      if (sub == t0) {
+    const int c0 = t0 * kTile;                    // keys below are counted from here
+    const int n_loc = min(L, t1 * kTile) - c0;
+    const int n_tiles = t1 - t0;
+    // Slot ids of half h: key k's at slots[k % (2 kHalf)]; keys past the last repeat it.
+    int64_t ids[kHalf / kWave];
+    auto fetch_ids = [&](int h) {
 #pragma unroll
-        for (int q = 0; q < C::NG; ++q) {
-          if (w != q % kWaves || q >= n_groups) continue;
-          int qrow, hq, s;
-          const bool ok = row_of(q, qrow, hq, s);
-          const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
+      for (int i = 0; i < kHalf / kWave; ++i)
+        ids[i] = rtt[c0 + min(h * kHalf + i * kWave + lane, n_loc - 1)];
+    };
+    auto stage_ids = [&](int h) {
 #pragma unroll
-          for (int kk = 0; kk < C::kSteps; ++kk) {
-            const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
-            sm.qfrag[q][kk][lane] =
-                ok && (!C::OTHER || d0 < D) ? ld_g16(qp + d0) : u32x4{0u, 0u, 0u, 0u};
-          }
-        }
-      }
-      __syncthreads();
+      for (int i = 0; i < kHalf / kWave; ++i)
+        slots[(h & 1) * kHalf + i * kWave + lane] =
+            (int32_t)pool_row(ids[i], a.pool_slots, false);
+      wave_lds_sync();
+    };
+    auto issue = [&](u32x4 (&x)[4][C::kS], int it, const uint8_t* base) {
+      issue_rows<C>(x, slots, it & (2 * kHalfTiles - 1), 2 * kHalf, g, n, base, slot_bytes,
+                    n_chunks);
+    };
+    wave_lds_sync();
+    fetch_ids(0);
+    stage_ids(0);
 
-      // ---- this wave's tiles, loads a tile ahead (see decode_kernel)
-      int it = w;
-      if (it < n_tiles) {
-        u32x4 qf[C::kSteps];
-        if (C::NG == 1) {
+    // ---- the tiles, loads a tile ahead (see decode_kernel)
+    KBuf<C> kb;
+    VBuf<C> vb;
+    auto scores = [&](int it, u32x2 (&pt)[C::NG], u32x2 (&pl)[C::NG][2]) {
+      u32x4 kf[C::kSteps];
+      k_frags<C>(ks, g, n, kf);
 #pragma unroll
-          for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.qfrag[0][kk][lane];
+      for (int q = 0; q < C::NG; ++q) {
+        if (C::NG > 1) {
+          if (q >= n_groups) break;
+#pragma unroll
+          for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.wave[w].qfrag[q][kk][lane];
         }
-        KBuf<C> kb;
-        VBuf<C> vb;
-        const int32_t* slots = sm.u.loop.slots;
-        u32x4* ks = sm.u.loop.kstage[w];
-        auto scores = [&](int it, u32x2 (&pt)[C::NG], u32x2 (&pl)[C::NG][2]) {
-          u32x4 kf[C::kSteps];
-          k_frags<C>(ks, g, n, kf);
-#pragma unroll
-          for (int q = 0; q < C::NG; ++q) {
-            if (C::NG > 1) {
-              if (q >= n_groups) break;
-#pragma unroll
-              for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.qfrag[q][kk][lane];
-            }
-            const int lim = min(n_loc, seen[q] - c0);
-            pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q],
-                                  [](const float (&)[4]) {});
-          }
-        };
-        u32x2 pt[C::NG], pl[C::NG][2];
-        issue_rows<C>(kb.k, slots, it, n_loc, g, n, kbase, slot_bytes, n_chunks);
-        issue_rows<C>(vb.v, slots, it, n_loc, g, n, vbase, slot_bytes, n_chunks);
-        for (; it + kWaves < n_tiles; it += kWaves) {
-          stage_k<C>(kb, ks, g, n);
-          __builtin_amdgcn_sched_barrier(0);
-          issue_rows<C>(kb.k, slots, it + kWaves, n_loc, g, n, kbase, slot_bytes, n_chunks);
-          __builtin_amdgcn_sched_barrier(0);
-          scores(it, pt, pl);
-          pv<C>(vb, pt, pl, st, n_groups);
-          __builtin_amdgcn_sched_barrier(0);
-          issue_rows<C>(vb.v, slots, it + kWaves, n_loc, g, n, vbase, slot_bytes, n_chunks);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        stage_k<C>(kb, ks, g, n);
-        scores(it, pt, pl);
-        pv<C>(vb, pt, pl, st, n_groups);
+        const int lim = min(n_loc, seen[q] - c0);
+        pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [](const float (&)[4]) {});
       }
+    };
+    u32x2 pt[C::NG], pl[C::NG][2];
+    issue(kb.k, 0, kbase);
+    issue(vb.v, 0, vbase);
+    int it = 0;
+    for (; it + 1 < n_tiles; ++it) {
+      // The ids of the next half, read while this one's tiles go by; its place held the
+      // half before, whose last tile is issued.
+      const int at = it & (kHalfTiles - 1);
+      if (at == 0)
+        fetch_ids(it / kHalfTiles + 1);
+      else if (at == kHalfTiles / 2)
+        stage_ids(it / kHalfTiles + 1);
+      wave_lds_sync();
+      stage_k<C>(kb, ks, g, n);
+      wave_lds_sync();
+      __builtin_amdgcn_sched_barrier(0);
+      issue(kb.k, it + 1, kbase);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(it, pt, pl);
+      pv<C>(vb, pt, pl, st, n_groups);
+      __builtin_amdgcn_sched_barrier(0);
+      issue(vb.v, it + 1, vbase);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    wave_lds_sync();
+    stage_k<C>(kb, ks, g, n);
+    wave_lds_sync();
+    scores(it, pt, pl);
+    pv<C>(vb, pt, pl, st, n_groups);
 
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
       st.l[q] += __shfl_xor(st.l[q], 16, kWave);
       st.l[q] += __shfl_xor(st.l[q], 32, kWave);
     }
-    block_merge<C>(sm.u.merge, w, lane, st, n_groups);
-    if (w != 0) continue;
-    // Partials of (workgroup, unit), a row's dims side by side.  Lane (g, n) holds of
+    // Partials of (worker, unit), a row's dims side by side.  Lane (g, n) holds of
     // row n the dims 128 s + 32 g + 8 r + e (bf16: accumulator 8 s + e) or 64 g + 16 r
     // + e (fp8), four neighbours per store.
-    const int64_t slot = (int64_t)blockIdx.x + (int64_t)item * a.hkv + hk;
+    const int64_t slot = (int64_t)me + (int64_t)item * a.hkv + hk;
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
       if (16 * q + n >= n_rows) continue;
@@ -245,13 +286,13 @@ struct Owners {
   int count;
 };
 __device__ __forceinline__ Owners unit_owners(const PartArgs& a, int item, int hk) {
-  const int before = a.ipre[item], Ti = a.ipre[item + 1] - before, total = a.ipre[a.n_items];
-  if (Ti == 0) return Owners{0, 0};
-  const int64_t N = (int64_t)a.hkv * total;
-  const int64_t p = (int64_t)a.hkv * before + (int64_t)hk * Ti;
-  const int P = (int)min<int64_t>(a.n_blocks, N);
-  const int b0 = owner_of(p, N, P);
-  return Owners{b0 + (int64_t)item * a.hkv + hk, owner_of(p + Ti - 1, N, P) - b0 + 1};
+  const int before = a.ipre[item], span = a.ipre[item + 1] - before;
+  if (span == 0) return Owners{0, 0};
+  const int64_t N = (int64_t)a.hkv * a.ipre[a.n_items];
+  const int64_t p = (int64_t)a.hkv * before + (int64_t)hk * span;
+  const int P = (int)min<int64_t>(a.n_workers, N);
+  const int b0 = owner_of(p + kUnitTiles, N, P);
+  return Owners{b0 + (int64_t)item * a.hkv + hk, owner_of(p + span - 1, N, P) - b0 + 1};
 }
 
 template <int DP, bool FP8, int WPR>
@@ -395,7 +436,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
 struct PartPlan {
   bool fp8, narrow, other;
   int32_t unit_rows;    // 16 or 32
-  int32_t n_blocks;     // persistent workgroups
+  int32_t n_workers;    // persistent waves
   int64_t ipre_bytes, ml_bytes, o_bytes, piece_ml_bytes, piece_o_bytes;
   int64_t total() const {
     return ipre_bytes + ml_bytes + o_bytes + piece_ml_bytes + piece_o_bytes;
@@ -426,8 +467,12 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   p->other = head_dim != 256;
   p->narrow = head_dim <= 128 && !p->fp8;
   p->unit_rows = 16 * row_groups;
-  p->n_blocks = device_cu_count() * (p->narrow ? 2 : 1);
-  const int64_t rows = (p->n_blocks + (int64_t)n_items * num_kv_heads) * slot_rows;
+  // Four waves per CU, eight of the 128-dim ones (measured with half and twice as many:
+  // 64 requests of 1 to 1024 keys 30 us, 42 with eight waves per CU; 16 of 1 to 2048 in
+  // units of 32 rows 28 and 37 us with two; 96 of 1 to 700 at 32 / 8 heads of 128 56 us,
+  // 83 with four).
+  p->n_workers = kWaves * device_cu_count() * (p->narrow ? 2 : 1);
+  const int64_t rows = (p->n_workers + (int64_t)n_items * num_kv_heads) * slot_rows;
   p->ipre_bytes = ((int64_t)(n_items + 1) * 4 + 255) / 256 * 256;
   p->ml_bytes = (rows * 8 + 255) / 256 * 256;
   p->o_bytes = rows * (p->narrow ? 128 : 256) * 4;
@@ -438,8 +483,8 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
 
 template <class C>
 void launch_stream(const PartArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((part_stream_kernel<C>), dim3((unsigned)a.n_blocks), dim3(kWaves * kWave), 0,
-                     s, a);
+  hipLaunchKernelGGL((part_stream_kernel<C>), dim3((unsigned)(a.n_workers / kWaves)),
+                     dim3(kWaves * kWave), 0, s, a);
 }
 
 template <int NG>
@@ -532,7 +577,7 @@ extern "C" int32_t tf_attn_shared(
   a.hkv = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
   a.head_dim = head_dim;
-  a.n_blocks = p.n_blocks;
+  a.n_workers = p.n_workers;
   a.scale_log2 = scale * kLog2e;
   a.out = static_cast<__bf16*>(out);
   a.out_stride = out_row_stride;
