@@ -337,6 +337,28 @@ int32_t tf_attn_shared(
     void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
 
+/* tf_attn_scored: tf_attn_decode (every request one token, q row b) and tf_attn_weights in
+ * one pass: the scores of the attention itself are kept in the workspace and become
+ * weights once every row's sum is known.  head_dim a multiple of 8 (fp8 pools: 16) up to
+ * 256; batch_size * ceil(num_q_heads / num_kv_heads / 16) at most 2048; max_len: the keys
+ * per request whose scores the workspace holds (a longer context's weights end there).
+ * Workspace: tf_attn_scored_workspace_bytes of the same sizes, 16-byte aligned; calls that
+ * overlap in time must not share it. */
+int64_t tf_attn_scored_workspace_bytes(int32_t batch_size, int32_t max_len, int32_t num_q_heads,
+                                       int32_t num_kv_heads, int32_t head_dim,
+                                       int32_t kv_dtype);
+
+int32_t tf_attn_scored(
+    const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+    int64_t pool_slots, int32_t kv_dtype, const float* k_scale, const float* v_scale,
+    const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
+    const int64_t* req_pool_indices, const int64_t* seq_lens, int32_t seq_len_override,
+    int32_t batch_size, int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, float scale, void* out, int64_t out_row_stride, float* scores,
+    int64_t scores_row_stride, int32_t add, void* workspace, int64_t workspace_bytes,
+    const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax,
+    tf_stream_t stream);
+
 /* tf_attn_weights: scores[req_pool_indices[b], k] += (add 0: =) the softmax weights that
  * request b's last min(window, extend_lens[b]) new tokens give key k, summed in fp32 over
  * those tokens and all query heads, for k < seq_lens[b] (each a table row of its own;

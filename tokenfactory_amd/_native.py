@@ -129,6 +129,20 @@ SIGNATURES = {
         _p, _i64, _i64,
         _p, _p,
     ]),
+    "tf_attn_scored_workspace_bytes": (_i64, [_i32] * 6),
+    "tf_attn_scored": (_i32, [
+        _p, _i64,
+        _p, _p, _i64, _i32, _p, _p,
+        _p, _i64, _i64, _i64,
+        _p, _p, _i32,                  # req_pool_indices, seq_lens, its override
+        _i32, _i32,                    # batch_size, max_len
+        _i32, _i32, _i32, _f32,
+        _p, _i64,
+        _p, _i64, _i32,                # scores, scores_row_stride, add
+        _p, _i64,                      # workspace, workspace_bytes
+        _p, _i64, _i64,
+        _p, _p,
+    ]),
     "tf_attn_weights_workspace_bytes": (_i64, [_i32] * 7),
     "tf_attn_weights": (_i32, [
         _p, _i64, _i64,                # q, q_row_stride, q_rows

@@ -32,8 +32,12 @@ struct PartArgs {
   int64_t rtt_rows, rtt_stride, rtt_cols;
   const int64_t* rpi;
   const int64_t* seq_lens;
-  const PartItem* items;   // shared parts, then the requests' own (from own0)
+  int32_t seq_override;
+  // Shared parts, then the requests' own (from own0).  NULL (and toks): one new token per
+  // request, item i the i % head_blocks-th block of its heads.
+  const PartItem* items;
   const PartTok* toks;
+  int32_t head_blocks;
   int32_t n_items, own0;
   int32_t unit_rows;       // query rows of a unit
   int32_t slot_rows;       // of them that any unit uses: rows of a partial slot
@@ -53,6 +57,11 @@ struct PartArgs {
   const int2* units;
   const float2* piece_ml;  // [slot][256], [slot][256][256]
   const float* piece_o;
+  // Scored calls: every row's scores (log2 units, -inf where masked) of its first
+  // score_cap keys, row q_row * q heads + head, and its log2 of the sum of 2^score.
+  float* row_scores;
+  int64_t score_cap;
+  float* row_lse;
 };
 
 }  // namespace tfa

@@ -32,8 +32,18 @@ namespace {
 
 // The context length of a request, clamped to its table row.
 __device__ __forceinline__ int context_len(const PartArgs& a, int b) {
-  const int64_t len = min(a.seq_lens[b], a.rtt_cols);
+  const int64_t len =
+      min(a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b], a.rtt_cols);
   return len > 0 ? (int)len : 0;
+}
+
+__device__ __forceinline__ PartItem item_at(const PartArgs& a, int i) {
+  if (a.items) return a.items[i];
+  const int b = i / a.head_blocks;
+  return PartItem{b, b, 1, (i - b * a.head_blocks) * a.unit_rows, 0, -1, -1, 0};
+}
+__device__ __forceinline__ PartTok tok_at(const PartArgs& a, int i) {
+  return a.toks ? a.toks[i] : PartTok{i, i, 0, 0};
 }
 
 // Keys that token t of an item sees, counted from key 0.
@@ -51,7 +61,7 @@ __device__ __forceinline__ int part_keys(const PartArgs& a, const PartItem& it) 
     end = min((int64_t)it.k1, a.rtt_cols);
   } else {
     const int last = min(it.row0 + C::kRows, it.n_tok * a.group) - 1;
-    end = token_seen(a, a.toks[it.tok0 + last / a.group]);
+    end = token_seen(a, tok_at(a, it.tok0 + last / a.group));
   }
   return max(0, end - it.k0);
 }
@@ -75,7 +85,9 @@ struct StreamSmem {
   int32_t wsum[kWaves];
 };
 
-template <class C>
+// SCORED: the scores are kept (16 bytes per row and four keys, a few percent of the keys'
+// own bytes), for the weights that follow.
+template <class C, bool SCORED>
 __global__ void __launch_bounds__(kWaves * kWave, C::NG == 1 || C::DP == 128 ? 2 : 1)
 part_stream_kernel(PartArgs a) {
   __shared__ StreamSmem<C> sm;
@@ -93,7 +105,7 @@ part_stream_kernel(PartArgs a) {
   int32_t* spans = reinterpret_cast<int32_t*>(&sm.wave[0]);
   static_assert(sizeof(sm.wave) >= 4 * kMaxItems, "spans of the items");
   for (int i = tid; i < a.n_items; i += kWaves * kWave)
-    spans[i] = unit_span((part_keys<C>(a, a.items[i]) + kTile - 1) / kTile);
+    spans[i] = unit_span((part_keys<C>(a, item_at(a, i)) + kTile - 1) / kTile);
   __syncthreads();
   item_prefix(a.n_items, [&](int i) { return spans[i]; }, sm.ipre, sm.wsum);
   if (blockIdx.x == 0)
@@ -134,7 +146,7 @@ part_stream_kernel(PartArgs a) {
     const int t0 = max(0, v0 - kUnitTiles), t1 = v1 - kUnitTiles;
     if (t0 >= t1) continue;
 
-    const PartItem im = a.items[item];
+    const PartItem im = item_at(a, item);
     const int L = part_keys<C>(a, im);
     const int n_rows = im.n_tok * a.group - im.row0;       // of kRows
     const int n_groups = min((n_rows + 15) / 16, C::NG);
@@ -146,7 +158,7 @@ part_stream_kernel(PartArgs a) {
     auto row_of = [&](int q, int& qrow, int& hq, int& seen) {
       const int rho = im.row0 + min(16 * q + n, n_rows - 1);
       const int t = rho / a.group;
-      const PartTok tok = a.toks[im.tok0 + t];
+      const PartTok tok = tok_at(a, im.tok0 + t);
       qrow = tok.qrow;
       hq = hk * a.group + rho - t * a.group;
       seen = token_seen(a, tok) - im.k0;
@@ -154,11 +166,14 @@ part_stream_kernel(PartArgs a) {
     };
     u32x4 qf[C::kSteps];
     int seen[C::NG];
+    float* kept[C::NG];   // where the lane's row n of group q keeps its scores (or NULL)
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
       int qrow, hq;
       const bool ok = row_of(q, qrow, hq, seen[q]);
       const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
+      kept[q] = SCORED && ok ? a.row_scores + ((int64_t)qrow * a.hkv * a.group + hq) * a.score_cap
+                             : nullptr;
 #pragma unroll
       for (int kk = 0; kk < C::kSteps; ++kk) {
         const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
@@ -186,7 +201,7 @@ part_stream_kernel(PartArgs a) {
 #pragma unroll
       for (int i = 0; i < kHalf / kWave; ++i)
         slots[(h & 1) * kHalf + i * kWave + lane] =
-            (int32_t)pool_row(ids[i], a.pool_slots, false);
+            (int32_t)pool_row(ids[i], a.pool_slots, a.seq_override > 0);
       wave_lds_sync();
     };
     auto issue = [&](u32x4 (&x)[4][C::kS], int it, const uint8_t* base) {
@@ -211,7 +226,11 @@ part_stream_kernel(PartArgs a) {
           for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.wave[w].qfrag[q][kk][lane];
         }
         const int lim = min(n_loc, seen[q] - c0);
-        pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [](const float (&)[4]) {});
+        pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [&](const float (&sc)[4]) {
+          const int k = im.k0 + c0 + it * kTile;
+          if (SCORED && kept[q] && k < a.score_cap)
+            *reinterpret_cast<f32x4*>(kept[q] + k + 4 * g) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+        });
       }
     };
     u32x2 pt[C::NG], pl[C::NG][2];
@@ -304,7 +323,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
   const int w = wave_id();
   const int item = a.own0 + (int)(blockIdx.x / a.hkv);
   const int hk = (int)(blockIdx.x % a.hkv);
-  const PartItem im = a.items[item];
+  const PartItem im = item_at(a, item);
   const int n = (int)blockIdx.y * kRows + w / WPR;     // the wave's row of the unit
   const int n_rows = im.b < 0 ? 0 : min(im.n_tok * a.group - im.row0, a.unit_rows);
   if ((int)blockIdx.y * kRows >= n_rows) return;
@@ -312,7 +331,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
 
   const int rho = im.row0 + min(n, n_rows - 1);
   const int t = rho / a.group;
-  const PartTok tok = a.toks[im.tok0 + t];
+  const PartTok tok = tok_at(a, im.tok0 + t);
   const int hq = hk * a.group + rho - t * a.group;
   const int D = a.head_dim;
   const bool lane_in = 4 * lane < DP, lane_out = 4 * lane < D;
@@ -398,6 +417,9 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     }
   }
 
+  // (+inf for a row without a visible key: its weights are zeros)
+  if (write && a.row_lse && lane == 0)
+    a.row_lse[(int64_t)tok.qrow * a.hkv * a.group + hq] = l == 0.f ? INFINITY : m + log2f(l);
   uint32_t om = 0;
   const float vscale = FP8 ? a.v_scale[0] : 1.f;
   __bf16* orow = a.out + (int64_t)tok.qrow * a.out_stride + (int64_t)hq * D;
@@ -408,7 +430,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     attend_row<FP8>(rs, a.q + (int64_t)tok.qrow * a.q_stride + (int64_t)hq * D,
                     reinterpret_cast<uint32_t*>(&so[w][0]), D,
                     a.rtt + clamp_i64(a.rpi[im.b], 0, a.rtt_rows - 1) * a.rtt_stride, 0, seen,
-                    a.pool_slots, false, a.k_pool + (int64_t)hk * row_bytes,
+                    a.pool_slots, a.seq_override > 0, a.k_pool + (int64_t)hk * row_bytes,
                     a.v_pool + (int64_t)hk * row_bytes, (int64_t)a.hkv * row_bytes,
                     a.scale_log2 * (FP8 ? a.k_scale[0] : 1.f), lane);
     om = write_row(rs, seen > 0 ? vscale / rs.l : 0.f, D, orow,
@@ -430,6 +452,52 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     *reinterpret_cast<u32x2*>(orow + 4 * lane) = o;
   }
   amax_commit(a.amax, om);
+}
+
+// scores[row, k] (+)= sum of 2^(score - lse) over the request's heads, four keys a thread.
+constexpr int kScoreThreads = 256;
+struct ScoreArgs {
+  const float* row_scores;
+  const float* row_lse;
+  int64_t score_cap;
+  const int64_t* rpi;
+  const int64_t* seq_lens;
+  int64_t rtt_rows, rtt_cols;
+  int32_t seq_override, hq, add;
+  float* scores;
+  int64_t scores_stride;
+};
+__global__ void __launch_bounds__(kScoreThreads) add_weights_kernel(ScoreArgs a) {
+  const int b = blockIdx.y;
+  int64_t len = min(min(a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b], a.rtt_cols),
+                    a.score_cap);
+  const float* rows = a.row_scores + (int64_t)b * a.hq * a.score_cap;
+  const float* lse = a.row_lse + (int64_t)b * a.hq;
+  float* out = a.scores + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.scores_stride;
+  constexpr int kStep = 4;   // heads in flight
+  for (int64_t k = 4 * ((int64_t)blockIdx.x * kScoreThreads + threadIdx.x); k < len;
+       k += 4 * (int64_t)gridDim.x * kScoreThreads) {
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    for (int h0 = 0; h0 < a.hq; h0 += kStep) {
+      f32x4 s[kStep];
+      float off[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int h = min(h0 + i, a.hq - 1);
+        s[i] = *reinterpret_cast<const f32x4*>(rows + h * a.score_cap + k);
+        off[i] = h0 + i < a.hq ? lse[h] : INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        if (h0 + i >= a.hq) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] += fast_exp2(s[i][e] - off[i]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < len) out[k + e] = a.add ? out[k + e] + w[e] : w[e];
+  }
 }
 
 // Kernel shape and workspace of a call.
@@ -481,19 +549,19 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   return TF_OK;
 }
 
-template <class C>
+template <class C, bool SCORED>
 void launch_stream(const PartArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((part_stream_kernel<C>), dim3((unsigned)(a.n_workers / kWaves)),
+  hipLaunchKernelGGL((part_stream_kernel<C, SCORED>), dim3((unsigned)(a.n_workers / kWaves)),
                      dim3(kWaves * kWave), 0, s, a);
 }
 
-template <int NG>
+template <int NG, bool SCORED>
 void launch_stream_groups(const PartArgs& a, const PartPlan& p, hipStream_t s) {
-  if (p.narrow) return launch_stream<Cfg<128, false, NG, true, true>>(a, s);
-  if (p.other && p.fp8) return launch_stream<Cfg<256, true, NG, true, true>>(a, s);
-  if (p.other) return launch_stream<Cfg<256, false, NG, true, true>>(a, s);
-  if (p.fp8) return launch_stream<Cfg<256, true, NG, false, true>>(a, s);
-  return launch_stream<Cfg<256, false, NG, false, true>>(a, s);
+  if (p.narrow) return launch_stream<Cfg<128, false, NG, true, true>, SCORED>(a, s);
+  if (p.other && p.fp8) return launch_stream<Cfg<256, true, NG, true, true>, SCORED>(a, s);
+  if (p.other) return launch_stream<Cfg<256, false, NG, true, true>, SCORED>(a, s);
+  if (p.fp8) return launch_stream<Cfg<256, true, NG, false, true>, SCORED>(a, s);
+  return launch_stream<Cfg<256, false, NG, false, true>, SCORED>(a, s);
 }
 
 template <int WPR>
@@ -507,6 +575,49 @@ void launch_merge(const PartArgs& a, const PartPlan& p, int n_own, int rows, hip
     hipLaunchKernelGGL((part_merge_kernel<256, true, WPR>), grid, block, 0, s, a);
   else
     hipLaunchKernelGGL((part_merge_kernel<256, false, WPR>), grid, block, 0, s, a);
+}
+
+PartArgs part_args(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                   int64_t pool_slots, const float* k_scale, const float* v_scale,
+                   const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride,
+                   int64_t rtt_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                   int32_t n_items, int32_t slot_rows, int32_t num_q_heads, int32_t num_kv_heads,
+                   int32_t head_dim, float scale, void* out, int64_t out_row_stride,
+                   void* workspace, const void* gate, int64_t gate_row_stride,
+                   int64_t gate_head_stride, uint32_t* out_amax, const PartPlan& p) {
+  PartArgs a = {};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_stride = q_row_stride;
+  a.k_pool = static_cast<const uint8_t*>(k_pool);
+  a.v_pool = static_cast<const uint8_t*>(v_pool);
+  a.pool_slots = pool_slots;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.rtt = req_to_token;
+  a.rtt_rows = rtt_rows;
+  a.rtt_stride = rtt_row_stride;
+  a.rtt_cols = rtt_cols;
+  a.rpi = req_pool_indices;
+  a.seq_lens = seq_lens;
+  a.n_items = n_items;
+  a.unit_rows = p.unit_rows;
+  a.slot_rows = slot_rows;
+  a.hkv = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.head_dim = head_dim;
+  a.n_workers = p.n_workers;
+  a.scale_log2 = scale * kLog2e;
+  a.out = static_cast<__bf16*>(out);
+  a.out_stride = out_row_stride;
+  a.gate = static_cast<const __bf16*>(gate);
+  a.gate_stride = gate_row_stride;
+  a.gate_hstride = gate_head_stride;
+  a.amax = out_amax;
+  char* ws = static_cast<char*>(workspace);
+  a.ipre = reinterpret_cast<int32_t*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ipre_bytes);
+  a.part_o = reinterpret_cast<float*>(ws + p.ipre_bytes + p.ml_bytes);
+  return a;
 }
 
 }  // namespace
@@ -554,45 +665,18 @@ extern "C" int32_t tf_attn_shared(
     return fail(TF_ERR_INVALID, "shared: items and tokens must be 16-byte aligned");
   if (n_pieces && (!pieces || !units || !aligned16(pieces) || !aligned8(units)))
     return fail(TF_ERR_INVALID, "shared: pieces and units must be 16- and 8-byte aligned");
-  PartArgs a = {};
-  a.q = static_cast<const __bf16*>(q);
-  a.q_stride = q_row_stride;
-  a.k_pool = static_cast<const uint8_t*>(k_pool);
-  a.v_pool = static_cast<const uint8_t*>(v_pool);
-  a.pool_slots = pool_slots;
-  a.k_scale = k_scale;
-  a.v_scale = v_scale;
-  a.rtt = req_to_token;
-  a.rtt_rows = rtt_rows;
-  a.rtt_stride = rtt_row_stride;
-  a.rtt_cols = rtt_cols;
-  a.rpi = req_pool_indices;
-  a.seq_lens = seq_lens;
+  PartArgs a = part_args(q, q_row_stride, k_pool, v_pool, pool_slots, k_scale, v_scale,
+                         req_to_token, rtt_rows, rtt_row_stride, rtt_cols, req_pool_indices,
+                         seq_lens, n_items, slot_rows, num_q_heads, num_kv_heads, head_dim, scale,
+                         out, out_row_stride, workspace, gate, gate_row_stride, gate_head_stride,
+                         out_amax, p);
   a.items = reinterpret_cast<const PartItem*>(items);
   a.toks = reinterpret_cast<const PartTok*>(tokens);
-  a.n_items = n_items;
   a.own0 = n_shared;
-  a.unit_rows = p.unit_rows;
-  a.slot_rows = slot_rows;
-  a.hkv = num_kv_heads;
-  a.group = num_q_heads / num_kv_heads;
-  a.head_dim = head_dim;
-  a.n_workers = p.n_workers;
-  a.scale_log2 = scale * kLog2e;
-  a.out = static_cast<__bf16*>(out);
-  a.out_stride = out_row_stride;
-  a.gate = static_cast<const __bf16*>(gate);
-  a.gate_stride = gate_row_stride;
-  a.gate_hstride = gate_head_stride;
-  a.amax = out_amax;
-  char* ws = static_cast<char*>(workspace);
-  a.ipre = reinterpret_cast<int32_t*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.ipre_bytes);
-  a.part_o = reinterpret_cast<float*>(ws + p.ipre_bytes + p.ml_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (n_pieces) {
     a.units = reinterpret_cast<const int2*>(units);
-    char* at = ws + p.ipre_bytes + p.ml_bytes + p.o_bytes;
+    char* at = static_cast<char*>(workspace) + p.ipre_bytes + p.ml_bytes + p.o_bytes;
     a.piece_ml = reinterpret_cast<float2*>(at);
     a.piece_o = reinterpret_cast<float*>(at + p.piece_ml_bytes);
     ExtendArgs e = {};
@@ -620,11 +704,118 @@ extern "C" int32_t tf_attn_shared(
     if (rc != TF_OK) return rc;
   }
   if (row_groups == 1)
-    launch_stream_groups<1>(a, p, s);
+    launch_stream_groups<1, false>(a, p, s);
   else
-    launch_stream_groups<2>(a, p, s);
+    launch_stream_groups<2, false>(a, p, s);
   rc = launch_status("tf_attn_shared stream launch");
   if (rc != TF_OK) return rc;
   launch_merge<4>(a, p, n_items - n_shared, slot_rows, s);
   return launch_status("tf_attn_shared merge launch");
+}
+
+namespace tfa {
+namespace {
+
+// tf_attn_scored: one new token per request.
+struct ScoredPlan {
+  PartPlan p;
+  int32_t n_items, head_blocks, slot_rows;
+  int64_t cap, scores_bytes, lse_bytes;
+  int64_t total() const { return p.total() + scores_bytes + lse_bytes; }
+};
+
+int make_scored_plan(int32_t batch, int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads,
+                     int32_t head_dim, int32_t kv_dtype, ScoredPlan* r) {
+  if (batch < 0 || max_len < 1 || num_kv_heads <= 0 || num_q_heads <= 0)
+    return fail(TF_ERR_INVALID, "scored: batch=%d max_len=%d heads %d/%d", batch, max_len,
+                num_q_heads, num_kv_heads);
+  const int32_t group = num_q_heads / num_kv_heads;
+  r->head_blocks = (group + 15) / 16;
+  r->slot_rows = group < 1 ? 1 : group < 16 ? group : 16;
+  if ((int64_t)batch * r->head_blocks > kMaxItems)
+    return fail(TF_ERR_UNSUPPORTED, "scored: %d requests of %d head blocks (at most %d)", batch,
+                r->head_blocks, kMaxItems);
+  r->n_items = batch * r->head_blocks;
+  const int rc = make_part_plan("scored", r->n_items, 1, r->slot_rows, 0, num_q_heads,
+                                num_kv_heads, head_dim, kv_dtype, &r->p);
+  if (rc != TF_OK) return rc;
+  r->p.o_bytes = (r->p.o_bytes + 255) / 256 * 256;
+  r->cap = ((int64_t)max_len + kTile - 1) / kTile * kTile;
+  r->scores_bytes = (int64_t)batch * num_q_heads * r->cap * 4;
+  r->lse_bytes = (int64_t)batch * num_q_heads * 4;
+  return TF_OK;
+}
+
+}  // namespace
+}  // namespace tfa
+
+extern "C" int64_t tf_attn_scored_workspace_bytes(int32_t batch_size, int32_t max_len,
+                                                  int32_t num_q_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim, int32_t kv_dtype) {
+  using namespace tfa;
+  clear_error();
+  ScoredPlan r;
+  const int rc = make_scored_plan(batch_size, max_len, num_q_heads, num_kv_heads, head_dim,
+                                  kv_dtype, &r);
+  return rc != TF_OK ? rc : r.total();
+}
+
+extern "C" int32_t tf_attn_scored(
+    const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+    int64_t pool_slots, int32_t kv_dtype, const float* k_scale, const float* v_scale,
+    const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
+    const int64_t* req_pool_indices, const int64_t* seq_lens, int32_t seq_len_override,
+    int32_t batch_size, int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, float scale, void* out, int64_t out_row_stride, float* scores,
+    int64_t scores_row_stride, int32_t add, void* workspace, int64_t workspace_bytes,
+    const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax,
+    tf_stream_t stream) {
+  using namespace tfa;
+  clear_error();
+  ScoredPlan r;
+  int rc = make_scored_plan(batch_size, max_len, num_q_heads, num_kv_heads, head_dim, kv_dtype,
+                            &r);
+  if (rc != TF_OK) return rc;
+  if (batch_size == 0) return TF_OK;
+  rc = check_slot_call("scored", q, q_row_stride, k_pool, v_pool, pool_slots, kv_dtype, k_scale,
+                       v_scale, req_to_token, rtt_rows, rtt_row_stride, rtt_cols,
+                       req_pool_indices, seq_lens, seq_len_override, num_q_heads, head_dim, out,
+                       out_row_stride, gate, gate_row_stride, gate_head_stride, workspace,
+                       workspace_bytes, r.total());
+  if (rc != TF_OK) return rc;
+  if (!scores || scores_row_stride < rtt_cols)
+    return fail(TF_ERR_INVALID, "scored: scores need rows of at least %lld", (long long)rtt_cols);
+  PartArgs a = part_args(q, q_row_stride, k_pool, v_pool, pool_slots, k_scale, v_scale,
+                         req_to_token, rtt_rows, rtt_row_stride, rtt_cols, req_pool_indices,
+                         seq_lens, r.n_items, r.slot_rows, num_q_heads, num_kv_heads, head_dim,
+                         scale, out, out_row_stride, workspace, gate, gate_row_stride,
+                         gate_head_stride, out_amax, r.p);
+  a.seq_override = seq_len_override;
+  a.head_blocks = r.head_blocks;
+  a.row_scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + r.p.total());
+  a.score_cap = r.cap;
+  a.row_lse = a.row_scores + r.scores_bytes / 4;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  launch_stream_groups<1, true>(a, r.p, s);
+  rc = launch_status("tf_attn_scored stream launch");
+  if (rc != TF_OK) return rc;
+  launch_merge<4>(a, r.p, r.n_items, r.slot_rows, s);
+  ScoreArgs sa = {};
+  sa.row_scores = a.row_scores;
+  sa.row_lse = a.row_lse;
+  sa.score_cap = r.cap;
+  sa.rpi = req_pool_indices;
+  sa.seq_lens = seq_lens;
+  sa.rtt_rows = rtt_rows;
+  sa.rtt_cols = rtt_cols;
+  sa.seq_override = seq_len_override;
+  sa.hq = num_q_heads;
+  sa.add = add;
+  sa.scores = scores;
+  sa.scores_stride = scores_row_stride;
+  const int64_t blocks = (r.cap + 4 * kScoreThreads - 1) / (4 * kScoreThreads);
+  hipLaunchKernelGGL(add_weights_kernel,
+                     dim3((unsigned)(blocks < 256 ? blocks : 256), (unsigned)batch_size),
+                     dim3(kScoreThreads), 0, s, sa);
+  return launch_status("tf_attn_scored launch");
 }

@@ -14,7 +14,8 @@ from typing import Optional
 import torch
 
 from . import _native
-from .attention import _KV_DTYPES, _check_inputs, _pool_scales, slot_based_attention
+from .attention import (_KV_DTYPES, _check_inputs, _epilogue, _output, _pool_scales,
+                        slot_based_attention)
 from .block_fp8 import workspace
 from .fp8_linear import _ptr
 
@@ -25,6 +26,28 @@ def check_scores(fn: str, scores: torch.Tensor, table: torch.Tensor) -> None:
             or scores.stride(1) != 1 or (scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]):
         raise ValueError(f"{fn}: scores must be fp32 with req_to_token's rows and columns "
                          f"{tuple(table.shape)}, on its device, row-major")
+
+
+MAX_ITEMS = 2048               # blocks of 16 heads of a kv head in one launch
+MAX_KEPT_BYTES = 4 << 30       # scores kept between the two halves of a step
+
+
+def _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span) -> bool:
+    """Whether a decode step keeps the attention's own scores for the weights (tf_attn_scored)
+    instead of computing them again: 4 bytes per head and key, where K and V are 4 to 16
+    times that, unless the table is so wide that the longest context's room for every
+    request is too much."""
+    if n_q % n_kv or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
+        return False
+    return (bsz * -(-(n_q // n_kv) // 16) <= MAX_ITEMS
+            and 4 * bsz * n_q * span <= MAX_KEPT_BYTES)
+
+
+def _check_tokens(fn: str, batch, n_tok: int) -> None:
+    ext = batch.extend_lens
+    if len(ext) != batch.batch_size or sum(int(e) for e in ext) != n_tok:
+        raise ValueError(f"{fn}: extend_lens {list(ext)[:8]}... do not match "
+                         f"batch_size={batch.batch_size}, T={n_tok}")
 
 
 def scored_attention(
@@ -77,23 +100,36 @@ def scored_attention(
         k_scale, v_scale = _pool_scales(q, kv_dtype, k_scale, v_scale)
         if q.stride(2) != 1 or q.stride(1) != head_dim:
             q = q.contiguous()
+        rtt = batch.req_to_token
+        span = (rtt.shape[1] if torch.cuda.is_current_stream_capturing()
+                else max(1, int(batch.max_seq_len)))
+        scale = head_dim ** -0.5 if scaling is None else float(scaling)
+        override = int(batch.max_seq_len) if bsz == 1 else 0
+        table = (rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
+                 batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr(), override)
+        if n_tok and longest == 1 and _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span):
+            _check_tokens(fn, batch, n_tok)
+            out = _output(q, out)
+            ws, nbytes = workspace("tf_attn_scored_workspace_bytes", device, bsz, span, n_q, n_kv,
+                                   head_dim, kv_dtype)
+            _native.call("tf_attn_scored", q.data_ptr(), q.stride(0), layer_k_buffer.data_ptr(),
+                         layer_v_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale),
+                         _ptr(v_scale), *table, bsz, span, n_q, n_kv, head_dim, scale,
+                         out.data_ptr(), out.stride(0), scores.data_ptr(), scores.stride(0),
+                         int(bool(add)), ws.data_ptr(), nbytes, *_epilogue(q, gate, out_amax),
+                         _native.current_stream(device))
+            return out
         out = slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, scaling=scaling,
                                    k_scale=k_scale, v_scale=v_scale, out=out, gate=gate,
                                    out_amax=out_amax)
         if n_tok == 0:
             return out
-        rtt = batch.req_to_token
-        span = (rtt.shape[1] if torch.cuda.is_current_stream_capturing()
-                else max(1, int(batch.max_seq_len)))
         window = min(int(window), longest)
         ws, nbytes = workspace("tf_attn_weights_workspace_bytes", device, bsz, window, span, n_q,
                                n_kv, head_dim, kv_dtype)
         _native.call("tf_attn_weights", q.data_ptr(), q.stride(0), n_tok,
-                     layer_k_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale), rtt.data_ptr(), rtt.shape[0],
-                     rtt.stride(0), rtt.shape[1], batch.req_pool_indices.data_ptr(),
-                     batch.seq_lens.data_ptr(), int(batch.max_seq_len) if bsz == 1 else 0,
+                     layer_k_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale), *table,
                      _ptr(ext_t) if longest > 1 else None, bsz, window, span, n_q, n_kv, head_dim,
-                     head_dim ** -0.5 if scaling is None else float(scaling), scores.data_ptr(),
-                     scores.stride(0), int(bool(add)), ws.data_ptr(), nbytes,
-                     _native.current_stream(device))
+                     scale, scores.data_ptr(), scores.stride(0), int(bool(add)), ws.data_ptr(),
+                     nbytes, _native.current_stream(device))
     return out
