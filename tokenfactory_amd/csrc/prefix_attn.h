@@ -58,10 +58,13 @@ struct PartArgs {
   const float2* piece_ml;  // [slot][256], [slot][256][256]
   const float* piece_o;
   // Scored calls: every row's scores (log2 units, -inf where masked) of its first
-  // score_cap keys, row q_row * q heads + head, and its log2 of the sum of 2^score.
+  // score_cap keys, row q_row * q heads + head, and the table that their weights go to.
   float* row_scores;
   int64_t score_cap;
-  float* row_lse;
+  float* scores;
+  int64_t scores_stride;
+  int32_t add_scores;
+  int32_t weight_blocks, n_weights;   // workgroups for them: per request, and in all
 };
 
 }  // namespace tfa

@@ -21,6 +21,8 @@
 // HBM, or by the latency of a unit's first loads where contexts are short.
 #include <math.h>
 
+#include <algorithm>
+
 #include "attn_row.h"
 #include "prefix_attn.h"
 #include "stream_tile.h"
@@ -74,12 +76,18 @@ constexpr int kHalf = kHalfTiles * kTile;        // in two halves by turns
 // Positions of an item's units: its tiles behind kUnitTiles positions without work.
 __device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUnitTiles : 0; }
 
-template <class C>
+// Scores of 8 tiles on their way to memory (SCORED): 512 bytes of a row per store, where
+// a tile's own are 64, whose stores took a fifth of the kernel's time.
+constexpr int kKeptTiles = 8;
+constexpr int kKeptRow = kKeptTiles * kTile + 4;   // floats, padded
+
+template <class C, bool SCORED>
 struct StreamSmem {
   struct {
     int32_t slots[2 * kHalf];
     u32x4 kstage[kTile * C::kChunks];          // see stage_k
-    u32x4 qfrag[C::NG][C::kSteps][kWave];
+    u32x4 qfrag[C::NG > 1 ? C::NG : 0][C::kSteps][kWave];   // (one group's stay in registers)
+    float kept[SCORED ? 16 : 0][kKeptRow];
   } wave[kWaves];
   int32_t ipre[kMaxItems + 1];                 // exclusive prefix of the items' spans
   int32_t wsum[kWaves];
@@ -90,7 +98,8 @@ struct StreamSmem {
 template <class C, bool SCORED>
 __global__ void __launch_bounds__(kWaves * kWave, C::NG == 1 || C::DP == 128 ? 2 : 1)
 part_stream_kernel(PartArgs a) {
-  __shared__ StreamSmem<C> sm;
+  __shared__ StreamSmem<C, SCORED> sm;
+  static_assert(!SCORED || C::NG == 1, "scored items are the heads of one token");
   const int D = C::OTHER ? a.head_dim : C::DP;
   const int row_bytes = C::FP8 ? D : 2 * D;
   const int n_chunks = row_bytes / 16;
@@ -166,20 +175,17 @@ part_stream_kernel(PartArgs a) {
     };
     u32x4 qf[C::kSteps];
     int seen[C::NG];
-    float* kept[C::NG];   // where the lane's row n of group q keeps its scores (or NULL)
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
       int qrow, hq;
       const bool ok = row_of(q, qrow, hq, seen[q]);
       const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
-      kept[q] = SCORED && ok ? a.row_scores + ((int64_t)qrow * a.hkv * a.group + hq) * a.score_cap
-                             : nullptr;
 #pragma unroll
       for (int kk = 0; kk < C::kSteps; ++kk) {
         const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
         qf[kk] = ok && (!C::OTHER || d0 < D) ? ld_g16(qp + d0) : u32x4{0u, 0u, 0u, 0u};
       }
-      if (C::NG > 1) {   // (one group's stay in registers)
+      if constexpr (C::NG > 1) {
 #pragma unroll
         for (int kk = 0; kk < C::kSteps; ++kk) sm.wave[w].qfrag[q][kk][lane] = qf[kk];
       }
@@ -220,17 +226,36 @@ part_stream_kernel(PartArgs a) {
       k_frags<C>(ks, g, n, kf);
 #pragma unroll
       for (int q = 0; q < C::NG; ++q) {
-        if (C::NG > 1) {
+        if constexpr (C::NG > 1) {
           if (q >= n_groups) break;
 #pragma unroll
           for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.wave[w].qfrag[q][kk][lane];
         }
         const int lim = min(n_loc, seen[q] - c0);
         pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [&](const float (&sc)[4]) {
-          const int k = im.k0 + c0 + it * kTile;
-          if (SCORED && kept[q] && k < a.score_cap)
-            *reinterpret_cast<f32x4*>(kept[q] + k + 4 * g) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+          if constexpr (SCORED)
+            *reinterpret_cast<f32x4*>(
+                &sm.wave[w].kept[n][((t0 + it) % kKeptTiles) * kTile + 4 * g]) =
+                f32x4{sc[0], sc[1], sc[2], sc[3]};
         });
+      }
+    };
+    // Scores of the tiles from the last multiple of kKeptTiles (or the first) to tile it, at
+    // the last of them: two rows at a time.
+    auto flush = [&](int it, bool last) {
+      if constexpr (SCORED) {
+        const int tile = t0 + it;
+        if (!last && tile % kKeptTiles != kKeptTiles - 1) return;
+        const int from = max(t0, tile - tile % kKeptTiles);
+        const int i = lane & 31;
+        const int k = (tile - tile % kKeptTiles) * kTile + 4 * i;
+        float* rows = a.row_scores + ((int64_t)a.hkv * im.b + hk) * a.group * a.score_cap;
+        wave_lds_sync();
+        if (k >= from * kTile && k < min((tile + 1) * (int64_t)kTile, a.score_cap))
+          for (int r = lane >> 5; r < min(n_rows, 16); r += 2)
+            *reinterpret_cast<f32x4*>(rows + (im.row0 + r) * a.score_cap + k) =
+                *reinterpret_cast<const f32x4*>(&sm.wave[w].kept[r][4 * i]);
+        wave_lds_sync();
       }
     };
     u32x2 pt[C::NG], pl[C::NG][2];
@@ -256,12 +281,14 @@ part_stream_kernel(PartArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       issue(vb.v, it + 1, vbase);
       __builtin_amdgcn_sched_barrier(0);
+      flush(it, false);
     }
     wave_lds_sync();
     stage_k<C>(kb, ks, g, n);
     wave_lds_sync();
     scores(it, pt, pl);
     pv<C>(vb, pt, pl, st, n_groups);
+    flush(it, true);
 
 #pragma unroll
     for (int q = 0; q < C::NG; ++q) {
@@ -314,15 +341,105 @@ __device__ __forceinline__ Owners unit_owners(const PartArgs& a, int item, int h
   return Owners{b0 + (int64_t)item * a.hkv + hk, owner_of(p + span - 1, N, P) - b0 + 1};
 }
 
-template <int DP, bool FP8, int WPR>
+// The weights of a scored call: workgroups of the merge launch in front of the units'
+// (neither reads what the other writes).  Each takes the sums of 2^score of its request's
+// rows from the partials, then of kWeightKeys keys at a time
+//   scores[row, k] (+)= sum over the heads of 2^(score - lse),
+// four keys a thread, a quarter of the threads for every fourth head, added in a fixed
+// order.  Bound by latency (of few keys) or by reading the scores.
+constexpr int kMergeThreads = kMergeWaves * kWave;
+constexpr int kWeightHeads = kMergeThreads / 16;   // heads at a time
+constexpr int kWeightKeys = kMergeThreads;
+
+__device__ void add_weights(const PartArgs& a, int block) {
+  __shared__ float lse[kWeightHeads];
+  __shared__ f32x4 part[3][kWeightKeys / 4];
+  const int lane = threadIdx.x & 63;
+  const int quarter = wave_id() / 2, at = threadIdx.x % (kWeightKeys / 4);
+  const int b = block / a.weight_blocks;
+  const int hq = a.hkv * a.group;
+  const int64_t len = min((int64_t)context_len(a, b), a.score_cap);
+  const int64_t first = (int64_t)(block % a.weight_blocks) * kWeightKeys;
+  if (first >= len) return;
+  float* out = a.scores + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.scores_stride;
+  for (int h0 = 0; h0 < hq; h0 += kWeightHeads) {
+    const int n_heads = min(kWeightHeads, hq - h0);
+    __syncthreads();   // (the heads before are done with lse)
+    {   // sixteen lanes per head, four partials in flight each
+      const int i = threadIdx.x / 16, h = h0 + min(i, n_heads - 1);
+      const int hk = h / a.group, r = h - hk * a.group;
+      const Owners own = unit_owners(a, b * a.head_blocks + r / a.unit_rows, hk);
+      float m = -INFINITY, l = 0.f;
+      auto join = [&](float m2, float l2) {
+        const float mn = fmaxf(m, m2);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        l = l * fast_exp2(m - ref) + l2 * fast_exp2(m2 - ref);
+        m = mn;
+      };
+      for (int k = lane & 15; k < own.count; k += 64) {
+        float2 ml[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          ml[c] = a.part_ml[(own.first + min(k + 16 * c, own.count - 1)) * a.slot_rows +
+                            r % a.unit_rows];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (k + 16 * c < own.count) join(ml[c].x, ml[c].y);
+      }
+#pragma unroll
+      for (int d = 8; d >= 1; d >>= 1)
+        join(__shfl_xor(m, d, kWave), __shfl_xor(l, d, kWave));
+      // (a NaN sum makes every weight of its row NaN)
+      if ((lane & 15) == 0) lse[i] = l == 0.f ? INFINITY : m + log2f(l);
+    }
+    const float* rows = a.row_scores + ((int64_t)b * hq + h0) * a.score_cap;
+    for (int64_t k0 = first; k0 < len; k0 += (int64_t)a.weight_blocks * kWeightKeys) {
+      const int64_t k = k0 + 4 * at;
+      constexpr int kMine = kWeightHeads / 4;
+      f32x4 s[kMine], sum = {0.f, 0.f, 0.f, 0.f};
+      const bool live = k < len;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (live && quarter + 4 * i < n_heads)
+          s[i] = *reinterpret_cast<const f32x4*>(rows + (quarter + 4 * i) * a.score_cap + k);
+      __syncthreads();   // lse is there, and the keys before are done with part
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (quarter + 4 * i >= n_heads) break;
+        const float off = lse[quarter + 4 * i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(s[i][e] - off);
+      }
+      if (quarter) part[quarter - 1][at] = sum;
+      __syncthreads();
+      if (quarter == 0 && live) {
+        for (int c = 0; c < 3; ++c) sum += part[c][at];
+        const bool adds = a.add_scores || h0 > 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k + e < len) out[k + e] = adds ? out[k + e] + sum[e] : sum[e];
+      }
+    }
+  }
+}
+
+template <int DP, bool FP8, int WPR, bool SCORED>
 __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArgs a) {
+  int unit = blockIdx.x;
+  if constexpr (SCORED) {
+    unit -= a.n_weights;
+    if (unit < 0) {
+      if (blockIdx.y == 0) add_weights(a, blockIdx.x);
+      return;
+    }
+  }
   constexpr int kRows = kMergeWaves / WPR;   // rows of the unit side by side
   __shared__ f32x4 so[kMergeWaves][kWave];
   __shared__ float sm_m[kMergeWaves], sm_l[kMergeWaves];
   const int lane = threadIdx.x & 63;
   const int w = wave_id();
-  const int item = a.own0 + (int)(blockIdx.x / a.hkv);
-  const int hk = (int)(blockIdx.x % a.hkv);
+  const int item = a.own0 + unit / a.hkv;
+  const int hk = unit % a.hkv;
   const PartItem im = item_at(a, item);
   const int n = (int)blockIdx.y * kRows + w / WPR;     // the wave's row of the unit
   const int n_rows = im.b < 0 ? 0 : min(im.n_tok * a.group - im.row0, a.unit_rows);
@@ -417,9 +534,6 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     }
   }
 
-  // (+inf for a row without a visible key: its weights are zeros)
-  if (write && a.row_lse && lane == 0)
-    a.row_lse[(int64_t)tok.qrow * a.hkv * a.group + hq] = l == 0.f ? INFINITY : m + log2f(l);
   uint32_t om = 0;
   const float vscale = FP8 ? a.v_scale[0] : 1.f;
   __bf16* orow = a.out + (int64_t)tok.qrow * a.out_stride + (int64_t)hq * D;
@@ -452,52 +566,6 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     *reinterpret_cast<u32x2*>(orow + 4 * lane) = o;
   }
   amax_commit(a.amax, om);
-}
-
-// scores[row, k] (+)= sum of 2^(score - lse) over the request's heads, four keys a thread.
-constexpr int kScoreThreads = 256;
-struct ScoreArgs {
-  const float* row_scores;
-  const float* row_lse;
-  int64_t score_cap;
-  const int64_t* rpi;
-  const int64_t* seq_lens;
-  int64_t rtt_rows, rtt_cols;
-  int32_t seq_override, hq, add;
-  float* scores;
-  int64_t scores_stride;
-};
-__global__ void __launch_bounds__(kScoreThreads) add_weights_kernel(ScoreArgs a) {
-  const int b = blockIdx.y;
-  int64_t len = min(min(a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b], a.rtt_cols),
-                    a.score_cap);
-  const float* rows = a.row_scores + (int64_t)b * a.hq * a.score_cap;
-  const float* lse = a.row_lse + (int64_t)b * a.hq;
-  float* out = a.scores + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.scores_stride;
-  constexpr int kStep = 4;   // heads in flight
-  for (int64_t k = 4 * ((int64_t)blockIdx.x * kScoreThreads + threadIdx.x); k < len;
-       k += 4 * (int64_t)gridDim.x * kScoreThreads) {
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    for (int h0 = 0; h0 < a.hq; h0 += kStep) {
-      f32x4 s[kStep];
-      float off[kStep];
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int h = min(h0 + i, a.hq - 1);
-        s[i] = *reinterpret_cast<const f32x4*>(rows + h * a.score_cap + k);
-        off[i] = h0 + i < a.hq ? lse[h] : INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        if (h0 + i >= a.hq) break;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] += fast_exp2(s[i][e] - off[i]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (k + e < len) out[k + e] = a.add ? out[k + e] + w[e] : w[e];
-  }
 }
 
 // Kernel shape and workspace of a call.
@@ -564,17 +632,17 @@ void launch_stream_groups(const PartArgs& a, const PartPlan& p, hipStream_t s) {
   return launch_stream<Cfg<256, false, NG, false, true>, SCORED>(a, s);
 }
 
-template <int WPR>
-void launch_merge(const PartArgs& a, const PartPlan& p, int n_own, int rows, hipStream_t s) {
-  const dim3 grid((unsigned)(n_own * a.hkv),
+template <int WPR, bool SCORED>
+void launch_merge(const PartArgs& a, const PartPlan& p, int rows, hipStream_t s) {
+  const dim3 grid((unsigned)((a.n_items - a.own0) * a.hkv + a.n_weights),
                   (unsigned)((rows + kMergeWaves / WPR - 1) / (kMergeWaves / WPR)));
   const dim3 block(kMergeWaves * kWave);
   if (p.narrow)
-    hipLaunchKernelGGL((part_merge_kernel<128, false, WPR>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((part_merge_kernel<128, false, WPR, SCORED>), grid, block, 0, s, a);
   else if (p.fp8)
-    hipLaunchKernelGGL((part_merge_kernel<256, true, WPR>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((part_merge_kernel<256, true, WPR, SCORED>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((part_merge_kernel<256, false, WPR>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((part_merge_kernel<256, false, WPR, SCORED>), grid, block, 0, s, a);
 }
 
 PartArgs part_args(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
@@ -709,7 +777,7 @@ extern "C" int32_t tf_attn_shared(
     launch_stream_groups<2, false>(a, p, s);
   rc = launch_status("tf_attn_shared stream launch");
   if (rc != TF_OK) return rc;
-  launch_merge<4>(a, p, n_items - n_shared, slot_rows, s);
+  launch_merge<4, false>(a, p, slot_rows, s);
   return launch_status("tf_attn_shared merge launch");
 }
 
@@ -720,8 +788,8 @@ namespace {
 struct ScoredPlan {
   PartPlan p;
   int32_t n_items, head_blocks, slot_rows;
-  int64_t cap, scores_bytes, lse_bytes;
-  int64_t total() const { return p.total() + scores_bytes + lse_bytes; }
+  int64_t cap, scores_bytes;
+  int64_t total() const { return p.total() + scores_bytes; }
 };
 
 int make_scored_plan(int32_t batch, int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads,
@@ -742,7 +810,6 @@ int make_scored_plan(int32_t batch, int32_t max_len, int32_t num_q_heads, int32_
   r->p.o_bytes = (r->p.o_bytes + 255) / 256 * 256;
   r->cap = ((int64_t)max_len + kTile - 1) / kTile * kTile;
   r->scores_bytes = (int64_t)batch * num_q_heads * r->cap * 4;
-  r->lse_bytes = (int64_t)batch * num_q_heads * 4;
   return TF_OK;
 }
 
@@ -794,28 +861,18 @@ extern "C" int32_t tf_attn_scored(
   a.head_blocks = r.head_blocks;
   a.row_scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + r.p.total());
   a.score_cap = r.cap;
-  a.row_lse = a.row_scores + r.scores_bytes / 4;
+  a.scores = scores;
+  a.scores_stride = scores_row_stride;
+  a.add_scores = add;
+  const int64_t blocks = (r.cap + kWeightKeys - 1) / kWeightKeys;
+  // (as many as CUs over all requests: each takes the sums of every row of its request)
+  const int64_t most = std::max<int64_t>(1, device_cu_count() / batch_size);
+  a.weight_blocks = (int32_t)std::min(blocks, most);
+  a.n_weights = a.weight_blocks * batch_size;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   launch_stream_groups<1, true>(a, r.p, s);
   rc = launch_status("tf_attn_scored stream launch");
   if (rc != TF_OK) return rc;
-  launch_merge<4>(a, r.p, r.n_items, r.slot_rows, s);
-  ScoreArgs sa = {};
-  sa.row_scores = a.row_scores;
-  sa.row_lse = a.row_lse;
-  sa.score_cap = r.cap;
-  sa.rpi = req_pool_indices;
-  sa.seq_lens = seq_lens;
-  sa.rtt_rows = rtt_rows;
-  sa.rtt_cols = rtt_cols;
-  sa.seq_override = seq_len_override;
-  sa.hq = num_q_heads;
-  sa.add = add;
-  sa.scores = scores;
-  sa.scores_stride = scores_row_stride;
-  const int64_t blocks = (r.cap + 4 * kScoreThreads - 1) / (4 * kScoreThreads);
-  hipLaunchKernelGGL(add_weights_kernel,
-                     dim3((unsigned)(blocks < 256 ? blocks : 256), (unsigned)batch_size),
-                     dim3(kScoreThreads), 0, s, sa);
+  launch_merge<4, true>(a, r.p, r.slot_rows, s);
   return launch_status("tf_attn_scored launch");
 }
