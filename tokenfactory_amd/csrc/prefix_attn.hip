@@ -76,10 +76,11 @@ constexpr int kHalf = kHalfTiles * kTile;        // in two halves by turns
 // Positions of an item's units: its tiles behind kUnitTiles positions without work.
 __device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUnitTiles : 0; }
 
-// Scores of 8 tiles on their way to memory (SCORED): 512 bytes of a row per store, where
-// a tile's own are 64, whose stores took a fifth of the kernel's time.
-constexpr int kKeptTiles = 8;
-constexpr int kKeptRow = kKeptTiles * kTile + 4;   // floats, padded
+// Scores on their way to memory (SCORED) wait in LDS, as many tiles' as there is room for
+// (28 KB a wave: 72 tiles of 6 rows), since loads issued after a store are waited for
+// behind it: stored at every tile, or at every 8 tiles, they took a fifth of the kernel's
+// time (64 requests of 1k to 8k keys 239 us, 201 without stores).
+template <class C> constexpr int kKeptFloats = C::DP == 128 ? 3072 : 7168;
 
 template <class C, bool SCORED>
 struct StreamSmem {
@@ -87,7 +88,7 @@ struct StreamSmem {
     int32_t slots[2 * kHalf];
     u32x4 kstage[kTile * C::kChunks];          // see stage_k
     u32x4 qfrag[C::NG > 1 ? C::NG : 0][C::kSteps][kWave];   // (one group's stay in registers)
-    float kept[SCORED ? 16 : 0][kKeptRow];
+    float kept[SCORED ? kKeptFloats<C> : 0];
   } wave[kWaves];
   int32_t ipre[kMaxItems + 1];                 // exclusive prefix of the items' spans
   int32_t wsum[kWaves];
@@ -96,7 +97,8 @@ struct StreamSmem {
 // SCORED: the scores are kept (16 bytes per row and four keys, a few percent of the keys'
 // own bytes), for the weights that follow.
 template <class C, bool SCORED>
-__global__ void __launch_bounds__(kWaves * kWave, C::NG == 1 || C::DP == 128 ? 2 : 1)
+__global__ void __launch_bounds__(kWaves * kWave,
+                                  (C::NG == 1 && !SCORED) || C::DP == 128 ? 2 : 1)
 part_stream_kernel(PartArgs a) {
   __shared__ StreamSmem<C, SCORED> sm;
   static_assert(!SCORED || C::NG == 1, "scored items are the heads of one token");
@@ -218,6 +220,11 @@ part_stream_kernel(PartArgs a) {
     fetch_ids(0);
     stage_ids(0);
 
+    // (rows of a multiple of 16 floats and 4: no two of a lane group on one bank)
+    const int kept_tiles = SCORED ? (kKeptFloats<C> / min(n_rows, 16) - 4) / kTile : 0;
+    const int kept_row = kept_tiles * kTile + 4;
+    int kept_from = 0;
+
     // ---- the tiles, loads a tile ahead (see decode_kernel)
     KBuf<C> kb;
     VBuf<C> vb;
@@ -233,29 +240,31 @@ part_stream_kernel(PartArgs a) {
         }
         const int lim = min(n_loc, seen[q] - c0);
         pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [&](const float (&sc)[4]) {
-          if constexpr (SCORED)
-            *reinterpret_cast<f32x4*>(
-                &sm.wave[w].kept[n][((t0 + it) % kKeptTiles) * kTile + 4 * g]) =
-                f32x4{sc[0], sc[1], sc[2], sc[3]};
+          if constexpr (SCORED) {
+            if (n < n_rows)
+              *reinterpret_cast<f32x4*>(
+                  &sm.wave[w].kept[n * kept_row + (it - kept_from) * kTile + 4 * g]) =
+                  f32x4{sc[0], sc[1], sc[2], sc[3]};
+          }
         });
       }
     };
-    // Scores of the tiles from the last multiple of kKeptTiles (or the first) to tile it, at
-    // the last of them: two rows at a time.
+    // The kept scores of tiles kept_from .. it go out once there is no room for more, and
+    // at the last tile.
     auto flush = [&](int it, bool last) {
       if constexpr (SCORED) {
-        const int tile = t0 + it;
-        if (!last && tile % kKeptTiles != kKeptTiles - 1) return;
-        const int from = max(t0, tile - tile % kKeptTiles);
-        const int i = lane & 31;
-        const int k = (tile - tile % kKeptTiles) * kTile + 4 * i;
-        float* rows = a.row_scores + ((int64_t)a.hkv * im.b + hk) * a.group * a.score_cap;
+        if (!last && it - kept_from + 1 < kept_tiles) return;
+        const int64_t k0 = c0 + kept_from * kTile;
+        const int keys = (int)min<int64_t>((it - kept_from + 1) * kTile, a.score_cap - k0);
+        float* rows = a.row_scores + ((int64_t)a.hkv * im.b + hk) * a.group * a.score_cap +
+                      im.row0 * a.score_cap + k0;
         wave_lds_sync();
-        if (k >= from * kTile && k < min((tile + 1) * (int64_t)kTile, a.score_cap))
-          for (int r = lane >> 5; r < min(n_rows, 16); r += 2)
-            *reinterpret_cast<f32x4*>(rows + (im.row0 + r) * a.score_cap + k) =
-                *reinterpret_cast<const f32x4*>(&sm.wave[w].kept[r][4 * i]);
+        for (int r = 0; r < min(n_rows, 16); ++r)
+          for (int k = 4 * lane; k < keys; k += 4 * kWave)
+            *reinterpret_cast<f32x4*>(rows + r * a.score_cap + k) =
+                *reinterpret_cast<const f32x4*>(&sm.wave[w].kept[r * kept_row + k]);
         wave_lds_sync();
+        kept_from = it + 1;
       }
     };
     u32x2 pt[C::NG], pl[C::NG][2];
