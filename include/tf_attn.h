@@ -391,13 +391,17 @@ int32_t tf_attn_weights(
  * rtt_cols)].  out_rows: rows that receive the result (NULL: in place); no row may be
  * written for two requests, or written for one and read for another.  new_lens: int64
  * [batch_size]; freed: int64 [batch_size][freed_width], the slots that left, in order, -1
- * behind them; freed_width >= min(max_len, rtt_cols) - keep. */
+ * behind them; freed_width >= min(max_len, rtt_cols) - keep.  Long rows take a workspace
+ * of tf_evict_workspace_bytes (0: none), 16-byte aligned, that calls overlapping in time
+ * must not share. */
+int64_t tf_evict_workspace_bytes(int64_t max_len, int64_t rtt_cols, int32_t batch_size);
+
 int32_t tf_evict_tokens(
     int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride, int64_t rtt_cols,
     float* scores, int64_t scores_row_stride, const int64_t* rows, const int64_t* out_rows,
     const int64_t* seq_lens, const int64_t* first, int64_t first_n, int64_t recent, int64_t keep,
     int64_t max_len, int32_t batch_size, int64_t* new_lens, int64_t* freed, int64_t freed_width,
-    tf_stream_t stream);
+    void* workspace, int64_t workspace_bytes, tf_stream_t stream);
 
 /* tf_attn_plan_blocks: the row blocks of a step, built on the device from its
  * work list and decode items (of either planner, padding included): the decode

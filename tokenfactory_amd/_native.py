@@ -154,12 +154,14 @@ SIGNATURES = {
         _p, _i64, _i32,                # scores, scores_row_stride, add
         _p, _i64, _p,                  # workspace, workspace_bytes, stream
     ]),
+    "tf_evict_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "tf_evict_tokens": (_i32, [
         _p, _i64, _i64, _i64,          # req_to_token, rtt_rows, rtt_row_stride, rtt_cols
         _p, _i64,                      # scores, scores_row_stride
         _p, _p, _p, _p, _i64,          # rows, out_rows, seq_lens, first, first_n
         _i64, _i64, _i64, _i32,        # recent, keep, max_len, batch_size
-        _p, _p, _i64, _p,              # new_lens, freed, freed_width, stream
+        _p, _p, _i64,                  # new_lens, freed, freed_width
+        _p, _i64, _p,                  # workspace, workspace_bytes, stream
     ]),
     "tf_attn_plan_decode_items": (_i32, [_p, _i32, _p, _p, _i32]),
     "tf_req_to_token_sync": (_i32, [
