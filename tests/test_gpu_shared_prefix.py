@@ -278,3 +278,72 @@ def test_many_requests(gpu):
                     dtype=torch.bfloat16, groups=[0] * b, prefixes=[30])
     want = slot_based_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, scaling=wl.scale)
     assert torch.equal(call(wl, SharedPrefixes([(list(range(b)), 30)])), want)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [(24, 4), (16, 2), (6, 1), (8, 8), (20, 1), (34, 2)])
+def test_long_prefixes_in_pieces(gpu, heads, fp8):
+    wl, groups = shared_case([1700], [5, 1, 40, 17, 16], [0] * 5, heads=heads, seed=21, fp8=fp8)
+    check(wl, groups, f"pieces {heads} fp8={fp8}")
+
+
+@pytest.mark.parametrize("prefix", [1537, 1568, 1600, 2047, 2049, 4133, 8191])
+def test_long_prefix_lengths(gpu, prefix):
+    wl, groups = shared_case([prefix], [1, 2, 9], [0] * 3, heads=(6, 1), seed=prefix)
+    check(wl, groups, f"pieces of {prefix}")
+
+
+@pytest.mark.parametrize("members", [2, 3, 5, 6, 11, 43, 90])
+def test_pieces_of_group_sizes(gpu, members):
+    """Row blocks of 256, whole waves of them without rows, several groups in one launch."""
+    b = 2 * members
+    wl, groups = shared_case([1600, 333], [1 + 7 * i % 50 for i in range(b)],
+                             [i % 2 for i in range(b)], heads=(6, 1), seed=members)
+    check(wl, groups, f"pieces of {members} members")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_pieces_with_several_tokens_and_prompts(gpu, fp8):
+    groups = [0, 1, 2, 0, 1, 0, 0, 1, 0]
+    ext = [4, 1, 2, 3, 1, 10, 1, 6, 40]
+    own = [9, 1, 30, 3, 200, 11, 64, 6, 50]
+    wl, members = shared_case([1900, 90, 0], own, groups, ext=ext, seed=25, fp8=fp8)
+    check(wl, members, f"pieces, tokens, fp8={fp8}")
+
+
+def test_pieces_with_short_members_and_masked_values(gpu):
+    """Contexts that end inside the shared part, before its first key, or nowhere near;
+    NaN in slots that nothing uses."""
+    wl, members = shared_case([1800], [5, 8, 1, 30], [0] * 4, seed=27, ext=[1, 3, 1, 2])
+    table = wl.batch.req_to_token
+    bad = torch.ones(wl.k_pool.shape[0], dtype=torch.bool, device=gpu)
+    bad[table[table >= 0].unique()] = False
+    wl.k_pool[bad] = float("nan")
+    wl.v_pool[bad] = float("nan")
+    shared = SharedPrefixes(members)
+    for lens in ([1805, 1808, 0, 1700], [0, 2, 1, 1], [1805, 1799, 17, 1830]):
+        wl.batch.seq_lens.copy_(torch.tensor(lens))
+        want, spread, _ = attention64(wl, seq_lens=lens)
+        assert_attention(call(wl, shared), want, spread, wl, f"lens {lens}")
+
+
+def test_pieces_large_scores(gpu):
+    wl, members = shared_case([1600], [40, 3, 1], [0] * 3, seed=23, q_std=40.0)
+    check(wl, members, "pieces, large scores")
+
+
+def test_pieces_captured_and_replayed(gpu):
+    wl, members = shared_case([1600], [40, 50, 60], [0] * 3, seed=13)
+    shared = SharedPrefixes(members)
+    full = wl.batch.seq_lens.clone()
+    call(wl, shared)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(wl, shared)
+    for step in range(3):
+        wl.batch.seq_lens.copy_(full - 7 * step)
+        wl.q.copy_(torch.randn_like(wl.q))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(wl, SharedPrefixes(members))), step

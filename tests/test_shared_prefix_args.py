@@ -32,9 +32,9 @@ def test_groups_must_fit_the_batch():
     wl = small_case([9, 9], [1, 1], d=64, dtype=torch.bfloat16)
     dev = torch.device("cpu")
     with pytest.raises(ValueError, match="batch of 2"):
-        SharedPrefixes([([0, 2], 4)])._plan(wl.batch, [1, 1], 4, 1, 64, dev)
+        SharedPrefixes([([0, 2], 4)])._plan(wl.batch, 2, 4, 1, 64, dev)
     with pytest.raises(ValueError, match="width"):
-        SharedPrefixes([([0, 1], 400)])._plan(wl.batch, [1, 1], 4, 1, 64, dev)
+        SharedPrefixes([([0, 1], 400)])._plan(wl.batch, 2, 4, 1, 64, dev)
 
 
 def lists(plan):
@@ -45,7 +45,15 @@ def lists(plan):
 
 
 EXT = [1, 4, 2, 1, 70, 1] + [1] * 60
-GROUPS = [([0, 1, 5] + list(range(6, 60)), 1000), ([2, 4, 62], 50)]
+GROUPS = [([0, 1, 5] + list(range(6, 60)), 2000), ([2, 4, 62], 50)]
+
+
+def test_short_prefixes_are_streamed():
+    """(at head_dim 256: the items, no pieces)"""
+    plan = _Plan([([0, 1], 1000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256)
+    assert plan.n_shared == 1 and plan.n_pieces == 0 and plan.row_groups == 1
+    plan = _Plan([([0, 1], 2000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256)
+    assert plan.n_shared == 0 and plan.n_pieces > 4
 
 
 @pytest.mark.parametrize("head_dim", [256, 128])

@@ -21,6 +21,7 @@ by phase. Only ROCm device tensors are accepted; there is no CPU path.
 """
 from __future__ import annotations
 
+import functools
 import math
 import threading
 from typing import Dict, Optional, Tuple
@@ -463,6 +464,20 @@ def _check_inputs(q, k_buf, v_buf, batch):
                          f"{rtt.shape[1]}")
 
 
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(name: str, device_index: int, *sizes) -> int:
+    """What entry point ``name`` asks for, for sizes on the current device."""
+    return _native.call(name, *sizes)
+
+
+def _scratch(name: str, device: torch.device, *sizes):
+    """(scratch or None, bytes) of a call, from torch on the current stream."""
+    nbytes = _scratch_bytes(name, device.index, *sizes)
+    if not nbytes:
+        return None, 0
+    return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device), nbytes
+
+
 def _pool_scales(q, kv_dtype: int, k_scale, v_scale):
     """The scales as the entry points take them (None for a bf16 pool)."""
     if kv_dtype != _native.TF_DTYPE_FP8_E4M3:
@@ -475,7 +490,7 @@ def _pool_scales(q, kv_dtype: int, k_scale, v_scale):
 
 def _output(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return q.new_empty(q.shape)
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 \
             or out.stride(1) != q.shape[2]:
         raise ValueError("out must match q's shape/dtype with dense heads and dims")

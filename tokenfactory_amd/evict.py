@@ -12,7 +12,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native
-from .block_fp8 import workspace
+from .attention import _scratch
 from .fp8_linear import _ptr
 from .scored_attention import check_scores
 
@@ -77,8 +77,8 @@ def evict_tokens(
         lens = torch.empty_strided((bsz,), (1,), dtype=torch.int64, device=device)
         freed = torch.empty_strided((bsz, width), (width, 1), dtype=torch.int64, device=device)
         if bsz:
-            ws, nbytes = workspace("tf_evict_workspace_bytes", device, max_seq_len,
-                                   table.shape[1], bsz)
+            ws, nbytes = _scratch("tf_evict_workspace_bytes", device, max_seq_len,
+                                  table.shape[1], bsz)
             _native.call("tf_evict_tokens", table.data_ptr(), table.shape[0], table.stride(0),
                          table.shape[1], scores.data_ptr(), scores.stride(0),
                          req_pool_indices.data_ptr(), _ptr(out_rows), seq_lens.data_ptr(),

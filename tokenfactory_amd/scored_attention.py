@@ -14,9 +14,8 @@ from typing import Optional
 import torch
 
 from . import _native
-from .attention import (_KV_DTYPES, _check_inputs, _epilogue, _output, _pool_scales,
+from .attention import (_KV_DTYPES, _check_inputs, _epilogue, _output, _pool_scales, _scratch,
                         slot_based_attention)
-from .block_fp8 import workspace
 from .fp8_linear import _ptr
 
 
@@ -41,13 +40,6 @@ def _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span) -> bool:
         return False
     return (bsz * -(-(n_q // n_kv) // 16) <= MAX_ITEMS
             and 4 * bsz * n_q * span <= MAX_KEPT_BYTES)
-
-
-def _check_tokens(fn: str, batch, n_tok: int) -> None:
-    ext = batch.extend_lens
-    if len(ext) != batch.batch_size or sum(int(e) for e in ext) != n_tok:
-        raise ValueError(f"{fn}: extend_lens {list(ext)[:8]}... do not match "
-                         f"batch_size={batch.batch_size}, T={n_tok}")
 
 
 def scored_attention(
@@ -90,7 +82,7 @@ def scored_attention(
     n_slots, n_kv, _ = layer_k_buffer.shape
     bsz, device = batch.batch_size, q.device
     kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
-    longest = max((int(e) for e in batch.extend_lens), default=1)
+    longest = int(batch.max_extend_len)
     ext_t = batch.extend_lens_tensor
     if longest > 1 and (ext_t is None or ext_t.device != device or ext_t.dtype != torch.long
                         or ext_t.numel() != bsz or not ext_t.is_contiguous()):
@@ -108,10 +100,12 @@ def scored_attention(
         table = (rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
                  batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr(), override)
         if n_tok and longest == 1 and _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span):
-            _check_tokens(fn, batch, n_tok)
+            if n_tok != bsz or len(batch.extend_lens) != bsz:
+                raise ValueError(f"{fn}: {n_tok} tokens, {len(batch.extend_lens)} extend_lens of "
+                                 f"a decode batch of {bsz}")
             out = _output(q, out)
-            ws, nbytes = workspace("tf_attn_scored_workspace_bytes", device, bsz, span, n_q, n_kv,
-                                   head_dim, kv_dtype)
+            ws, nbytes = _scratch("tf_attn_scored_workspace_bytes", device, bsz, span, n_q, n_kv,
+                                  head_dim, kv_dtype)
             _native.call("tf_attn_scored", q.data_ptr(), q.stride(0), layer_k_buffer.data_ptr(),
                          layer_v_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale),
                          _ptr(v_scale), *table, bsz, span, n_q, n_kv, head_dim, scale,
@@ -125,8 +119,8 @@ def scored_attention(
         if n_tok == 0:
             return out
         window = min(int(window), longest)
-        ws, nbytes = workspace("tf_attn_weights_workspace_bytes", device, bsz, window, span, n_q,
-                               n_kv, head_dim, kv_dtype)
+        ws, nbytes = _scratch("tf_attn_weights_workspace_bytes", device, bsz, window, span, n_q,
+                              n_kv, head_dim, kv_dtype)
         _native.call("tf_attn_weights", q.data_ptr(), q.stride(0), n_tok,
                      layer_k_buffer.data_ptr(), n_slots, kv_dtype, _ptr(k_scale), *table,
                      _ptr(ext_t) if longest > 1 else None, bsz, window, span, n_q, n_kv, head_dim,

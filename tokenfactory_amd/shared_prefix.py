@@ -21,8 +21,8 @@ import torch
 
 from . import _native
 from .attention import (SHORT_ROWS, _KV_DTYPES, _check_inputs, _cu_count, _epilogue, _output,
-                        _plan_event, _pool_scales, _upload, _ws_lock, slot_based_attention)
-from .block_fp8 import workspace
+                        _plan_event, _pool_scales, _scratch, _upload, _ws_lock,
+                        slot_based_attention)
 from .planning import EXTEND_TILE_ROWS, plan_extend
 
 MAX_PARTS = 2048          # parts of contexts in one launch
@@ -55,13 +55,22 @@ class SharedPrefixes:
         self._lock = threading.Lock()
         self._plans: Dict[tuple, _Plan] = {}
 
-    def _plan(self, batch, ext_lens, n_q, n_kv, head_dim, device) -> "_Plan":
+    def _plan(self, batch, n_tok, n_q, n_kv, head_dim, device) -> "_Plan":
+        key = (device.index, batch.batch_size, n_tok, n_q, n_kv, head_dim,
+               batch.req_to_token.shape[1], tuple(batch.extend_lens))
+        plan = self._plans.get(key)
+        if plan is not None:
+            return plan
+        ext_lens = [int(e) for e in batch.extend_lens]
+        if len(ext_lens) != batch.batch_size or sum(ext_lens) != n_tok \
+                or min(ext_lens, default=1) < 1:
+            raise ValueError(f"extend_lens {ext_lens[:8]}... do not match "
+                             f"batch_size={batch.batch_size}, T={n_tok}")
         if self._last >= batch.batch_size:
             raise ValueError(f"request {self._last} of a batch of {batch.batch_size}")
         width = batch.req_to_token.shape[1]
         if any(n > width for _, n in self.groups):
             raise ValueError(f"a shared prefix exceeds req_to_token's width {width}")
-        key = (device.index, tuple(ext_lens), n_q, n_kv, head_dim)
         with self._lock:
             plan = self._plans.get(key)
             if plan is None:
@@ -87,6 +96,16 @@ def cut_units(steps: Sequence[int], cus: int) -> List[int]:
     return [max(1, -(-s // lo)) for s in steps]
 
 
+def _streams(groups, rows, n_kv: int) -> bool:
+    """Whether the shared parts of a step at head_dim 256 are streamed with the others,
+    32 rows at a time, rather than taken in MFMA pieces, whose launch and partials cost
+    12 to 20 us whatever the length: short ones of few rows (24 / 4 heads, one group of 2
+    on 1000 keys 21 us streamed, 26 in pieces, of 64 on 500 40 and 45, of 4 on 4000 36 and
+    28; 4 groups of 4 on 2500 36 both ways, of 64 on 2000 57 both ways)."""
+    units = sum(-(-r // 32) * n_kv * -(-n // 16) for (_, n), r in zip(groups, rows))
+    return max((n for _, n in groups), default=0) <= 1536 and units <= 4096
+
+
 class _Plan:
     """The device lists of one step layout: parts of contexts and their tokens; at head_dim
     256 the pieces of the shared ones; and the extend kernel's entries of long prompts,
@@ -95,14 +114,15 @@ class _Plan:
     def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus):
         group = n_q // n_kv
         self.device = device
-        mfma = head_dim == 256
-        long_ = {b for b, e in enumerate(ext_lens) if mfma and e * group > SHORT_ROWS}
+        long_ = {b for b, e in enumerate(ext_lens)
+                 if head_dim == 256 and e * group > SHORT_ROWS}
         starts = [0, *np.cumsum(ext_lens).tolist()]
         groups = [([b for b in m if b not in long_], n) for m, n in groups]
         groups = [(m, n) for m, n in groups if len(m) > 1]
         self.shares = bool(groups)
         shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
         rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
+        mfma = head_dim == 256 and not _streams(groups, shared_rows, n_kv)
         if not mfma:
             rows += shared_rows
         self.row_groups = 2 if max(rows, default=1) > 16 else 1
@@ -160,35 +180,36 @@ class _Plan:
         self._lists: Optional[torch.Tensor] = None
         self._users: set = set()
         self._event = None
-        self._uploaded_on = 0
+        self._addresses: List[int] = []
         self._kept = False
 
     def lists(self) -> List[int]:
         """Addresses of (items, work, pieces, tokens, units) for launches on the current
         stream."""
-        stream = torch.cuda.current_stream(self.device)
         capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing and _native.current_stream(self.device) in self._users:
+            return self._addresses
+        stream = torch.cuda.current_stream(self.device)
         with self._lock:
             if self._lists is None:
                 if capturing:
                     raise RuntimeError("shared prefixes cannot be planned in a graph capture: "
                                        "run the call once before it")
                 self._lists = _upload(self._host, self.device, stream)
-                self._uploaded_on = stream.cuda_stream
-                self._users.add(stream.cuda_stream)
+                self._addresses = [self._lists.data_ptr() + at for at in self._offsets]
                 with _ws_lock:
                     self._event = _plan_event(self.device, stream)
                     self._event.record(stream)
-            elif stream.cuda_stream not in self._users:
-                if not capturing:   # (torch waits for the device before it captures)
-                    self._users.add(stream.cuda_stream)
-                    self._lists.record_stream(stream)
-                    stream.wait_event(self._event)
+                self._users.add(stream.cuda_stream)
+            elif stream.cuda_stream not in self._users and not capturing:
+                # (torch waits for the device before it captures)
+                self._lists.record_stream(stream)
+                stream.wait_event(self._event)
+                self._users.add(stream.cuda_stream)
             if capturing and not self._kept:
                 self._kept = True
                 _captured.append(self._lists)
-            base = self._lists.data_ptr()
-        return [base + at for at in self._offsets]
+        return self._addresses
 
 
 def shared_prefix_attention(
@@ -222,12 +243,8 @@ def shared_prefix_attention(
     n_slots, n_kv, _ = layer_k_buffer.shape
     if n_q % n_kv:
         raise ValueError(f"num_q_heads {n_q} is not a multiple of num_kv_heads {n_kv}")
-    ext_lens = [int(e) for e in batch.extend_lens]
-    if len(ext_lens) != batch.batch_size or sum(ext_lens) != n_tok or min(ext_lens, default=1) < 1:
-        raise ValueError(f"extend_lens {ext_lens[:8]}... do not match "
-                         f"batch_size={batch.batch_size}, T={n_tok}")
     kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
-    plan = shared._plan(batch, ext_lens, n_q, n_kv, head_dim, q.device)
+    plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, q.device)
     with _native.launching(q.device, stream):
         if not plan.shares or plan.n_items > MAX_PARTS \
                 or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
@@ -248,9 +265,9 @@ def shared_prefix_attention(
                 None if v_scale is None else v_scale.data_ptr(),
                 rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
                 batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
-        ws, nbytes = workspace("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
-                               plan.row_groups, plan.slot_rows, plan.n_pieces, n_q, n_kv,
-                               head_dim, kv_dtype)
+        ws, nbytes = _scratch("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
+                              plan.row_groups, plan.slot_rows, plan.n_pieces, n_q, n_kv,
+                              head_dim, kv_dtype)
         if plan.n_work:
             _native.call("tf_attn_extend", q.data_ptr(), q.stride(0), *pool, 0, work, plan.n_work,
                          n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), *epilogue,
