@@ -317,14 +317,16 @@ int32_t tf_attn_rows(
  * keys [k0, k1) of request b's table row; slots are 0 .. n_pieces - 1, a unit's (kv head
  * and 256 rows of a shared part) one behind the other, units = device int32 [..][2] =
  * {first slot, slots}, of a shared part's row block i and kv head h at pfx +
- * i * num_kv_heads + h, pfx being what the requests' own items then hold.
+ * i * num_kv_heads + h, pfx being what the requests' own items then hold.  n_stream
+ * (with row_groups 1): workgroups that stream the items in the pieces' launch, beside
+ * them; 0: a launch of their own.
  * The other arguments are tf_attn_decode's; rows that see no key are zeros.  Workspace:
  * tf_attn_shared_workspace_bytes of the same sizes, 16-byte aligned; calls that overlap
  * in time must not share it. */
 int64_t tf_attn_shared_workspace_bytes(int32_t n_items, int32_t row_groups, int32_t slot_rows,
-                                       int32_t n_pieces, int32_t num_q_heads,
-                                       int32_t num_kv_heads, int32_t head_dim,
-                                       int32_t kv_dtype);
+                                       int32_t n_pieces, int32_t n_stream,
+                                       int32_t num_q_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t kv_dtype);
 
 int32_t tf_attn_shared(
     const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
@@ -333,7 +335,7 @@ int32_t tf_attn_shared(
     const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* items,
     int32_t n_items, int32_t n_shared, const int32_t* tokens, int32_t row_groups,
     int32_t slot_rows, const int32_t* pieces, int32_t n_pieces, const int32_t* units,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    int32_t n_stream, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
     void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
 

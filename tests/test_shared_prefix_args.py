@@ -32,9 +32,9 @@ def test_groups_must_fit_the_batch():
     wl = small_case([9, 9], [1, 1], d=64, dtype=torch.bfloat16)
     dev = torch.device("cpu")
     with pytest.raises(ValueError, match="batch of 2"):
-        SharedPrefixes([([0, 2], 4)])._plan(wl.batch, 2, 4, 1, 64, dev)
+        SharedPrefixes([([0, 2], 4)])._plan(wl.batch, 2, 4, 1, 64, 0, dev)
     with pytest.raises(ValueError, match="width"):
-        SharedPrefixes([([0, 1], 400)])._plan(wl.batch, 2, 4, 1, 64, dev)
+        SharedPrefixes([([0, 1], 400)])._plan(wl.batch, 2, 4, 1, 64, 0, dev)
 
 
 def lists(plan):
@@ -50,9 +50,9 @@ GROUPS = [([0, 1, 5] + list(range(6, 60)), 2000), ([2, 4, 62], 50)]
 
 def test_short_prefixes_are_streamed():
     """(at head_dim 256: the items, no pieces)"""
-    plan = _Plan([([0, 1], 1000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256)
+    plan = _Plan([([0, 1], 1000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256, 3000, False)
     assert plan.n_shared == 1 and plan.n_pieces == 0 and plan.row_groups == 1
-    plan = _Plan([([0, 1], 2000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256)
+    plan = _Plan([([0, 1], 2000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256, 3000, False)
     assert plan.n_shared == 0 and plan.n_pieces > 4
 
 
@@ -61,7 +61,7 @@ def test_plan_covers_every_row_and_key_once(head_dim):
     """Each output row has one own part; own and shared parts meet at the shared length; a
     row's place in the shared part names the same token; pieces cover a unit's keys."""
     group, n_kv = 6, 4
-    plan = _Plan(GROUPS, EXT, 24, n_kv, head_dim, torch.device("cpu"), 64)
+    plan = _Plan(GROUPS, EXT, 24, n_kv, head_dim, torch.device("cpu"), 64, 3000, False)
     long_ = {4} if head_dim == 256 else set()
     items, work, pieces, toks, units = lists(plan)
     unit = 16 * plan.row_groups

@@ -115,14 +115,15 @@ SIGNATURES = {
         _p, _p,
     ]),
     "tf_attn_extend_split_workspace_bytes": (_i64, []),
-    "tf_attn_shared_workspace_bytes": (_i64, [_i32] * 8),
+    "tf_attn_shared_workspace_bytes": (_i64, [_i32] * 9),
     "tf_attn_shared": (_i32, [
         _p, _i64,
         _p, _p, _i64, _i32, _p, _p,
         _p, _i64, _i64, _i64,
         _p, _p,                        # req_pool_indices, seq_lens
         _p, _i32, _i32, _p,            # items, n_items, n_shared, tokens
-        _i32, _i32, _p, _i32, _p,      # row_groups, slot_rows, pieces, n_pieces, units
+        _i32, _i32,                    # row_groups, slot_rows
+        _p, _i32, _p, _i32,            # pieces, n_pieces, units, n_stream
         _i32, _i32, _i32, _f32,
         _p, _i64,
         _p, _i64,                      # workspace, workspace_bytes

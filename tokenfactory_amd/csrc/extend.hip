@@ -44,6 +44,7 @@
 
 #include <type_traits>
 
+#include "part_stream.h"
 #include "prefix_attn.h"
 #include "tf_common.h"
 #include "tf_internal.h"
@@ -403,12 +404,31 @@ constexpr float kNoKeys = -1e30f;
 
 // What the work list holds: whole entries; pieces of entries too (an instance of its
 // own: as one kernel, large prefills took 0.4 % and mixed steps 2 % longer); or pieces of
-// shared prefixes, whose rows are of the tokens that the entry lists (prefix_attn.hip).
+// shared prefixes, whose rows are of the tokens that the entry lists (prefix_attn.hip),
+// alone or beside workgroups that stream the requests' own parts (Beside: their arguments
+// and how many they are, the first of the grid).
 enum : int { kWhole = 0, kPieces = 1, kPrefix = 2 };
 
-template <bool FP8, int kList>
-__global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
+struct OwnParts {
+  PartArgs a;
+  int32_t n_stream;
+};
+
+template <bool FP8, int kList, class... Beside>
+__global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a, Beside... beside) {
   __shared__ Smem<FP8> sm;
+  int entry = blockIdx.x;
+  if constexpr (sizeof...(Beside) > 0) {
+    const OwnParts& own = (beside, ...);
+    if (entry < own.n_stream) {
+      using C = Cfg<kD, FP8, 1, false, true>;
+      static_assert(sizeof(StreamSmem<C, false, kWaves>) <= sizeof(sm), "LDS");
+      part_stream<C, false, kWaves>(own.a, reinterpret_cast<StreamSmem<C, false, kWaves>&>(sm),
+                                    entry);
+      return;
+    }
+    entry -= own.n_stream;
+  }
   constexpr bool kSplit = kList != kWhole;
   constexpr bool kShared = kList == kPrefix;
   constexpr int kKS = kStagesOf<FP8>, kVS = kVStagesOf<FP8>;
@@ -419,7 +439,7 @@ __global__ void __launch_bounds__(kThreads) extend_mfma_kernel(ExtendArgs a) {
   const int g = lane >> 5;
   const int n = lane & 31;
 
-  const int32_t* wk = a.work + 8 * (int64_t)blockIdx.x;
+  const int32_t* wk = a.work + 8 * (int64_t)entry;
   const int b = wk[0];
   const int hk = wk[1];
   const int row0 = wk[2];
@@ -887,13 +907,25 @@ int64_t part_bytes(int64_t n) { return part_ml_bytes(n) + n * kExtendItemRows * 
 
 }  // namespace
 
-int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, bool fp8, hipStream_t s) {
-  if (fp8)
-    hipLaunchKernelGGL((extend_mfma_kernel<true, kPrefix>), dim3((unsigned)n_pieces),
-                       dim3(kThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((extend_mfma_kernel<false, kPrefix>), dim3((unsigned)n_pieces),
-                       dim3(kThreads), 0, s, a);
+int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, const PartArgs* own,
+                         int32_t n_stream, bool fp8, hipStream_t s) {
+  const dim3 block(kThreads);
+  if (own) {
+    const OwnParts beside{*own, n_stream};
+    const dim3 grid((unsigned)(n_stream + n_pieces));
+    if (fp8)
+      hipLaunchKernelGGL((extend_mfma_kernel<true, kPrefix, OwnParts>), grid, block, 0, s, a,
+                         beside);
+    else
+      hipLaunchKernelGGL((extend_mfma_kernel<false, kPrefix, OwnParts>), grid, block, 0, s, a,
+                         beside);
+  } else if (fp8) {
+    hipLaunchKernelGGL((extend_mfma_kernel<true, kPrefix>), dim3((unsigned)n_pieces), block, 0, s,
+                       a);
+  } else {
+    hipLaunchKernelGGL((extend_mfma_kernel<false, kPrefix>), dim3((unsigned)n_pieces), block, 0,
+                       s, a);
+  }
   return launch_status("tf_attn_shared prefix launch");
 }
 
@@ -1082,7 +1114,7 @@ int32_t extend_launch(const void* q, int64_t q_row_stride, const void* k_pool,
     hipLaunchKernelGGL((extend_mfma_kernel<false, kWhole>), items, block, 0, s, a);
   const int rc = launch_status("tf_attn_extend launch");
   if (rc != TF_OK || n_merges == 0) return rc;
-  const dim3 grid((unsigned)n_merges, kWaves);
+  const dim3 grid((unsigned)n_merges, kExtendItemRows / kRowsPerWave);
   if (fp8)
     hipLaunchKernelGGL(extend_merge_kernel<true>, grid, block, 0, s, a, merges);
   else

@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "attn_row.h"
+#include "part_stream.h"
 #include "prefix_attn.h"
 #include "stream_tile.h"
 #include "tf_common.h"
@@ -32,298 +33,12 @@
 namespace tfa {
 namespace {
 
-// The context length of a request, clamped to its table row.
-__device__ __forceinline__ int context_len(const PartArgs& a, int b) {
-  const int64_t len =
-      min(a.seq_override > 0 ? (int64_t)a.seq_override : a.seq_lens[b], a.rtt_cols);
-  return len > 0 ? (int)len : 0;
-}
-
-__device__ __forceinline__ PartItem item_at(const PartArgs& a, int i) {
-  if (a.items) return a.items[i];
-  const int b = i / a.head_blocks;
-  return PartItem{b, b, 1, (i - b * a.head_blocks) * a.unit_rows, 0, -1, -1, 0};
-}
-__device__ __forceinline__ PartTok tok_at(const PartArgs& a, int i) {
-  return a.toks ? a.toks[i] : PartTok{i, i, 0, 0};
-}
-
-// Keys that token t of an item sees, counted from key 0.
-__device__ __forceinline__ int token_seen(const PartArgs& a, const PartTok& t) {
-  return context_len(a, t.b) - t.back;
-}
-
-// Keys of an item: a shared part's own bounds (a row of a shorter context masks what
-// lies behind it), else up to the last key that its last row sees.
-template <class C>
-__device__ __forceinline__ int part_keys(const PartArgs& a, const PartItem& it) {
-  if (it.b < 0) return 0;
-  int end;
-  if (it.k1 >= 0) {
-    end = min((int64_t)it.k1, a.rtt_cols);
-  } else {
-    const int last = min(it.row0 + C::kRows, it.n_tok * a.group) - 1;
-    end = token_seen(a, tok_at(a, it.tok0 + last / a.group));
-  }
-  return max(0, end - it.k0);
-}
-
-// What a unit costs beside its tiles (its slot ids, queries and partials), in tiles.
-constexpr int kUnitTiles = 8;
-constexpr int kHalfTiles = 8;                    // a wave stages slot ids for 8 tiles ahead,
-constexpr int kHalf = kHalfTiles * kTile;        // in two halves by turns
-
-// Positions of an item's units: its tiles behind kUnitTiles positions without work.
-__device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUnitTiles : 0; }
-
-// Scores on their way to memory (SCORED) wait in LDS, as many tiles' as there is room for
-// (28 KB a wave: 72 tiles of 6 rows), since loads issued after a store are waited for
-// behind it: stored at every tile, or at every 8 tiles, they took a fifth of the kernel's
-// time (64 requests of 1k to 8k keys 239 us, 201 without stores).
-template <class C> constexpr int kKeptFloats = C::DP == 128 ? 3072 : 7168;
-
-template <class C, bool SCORED>
-struct StreamSmem {
-  struct {
-    int32_t slots[2 * kHalf];
-    u32x4 kstage[kTile * C::kChunks];          // see stage_k
-    u32x4 qfrag[C::NG > 1 ? C::NG : 0][C::kSteps][kWave];   // (one group's stay in registers)
-    float kept[SCORED ? kKeptFloats<C> : 0];
-  } wave[kWaves];
-  int32_t ipre[kMaxItems + 1];                 // exclusive prefix of the items' spans
-  int32_t wsum[kWaves];
-};
-
-// SCORED: the scores are kept (16 bytes per row and four keys, a few percent of the keys'
-// own bytes), for the weights that follow.
 template <class C, bool SCORED>
 __global__ void __launch_bounds__(kWaves * kWave,
                                   (C::NG == 1 && !SCORED) || C::DP == 128 ? 2 : 1)
 part_stream_kernel(PartArgs a) {
-  __shared__ StreamSmem<C, SCORED> sm;
-  static_assert(!SCORED || C::NG == 1, "scored items are the heads of one token");
-  const int D = C::OTHER ? a.head_dim : C::DP;
-  const int row_bytes = C::FP8 ? D : 2 * D;
-  const int n_chunks = row_bytes / 16;
-
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int w = wave_id();
-  const int g = lane >> 4;
-  const int n = lane & 15;
-
-  // (every item by a thread of its own first: three loads in a row each)
-  int32_t* spans = reinterpret_cast<int32_t*>(&sm.wave[0]);
-  static_assert(sizeof(sm.wave) >= 4 * kMaxItems, "spans of the items");
-  for (int i = tid; i < a.n_items; i += kWaves * kWave)
-    spans[i] = unit_span((part_keys<C>(a, item_at(a, i)) + kTile - 1) / kTile);
-  __syncthreads();
-  item_prefix(a.n_items, [&](int i) { return spans[i]; }, sm.ipre, sm.wsum);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.n_items; i += kWaves * kWave) a.ipre[i] = sm.ipre[i];
-  // Every wave is a worker of its own: what a unit costs in front of its tiles (loads in
-  // a row) is then hidden by the other waves of the CU, and nothing is joined here.
-  const int64_t N = (int64_t)a.hkv * sm.ipre[a.n_items];
-  const int P = (int)min<int64_t>(a.n_workers, N);   // (owners of a unit are consecutive)
-  const int me = blockIdx.x * kWaves + w;
-  if (me >= P) return;
-  const int64_t x_end = (int64_t)(me + 1) * N / P;
-  int64_t x = (int64_t)me * N / P;
-
-  const float sl2 = a.scale_log2 * (C::FP8 ? a.k_scale[0] : 1.f);
-  const int64_t slot_bytes = (int64_t)a.hkv * row_bytes;
-  int32_t* const slots = sm.wave[w].slots;
-  u32x4* const ks = sm.wave[w].kstage;
-
-  int item = 0;   // the first whose units reach x
-  {
-    int lo = 0, hi = a.n_items - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)a.hkv * sm.ipre[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    item = lo;
-  }
-
-  while (x < x_end) {
-    // ---- the segment: unit (item, hk), tiles [t0, t1)
-    while ((int64_t)a.hkv * sm.ipre[item + 1] <= x) ++item;
-    const int span = sm.ipre[item + 1] - sm.ipre[item];
-    const int64_t r = x - (int64_t)a.hkv * sm.ipre[item];
-    const int hk = (int)(r / span);
-    const int v0 = (int)(r - (int64_t)hk * span);
-    const int v1 = (int)min<int64_t>(span, v0 + (x_end - x));
-    x += v1 - v0;
-    const int t0 = max(0, v0 - kUnitTiles), t1 = v1 - kUnitTiles;
-    if (t0 >= t1) continue;
-
-    const PartItem im = item_at(a, item);
-    const int L = part_keys<C>(a, im);
-    const int n_rows = im.n_tok * a.group - im.row0;       // of kRows
-    const int n_groups = min((n_rows + 15) / 16, C::NG);
-    const int64_t row = clamp_i64(a.rpi[im.b], 0, a.rtt_rows - 1);
-    const int64_t* rtt = a.rtt + row * a.rtt_stride + im.k0;
-    const uint8_t* kbase = a.k_pool + (int64_t)hk * row_bytes;
-    const uint8_t* vbase = a.v_pool + (int64_t)hk * row_bytes;
-    // Row n of group q: its token and head, and how many of the part's keys it sees.
-    auto row_of = [&](int q, int& qrow, int& hq, int& seen) {
-      const int rho = im.row0 + min(16 * q + n, n_rows - 1);
-      const int t = rho / a.group;
-      const PartTok tok = tok_at(a, im.tok0 + t);
-      qrow = tok.qrow;
-      hq = hk * a.group + rho - t * a.group;
-      seen = token_seen(a, tok) - im.k0;
-      return 16 * q + n < n_rows;
-    };
-    u32x4 qf[C::kSteps];
-    int seen[C::NG];
-#pragma unroll
-    for (int q = 0; q < C::NG; ++q) {
-      int qrow, hq;
-      const bool ok = row_of(q, qrow, hq, seen[q]);
-      const __bf16* qp = a.q + (int64_t)qrow * a.q_stride + (int64_t)hq * D;
-#pragma unroll
-      for (int kk = 0; kk < C::kSteps; ++kk) {
-        const int d0 = C::FP8 ? (64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : (32 * kk + 8 * g);
-        qf[kk] = ok && (!C::OTHER || d0 < D) ? ld_g16(qp + d0) : u32x4{0u, 0u, 0u, 0u};
-      }
-      if constexpr (C::NG > 1) {
-#pragma unroll
-        for (int kk = 0; kk < C::kSteps; ++kk) sm.wave[w].qfrag[q][kk][lane] = qf[kk];
-      }
-    }
-
-    WaveState<C> st;
-    reset_state<C>(st);
-    const int c0 = t0 * kTile;                    // keys below are counted from here
-    const int n_loc = min(L, t1 * kTile) - c0;
-    const int n_tiles = t1 - t0;
-    // Slot ids of half h: key k's at slots[k % (2 kHalf)]; keys past the last repeat it.
-    int64_t ids[kHalf / kWave];
-    auto fetch_ids = [&](int h) {
-#pragma unroll
-      for (int i = 0; i < kHalf / kWave; ++i)
-        ids[i] = rtt[c0 + min(h * kHalf + i * kWave + lane, n_loc - 1)];
-    };
-    auto stage_ids = [&](int h) {
-#pragma unroll
-      for (int i = 0; i < kHalf / kWave; ++i)
-        slots[(h & 1) * kHalf + i * kWave + lane] =
-            (int32_t)pool_row(ids[i], a.pool_slots, a.seq_override > 0);
-      wave_lds_sync();
-    };
-    auto issue = [&](u32x4 (&x)[4][C::kS], int it, const uint8_t* base) {
-      issue_rows<C>(x, slots, it & (2 * kHalfTiles - 1), 2 * kHalf, g, n, base, slot_bytes,
-                    n_chunks);
-    };
-    wave_lds_sync();
-    fetch_ids(0);
-    stage_ids(0);
-
-    // (rows of a multiple of 16 floats and 4: no two of a lane group on one bank)
-    const int kept_tiles = SCORED ? (kKeptFloats<C> / min(n_rows, 16) - 4) / kTile : 0;
-    const int kept_row = kept_tiles * kTile + 4;
-    int kept_from = 0;
-
-    // ---- the tiles, loads a tile ahead (see decode_kernel)
-    KBuf<C> kb;
-    VBuf<C> vb;
-    auto scores = [&](int it, u32x2 (&pt)[C::NG], u32x2 (&pl)[C::NG][2]) {
-      u32x4 kf[C::kSteps];
-      k_frags<C>(ks, g, n, kf);
-#pragma unroll
-      for (int q = 0; q < C::NG; ++q) {
-        if constexpr (C::NG > 1) {
-          if (q >= n_groups) break;
-#pragma unroll
-          for (int kk = 0; kk < C::kSteps; ++kk) qf[kk] = sm.wave[w].qfrag[q][kk][lane];
-        }
-        const int lim = min(n_loc, seen[q] - c0);
-        pt[q] = qk_softmax<C>(kf, qf, it, lim, g, sl2, st, q, pl[q], [&](const float (&sc)[4]) {
-          if constexpr (SCORED) {
-            if (n < n_rows)
-              *reinterpret_cast<f32x4*>(
-                  &sm.wave[w].kept[n * kept_row + (it - kept_from) * kTile + 4 * g]) =
-                  f32x4{sc[0], sc[1], sc[2], sc[3]};
-          }
-        });
-      }
-    };
-    // The kept scores of tiles kept_from .. it go out once there is no room for more, and
-    // at the last tile.
-    auto flush = [&](int it, bool last) {
-      if constexpr (SCORED) {
-        if (!last && it - kept_from + 1 < kept_tiles) return;
-        const int64_t k0 = c0 + kept_from * kTile;
-        const int keys = (int)min<int64_t>((it - kept_from + 1) * kTile, a.score_cap - k0);
-        float* rows = a.row_scores + ((int64_t)a.hkv * im.b + hk) * a.group * a.score_cap +
-                      im.row0 * a.score_cap + k0;
-        wave_lds_sync();
-        for (int r = 0; r < min(n_rows, 16); ++r)
-          for (int k = 4 * lane; k < keys; k += 4 * kWave)
-            *reinterpret_cast<f32x4*>(rows + r * a.score_cap + k) =
-                *reinterpret_cast<const f32x4*>(&sm.wave[w].kept[r * kept_row + k]);
-        wave_lds_sync();
-        kept_from = it + 1;
-      }
-    };
-    u32x2 pt[C::NG], pl[C::NG][2];
-    issue(kb.k, 0, kbase);
-    issue(vb.v, 0, vbase);
-    int it = 0;
-    for (; it + 1 < n_tiles; ++it) {
-      // The ids of the next half, read while this one's tiles go by; its place held the
-      // half before, whose last tile is issued.
-      const int at = it & (kHalfTiles - 1);
-      if (at == 0)
-        fetch_ids(it / kHalfTiles + 1);
-      else if (at == kHalfTiles / 2)
-        stage_ids(it / kHalfTiles + 1);
-      wave_lds_sync();
-      stage_k<C>(kb, ks, g, n);
-      wave_lds_sync();
-      __builtin_amdgcn_sched_barrier(0);
-      issue(kb.k, it + 1, kbase);
-      __builtin_amdgcn_sched_barrier(0);
-      scores(it, pt, pl);
-      pv<C>(vb, pt, pl, st, n_groups);
-      __builtin_amdgcn_sched_barrier(0);
-      issue(vb.v, it + 1, vbase);
-      __builtin_amdgcn_sched_barrier(0);
-      flush(it, false);
-    }
-    wave_lds_sync();
-    stage_k<C>(kb, ks, g, n);
-    wave_lds_sync();
-    scores(it, pt, pl);
-    pv<C>(vb, pt, pl, st, n_groups);
-    flush(it, true);
-
-#pragma unroll
-    for (int q = 0; q < C::NG; ++q) {
-      st.l[q] += __shfl_xor(st.l[q], 16, kWave);
-      st.l[q] += __shfl_xor(st.l[q], 32, kWave);
-    }
-    // Partials of (worker, unit), a row's dims side by side.  Lane (g, n) holds of
-    // row n the dims 128 s + 32 g + 8 r + e (bf16: accumulator 8 s + e) or 64 g + 16 r
-    // + e (fp8), four neighbours per store.
-    const int64_t slot = (int64_t)me + (int64_t)item * a.hkv + hk;
-#pragma unroll
-    for (int q = 0; q < C::NG; ++q) {
-      if (16 * q + n >= n_rows) continue;
-      const int64_t pr = slot * a.slot_rows + 16 * q + n;
-      float* po = a.part_o + pr * C::DP;
-#pragma unroll
-      for (int i = 0; i < C::kAcc; i += 4)
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr)
-          *reinterpret_cast<f32x4*>(po + (C::FP8 ? 64 * g + 16 * rr + i
-                                                 : 128 * (i >> 3) + 32 * g + 8 * rr + (i & 7))) =
-              f32x4{st.acc[q][i][rr], st.acc[q][i + 1][rr], st.acc[q][i + 2][rr],
-                    st.acc[q][i + 3][rr]};
-      if (g == 0) a.part_ml[pr] = float2{st.m[q], st.l[q]};
-    }
-  }
+  __shared__ StreamSmem<C, SCORED, kWaves> sm;
+  part_stream<C, SCORED, kWaves>(a, sm, blockIdx.x);
 }
 
 // Joins the parts of every row: WPR waves per row take its partials in turn, kAhead of
@@ -577,6 +292,8 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
   amax_commit(a.amax, om);
 }
 
+constexpr int kStepWaves = 8;   // of a workgroup that streams beside MFMA pieces
+
 // Kernel shape and workspace of a call.
 struct PartPlan {
   bool fp8, narrow, other;
@@ -589,7 +306,7 @@ struct PartPlan {
 };
 
 int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t slot_rows,
-                   int32_t n_pieces, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
+                   int32_t n_pieces, int32_t n_stream, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
                    PartPlan* p) {
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
     return fail(TF_ERR_INVALID, "%s: num_q_heads=%d not a multiple of num_kv_heads=%d", fn,
@@ -609,6 +326,9 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
                 kMaxItems);
   if (n_pieces < 0 || (n_pieces && head_dim != 256))
     return fail(TF_ERR_INVALID, "%s: n_pieces=%d at head_dim=%d", fn, n_pieces, head_dim);
+  if (n_stream < 0 || n_stream > 4096 || (n_stream && (!n_pieces || row_groups != 1)))
+    return fail(TF_ERR_INVALID, "%s: n_stream=%d beside %d pieces, row_groups=%d", fn, n_stream,
+                n_pieces, row_groups);
   p->other = head_dim != 256;
   p->narrow = head_dim <= 128 && !p->fp8;
   p->unit_rows = 16 * row_groups;
@@ -617,6 +337,7 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   // units of 32 rows 28 and 37 us with two; 96 of 1 to 700 at 32 / 8 heads of 128 56 us,
   // 83 with four).
   p->n_workers = kWaves * device_cu_count() * (p->narrow ? 2 : 1);
+  if (n_stream) p->n_workers = kStepWaves * n_stream;
   const int64_t rows = (p->n_workers + (int64_t)n_items * num_kv_heads) * slot_rows;
   p->ipre_bytes = ((int64_t)(n_items + 1) * 4 + 255) / 256 * 256;
   p->ml_bytes = (rows * 8 + 255) / 256 * 256;
@@ -642,9 +363,10 @@ void launch_stream_groups(const PartArgs& a, const PartPlan& p, hipStream_t s) {
 }
 
 template <int WPR, bool SCORED>
-void launch_merge(const PartArgs& a, const PartPlan& p, int rows, hipStream_t s) {
+void launch_merge_rows(const PartArgs& a, const PartPlan& p, hipStream_t s) {
+  constexpr int kRows = kMergeWaves / WPR;
   const dim3 grid((unsigned)((a.n_items - a.own0) * a.hkv + a.n_weights),
-                  (unsigned)((rows + kMergeWaves / WPR - 1) / (kMergeWaves / WPR)));
+                  (unsigned)((a.slot_rows + kRows - 1) / kRows));
   const dim3 block(kMergeWaves * kWave);
   if (p.narrow)
     hipLaunchKernelGGL((part_merge_kernel<128, false, WPR, SCORED>), grid, block, 0, s, a);
@@ -652,6 +374,16 @@ void launch_merge(const PartArgs& a, const PartPlan& p, int rows, hipStream_t s)
     hipLaunchKernelGGL((part_merge_kernel<256, true, WPR, SCORED>), grid, block, 0, s, a);
   else
     hipLaunchKernelGGL((part_merge_kernel<256, false, WPR, SCORED>), grid, block, 0, s, a);
+}
+
+// Four waves per row, one where the rows alone fill the CUs (72 rows 5.0 and 7.1 us, 1536
+// rows 9.0 and 9.3, 3072 rows of 128 dims 23.0 and 10.4, 6144 rows of 256 28.4 and 17.2).
+template <bool SCORED>
+void launch_merge(const PartArgs& a, const PartPlan& p, hipStream_t s) {
+  if ((int64_t)(a.n_items - a.own0) * a.hkv * a.slot_rows > 2048)
+    launch_merge_rows<1, SCORED>(a, p, s);
+  else
+    launch_merge_rows<4, SCORED>(a, p, s);
 }
 
 PartArgs part_args(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
@@ -702,13 +434,14 @@ PartArgs part_args(const void* q, int64_t q_row_stride, const void* k_pool, cons
 
 extern "C" int64_t tf_attn_shared_workspace_bytes(int32_t n_items, int32_t row_groups,
                                                   int32_t slot_rows, int32_t n_pieces,
-                                                  int32_t num_q_heads, int32_t num_kv_heads,
+                                                  int32_t n_stream, int32_t num_q_heads,
+                                                  int32_t num_kv_heads,
                                                   int32_t head_dim, int32_t kv_dtype) {
   using namespace tfa;
   clear_error();
   PartPlan p;
-  const int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, num_q_heads,
-                                num_kv_heads, head_dim, kv_dtype, &p);
+  const int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, n_stream,
+                                num_q_heads, num_kv_heads, head_dim, kv_dtype, &p);
   return rc != TF_OK ? rc : p.total();
 }
 
@@ -719,13 +452,13 @@ extern "C" int32_t tf_attn_shared(
     const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* items,
     int32_t n_items, int32_t n_shared, const int32_t* tokens, int32_t row_groups,
     int32_t slot_rows, const int32_t* pieces, int32_t n_pieces, const int32_t* units,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    int32_t n_stream, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
     void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, const void* gate,
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream) {
   using namespace tfa;
   clear_error();
   PartPlan p;
-  int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, num_q_heads,
+  int rc = make_part_plan("shared", n_items, row_groups, slot_rows, n_pieces, n_stream, num_q_heads,
                           num_kv_heads, head_dim, kv_dtype, &p);
   if (rc != TF_OK) return rc;
   if (n_shared < 0 || n_shared > n_items || (n_shared && n_pieces))
@@ -777,16 +510,18 @@ extern "C" int32_t tf_attn_shared(
     e.part_ml = reinterpret_cast<float*>(at);
     e.part_o = reinterpret_cast<float*>(at + p.piece_ml_bytes);
     e.toks = a.toks;
-    rc = launch_prefix_pieces(e, n_pieces, p.fp8, s);
+    rc = launch_prefix_pieces(e, n_pieces, n_stream ? &a : nullptr, n_stream, p.fp8, s);
     if (rc != TF_OK) return rc;
   }
-  if (row_groups == 1)
-    launch_stream_groups<1, false>(a, p, s);
-  else
-    launch_stream_groups<2, false>(a, p, s);
-  rc = launch_status("tf_attn_shared stream launch");
-  if (rc != TF_OK) return rc;
-  launch_merge<4, false>(a, p, slot_rows, s);
+  if (!n_stream) {
+    if (row_groups == 1)
+      launch_stream_groups<1, false>(a, p, s);
+    else
+      launch_stream_groups<2, false>(a, p, s);
+    rc = launch_status("tf_attn_shared stream launch");
+    if (rc != TF_OK) return rc;
+  }
+  launch_merge<false>(a, p, s);
   return launch_status("tf_attn_shared merge launch");
 }
 
@@ -813,7 +548,7 @@ int make_scored_plan(int32_t batch, int32_t max_len, int32_t num_q_heads, int32_
     return fail(TF_ERR_UNSUPPORTED, "scored: %d requests of %d head blocks (at most %d)", batch,
                 r->head_blocks, kMaxItems);
   r->n_items = batch * r->head_blocks;
-  const int rc = make_part_plan("scored", r->n_items, 1, r->slot_rows, 0, num_q_heads,
+  const int rc = make_part_plan("scored", r->n_items, 1, r->slot_rows, 0, 0, num_q_heads,
                                 num_kv_heads, head_dim, kv_dtype, &r->p);
   if (rc != TF_OK) return rc;
   r->p.o_bytes = (r->p.o_bytes + 255) / 256 * 256;
@@ -882,6 +617,6 @@ extern "C" int32_t tf_attn_scored(
   launch_stream_groups<1, true>(a, r.p, s);
   rc = launch_status("tf_attn_scored stream launch");
   if (rc != TF_OK) return rc;
-  launch_merge<4, true>(a, r.p, r.slot_rows, s);
+  launch_merge<true>(a, r.p, s);
   return launch_status("tf_attn_scored launch");
 }

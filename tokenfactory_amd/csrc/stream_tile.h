@@ -313,13 +313,13 @@ __device__ __forceinline__ bool any_odd(const WaveState<C>& st) {
   return y != y;
 }
 // ipre[i] = sum of tiles(i) of items < i, ipre[n_items] = total (block-wide scan).
-template <class Tiles>
+template <int WAVES = kWaves, class Tiles>
 __device__ __forceinline__ void item_prefix(int n_items, const Tiles& tiles, int32_t* ipre,
                                             int32_t* wsum) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = wave_id();
-  constexpr int kPer = kMaxItems / (kWaves * kWave);
+  constexpr int kPer = kMaxItems / (WAVES * kWave);
   int t[kPer];
   int sum = 0;
 #pragma unroll
@@ -344,7 +344,7 @@ __device__ __forceinline__ void item_prefix(int n_items, const Tiles& tiles, int
     if (i <= n_items) ipre[i] = excl;
     excl += t[k];
   }
-  if (tid == kWaves * kWave - 1 && n_items == kMaxItems) ipre[kMaxItems] = excl;
+  if (tid == WAVES * kWave - 1 && n_items == kMaxItems) ipre[kMaxItems] = excl;
   __syncthreads();
 }
 // Workgroup that owns global tile x when N tiles are split over P workgroups.

@@ -59,6 +59,7 @@ void plan_units(int32_t n_items, int32_t num_kv_heads, int32_t n_hgroups, int32_
 // kExtendItemRows flattened (token, q-head-of-group) rows each.
 constexpr int kExtendItemRows = 256;
 struct PartTok;
+struct PartArgs;
 struct ExtendArgs {
   const __bf16* q;
   int64_t q_stride;
@@ -86,8 +87,10 @@ struct ExtendArgs {
 };
 // The extend kernel over pieces of shared prefixes (head_dim 256): work entries {b, kv
 // head, row0, first token, tokens, first key, end key, slot + 1}, b's table row read for
-// all of them; partials [slot][256 rows][256], as prefix_attn.hip merges them.
-int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, bool fp8, hipStream_t s);
+// all of them; partials [slot][256 rows][256], as prefix_attn.hip merges them.  own (or
+// NULL): items that n_stream workgroups of 8 waves stream in the same launch.
+int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, const PartArgs* own,
+                         int32_t n_stream, bool fp8, hipStream_t s);
 
 // Slot attention for head dims other than 256 (attn_generic.hip): one wave per
 // query row.  work != NULL: the rows of n_rows extend work entries; else the

@@ -55,8 +55,8 @@ class SharedPrefixes:
         self._lock = threading.Lock()
         self._plans: Dict[tuple, _Plan] = {}
 
-    def _plan(self, batch, n_tok, n_q, n_kv, head_dim, device) -> "_Plan":
-        key = (device.index, batch.batch_size, n_tok, n_q, n_kv, head_dim,
+    def _plan(self, batch, n_tok, n_q, n_kv, head_dim, kv_dtype, device) -> "_Plan":
+        key = (device.index, batch.batch_size, n_tok, n_q, n_kv, head_dim, kv_dtype,
                batch.req_to_token.shape[1], tuple(batch.extend_lens))
         plan = self._plans.get(key)
         if plan is not None:
@@ -75,7 +75,8 @@ class SharedPrefixes:
             plan = self._plans.get(key)
             if plan is None:
                 plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device,
-                                                _cu_count(device))
+                                                _cu_count(device), int(batch.max_seq_len),
+                                                kv_dtype == _native.TF_DTYPE_FP8_E4M3)
             return plan
 
 
@@ -106,12 +107,26 @@ def _streams(groups, rows, n_kv: int) -> bool:
     return max((n for _, n in groups), default=0) <= 1536 and units <= 4096
 
 
+def _stream_share(steps: int, longest: Sequence[int], n_kv: int, fp8: bool, cus: int) -> int:
+    """Workgroups, of one per CU, that stream the requests' own parts beside the pieces of
+    the shared ones, which take ``steps`` steps of the MFMA tiles in all: in proportion to
+    what either takes of a CU's time (a step 2 us; a unit 3 us and 0.45 us per 16 keys, or
+    half of an fp8 pool's), the own parts being half of the longest that they can be (the
+    host knows that alone).  Measured with 0 (two launches), 64, 128 and 160 of 256: 64
+    requests on 8192 shared keys 76, 74, 56 and 52 us, 256 on 32768 of an fp8 pool 361,
+    284, 364 and 440."""
+    first, tile = (1.7, 0.23) if fp8 else (3.0, 0.45)
+    own = n_kv * sum(first + tile * 0.5 * max(0, n) / 16 for n in longest)
+    share = cus * own / (own + 2.0 * steps)
+    return int(min(max(share, cus / 16), cus * 5 / 8))
+
+
 class _Plan:
     """The device lists of one step layout: parts of contexts and their tokens; at head_dim
     256 the pieces of the shared ones; and the extend kernel's entries of long prompts,
     which share nothing (MFMA-bound)."""
 
-    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus):
+    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus, max_len, fp8):
         group = n_q // n_kv
         self.device = device
         long_ = {b for b, e in enumerate(ext_lens)
@@ -125,7 +140,9 @@ class _Plan:
         mfma = head_dim == 256 and not _streams(groups, shared_rows, n_kv)
         if not mfma:
             rows += shared_rows
-        self.row_groups = 2 if max(rows, default=1) > 16 else 1
+        # (Units of 16 rows stream beside the pieces, which outweighs that 17 to 32 rows read
+        # their keys twice: 4 groups of 4 of 1 to 4 tokens 60 us in units of 32, 55 so.)
+        self.row_groups = 2 if max(rows, default=1) > (32 if mfma else 16) else 1
         unit = 16 * self.row_groups
         self.slot_rows = min(unit, max(rows, default=1))
 
@@ -142,8 +159,16 @@ class _Plan:
             return at
 
         n_blocks = [-(-r // EXTEND_TILE_ROWS) for r in shared_rows]
-        cuts = cut_units([-(-n // KEYS_PER_STEP) for (_, n), k in zip(groups, n_blocks)
-                          for _ in range(k * n_kv)], cus) if mfma else []
+        self.n_stream, cuts = 0, []
+        if mfma:
+            steps = [-(-n // KEYS_PER_STEP) for (_, n), k in zip(groups, n_blocks)
+                     for _ in range(k * n_kv)]
+            if self.row_groups == 1:
+                prefix_of = {b: n for m, n in groups for b in m}
+                self.n_stream = _stream_share(
+                    sum(steps), [max_len - prefix_of.get(b, 0) for b in range(len(ext_lens))
+                                 if b not in long_], n_kv, fp8, cus)
+            cuts = cut_units(steps, cus - self.n_stream)
         for (members, length), blocks in zip(groups, n_blocks):
             tok0 = len(tokens)
             for b in members:
@@ -244,7 +269,7 @@ def shared_prefix_attention(
     if n_q % n_kv:
         raise ValueError(f"num_q_heads {n_q} is not a multiple of num_kv_heads {n_kv}")
     kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
-    plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, q.device)
+    plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, q.device)
     with _native.launching(q.device, stream):
         if not plan.shares or plan.n_items > MAX_PARTS \
                 or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
@@ -266,14 +291,14 @@ def shared_prefix_attention(
                 rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
                 batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
         ws, nbytes = _scratch("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
-                              plan.row_groups, plan.slot_rows, plan.n_pieces, n_q, n_kv,
-                              head_dim, kv_dtype)
+                              plan.row_groups, plan.slot_rows, plan.n_pieces, plan.n_stream,
+                              n_q, n_kv, head_dim, kv_dtype)
         if plan.n_work:
             _native.call("tf_attn_extend", q.data_ptr(), q.stride(0), *pool, 0, work, plan.n_work,
                          n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), *epilogue,
                          handle)
         _native.call("tf_attn_shared", q.data_ptr(), q.stride(0), *pool, items, plan.n_items,
                      plan.n_shared, tokens, plan.row_groups, plan.slot_rows, pieces,
-                     plan.n_pieces, units, n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
+                     plan.n_pieces, units, plan.n_stream, n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
                      handle)
     return out
