@@ -16,6 +16,13 @@ What the attention path reads:
 
 ``prefix_lens`` and ``is_prefill`` are carried but not read by attention (the
 prefix is ``seq_lens - extend_lens``, as at ``qwen3_8/full_attention.py:267``).
+
+Additions, which ``FullAttention.forward`` picks up: ``shared_prefixes`` (a
+``SharedPrefixes``: requests whose rows begin with the same slots, read once per group)
+and ``token_scores`` (fp32 of ``req_to_token``'s shape, to which every full-attention layer
+adds the weights that the last ``score_window`` new tokens of each request give its keys;
+zero a row when a request takes it).  A step with both is scored and reads every
+request's whole context.
 """
 from __future__ import annotations
 
@@ -40,6 +47,9 @@ class ForwardBatch:
     max_extend_len: int = 0
     extend_lens_tensor: Optional[torch.Tensor] = None
     req_pool_indices_list: Optional[List[int]] = None
+    shared_prefixes: Optional[object] = None
+    token_scores: Optional[torch.Tensor] = None
+    score_window: int = 32
 
     def __post_init__(self) -> None:
         # Defaulting order and rules follow qwen3_8/forward_batch.py:33-45.

@@ -21,6 +21,9 @@ projection). With an FP8 ``quantization_config`` (``quant_method == "fp8"``,
 projections are ``Fp8Linear`` (dynamic e4m3 activations x block-scaled e4m3
 weights on the gfx950 FP8 GEMM, like the reference's Triton path); otherwise
 plain bf16 ``nn.Linear``.
+
+A batch that carries ``shared_prefixes`` or ``token_scores`` runs
+``shared_prefix_attention`` or ``scored_attention`` instead, with the same output.
 """
 from __future__ import annotations
 
@@ -31,6 +34,8 @@ import torch.nn as nn
 
 from .attention import qk_norm_rope_kv_write, slot_based_attention
 from .fp8_linear import Fp8Linear, fp8_linears
+from .scored_attention import scored_attention
+from .shared_prefix import shared_prefix_attention
 
 
 def _fp8_block_size(config):
@@ -177,9 +182,18 @@ class FullAttention(nn.Module):
         # (fp8_triton.py:128), which saves that pass a read of the output.
         fp8_out = isinstance(self.o_proj, Fp8Linear)
         amax = torch.zeros((1,), dtype=torch.int32, device=q.device) if fp8_out else None
-        attn = slot_based_attention(q, k_buf, v_buf, forward_batch, scaling=self.scaling,
-                                    k_scale=scales[0], v_scale=scales[1], gate=gate,
-                                    out_amax=amax)
+        attention = dict(scaling=self.scaling, k_scale=scales[0], v_scale=scales[1], gate=gate,
+                         out_amax=amax)
+        scores = getattr(forward_batch, "token_scores", None)
+        shared = getattr(forward_batch, "shared_prefixes", None)
+        if scores is not None:
+            attn = scored_attention(q, k_buf, v_buf, forward_batch, scores,
+                                    window=getattr(forward_batch, "score_window", 32),
+                                    **attention)
+        elif shared is not None:
+            attn = shared_prefix_attention(q, k_buf, v_buf, forward_batch, shared, **attention)
+        else:
+            attn = slot_based_attention(q, k_buf, v_buf, forward_batch, **attention)
         x = attn.reshape(n_tok, self.num_heads * self.head_dim)
         return self.o_proj(x, x_amax=amax) if fp8_out else self.o_proj(x)
 
