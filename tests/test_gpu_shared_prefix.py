@@ -347,3 +347,64 @@ def test_pieces_captured_and_replayed(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, call(wl, SharedPrefixes(members))), step
+
+
+@pytest.mark.parametrize("d", [128, 64, 32, 80, 8, 120])
+@pytest.mark.parametrize("heads", [(32, 8), (6, 1), (34, 2)])
+def test_pieces_at_other_head_dims(gpu, d, heads):
+    wl, groups = shared_case([1700, 130], [5, 1, 40, 17, 16, 8], [0, 0, 1, 0, 1, 0], heads=heads,
+                             d=d, seed=31)
+    check(wl, groups, f"pieces {heads} D={d}")
+
+
+@pytest.mark.parametrize("prefix", [1537, 1600, 1601, 1663, 4133])
+def test_piece_lengths_at_128_dims(gpu, prefix):
+    wl, groups = shared_case([prefix], [1, 2, 9], [0] * 3, heads=(4, 1), d=128, seed=prefix)
+    check(wl, groups, f"pieces of {prefix}, D=128")
+
+
+@pytest.mark.parametrize("members", [2, 9, 65, 130])
+def test_piece_rows_at_128_dims(gpu, members):
+    """Row blocks of 256, 4 rows a member; waves and blocks partly filled."""
+    wl, groups = shared_case([1600], [1 + 7 * i % 50 for i in range(members)], [0] * members,
+                             heads=(4, 1), d=128, seed=members)
+    check(wl, groups, f"pieces of {members} members, D=128")
+
+
+@pytest.mark.parametrize("d", [128, 64])
+def test_pieces_with_prompts_at_other_head_dims(gpu, d):
+    """Prompt chunks in a group: hundreds of rows of one request, causal in their own part."""
+    wl, members = shared_case([1700, 0], [1, 70, 20, 3, 100], [0, 0, 0, 0, 1],
+                              ext=[1, 70, 1, 3, 100], heads=(8, 2), d=d, seed=33)
+    check(wl, members, f"pieces, prompts, D={d}")
+
+
+def test_short_members_and_odd_values_at_128_dims(gpu):
+    wl, members = shared_case([1800], [5, 8, 1, 30], [0] * 4, seed=37, ext=[1, 3, 1, 2],
+                              heads=(8, 2), d=128)
+    table = wl.batch.req_to_token
+    bad = torch.ones(wl.k_pool.shape[0], dtype=torch.bool, device=gpu)
+    bad[table[table >= 0].unique()] = False
+    wl.k_pool[bad] = float("nan")
+    wl.v_pool[bad] = float("nan")
+    shared = SharedPrefixes(members)
+    for lens in ([1805, 1808, 0, 1700], [0, 2, 1, 1], [1805, 1799, 17, 1830]):
+        wl.batch.seq_lens.copy_(torch.tensor(lens))
+        want, spread, _ = attention64(wl, seq_lens=lens)
+        assert_attention(call(wl, shared), want, spread, wl, f"lens {lens}")
+    # a NaN value of a shared key: NaN for the rows that see it, the others as before
+    lens = [1805, 1808, 100, 1700]
+    wl.batch.seq_lens.copy_(torch.tensor(lens))
+    want, spread, _ = attention64(wl, seq_lens=lens)
+    wl.v_pool[table[wl.rows[0], 900]] = float("nan")
+    got = call(wl, shared)
+    at = [0, 1, 4, 5, 7]       # first q row of each request (new tokens 1, 3, 1, 2)
+    assert torch.isnan(got[[0, 1, 2, 3, 5, 6]].float()).all()
+    assert_attention(got[4:5], want[4:5], spread[4:5], wl, "a row that ends before it")
+    assert at[-1] == got.shape[0]
+
+
+def test_large_scores_at_128_dims(gpu):
+    wl, members = shared_case([1600], [40, 3, 1], [0] * 3, heads=(8, 2), d=128, seed=39,
+                              q_std=40.0)
+    check(wl, members, "pieces, large scores, D=128")

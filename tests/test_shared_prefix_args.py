@@ -56,7 +56,7 @@ def test_short_prefixes_are_streamed():
     assert plan.n_shared == 0 and plan.n_pieces > 4
 
 
-@pytest.mark.parametrize("head_dim", [256, 128])
+@pytest.mark.parametrize("head_dim", [256, 128, 192])
 def test_plan_covers_every_row_and_key_once(head_dim):
     """Each output row has one own part; own and shared parts meet at the shared length; a
     row's place in the shared part names the same token; pieces cover a unit's keys."""
@@ -78,7 +78,7 @@ def test_plan_covers_every_row_and_key_once(head_dim):
             if pfx < 0:
                 continue
             rp = (pfx_tok + t) * group + rho % group
-            if head_dim != 256:
+            if head_dim == 192:
                 front = items[pfx + rp // unit]
                 assert front[3] == rp // unit * unit and front[4] == 0 and front[5] == k0
                 assert toks[front[1] + pfx_tok + t].tolist() == toks[tok0 + t].tolist()
@@ -96,7 +96,7 @@ def test_plan_covers_every_row_and_key_once(head_dim):
                     assert rp < n_front * group
     assert rows == {(b, r) for b, e in enumerate(EXT) if b not in long_ for r in range(e * group)}
     assert set(work[:, 0].tolist()) == long_
-    assert (len(pieces) > 0) == (head_dim == 256) and len(pieces) <= 64
+    assert (len(pieces) > 0) == (head_dim != 192) and len(pieces) <= 64
 
 
 @pytest.mark.parametrize("steps,cus", [([256] * 8, 256), ([1024] * 24, 256), ([1], 256),

@@ -20,7 +20,7 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libtf_attn.so"
 SOURCES = ["abi.hip", "add_norm.hip", "attn_generic.hip", "attn_weights.hip", "block_fp8.hip", "decode.hip",
            "evict.hip", "extend.hip", "fp8_linear.hip", "gdn.hip", "kv_ops.hip", "narrow_linear.hip", "plan.hip",
-           "prefix_attn.hip", "qk_prep.hip"]
+           "prefix_attn.hip", "prefix_tiles.hip", "qk_prep.hip"]
 ARCH = "gfx950"
 
 
@@ -51,8 +51,9 @@ def compile_flags() -> list:
 # of a wave.  fp8_linear.hip, block_fp8.hip: the GEMMs fold each MFMA product into fp32
 # accumulators with a VALU FMA, which reads VGPRs only.  gdn.hip: the chunked
 # recurrence feeds its accumulators (state, P, Delta) back to VALU work and
-# MFMA operands.
-EXTRA_FLAGS = {"extend.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"],
+# MFMA operands.  prefix_tiles.hip: as extend.hip.
+EXTRA_FLAGS = {"prefix_tiles.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"],
+               "extend.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"],
                "block_fp8.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"],
                "fp8_linear.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"],
                "gdn.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form=1"]}

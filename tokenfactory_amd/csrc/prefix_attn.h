@@ -52,10 +52,10 @@ struct PartArgs {
   int32_t* ipre;           // prefix of the items' spans, for the merge
   float2* part_ml;         // partials of (worker + unit) slots
   float* part_o;
-  // Shared parts that the extend kernel took in pieces (NULL: they are items): unit
+  // Shared parts that MFMA tiles took in pieces (NULL: they are items): unit
   // pfx + (row / 256) * hkv + kv head is {first slot, slots}.
   const int2* units;
-  const float2* piece_ml;  // [slot][256], [slot][256][256]
+  const float2* piece_ml;  // [slot][256], [slot][256][256 or 128]
   const float* piece_o;
   // Scored calls: every row's scores (log2 units, -inf where masked) of its first
   // score_cap keys, row q_row * q heads + head, and the table that their weights go to.

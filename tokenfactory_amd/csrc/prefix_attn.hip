@@ -9,8 +9,11 @@
 // one item per request, or several where it has more rows than a unit.  Every item
 // leaves fp32 partials, which part_merge_kernel joins.
 //
-// At head_dim 256 the shared parts go through the extend kernel's MFMA tiles instead
-// (extend.hip, kPrefix), cut over their keys so that every CU has a piece.
+// Long shared parts go through MFMA tiles instead, cut over their keys so that every CU has a
+// piece: the extend kernel's at head_dim 256 (extend.hip, kPrefix), prefix_tiles.hip's up
+// to 128.  Where a request's own rows fit one or two units of 16, its own part is streamed
+// by other workgroups of the same launch: the tiles are bound by MFMA, the streams by HBM,
+// which about half of the CUs saturate.
 //
 // part_stream_kernel does the decode kernel's tile work (decode.hip) with waves that
 // work alone: a persistent wave owns an equal share of all units' tiles (unit = (item, kv
@@ -324,13 +327,14 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   if (n_items > kMaxItems)
     return fail(TF_ERR_UNSUPPORTED, "%s: %d parts in one call (at most %d)", fn, n_items,
                 kMaxItems);
-  if (n_pieces < 0 || (n_pieces && head_dim != 256))
-    return fail(TF_ERR_INVALID, "%s: n_pieces=%d at head_dim=%d", fn, n_pieces, head_dim);
   if (n_stream < 0 || n_stream > 4096 || (n_stream && (!n_pieces || row_groups != 1)))
     return fail(TF_ERR_INVALID, "%s: n_stream=%d beside %d pieces, row_groups=%d", fn, n_stream,
                 n_pieces, row_groups);
   p->other = head_dim != 256;
   p->narrow = head_dim <= 128 && !p->fp8;
+  if (n_pieces < 0 || (n_pieces && p->other && !p->narrow))
+    return fail(TF_ERR_INVALID, "%s: n_pieces=%d at head_dim=%d, kv_dtype=%d", fn, n_pieces,
+                head_dim, kv_dtype);
   p->unit_rows = 16 * row_groups;
   // Four waves per CU, eight of the 128-dim ones (measured with half and twice as many:
   // 64 requests of 1 to 1024 keys 30 us, 42 with eight waves per CU; 16 of 1 to 2048 in
@@ -343,7 +347,7 @@ int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t 
   p->ml_bytes = (rows * 8 + 255) / 256 * 256;
   p->o_bytes = rows * (p->narrow ? 128 : 256) * 4;
   p->piece_ml_bytes = (int64_t)n_pieces * kExtendItemRows * 8;
-  p->piece_o_bytes = (int64_t)n_pieces * kExtendItemRows * 256 * 4;
+  p->piece_o_bytes = (int64_t)n_pieces * kExtendItemRows * (p->narrow ? 128 : 256) * 4;
   return TF_OK;
 }
 
@@ -510,7 +514,9 @@ extern "C" int32_t tf_attn_shared(
     e.part_ml = reinterpret_cast<float*>(at);
     e.part_o = reinterpret_cast<float*>(at + p.piece_ml_bytes);
     e.toks = a.toks;
-    rc = launch_prefix_pieces(e, n_pieces, n_stream ? &a : nullptr, n_stream, p.fp8, s);
+    const PartArgs* own = n_stream ? &a : nullptr;
+    rc = p.narrow ? launch_prefix_tiles(e, head_dim, n_pieces, own, n_stream, s)
+                  : launch_prefix_pieces(e, n_pieces, own, n_stream, p.fp8, s);
     if (rc != TF_OK) return rc;
   }
   if (!n_stream) {

@@ -91,6 +91,10 @@ struct ExtendArgs {
 // NULL): items that n_stream workgroups of 8 waves stream in the same launch.
 int launch_prefix_pieces(const ExtendArgs& a, int32_t n_pieces, const PartArgs* own,
                          int32_t n_stream, bool fp8, hipStream_t s);
+// The same at head dims up to 128 of bf16 pools (prefix_tiles.hip): partials [slot][256
+// rows][128].
+int launch_prefix_tiles(const ExtendArgs& a, int32_t head_dim, int32_t n_pieces,
+                        const PartArgs* own, int32_t n_stream, hipStream_t s);
 
 // Slot attention for head dims other than 256 (attn_generic.hip): one wave per
 // query row.  work != NULL: the rows of n_rows extend work entries; else the

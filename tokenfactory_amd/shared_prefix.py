@@ -122,9 +122,9 @@ def _stream_share(steps: int, longest: Sequence[int], n_kv: int, fp8: bool, cus:
 
 
 class _Plan:
-    """The device lists of one step layout: parts of contexts and their tokens; at head_dim
-    256 the pieces of the shared ones; and the extend kernel's entries of long prompts,
-    which share nothing (MFMA-bound)."""
+    """The device lists of one step layout: parts of contexts and their tokens; the pieces of
+    long shared ones where MFMA tiles take them; and at head_dim 256 the extend kernel's
+    entries of long prompts, which share nothing (MFMA-bound)."""
 
     def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus, max_len, fp8):
         group = n_q // n_kv
@@ -137,7 +137,8 @@ class _Plan:
         self.shares = bool(groups)
         shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
         rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
-        mfma = head_dim == 256 and not _streams(groups, shared_rows, n_kv)
+        mfma = (head_dim == 256 or (head_dim <= 128 and not fp8)) \
+            and not _streams(groups, shared_rows, n_kv)
         if not mfma:
             rows += shared_rows
         # (Units of 16 rows stream beside the pieces, which outweighs that 17 to 32 rows read
