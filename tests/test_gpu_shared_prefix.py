@@ -271,13 +271,19 @@ def test_slots_behind_2_gib(gpu):
     assert_attention(got, want, spread, wl, "far slots")
 
 
-def test_many_requests(gpu):
-    """More parts than one launch takes: the unshared path answers."""
+@pytest.mark.parametrize("d", [64, 192])
+def test_many_requests(gpu, d):
+    """As many parts as one launch takes; at 192 dims, where the shared ones are parts too,
+    more than that: the unshared path answers."""
     b = 2000
-    wl = small_case([40] * b, [1] * b, hq=2, hkv=1, d=64, seed=17, device=gpu,
+    wl = small_case([40] * b, [1] * b, hq=2, hkv=1, d=d, seed=17, device=gpu,
                     dtype=torch.bfloat16, groups=[0] * b, prefixes=[30])
-    want = slot_based_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, scaling=wl.scale)
-    assert torch.equal(call(wl, SharedPrefixes([(list(range(b)), 30)])), want)
+    groups = [(list(range(b)), 30)]
+    if d == 64:
+        check(wl, groups, "2000 requests")
+    else:
+        want = slot_based_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, scaling=wl.scale)
+        assert torch.equal(call(wl, SharedPrefixes(groups)), want)
 
 
 @pytest.mark.parametrize("fp8", [False, True])

@@ -48,12 +48,27 @@ EXT = [1, 4, 2, 1, 70, 1] + [1] * 60
 GROUPS = [([0, 1, 5] + list(range(6, 60)), 2000), ([2, 4, 62], 50)]
 
 
-def test_short_prefixes_are_streamed():
-    """(at head_dim 256: the items, no pieces)"""
-    plan = _Plan([([0, 1], 1000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256, 3000, False)
-    assert plan.n_shared == 1 and plan.n_pieces == 0 and plan.row_groups == 1
-    plan = _Plan([([0, 1], 2000)], [1, 1], 24, 4, 256, torch.device("cpu"), 256, 3000, False)
-    assert plan.n_shared == 0 and plan.n_pieces > 4
+@pytest.mark.parametrize("head_dim,fp8,pieces", [(256, False, True), (256, True, True),
+                                                 (128, False, True), (128, True, False),
+                                                 (8, False, True), (136, False, False)])
+def test_what_takes_the_shared_parts(head_dim, fp8, pieces):
+    plan = _Plan([([0, 1], 1000)], [1, 1], 24, 4, head_dim, torch.device("cpu"), 256, 1100, fp8)
+    assert (plan.n_pieces > 0) == pieces and (plan.n_shared > 0) != pieces
+    assert (plan.n_stream > 0) == pieces and plan.row_groups == 1
+
+
+@pytest.mark.parametrize("head_dim", [256, 128, 192])
+@pytest.mark.parametrize("groups", [[], [([1, 2], 60)]])
+def test_steps_that_share_nothing(head_dim, groups):
+    """No group, or (at 256 dims) one whose other member is a long prompt."""
+    ext = [1, 1, 100]
+    plan = _Plan(groups, ext, 24, 4, head_dim, torch.device("cpu"), 256, 1100, False)
+    assert plan.shares == (bool(groups) and head_dim != 256)
+
+
+def test_rows_too_many_to_stream_beside():
+    plan = _Plan([([0, 1], 1000)], [1, 9], 24, 4, 256, torch.device("cpu"), 256, 1100, False)
+    assert plan.n_pieces and not plan.n_stream and plan.row_groups == 2
 
 
 @pytest.mark.parametrize("head_dim", [256, 128, 192])

@@ -81,7 +81,7 @@ class SharedPrefixes:
 
 
 KEYS_PER_STEP = 32   # of the extend kernel
-MIN_STEPS = 8        # of a piece of a prefix
+MIN_STEPS = 2        # of a piece: 3 requests on 300 keys 13.7 us, with 8 17.1, with 16 20.7
 
 
 def cut_units(steps: Sequence[int], cus: int) -> List[int]:
@@ -97,28 +97,34 @@ def cut_units(steps: Sequence[int], cus: int) -> List[int]:
     return [max(1, -(-s // lo)) for s in steps]
 
 
-def _streams(groups, rows, n_kv: int) -> bool:
-    """Whether the shared parts of a step at head_dim 256 are streamed with the others,
-    32 rows at a time, rather than taken in MFMA pieces, whose launch and partials cost
-    12 to 20 us whatever the length: short ones of few rows (24 / 4 heads, one group of 2
-    on 1000 keys 21 us streamed, 26 in pieces, of 64 on 500 40 and 45, of 4 on 4000 36 and
-    28; 4 groups of 4 on 2500 36 both ways, of 64 on 2000 57 both ways)."""
-    units = sum(-(-r // 32) * n_kv * -(-n // 16) for (_, n), r in zip(groups, rows))
-    return max((n for _, n in groups), default=0) <= 1536 and units <= 4096
+# Times in us that the split of a step is estimated with, by (narrow tiles, fp8 pool): of a
+# streaming workgroup (8 waves) per unit and per 16 keys of it, of a step of 32 keys by MFMA
+# tiles without and with all of their 256 rows.
+_STEP_US = {(False, False): (3.0, 0.40, 0.35, 1.5), (False, True): (1.7, 0.21, 0.4, 1.9),
+            (True, False): (2.0, 0.18, 0.3, 1.0)}
 
 
-def _stream_share(steps: int, longest: Sequence[int], n_kv: int, fp8: bool, cus: int) -> int:
-    """Workgroups, of one per CU, that stream the requests' own parts beside the pieces of
-    the shared ones, which take ``steps`` steps of the MFMA tiles in all: in proportion to
-    what either takes of a CU's time (a step 2 us; a unit 3 us and 0.45 us per 16 keys, or
-    half of an fp8 pool's), the own parts being half of the longest that they can be (the
-    host knows that alone).  Measured with 0 (two launches), 64, 128 and 160 of 256: 64
-    requests on 8192 shared keys 76, 74, 56 and 52 us, 256 on 32768 of an fp8 pool 361,
-    284, 364 and 440."""
-    first, tile = (1.7, 0.23) if fp8 else (3.0, 0.45)
-    own = n_kv * sum(first + tile * 0.5 * max(0, n) / 16 for n in longest)
-    share = cus * own / (own + 2.0 * steps)
-    return int(min(max(share, cus / 16), cus * 5 / 8))
+def _stream_share(steps: Sequence[Tuple[int, int]], own: Sequence[Tuple[int, int]], n_kv: int,
+                  narrow: bool, fp8: bool, cus: int) -> int:
+    """Workgroups, one per CU, that stream the requests' own parts beside the pieces of the
+    shared ones: where both are estimated to end together.  steps: (steps, rows) of each
+    MFMA unit; own: (units of 16 rows, longest own part) per request, which is taken to
+    be half full (the host knows no more).  Measured with 64, 112, 160 and 192 of 256: 64
+    requests on 8192 shared keys 75, 58, 52 and 63 us (two launches 71), branches of 4
+    groups 74, 61, 54 and 51 (57), 96 on 2000 of 128 dims 84, 62, 51 and 44 (62), 256 on
+    32768 of an fp8 pool 294, 318, 429 and 821 (330)."""
+    unit, tile, step, full = _STEP_US[narrow, fp8]
+    streams = n_kv * sum(u * (unit + tile * 0.5 * max(0, n) / 16) for u, n in own)
+    total, longest = sum(k for k, _ in steps), max(k for k, _ in steps)
+    per_step = sum(k * (step + (full - step) * min(r, EXTEND_TILE_ROWS) / EXTEND_TILE_ROWS)
+                   for k, r in steps) / total
+
+    def end(n):   # (pieces are whole: the longest unit is cut into as many as it can)
+        parts = max(1, (cus - n) * longest // total)
+        rounds = max(1.0, len(steps) / (cus - n))
+        return max(10 + streams / n, 12 + per_step * rounds * -(-longest // parts))
+
+    return min(range(max(1, cus // 16), cus * 3 // 4 + 1, max(1, cus // 32)), key=end)
 
 
 class _Plan:
@@ -137,8 +143,7 @@ class _Plan:
         self.shares = bool(groups)
         shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
         rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
-        mfma = (head_dim == 256 or (head_dim <= 128 and not fp8)) \
-            and not _streams(groups, shared_rows, n_kv)
+        mfma = self.shares and (head_dim == 256 or (head_dim <= 128 and not fp8))
         if not mfma:
             rows += shared_rows
         # (Units of 16 rows stream beside the pieces, which outweighs that 17 to 32 rows read
@@ -162,14 +167,16 @@ class _Plan:
         n_blocks = [-(-r // EXTEND_TILE_ROWS) for r in shared_rows]
         self.n_stream, cuts = 0, []
         if mfma:
-            steps = [-(-n // KEYS_PER_STEP) for (_, n), k in zip(groups, n_blocks)
-                     for _ in range(k * n_kv)]
+            steps = [(-(-n // KEYS_PER_STEP), r - EXTEND_TILE_ROWS * i)
+                     for (_, n), r, k in zip(groups, shared_rows, n_blocks)
+                     for i in range(k) for _ in range(n_kv)]
             if self.row_groups == 1:
                 prefix_of = {b: n for m, n in groups for b in m}
                 self.n_stream = _stream_share(
-                    sum(steps), [max_len - prefix_of.get(b, 0) for b in range(len(ext_lens))
-                                 if b not in long_], n_kv, fp8, cus)
-            cuts = cut_units(steps, cus - self.n_stream)
+                    steps, [(-(-e * group // 16), max_len - prefix_of.get(b, 0))
+                            for b, e in enumerate(ext_lens) if b not in long_],
+                    n_kv, head_dim != 256, fp8, cus)
+            cuts = cut_units([k for k, _ in steps], cus - self.n_stream)
         for (members, length), blocks in zip(groups, n_blocks):
             tok0 = len(tokens)
             for b in members:
