@@ -47,7 +47,7 @@ def score_error(wl):
     |q k|, itself at most |q| |k|), the sum is scaled and exponentiated."""
     qn = wl.q.double().norm(dim=2).max().item()
     kn = pool64(wl.k_pool, wl.k_scale).nan_to_num(0.0).norm(dim=2).max().item()
-    return (wl.head_dim + 3) * 2.0 ** -24 * qn * kn * wl.scale + 2.0 ** -21
+    return (wl.head_dim + 3) * 2.0 ** -24 * qn * kn * abs(wl.scale) + 2.0 ** -21
 
 
 def assert_attention(got, want, spread, wl, what=""):

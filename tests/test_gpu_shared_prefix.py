@@ -414,3 +414,52 @@ def test_large_scores_at_128_dims(gpu):
     wl, members = shared_case([1600], [40, 3, 1], [0] * 3, heads=(8, 2), d=128, seed=39,
                               q_std=40.0)
     check(wl, members, "pieces, large scores, D=128")
+
+
+@pytest.mark.parametrize("d,fp8", [(256, False), (256, True), (128, False)])
+def test_many_pairs(gpu, d, fp8):
+    """Shared parts of at most 16 rows, streamed with the requests' own: 40 pairs, some of
+    contexts that end inside the shared part."""
+    groups = [b % 40 for b in range(80)]
+    wl, members = shared_case([1 + 17 * g for g in range(40)],
+                              [1 + 11 * b % 60 for b in range(80)], groups, d=d, seed=40, fp8=fp8)
+    wl.batch.seq_lens[77] = 1 + 17 * 37 - 30
+    got = call(wl, SharedPrefixes(members))
+    want, spread, _ = attention64(wl, seq_lens=wl.batch.seq_lens.tolist())
+    assert_attention(got, want, spread, wl, f"pairs D={d} fp8={fp8}")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_long_prompts_on_long_contexts(gpu, fp8):
+    """A prompt's entries cut over their keys beside decodes that share, then the same plan
+    for other lengths, and captured."""
+    ext = [1, 1, 1, 1, 30, 1]
+    wl, members = shared_case([700, 0], [9, 1, 40, 3, 5000, 2], [0, 0, 0, 0, 1, 0], ext=ext,
+                              seed=12, fp8=fp8)
+    shared = SharedPrefixes(members)
+
+    def right(got, what):
+        want, spread, _ = attention64(wl, seq_lens=wl.batch.seq_lens.tolist())
+        assert_attention(got, want, spread, wl, what)
+
+    right(call(wl, shared), "split")
+    out = torch.zeros_like(wl.q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(wl, shared, out=out)
+    for seq in ([709, 701, 740, 703, 5000, 702], [705, 701, 703, 703, 200, 702],
+                [709, 701, 740, 703, 3001, 702], [709, 701, 740, 703, 30, 702]):
+        wl.batch.seq_lens.copy_(torch.tensor(seq))
+        right(call(wl, shared), f"eager {seq}")
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        right(out, f"replayed {seq}")
+
+
+def test_negative_scaling(gpu):
+    wl, members = shared_case([200], [5, 9, 1, 30], [0] * 4, seed=13)
+    wl.scale = -wl.scale
+    got = call(wl, SharedPrefixes(members))
+    want, spread, _ = attention64(wl)
+    assert_attention(got, want, spread, wl, "negative scaling")

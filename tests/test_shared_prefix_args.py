@@ -5,7 +5,7 @@ import torch
 
 from tests.helpers import small_case
 from tokenfactory_amd import SharedPrefixes, shared_prefix_attention
-from tokenfactory_amd.shared_prefix import MIN_STEPS, _Plan, cut_units
+from tokenfactory_amd.shared_prefix import MAX_LAYOUTS, MIN_STEPS, _Plan, cut_units
 
 
 @pytest.mark.parametrize("groups", [[([0, 0], 5)], [([0, 1], 5), ([1, 2], 5)], [([0, -1], 5)],
@@ -66,9 +66,46 @@ def test_steps_that_share_nothing(head_dim, groups):
     assert plan.shares == (bool(groups) and head_dim != 256)
 
 
-def test_rows_too_many_to_stream_beside():
-    plan = _Plan([([0, 1], 1000)], [1, 9], 24, 4, 256, torch.device("cpu"), 256, 1100, False)
-    assert plan.n_pieces and not plan.n_stream and plan.row_groups == 2
+@pytest.mark.parametrize("head_dim,new,beside", [(256, 9, True), (128, 10, True),
+                                                 (128, 11, False)])
+def test_rows_too_many_to_stream_beside(head_dim, new, beside):
+    plan = _Plan([([0, 1], 1000)], [1, new], 24, 4, head_dim, torch.device("cpu"), 256, 1100, 0)
+    assert plan.n_pieces and (plan.n_stream > 0) == beside
+    assert plan.row_groups == (1 if beside else 2)
+
+
+@pytest.mark.parametrize("head_dim", [256, 128])
+def test_parts_of_few_rows_are_streamed_where_they_are_many(head_dim):
+    """Pairs of 12 rows: by tiles alone, streamed where there are many or own keys are
+    nearly all; threes of 18 rows by tiles."""
+    def plan(n, members, max_len):
+        groups = [(list(range(g * members, (g + 1) * members)), 500) for g in range(n)]
+        return _Plan(groups, [1] * n * members, 24, 4, head_dim, torch.device("cpu"), 256,
+                     max_len, 0)
+    assert plan(2, 2, 600).n_pieces
+    assert not plan(40, 2, 600).n_pieces and plan(40, 2, 600).n_shared == 40
+    assert not plan(2, 2, 9000).n_pieces
+    assert plan(40, 3, 600).n_pieces
+
+
+def test_long_prompts_on_long_contexts_are_cut():
+    def plan(max_len):
+        return _Plan([([0, 1], 500)], [1, 1, 64], 24, 4, 256, torch.device("cpu"), 256, max_len, 0)
+    assert plan(60000).route.split and not plan(800).route.split
+    assert plan(800).n_work == plan(60000).n_work == 8
+
+
+def test_layouts_are_bounded(monkeypatch):
+    """One object over many layouts keeps the lists of the latest alone."""
+    monkeypatch.setattr("tokenfactory_amd.shared_prefix._cu_count", lambda device: 256)
+    shared = SharedPrefixes([([0, 1], 100)])
+    plans = []
+    for new in range(1, MAX_LAYOUTS + 3):
+        b = small_case([200, 200], [1, new], d=128, dtype=torch.bfloat16).batch
+        n_tok = sum(b.extend_lens)
+        plans.append(shared._plan(b, n_tok, 24, 4, 128, 0, torch.device("cpu")))
+        assert shared._plan(b, n_tok, 24, 4, 128, 0, torch.device("cpu")) is plans[-1]
+    assert len(shared._plans) == MAX_LAYOUTS
 
 
 @pytest.mark.parametrize("head_dim", [256, 128, 192])

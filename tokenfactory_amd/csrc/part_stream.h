@@ -56,7 +56,7 @@ __device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUn
 // (28 KB a wave: 72 tiles of 6 rows), since loads issued after a store are waited for
 // behind it: stored at every tile, or at every 8 tiles, they took a fifth of the kernel's
 // time (64 requests of 1k to 8k keys 239 us, 201 without stores).
-template <class C> constexpr int kKeptFloats = C::DP == 128 ? 3072 : 7168;
+template <class C> constexpr int kKeptFloats = C::DP == 128 ? 12 << 8 : 28 << 8;
 
 template <class C, bool SCORED, int WAVES>
 struct StreamSmem {

@@ -9,9 +9,10 @@
 // one item per request, or several where it has more rows than a unit.  Every item
 // leaves fp32 partials, which part_merge_kernel joins.
 //
-// Long shared parts go through MFMA tiles instead, cut over their keys so that every CU has a
-// piece: the extend kernel's at head_dim 256 (extend.hip, kPrefix), prefix_tiles.hip's up
-// to 128.  Where a request's own rows fit one or two units of 16, its own part is streamed
+// Shared parts go through MFMA tiles instead (but many parts of few rows, or where nearly all
+// keys are own ones: shared_prefix.py has the rule and its figures), cut over their keys so that
+// every CU has a piece: the extend kernel's at head_dim 256 (extend.hip, kPrefix),
+// prefix_tiles.hip's up to 128.  Where the requests' own rows fit units of 16, up to four each, its own part is streamed
 // by other workgroups of the same launch: the tiles are bound by MFMA, the streams by HBM,
 // which about half of the CUs saturate.
 //
@@ -381,7 +382,7 @@ void launch_merge_rows(const PartArgs& a, const PartPlan& p, hipStream_t s) {
 }
 
 // Four waves per row, one where the rows alone fill the CUs (72 rows 5.0 and 7.1 us, 1536
-// rows 9.0 and 9.3, 3072 rows of 128 dims 23.0 and 10.4, 6144 rows of 256 28.4 and 17.2).
+// rows 9.0 and 9.3, 96 x 32 rows of 128 dims 23.0 and 10.4, 6144 rows of 256 28.4 and 17.2).
 template <bool SCORED>
 void launch_merge(const PartArgs& a, const PartPlan& p, hipStream_t s) {
   if ((int64_t)(a.n_items - a.own0) * a.hkv * a.slot_rows > 2048)

@@ -20,12 +20,14 @@ import numpy as np
 import torch
 
 from . import _native
-from .attention import (SHORT_ROWS, _KV_DTYPES, _check_inputs, _cu_count, _epilogue, _output,
-                        _plan_event, _pool_scales, _scratch, _upload, _ws_lock,
-                        slot_based_attention)
+from .attention import (SHORT_ROWS, SPLIT_KEYS, Route, _KV_DTYPES, _check_inputs, _cu_count,
+                        _epilogue, _fork_join_events, _output, _plan_event, _pool_scales, _scratch,
+                        _side_stream, _upload, _ws_lock, slot_based_attention)
+from .fp8_linear import _ptr
 from .planning import EXTEND_TILE_ROWS, plan_extend
 
 MAX_PARTS = 2048          # parts of contexts in one launch
+MAX_LAYOUTS = 64          # step layouts whose lists an object keeps
 _captured: List[object] = []   # lists that captured graphs read
 
 
@@ -57,7 +59,8 @@ class SharedPrefixes:
 
     def _plan(self, batch, n_tok, n_q, n_kv, head_dim, kv_dtype, device) -> "_Plan":
         key = (device.index, batch.batch_size, n_tok, n_q, n_kv, head_dim, kv_dtype,
-               batch.req_to_token.shape[1], tuple(batch.extend_lens))
+               batch.req_to_token.shape[1], tuple(batch.extend_lens),
+               batch.max_extend_len > 1 and batch.max_seq_len >= SPLIT_KEYS)
         plan = self._plans.get(key)
         if plan is not None:
             return plan
@@ -74,9 +77,11 @@ class SharedPrefixes:
         with self._lock:
             plan = self._plans.get(key)
             if plan is None:
+                if len(self._plans) >= MAX_LAYOUTS:   # (calls under way hold their own)
+                    del self._plans[next(iter(self._plans))]
                 plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device,
                                                 _cu_count(device), int(batch.max_seq_len),
-                                                kv_dtype == _native.TF_DTYPE_FP8_E4M3)
+                                                kv_dtype)
             return plan
 
 
@@ -100,21 +105,20 @@ def cut_units(steps: Sequence[int], cus: int) -> List[int]:
 # Times in us that the split of a step is estimated with, by (narrow tiles, fp8 pool): of a
 # streaming workgroup (8 waves) per unit and per 16 keys of it, of a step of 32 keys by MFMA
 # tiles without and with all of their 256 rows.
-_STEP_US = {(False, False): (3.0, 0.40, 0.35, 1.5), (False, True): (1.7, 0.21, 0.4, 1.9),
-            (True, False): (2.0, 0.18, 0.3, 1.0)}
+_STEP_US = {(False, False): (3.0, 0.40, 0.45, 1.5), (False, True): (1.7, 0.21, 0.4, 1.9),
+            (True, False): (2.0, 0.18, 0.3, 1.5)}
 
 
 def _stream_share(steps: Sequence[Tuple[int, int]], own: Sequence[Tuple[int, int]], n_kv: int,
                   narrow: bool, fp8: bool, cus: int) -> int:
     """Workgroups, one per CU, that stream the requests' own parts beside the pieces of the
     shared ones: where both are estimated to end together.  steps: (steps, rows) of each
-    MFMA unit; own: (units of 16 rows, longest own part) per request, which is taken to
-    be half full (the host knows no more).  Measured with 64, 112, 160 and 192 of 256: 64
+    MFMA unit; own: (units of 16 rows, keys of the own part) per request.  Measured with 64, 112, 160 and 192 of 256: 64
     requests on 8192 shared keys 75, 58, 52 and 63 us (two launches 71), branches of 4
     groups 74, 61, 54 and 51 (57), 96 on 2000 of 128 dims 84, 62, 51 and 44 (62), 256 on
     32768 of an fp8 pool 294, 318, 429 and 821 (330)."""
     unit, tile, step, full = _STEP_US[narrow, fp8]
-    streams = n_kv * sum(u * (unit + tile * 0.5 * max(0, n) / 16) for u, n in own)
+    streams = n_kv * sum(u * (unit + tile * n / 16) for u, n in own)
     total, longest = sum(k for k, _ in steps), max(k for k, _ in steps)
     per_step = sum(k * (step + (full - step) * min(r, EXTEND_TILE_ROWS) / EXTEND_TILE_ROWS)
                    for k, r in steps) / total
@@ -124,17 +128,30 @@ def _stream_share(steps: Sequence[Tuple[int, int]], own: Sequence[Tuple[int, int
         rounds = max(1.0, len(steps) / (cus - n))
         return max(10 + streams / n, 12 + per_step * rounds * -(-longest // parts))
 
-    return min(range(max(1, cus // 16), cus * 3 // 4 + 1, max(1, cus // 32)), key=end)
+    return min(range(max(1, cus // 16), cus * 7 // 8 + 1, max(1, cus // 32)), key=end)
+
+
+def _streams_all(shared: Sequence[Tuple[int, int]], own_keys: int, n_kv: int, cus: int) -> bool:
+    """Whether the shared parts ((rows, keys) each) are streamed as the requests' own are, in
+    units of 16 rows, and not by MFMA tiles: where a unit holds a part's rows, so that its
+    keys are still read once, and either the parts are many (32 groups of 2 on 500 keys 37
+    us, 50 by tiles, 500 of 2 on 2000 964 and 1046) or own keys are nearly all (2 requests
+    on 100 keys beside 62 of 4k: 119 and 128).  One group of 4 on 8000 keys, 16 rows of
+    128 dims: 39 us streamed, whose merge joins hundreds of waves' partials, 22 by tiles."""
+    return max(r for r, _ in shared) <= 16 and (
+        4 * n_kv * len(shared) >= cus or 8 * sum(n for _, n in shared) <= own_keys)
 
 
 class _Plan:
     """The device lists of one step layout: parts of contexts and their tokens; the pieces of
     long shared ones where MFMA tiles take them; and at head_dim 256 the extend kernel's
-    entries of long prompts, which share nothing (MFMA-bound)."""
+    entries of long prompts, which share nothing (MFMA-bound) and may be cut over their
+    keys as in ``slot_based_attention``."""
 
-    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus, max_len, fp8):
+    def __init__(self, groups, ext_lens, n_q, n_kv, head_dim, device, cus, max_len, kv_dtype):
         group = n_q // n_kv
-        self.device = device
+        fp8 = kv_dtype == _native.TF_DTYPE_FP8_E4M3
+        self.device, self.n_q, self.n_kv = device, n_q, n_kv
         long_ = {b for b, e in enumerate(ext_lens)
                  if head_dim == 256 and e * group > SHORT_ROWS}
         starts = [0, *np.cumsum(ext_lens).tolist()]
@@ -143,12 +160,20 @@ class _Plan:
         self.shares = bool(groups)
         shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
         rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
-        mfma = self.shares and (head_dim == 256 or (head_dim <= 128 and not fp8))
+        prefix_of = {b: n for m, n in groups for b in m}
+        # (own parts are taken to be half full: the host knows the longest context alone)
+        own_keys = {b: max(0, max_len - prefix_of.get(b, 0)) // 2
+                    for b in range(len(ext_lens)) if b not in long_}
+        mfma = self.shares and (head_dim == 256 or (head_dim <= 128 and not fp8)) \
+            and not _streams_all([(r, n) for r, (_, n) in zip(shared_rows, groups)],
+                                 sum(own_keys.values()), n_kv, cus)
         if not mfma:
             rows += shared_rows
-        # (Units of 16 rows stream beside the pieces, which outweighs that 17 to 32 rows read
-        # their keys twice: 4 groups of 4 of 1 to 4 tokens 60 us in units of 32, 55 so.)
-        self.row_groups = 2 if max(rows, default=1) > (32 if mfma else 16) else 1
+        # (Units of 16 rows stream beside the pieces, which outweighs that up to 64 rows read
+        # their keys four times: 4 groups of 8 of 6 tokens on 4000 keys 58 us, 82 in units of
+        # 32; 12 of 10 on 1000 35 and 51; with own parts of up to 2000 keys, 4 groups of 8
+        # of 10, 149 and 132.)
+        self.row_groups = 2 if max(rows, default=1) > (64 if mfma else 16) else 1
         unit = 16 * self.row_groups
         self.slot_rows = min(unit, max(rows, default=1))
 
@@ -171,10 +196,8 @@ class _Plan:
                      for (_, n), r, k in zip(groups, shared_rows, n_blocks)
                      for i in range(k) for _ in range(n_kv)]
             if self.row_groups == 1:
-                prefix_of = {b: n for m, n in groups for b in m}
                 self.n_stream = _stream_share(
-                    steps, [(-(-e * group // 16), max_len - prefix_of.get(b, 0))
-                            for b, e in enumerate(ext_lens) if b not in long_],
+                    steps, [(-(-ext_lens[b] * group // 16), n) for b, n in own_keys.items()],
                     n_kv, head_dim != 256, fp8, cus)
             cuts = cut_units([k for k, _ in steps], cus - self.n_stream)
         for (members, length), blocks in zip(groups, n_blocks):
@@ -205,18 +228,22 @@ class _Plan:
             work = plan_extend(ext_lens, n_q, n_kv, decode_to_decode_kernel=True)
             work = work[np.isin(work[:, 0], list(long_))]
         self.n_work, self.n_pieces = len(work), len(pieces)
+        long_lens = [ext_lens[b] for b in sorted(long_)]
+        self.route = Route(long_lens, sum(long_lens), n_q, n_kv, head_dim, kv_dtype, len(work),
+                           exact=True, max_len=max_len, cus=cus) if long_ else None
         parts = [np.asarray(x, dtype=np.int32).reshape(-1)
                  for x in (items, work, pieces, tokens, units)]
         self._offsets = np.cumsum([0] + [4 * len(x) for x in parts])[:5].tolist()
         self._host = np.concatenate(parts)
         self._lock = threading.Lock()
         self._lists: Optional[torch.Tensor] = None
+        self._split: Optional[torch.Tensor] = None   # pieces of the long prompts' entries
         self._users: set = set()
         self._event = None
         self._addresses: List[int] = []
         self._kept = False
 
-    def lists(self) -> List[int]:
+    def lists(self, batch) -> List[int]:
         """Addresses of (items, work, pieces, tokens, units) for launches on the current
         stream."""
         capturing = torch.cuda.is_current_stream_capturing()
@@ -229,19 +256,28 @@ class _Plan:
                     raise RuntimeError("shared prefixes cannot be planned in a graph capture: "
                                        "run the call once before it")
                 self._lists = _upload(self._host, self.device, stream)
-                self._addresses = [self._lists.data_ptr() + at for at in self._offsets]
+                addresses = [self._lists.data_ptr() + at for at in self._offsets]
+                if self.route is not None and self.route.split:
+                    # (shares by the lengths of now; right for any later ones)
+                    self._split = self.route.alloc(self.device)
+                    self.route.plan(self._split, addresses[1], self.n_work, None, None, 0,
+                                    self.n_q, self.n_kv, batch, stream)
+                    addresses[1] = self._split.data_ptr()
+                self._addresses = addresses
                 with _ws_lock:
                     self._event = _plan_event(self.device, stream)
                     self._event.record(stream)
                 self._users.add(stream.cuda_stream)
             elif stream.cuda_stream not in self._users and not capturing:
                 # (torch waits for the device before it captures)
-                self._lists.record_stream(stream)
+                for t in (self._lists, self._split):
+                    if t is not None:
+                        t.record_stream(stream)
                 stream.wait_event(self._event)
                 self._users.add(stream.cuda_stream)
             if capturing and not self._kept:
                 self._kept = True
-                _captured.append(self._lists)
+                _captured.append((self._lists, self._split))
         return self._addresses
 
 
@@ -268,7 +304,8 @@ def shared_prefix_attention(
     Steps in which nothing is shared run ``slot_based_attention`` itself: no group of two
     requests with few new tokens (prompts of more than 64 rows, new tokens x query heads
     per kv head, are bound by their products at head_dim 256, not by their keys' bytes),
-    an fp8 pool whose head_dim is not a multiple of 16, or more than 2048 parts."""
+    an fp8 pool whose head_dim is not a multiple of 16, more than 2048 parts, or a negative
+    ``scaling`` (the tiles follow a row's largest product)."""
     fn = "shared_prefix_attention"
     _native.refuse_gradients(fn, q, layer_k_buffer, layer_v_buffer, gate)
     _check_inputs(q, layer_k_buffer, layer_v_buffer, batch)
@@ -280,7 +317,7 @@ def shared_prefix_attention(
     plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, q.device)
     with _native.launching(q.device, stream):
         if not plan.shares or plan.n_items > MAX_PARTS \
-                or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
+                or (scaling is not None and not scaling >= 0) or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
             return slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, scaling=scaling,
                                         k_scale=k_scale, v_scale=v_scale, out=out, gate=gate,
                                         out_amax=out_amax)
@@ -290,23 +327,42 @@ def shared_prefix_attention(
             q = q.contiguous()
         out = _output(q, out)
         epilogue = _epilogue(q, gate, out_amax)
-        items, work, pieces, tokens, units = plan.lists()
-        handle = _native.current_stream(q.device)
+        items, work, pieces, tokens, units = plan.lists(batch)
         rtt = batch.req_to_token
         pool = (layer_k_buffer.data_ptr(), layer_v_buffer.data_ptr(), n_slots, kv_dtype,
-                None if k_scale is None else k_scale.data_ptr(),
-                None if v_scale is None else v_scale.data_ptr(),
-                rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
-                batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
+                _ptr(k_scale), _ptr(v_scale), rtt.data_ptr(), rtt.shape[0], rtt.stride(0),
+                rtt.shape[1], batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr())
         ws, nbytes = _scratch("tf_attn_shared_workspace_bytes", q.device, plan.n_items,
                               plan.row_groups, plan.slot_rows, plan.n_pieces, plan.n_stream,
                               n_q, n_kv, head_dim, kv_dtype)
-        if plan.n_work:
+
+        def parts(handle):
+            _native.call("tf_attn_shared", q.data_ptr(), q.stride(0), *pool, items, plan.n_items,
+                         plan.n_shared, tokens, plan.row_groups, plan.slot_rows, pieces,
+                         plan.n_pieces, units, plan.n_stream, n_q, n_kv, head_dim, scaling,
+                         out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue, handle)
+
+        if not plan.n_work:
+            parts(_native.current_stream(q.device))
+            return out
+        # Long prompts' entries, and the parts beside them on a second stream: they write
+        # other rows of out, and take the CUs that the entries leave.
+        main, side = torch.cuda.current_stream(q.device), _side_stream(q.device)
+        fork, join = _fork_join_events(q.device, main)
+        fork.record(main)
+        if plan.route.split:
+            split_ws = torch.empty(_native.load().tf_attn_extend_split_workspace_bytes(),
+                                   dtype=torch.uint8, device=q.device)
+            _native.call("tf_attn_extend_split", q.data_ptr(), q.stride(0), *pool, 0, work,
+                         plan.route.n_pieces, work + 32 * plan.route.n_pieces,
+                         plan.route.n_merges, split_ws.data_ptr(), split_ws.numel(), n_q, n_kv,
+                         scaling, out.data_ptr(), out.stride(0), *epilogue, main.cuda_stream)
+        else:
             _native.call("tf_attn_extend", q.data_ptr(), q.stride(0), *pool, 0, work, plan.n_work,
                          n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), *epilogue,
-                         handle)
-        _native.call("tf_attn_shared", q.data_ptr(), q.stride(0), *pool, items, plan.n_items,
-                     plan.n_shared, tokens, plan.row_groups, plan.slot_rows, pieces,
-                     plan.n_pieces, units, plan.n_stream, n_q, n_kv, head_dim, scaling, out.data_ptr(), out.stride(0), ws.data_ptr(), nbytes, *epilogue,
-                     handle)
+                         main.cuda_stream)
+        side.wait_event(fork)
+        parts(side.cuda_stream)
+        join.record(side)
+        main.wait_event(join)
     return out
