@@ -115,6 +115,12 @@ def test_prefix_lengths_per_request(gpu):
     run([500, 500, 500, 30, 700, 90], 200, first, 50, seed=5, moved=True)
 
 
+@pytest.mark.parametrize("which", ["keep", "first", "recent"])
+@pytest.mark.parametrize("longest", [300, 20000])
+def test_sizes_beyond_every_row(gpu, which, longest):
+    run([longest, 70, 0], **{"keep": 40, "first": 3, "recent": 5, which: 2 ** 63 - 1})
+
+
 def test_strided_tables_and_other_columns_stay(gpu):
     run([500, 300], 128, 4, 16, pad=5, width=900, seed=6)
 

@@ -18,6 +18,8 @@
 // and no chunk is written before the ones in front of it.
 #include <math.h>
 
+#include <algorithm>
+
 #include "tf_common.h"
 #include "tf_internal.h"
 
@@ -573,9 +575,9 @@ extern "C" int32_t tf_evict_tokens(
   a.out_rows = out_rows;
   a.seq_lens = seq_lens;
   a.first = first;
-  a.first_n = first_n;
-  a.recent = recent;
-  a.keep = keep;
+  a.first_n = std::min(first_n, max_len);   // (no row has more, and no sum of theirs overflows)
+  a.recent = std::min(recent, max_len);
+  a.keep = std::min(keep, max_len);
   a.max_len = max_len;
   a.lens_out = new_lens;
   a.freed = freed;

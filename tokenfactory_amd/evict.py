@@ -32,10 +32,10 @@ def evict_tokens(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Shortens the table rows of requests longer than ``max(keep, first + recent)`` tokens
     to that many: the first ``first`` stay (attention sinks, a shared prefix: an int, or
-    int64 ``[B]`` on the device, a negative one counting as 0), the last ``recent`` stay, and of those between the ones
-    with the largest score (equal scores: the earlier; NaN below every number), all in
-    their order, their scores beside them.  The entries behind, up to the old length,
-    become -1 with score 0.
+    int64 ``[B]`` on the device, a negative one counting as 0), the last ``recent`` stay,
+    and of those between the ones with the largest score (equal scores: the earlier; NaN
+    below every number), all in their order, their scores beside them.  The entries
+    behind, up to the old length, become -1 with score 0.
 
     ``req_to_token`` int64 and ``scores`` fp32 ``[max_reqs, max_context_len]`` change in
     place; ``seq_lens`` (int64 ``[B]``, at most ``max_seq_len``) is read.  ``out_rows``
@@ -72,7 +72,9 @@ def evict_tokens(
     if not 0 <= max_seq_len <= table.shape[1]:
         raise ValueError(f"{fn}: max_seq_len {max_seq_len} exceeds req_to_token width "
                          f"{table.shape[1]}")
-    width = max(0, max_seq_len - keep)
+    # (no row has more, and sums of theirs stay in 64 bits)
+    keep, recent, first_n = (min(n, max_seq_len) for n in (keep, recent, first_n))
+    width = max_seq_len - keep
     with _native.launching(device, stream):
         lens = torch.empty_strided((bsz,), (1,), dtype=torch.int64, device=device)
         freed = torch.empty_strided((bsz, width), (width, 1), dtype=torch.int64, device=device)
