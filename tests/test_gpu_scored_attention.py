@@ -247,3 +247,30 @@ def test_slots_behind_2_gib(gpu):
     wl.k_pool, wl.v_pool = small
     assert_attention(got, want, spread, wl, "far slots")
     assert_scores(scores, before, wl, weights, True, what="far slots")
+
+
+def test_refusals(gpu):
+    """Raised on the host before anything is launched: the scores stay."""
+    wl = case([9, 30, 4], [1, 1, 1], seed=30)
+    scores = new_scores(wl, 0.0)
+
+    def refused(match, error=ValueError, **kw):
+        with pytest.raises(error, match=match):
+            call(wl, scores, **kw)
+
+    refused("window", window=0)
+    refused("out must match", out=torch.empty_like(wl.q)[:2])
+    refused("gate", gate=torch.empty_like(wl.q, dtype=torch.float32))
+    refused("out_amax", out_amax=torch.zeros(1, device=gpu))
+    wl.batch.req_pool_indices_list = [1, 2, 1]
+    refused("twice")
+    wl.batch.req_pool_indices_list = None
+    wl.batch.extend_lens, wl.batch.max_extend_len = [1, 2], 1
+    refused("decode batch of 3")
+    wl.batch.extend_lens, wl.batch.max_extend_len = [1, 1, 1], 2
+    wl.batch.extend_lens_tensor = wl.batch.extend_lens_tensor.to(torch.int32)
+    refused("extend_lens_tensor")
+    assert not scores.any()
+    wl = case([9, 30], [1, 1], seed=31, fp8=True)
+    with pytest.raises(ValueError, match="k_scale"):
+        scored_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, new_scores(wl))

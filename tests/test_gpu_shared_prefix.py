@@ -463,3 +463,25 @@ def test_negative_scaling(gpu):
     got = call(wl, SharedPrefixes(members))
     want, spread, _ = attention64(wl)
     assert_attention(got, want, spread, wl, "negative scaling")
+
+
+def test_refusals(gpu):
+    """Raised on the host before anything is launched."""
+    wl, members = shared_case([200], [5, 9, 1], [0] * 3, seed=50, fp8=True)
+    shared = SharedPrefixes(members)
+
+    def refused(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            call(wl, shared, **kw)
+
+    refused("out must match", out=torch.empty_like(wl.q)[:2])
+    refused("gate", gate=torch.empty_like(wl.q, dtype=torch.float32))
+    refused("out_amax", out_amax=torch.zeros(1, device=gpu))
+    with pytest.raises(ValueError, match="k_scale"):
+        shared_prefix_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, shared)
+    with pytest.raises(ValueError, match="batch of 3"):
+        call(wl, SharedPrefixes([([0, 3], 10)]))
+    with pytest.raises(ValueError, match="width"):
+        call(wl, SharedPrefixes([([0, 1], 100000)]))
+    wl.batch.extend_lens = [1, 1, 2]
+    refused("extend_lens")

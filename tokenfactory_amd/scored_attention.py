@@ -68,7 +68,8 @@ def scored_attention(
 
     A captured call follows ``seq_lens`` (and ``extend_lens_tensor``) in place up to
     ``req_to_token``'s width; an eager one covers ``batch.max_seq_len`` keys, as the
-    batch promises."""
+    batch promises.  A batch of one has ``batch.max_seq_len`` keys in both, as in
+    ``slot_based_attention``."""
     fn = "scored_attention"
     _native.refuse_gradients(fn, q, layer_k_buffer, layer_v_buffer, gate, scores)
     _check_inputs(q, layer_k_buffer, layer_v_buffer, batch)
@@ -88,6 +89,9 @@ def scored_attention(
                         or ext_t.numel() != bsz or not ext_t.is_contiguous()):
         raise ValueError(f"{fn}: batch.extend_lens_tensor must be contiguous int64 [batch_size] "
                          "on q's device")
+    if n_tok and longest == 1 and (n_tok != bsz or len(batch.extend_lens) != bsz):
+        raise ValueError(f"{fn}: {n_tok} tokens, {len(batch.extend_lens)} extend_lens of a "
+                         f"decode batch of {bsz}")
     with _native.launching(device, stream):
         k_scale, v_scale = _pool_scales(q, kv_dtype, k_scale, v_scale)
         if q.stride(2) != 1 or q.stride(1) != head_dim:
@@ -100,9 +104,6 @@ def scored_attention(
         table = (rtt.data_ptr(), rtt.shape[0], rtt.stride(0), rtt.shape[1],
                  batch.req_pool_indices.data_ptr(), batch.seq_lens.data_ptr(), override)
         if n_tok and longest == 1 and _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span):
-            if n_tok != bsz or len(batch.extend_lens) != bsz:
-                raise ValueError(f"{fn}: {n_tok} tokens, {len(batch.extend_lens)} extend_lens of "
-                                 f"a decode batch of {bsz}")
             out = _output(q, out)
             ws, nbytes = _scratch("tf_attn_scored_workspace_bytes", device, bsz, span, n_q, n_kv,
                                   head_dim, kv_dtype)
