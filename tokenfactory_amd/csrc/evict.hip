@@ -6,16 +6,16 @@
 // One workgroup per request, or for rows that may be longer than 16384 five launches of
 // one per 8192 entries: the same digits counted per run, each launch deriving a digit from
 // the counts of the one before (kernel boundaries order them: no atomics, nothing to
-// clear), then the moves into scratch and back.  Bound by latency: 8 rows of 131072 take
-// 183 us by a workgroup each, whose CU moves 25 GB/s, and 44 in launches; of 24576 42 and
-// 34; of 16384 27 and 33 (longer ones are no longer read once for all three digits).
+// clear), then the moves into scratch and back.  Bound by latency: 3 rows of
+// up to 1500 entries 6.2 us on the device, 64 of up to 8192 13.6 (9.4 MB), a call on 8 rows
+// of 16384 23.6 us, of 24576 29.5, of 131072 39.7 (183 by a workgroup each, whose CU moves
+// 25 GB/s).
 //
 // The room-th largest score is found digit by digit (radix selection over the scores'
 // order-preserving integers, 11 bits at a time, counted in LDS), the entries above it
-// stay and of the equal ones the first.  Then one ordered pass moves slots and scores:
-// positions come from a scan over the workgroup and a running count.  In place: an entry
-// moves to its own or an earlier position, a chunk is read before any of it is written,
-// and no chunk is written before the ones in front of it.
+// stay and of the equal ones the first.  Every wave takes consecutive entries, 64 at a
+// time, so that an entry's place is what the waves before it keep (one sum per wave
+// through LDS), what its own wave kept so far, and a count over the lanes below.
 #include <math.h>
 
 #include <algorithm>
@@ -28,11 +28,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kPer = 4;                        // entries of a thread in a chunk
-constexpr int kChunk = kThreads * kPer;
 constexpr int kDigitBits = 11;
 constexpr int kBins = 1 << kDigitBits;
-constexpr int kAhead = 16;                     // scores of a thread in flight
 
 struct EvictArgs {
   int64_t* table;
@@ -81,12 +78,19 @@ __device__ __forceinline__ Range range_of(const EvictArgs& a, int b) {
   return r;
 }
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {   // inclusive
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int o = __shfl_up(v, off, kWave);
-    if (lane >= off) v += o;
-  }
+// Inclusive sums over the lanes: within rows of 16, then over the rows, by lane moves of
+// the vector unit (a shuffle goes through LDS: the three digits' scans took 1.5 us so).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += moved<0x111, 0xf>(v);   // from 1, 2, 4 and 8 lanes below in the row
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);   // the row's last lane to the next row (1 and 3)
+  v += moved<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
   return v;
 }
 
@@ -96,8 +100,9 @@ struct WaveSums {
   int before, all;
 };
 __device__ __forceinline__ WaveSums sum_waves(const int32_t* wsum, int lane, int w) {
-  const int v = wave_scan(lane < kWaves ? wsum[lane] : 0, lane);
-  return WaveSums{w ? __shfl(v, w - 1, kWave) : 0, __shfl(v, kWaves - 1, kWave)};
+  const int v = wave_scan(lane < kWaves ? wsum[lane] : 0);
+  return WaveSums{w ? __builtin_amdgcn_readlane(v, w - 1) : 0,
+                  __builtin_amdgcn_readlane(v, kWaves - 1)};
 }
 
 // One count for the lane's bin; a wave whose (active) lanes share one, as equal scores do,
@@ -124,7 +129,7 @@ __device__ __forceinline__ void find_digit(const int32_t* bins, int ties, int32_
                                            uint32_t* found, int lane, int w) {
   const int i0 = kBins - 1 - 2 * (int)threadIdx.x;
   const int c0 = bins[i0], c1 = bins[i0 - 1];
-  const int incl = wave_scan(c0 + c1, lane);
+  const int incl = wave_scan(c0 + c1);
   if (lane == kWave - 1) wsum[w] = incl;
   lds_barrier();
   const int before = sum_waves(wsum, lane, w).before + incl - c0 - c1;
@@ -142,54 +147,42 @@ __device__ __forceinline__ void find_digit(const int32_t* bins, int ties, int32_
 __device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __device__ __forceinline__ uint32_t digit_mask(int pass) { return pass == 2 ? 1023u : 2047u; }
 
-// Places of PER entries a thread, entry j being number j * kThreads + thread: how many
-// before it stay for certain (sure), and how many are ties, from counts per wave in LDS.
-template <int PER>
-struct Places {
-  int32_t counts[2][PER * kWaves];
+// The entries that stay (`sure`, a bit per entry of the lane) and the ties of a wave so far.
+struct Kept {
+  int gt, eq;
 };
+// How many entries of the wave stay for certain and how many are ties.
 template <int PER>
-__device__ __forceinline__ void places(Places<PER>& lds, int sure, int tie, int lane, int w,
-                                       int (&gt)[PER], int (&eq)[PER], int& all_gt, int& all_eq) {
-  static_assert(PER * kWaves == kWave || PER * kWaves == 2 * kWave, "one or two counts a lane");
-  constexpr int kEach = PER * kWaves / kWave;
-  int own[2][PER];   // before the entry within its wave
+__device__ __forceinline__ Kept wave_kept(int sure, int tie) {
+  Kept k{0, 0};
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const uint64_t below = (1ull << lane) - 1;
-    const uint64_t ms = __ballot(sure >> j & 1), mt = __ballot(tie >> j & 1);
-    own[0][j] = __popcll(ms & below);
-    own[1][j] = __popcll(mt & below);
-    if (lane == 0) {
-      lds.counts[0][j * kWaves + w] = __popcll(ms);
-      lds.counts[1][j * kWaves + w] = __popcll(mt);
-    }
+    k.gt += __popcll(__ballot(sure >> j & 1));
+    k.eq += __popcll(__ballot(tie >> j & 1));
   }
-  lds_barrier();
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    int n[kEach], sum = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) sum += n[e] = lds.counts[c][lane * kEach + e];
-    const int incl = wave_scan(sum, lane);
-    (c ? all_eq : all_gt) = __shfl(incl, kWave - 1, kWave);
-    int before[kEach];   // the lane's counts
-    before[0] = incl - sum;
-    if (kEach == 2) before[kEach - 1] = incl - n[kEach - 1];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int at = j * kWaves + w;
-      const int v = __shfl(before[0], at / kEach, kWave);
-      const int u = kEach == 2 ? __shfl(before[kEach - 1], at / kEach, kWave) : v;
-      (c ? eq : gt)[j] = own[c][j] + (at % kEach ? u : v);
-    }
-  }
+  return k;
+}
+// Where the lane's entry j goes: how many entries before it stay, of which `before` those of
+// the waves (and runs) in front, which is moved past the wave's entries j; and whether it
+// stays itself.
+__device__ __forceinline__ bool place(Kept& before, int sure, int tie, int j, int ties, int& at) {
+  const uint64_t ms = __ballot(sure >> j & 1), mt = __ballot(tie >> j & 1);
+  const int gt = before.gt + __builtin_amdgcn_mbcnt_hi((uint32_t)(ms >> 32),
+                                 __builtin_amdgcn_mbcnt_lo((uint32_t)ms, 0));
+  const int eq = before.eq + __builtin_amdgcn_mbcnt_hi((uint32_t)(mt >> 32),
+                                 __builtin_amdgcn_mbcnt_lo((uint32_t)mt, 0));
+  before.gt += __popcll(ms);
+  before.eq += __popcll(mt);
+  at = gt + min(eq, ties);
+  return (sure >> j & 1) || ((tie >> j & 1) && eq < ties);
 }
 
+// PER: entries of a thread.
+template <int PER>
 __global__ void __launch_bounds__(kThreads) evict_kernel(EvictArgs a) {
   __shared__ int32_t bins[kBins];
   __shared__ int32_t wsum[kWaves];
-  __shared__ Places<kPer> order;
+  __shared__ int32_t kept[2][kWaves];
   __shared__ uint32_t found[2];   // the digit of the room-th largest, and how many it needs
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = wave_id();
   const Range rg = range_of(a, b);
@@ -202,40 +195,38 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(EvictArgs a) {
   int64_t* freed = a.freed + (int64_t)b * a.freed_width;
   if (tid == 0) a.lens_out[b] = rg.left;
 
+  const bool nothing = rg.left == rg.n;
+  if (nothing && to == row) {
+    for (int64_t i = tid; i < a.freed_width; i += kThreads) freed[i] = -1;
+    return;
+  }
+  // The row, read once: entry j of a lane is number i0 + 64 j.  Every load has returned
+  // before the barrier that lets anything be written.
+  const int i0 = w * kWave * PER + lane;
+  float v[PER];
+  int64_t s[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) v[j] = i0 + j * kWave < rg.n ? scores[i0 + j * kWave] : 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) s[j] = i0 + j * kWave < rg.n ? slots[i0 + j * kWave] : 0;
+
   // ---- the room-th largest: `cut`, of which `ties` stay
   uint32_t cut = 0;
   int ties = rg.room;
-  const int mid = rg.end - rg.first;
-  const bool select = rg.room > 0 && rg.room < mid;
+  const bool select = rg.room > 0 && rg.room < rg.end - rg.first;
   if (select) {
-    // Scores kAhead at a time: those of a short range are read once and stay.
-    uint32_t key[kAhead];
-    auto load = [&](int base) {
-      float v[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int i = base + j * kThreads + tid;
-        v[j] = i < mid ? scores[rg.first + i] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) key[j] = order_of(v[j]);
-    };
-    constexpr int kRun = kAhead * kThreads;
-    if (mid <= kRun) load(0);
     uint32_t mask = 0;
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = digit_shift(pass);
       const uint32_t digit = digit_mask(pass);
       for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
       lds_barrier();
-      for (int base = 0; base < mid; base += kRun) {
-        if (mid > kRun) load(base);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          if (base + j * kThreads >= mid) break;
-          if (base + j * kThreads + tid < mid && (key[j] & mask) == cut)
-            count(bins, (key[j] >> shift) & digit);
-        }
+      for (int j = 0; j < PER; ++j) {
+        const int i = i0 + j * kWave;
+        if (PER == 16) asm volatile("" : "+v"(v[j]));   // (k is made again: 128 registers)
+        const uint32_t k = order_of(v[j]);
+        if (i >= rg.first && i < rg.end && (k & mask) == cut) count(bins, (k >> shift) & digit);
       }
       lds_barrier();
       find_digit(bins, ties, wsum, found, lane, w);
@@ -245,62 +236,37 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(EvictArgs a) {
     }
   }
 
-  // ---- the ordered pass, a chunk's entries read while the one before it moves
-  const bool nothing = rg.left == rg.n;
-  int gt0 = 0, eq0 = 0;   // entries before the chunk that stay for certain / that are ties
-  const int start = nothing && to == row ? rg.n : 0;
-  int64_t s[kPer];
-  float v[kPer];
-  auto read = [&](int c0) {
+  // ---- what stays moves together, the rest goes out
+  int sure = 0, tie = 0;   // bit per entry
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = c0 + j * kThreads + tid;
-      if (i < rg.n) {
-        s[j] = slots[i];
-        v[j] = scores[i];
-      }
+  for (int j = 0; j < PER; ++j) {
+    const int i = i0 + j * kWave;
+    const uint32_t k = order_of(v[j]);
+    const bool outside = nothing || i < rg.first || i >= rg.end;
+    sure |= (i < rg.n && (outside || (select && k > cut))) << j;
+    tie |= (i < rg.n && !outside && select && k == cut) << j;
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) asm volatile("" ::"v"(s[j]));   // (see above)
+  const Kept mine = wave_kept<PER>(sure, tie);
+  if (lane == 0) {
+    kept[0][w] = mine.gt;
+    kept[1][w] = mine.eq;
+  }
+  lds_barrier();
+  Kept before{sum_waves(kept[0], lane, w).before, sum_waves(kept[1], lane, w).before};
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = i0 + j * kWave;
+    int at;
+    const bool stays = place(before, sure, tie, j, ties, at);
+    if (i >= rg.n) continue;
+    if (stays) {
+      new_slots[at] = s[j];
+      new_scores[at] = v[j];
+    } else if (i - at < a.freed_width) {
+      freed[i - at] = s[j];
     }
-  };
-  if (start < rg.n) read(start);
-  for (int c0 = start; c0 < rg.n; c0 += kChunk) {
-    int64_t my_s[kPer];
-    float my_v[kPer];
-    int sure = 0, tie = 0;   // bit per entry
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = c0 + j * kThreads + tid;
-      my_s[j] = s[j];
-      my_v[j] = v[j];
-      if (i >= rg.n) continue;
-      if (nothing || i < rg.first || i >= rg.end) {
-        sure |= 1 << j;
-      } else if (select) {
-        const uint32_t k = order_of(my_v[j]);
-        sure |= (k > cut) << j;
-        tie |= (k == cut) << j;
-      }
-    }
-    // (the chunk's loads have returned before the barrier that lets others write there)
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) asm volatile("" ::"v"(my_s[j]), "v"(my_v[j]));
-    if (c0 + kChunk < rg.n) read(c0 + kChunk);
-    int gt[kPer], eq[kPer], all_gt, all_eq;
-    places<kPer>(order, sure, tie, lane, w, gt, eq, all_gt, all_eq);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = c0 + j * kThreads + tid;
-      if (i >= rg.n) continue;
-      const int at = gt0 + gt[j] + min(eq0 + eq[j], ties);
-      if ((sure >> j & 1) || ((tie >> j & 1) && eq0 + eq[j] < ties)) {
-        new_slots[at] = my_s[j];
-        new_scores[at] = my_v[j];
-      } else if (i - at < a.freed_width) {
-        freed[i - at] = my_s[j];
-      }
-    }
-    gt0 += all_gt;
-    eq0 += all_eq;
-    lds_barrier();
   }
   // ---- behind what stays: empty entries without weight
   for (int i = rg.left + tid; i < rg.n; i += kThreads) {
@@ -320,9 +286,11 @@ struct Found {
 };
 
 // The digits of passes 0 .. passes - 1: those before the last from the launch before, the
-// last from the runs' counts, by every workgroup for itself.
+// last from the runs' counts, by every workgroup for itself.  front: of the last pass, how
+// many entries of the runs before `run` have digits 2 thread and 2 thread + 1.
 __device__ Found find_cut(const EvictArgs& a, const Range& rg, int b, int passes, int32_t* bins,
-                          int32_t* wsum, uint32_t* found) {
+                          int32_t* wsum, uint32_t* found, int run, int2& front) {
+  front = int2{0, 0};
   if (passes == 0) return Found{0u, rg.room};
   const int lane = threadIdx.x & 63, w = wave_id();
   const int pass = passes - 1;
@@ -340,6 +308,10 @@ __device__ Found find_cut(const EvictArgs& a, const Range& rg, int b, int passes
     const int2 c = *reinterpret_cast<const int2*>(counts + (int64_t)r * kBins + i);
     c0 += c.x;
     c1 += c.y;
+    if (r < run) {
+      front.x += c.x;
+      front.y += c.y;
+    }
   }
   bins[i] = c0;
   bins[i + 1] = c1;
@@ -370,7 +342,8 @@ __global__ void __launch_bounds__(kThreads) evict_count_kernel(EvictArgs a) {
     const int i = j * kThreads + tid;
     v[j] = from + i < mid ? scores[i] : 0.f;
   }
-  const Found f = find_cut(a, rg, b, PASS, bins, wsum, found);
+  int2 front;
+  const Found f = find_cut(a, rg, b, PASS, bins, wsum, found, 0, front);
   constexpr uint32_t mask = PASS == 0 ? 0u : PASS == 1 ? 0xffe00000u : 0xfffffc00u;
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
   if (tid < kWaves) wsum[tid] = 0;
@@ -384,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) evict_count_kernel(EvictArgs a) {
     if (PASS == 2) above += (k & mask) > f.cut;
   }
   if (PASS == 2) {
-    above = wave_scan(above, tid & 63);
+    above = wave_scan(above);
     if ((tid & 63) == kWave - 1) wsum[wave_id()] = above;
   }
   lds_barrier();
@@ -402,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) evict_count_kernel(EvictArgs a) {
 __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
   __shared__ int32_t bins[kBins];
   __shared__ int32_t wsum[2][kWaves];
-  __shared__ Places<kRunPer> order;
+  __shared__ int32_t kept[2][kWaves];
   __shared__ uint32_t found[2];
   const int b = blockIdx.y, run = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = wave_id();
   const Range rg = range_of(a, b);
@@ -430,28 +403,24 @@ __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
   const bool select = rg.room > 0 && rg.room < mid, all = rg.room >= mid;
   int64_t s[kRunPer];
   float v[kRunPer];
+  const int i0 = from + w * kWave * kRunPer + lane;   // entry j of the lane is i0 + 64 j
 #pragma unroll
   for (int j = 0; j < kRunPer; ++j) {
-    const int i = from + j * kThreads + tid;
-    if (i >= mid) continue;
-    s[j] = slots[rg.first + i];
-    v[j] = scores[rg.first + i];
+    const int i = i0 + j * kWave;
+    s[j] = i < mid ? slots[rg.first + i] : 0;
+    v[j] = i < mid ? scores[rg.first + i] : 0.f;
   }
   Found f{0u, 0};
   int gt0 = 0, eq0 = 0;   // of the runs before: above the cut, equal to it
   if (select) {
-    f = find_cut(a, rg, b, 3, bins, wsum[0], found);
-    const int32_t* counts = a.counts + ((int64_t)b * 3 + 2) * a.n_runs * kBins;
-    const uint32_t digit = f.cut & digit_mask(2);
-    int g = 0, e = 0;
-#pragma unroll 8
-    for (int r = 0; r < run; ++r) {
-      const int c = counts[(int64_t)r * kBins + tid];   // (the pass has kThreads digits)
-      g += (uint32_t)tid > digit ? c : 0;
-      e += (uint32_t)tid == digit ? c : 0;
-    }
+    int g = 0;   // (counted above by the launch before)
     for (int r = tid; r < run; r += kThreads) g += a.above[(int64_t)b * a.n_runs + r];
-    const int gi = wave_scan(g, lane), ei = wave_scan(e, lane);
+    int2 front;
+    f = find_cut(a, rg, b, 3, bins, wsum[0], found, run, front);
+    const int digit = (int)(f.cut & digit_mask(2));
+    g += (2 * tid > digit ? front.x : 0) + (2 * tid + 1 > digit ? front.y : 0);
+    const int e = 2 * tid == digit ? front.x : 2 * tid + 1 == digit ? front.y : 0;
+    const int gi = wave_scan(g), ei = wave_scan(e);
     if (lane == kWave - 1) {
       wsum[0][w] = gi;
       wsum[1][w] = ei;
@@ -466,19 +435,25 @@ __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
   int sure = 0, tie = 0;
 #pragma unroll
   for (int j = 0; j < kRunPer; ++j) {
-    if (from + j * kThreads + tid >= mid) continue;
     const uint32_t k = order_of(v[j]);
-    sure |= (all || (select && k > f.cut)) << j;
-    tie |= (select && k == f.cut) << j;
+    const bool in = i0 + j * kWave < mid;
+    sure |= (in && (all || (select && k > f.cut))) << j;
+    tie |= (in && select && k == f.cut) << j;
   }
-  int gt[kRunPer], eq[kRunPer], all_gt, all_eq;
-  places<kRunPer>(order, sure, tie, lane, w, gt, eq, all_gt, all_eq);
+  const Kept mine = wave_kept<kRunPer>(sure, tie);
+  if (lane == 0) {
+    kept[0][w] = mine.gt;
+    kept[1][w] = mine.eq;
+  }
+  lds_barrier();
+  Kept before{gt0 + sum_waves(kept[0], lane, w).before, eq0 + sum_waves(kept[1], lane, w).before};
 #pragma unroll
   for (int j = 0; j < kRunPer; ++j) {
-    const int i = from + j * kThreads + tid;
+    const int i = i0 + j * kWave;
+    int at;
+    const bool stays = place(before, sure, tie, j, f.ties, at);
     if (i >= mid) continue;
-    const int at = gt0 + gt[j] + min(eq0 + eq[j], f.ties);
-    if ((sure >> j & 1) || ((tie >> j & 1) && eq0 + eq[j] < f.ties)) {
+    if (stays) {
       new_slots[rg.first + at] = s[j];
       new_scores[rg.first + at] = v[j];
     } else if (i - at < a.freed_width) {
@@ -523,7 +498,16 @@ SplitPlan split_plan(int64_t max_len, int32_t batch) {
   return p;
 }
 // Rows that may be this long are split (see the top).
-constexpr int64_t kSplitLen = kAhead * kThreads + 1;
+constexpr int64_t kSplitLen = 16 * kThreads + 1;
+
+// With as few entries a thread as hold the row: what the kernel does not need it does not
+// fetch (its unrolled code is read once, by every CU's first wave).
+template <int PER>
+void launch_evict(const EvictArgs& a, int32_t batch, hipStream_t s) {
+  if constexpr (PER < 16)
+    if (a.max_len > PER * kThreads) return launch_evict<2 * PER>(a, batch, s);
+  hipLaunchKernelGGL(evict_kernel<PER>, dim3((unsigned)batch), dim3(kThreads), 0, s, a);
+}
 
 }  // namespace
 }  // namespace tfa
@@ -584,7 +568,7 @@ extern "C" int32_t tf_evict_tokens(
   a.freed_width = freed_width;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (need == 0) {
-    hipLaunchKernelGGL(evict_kernel, dim3((unsigned)batch_size), dim3(kThreads), 0, s, a);
+    launch_evict<2>(a, batch_size, s);
     return launch_status("tf_evict_tokens launch");
   }
   const SplitPlan p = split_plan(max_len, batch_size);
