@@ -89,17 +89,18 @@ KEYS_PER_STEP = 32   # of the extend kernel
 MIN_STEPS = 2        # of a piece: 3 requests on 300 keys 13.7 us, with 8 17.1, with 16 20.7
 
 
-def cut_units(steps: Sequence[int], cus: int) -> List[int]:
+def cut_units(steps: Sequence[int], cus: int) -> np.ndarray:
     """Pieces per unit, steps[i] steps of keys long: the shortest pieces of which there are
     no more than CUs (a piece more would be a round more), of MIN_STEPS at least."""
-    lo, hi = MIN_STEPS, max([MIN_STEPS, *steps])
+    steps = np.asarray(steps, dtype=np.int64)
+    lo, hi = MIN_STEPS, max(MIN_STEPS, int(steps.max()))
     while lo < hi:
         mid = (lo + hi) // 2
-        if sum(-(-s // mid) for s in steps) <= cus:
+        if (-(-steps // mid)).sum() <= cus:
             hi = mid
         else:
             lo = mid + 1
-    return [max(1, -(-s // lo)) for s in steps]
+    return np.maximum(1, -(-steps // lo))
 
 
 # Times in us that the split of a step is estimated with, by (narrow tiles, fp8 pool): of a
@@ -109,19 +110,19 @@ _STEP_US = {(False, False): (3.0, 0.40, 0.45, 1.5), (False, True): (1.7, 0.21, 0
             (True, False): (2.0, 0.18, 0.3, 1.5)}
 
 
-def _stream_share(steps: Sequence[Tuple[int, int]], own: Sequence[Tuple[int, int]], n_kv: int,
-                  narrow: bool, fp8: bool, cus: int) -> int:
+def _stream_share(steps: np.ndarray, rows: np.ndarray, own_units: np.ndarray,
+                  own_keys: np.ndarray, n_kv: int, narrow: bool, fp8: bool, cus: int) -> int:
     """Workgroups, one per CU, that stream the requests' own parts beside the pieces of the
-    shared ones: where both are estimated to end together.  steps: (steps, rows) of each
-    MFMA unit; own: (units of 16 rows, keys of the own part) per request.  Measured with 64, 112, 160 and 192 of 256: 64
-    requests on 8192 shared keys 75, 58, 52 and 63 us (two launches 71), branches of 4
-    groups 74, 61, 54 and 51 (57), 96 on 2000 of 128 dims 84, 62, 51 and 44 (62), 256 on
-    32768 of an fp8 pool 294, 318, 429 and 821 (330)."""
+    shared ones: where both are estimated to end together.  steps, rows: of each MFMA unit;
+    own_units (of 16 rows), own_keys: of each request's own part.  Measured with 64, 112,
+    160 and 192 of 256: 64 requests on 8192 shared keys 75, 58, 52 and 63 us (two launches
+    71), branches of 4 groups 74, 61, 54 and 51 (57), 96 on 2000 of 128 dims 84, 62, 51 and
+    44 (62), 256 on 32768 of an fp8 pool 294, 318, 429 and 821 (330)."""
     unit, tile, step, full = _STEP_US[narrow, fp8]
-    streams = n_kv * sum(u * (unit + tile * n / 16) for u, n in own)
-    total, longest = sum(k for k, _ in steps), max(k for k, _ in steps)
-    per_step = sum(k * (step + (full - step) * min(r, EXTEND_TILE_ROWS) / EXTEND_TILE_ROWS)
-                   for k, r in steps) / total
+    streams = n_kv * float((own_units * (unit + tile * own_keys / 16)).sum())
+    total, longest = int(steps.sum()), int(steps.max())
+    filled = np.minimum(rows, EXTEND_TILE_ROWS) / EXTEND_TILE_ROWS
+    per_step = float((steps * (step + (full - step) * filled)).sum()) / total
 
     def end(n):   # (pieces are whole: the longest unit is cut into as many as it can)
         parts = max(1, (cus - n) * longest // total)
@@ -131,15 +132,25 @@ def _stream_share(steps: Sequence[Tuple[int, int]], own: Sequence[Tuple[int, int
     return min(range(max(1, cus // 16), cus * 7 // 8 + 1, max(1, cus // 32)), key=end)
 
 
-def _streams_all(shared: Sequence[Tuple[int, int]], own_keys: int, n_kv: int, cus: int) -> bool:
-    """Whether the shared parts ((rows, keys) each) are streamed as the requests' own are, in
+def _streams_all(rows: np.ndarray, keys: np.ndarray, own_keys: int, n_kv: int, cus: int) -> bool:
+    """Whether the shared parts (rows and keys of each) are streamed as the requests' own are, in
     units of 16 rows, and not by MFMA tiles: where a unit holds a part's rows, so that its
     keys are still read once, and either the parts are many (32 groups of 2 on 500 keys 37
     us, 50 by tiles, 500 of 2 on 2000 964 and 1046) or own keys are nearly all (2 requests
     on 100 keys beside 62 of 4k: 119 and 128).  One group of 4 on 8000 keys, 16 rows of
     128 dims: 39 us streamed, whose merge joins hundreds of waves' partials, 22 by tiles."""
-    return max(r for r, _ in shared) <= 16 and (
-        4 * n_kv * len(shared) >= cus or 8 * sum(n for _, n in shared) <= own_keys)
+    return rows.max() <= 16 and (4 * n_kv * len(rows) >= cus or 8 * keys.sum() <= own_keys)
+
+
+def _ragged(values: np.ndarray, counts: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
+    """values[i] counts[i] times, and each one's number among those of its i."""
+    ends = np.cumsum(counts)
+    total = int(ends[-1]) if len(ends) else 0
+    return np.repeat(values, counts), np.arange(total) - np.repeat(ends - counts, counts)
+
+
+def _items(*columns) -> np.ndarray:
+    return np.stack(np.broadcast_arrays(*columns), axis=1)
 
 
 class _Plan:
@@ -152,85 +163,86 @@ class _Plan:
         group = n_q // n_kv
         fp8 = kv_dtype == _native.TF_DTYPE_FP8_E4M3
         self.device, self.n_q, self.n_kv = device, n_q, n_kv
-        long_ = {b for b, e in enumerate(ext_lens)
-                 if head_dim == 256 and e * group > SHORT_ROWS}
-        starts = [0, *np.cumsum(ext_lens).tolist()]
-        groups = [([b for b in m if b not in long_], n) for m, n in groups]
+        ext = np.asarray(ext_lens, dtype=np.int64).reshape(-1)
+        starts = np.cumsum(ext) - ext
+        long_ = (ext * group > SHORT_ROWS) & (head_dim == 256)
+        own = np.flatnonzero(~long_)   # requests with parts
+        groups = [([b for b in m if not long_[b]], n) for m, n in groups]
         groups = [(m, n) for m, n in groups if len(m) > 1]
         self.shares = bool(groups)
-        shared_rows = [sum(ext_lens[b] for b in m) * group for m, _ in groups]
-        rows = [e * group for b, e in enumerate(ext_lens) if b not in long_]
-        prefix_of = {b: n for m, n in groups for b in m}
+        members = np.asarray([b for m, _ in groups for b in m], dtype=np.int64)
+        first = np.asarray([m[0] for m, _ in groups], dtype=np.int64)
+        sizes = np.asarray([len(m) for m, _ in groups], dtype=np.int64)
+        lengths = np.asarray([n for _, n in groups], dtype=np.int64)
+        group_of = np.repeat(np.arange(len(groups)), sizes)   # of members
+        n_toks = np.bincount(group_of, weights=ext[members],
+                             minlength=len(groups)).astype(np.int64)
+        shared_rows, rows = n_toks * group, ext[own] * group
+        prefix = np.zeros(len(ext), dtype=np.int64)
+        prefix[members] = lengths[group_of]
         # (own parts are taken to be half full: the host knows the longest context alone)
-        own_keys = {b: max(0, max_len - prefix_of.get(b, 0)) // 2
-                    for b in range(len(ext_lens)) if b not in long_}
+        own_keys = np.maximum(0, max_len - prefix[own]) // 2
         mfma = self.shares and (head_dim == 256 or (head_dim <= 128 and not fp8)) \
-            and not _streams_all([(r, n) for r, (_, n) in zip(shared_rows, groups)],
-                                 sum(own_keys.values()), n_kv, cus)
-        if not mfma:
-            rows += shared_rows
+            and not _streams_all(shared_rows, lengths, int(own_keys.sum()), n_kv, cus)
         # (Units of 16 rows stream beside the pieces, which outweighs that up to 64 rows read
         # their keys four times: 4 groups of 8 of 6 tokens on 4000 keys 58 us, 82 in units of
         # 32; 12 of 10 on 1000 35 and 51; with own parts of up to 2000 keys, 4 groups of 8
         # of 10, 149 and 132.)
-        self.row_groups = 2 if max(rows, default=1) > (64 if mfma else 16) else 1
+        most = int(max([1, *rows.tolist(), *([] if mfma else shared_rows.tolist())]))
+        self.row_groups = 2 if most > (64 if mfma else 16) else 1
         unit = 16 * self.row_groups
-        self.slot_rows = min(unit, max(rows, default=1))
+        self.slot_rows = min(unit, most)
 
-        items, tokens, pieces, units = [], [], [], []
-        front = {}   # request -> (its shared part, its first token there, keys)
+        # Tokens: the groups', then the requests' own.
+        reqs = np.concatenate([members, own])
+        b, t = _ragged(reqs, ext[reqs])
+        tokens = np.stack([starts[b] + t, b, ext[b] - 1 - t, np.zeros_like(b)], axis=1)
+        tok0 = np.cumsum(ext[reqs]) - ext[reqs]
+        group_tok0 = tok0[np.cumsum(sizes) - sizes] if len(groups) else lengths
+        part = np.full(len(ext), -1, dtype=np.int64)      # a request's shared part
+        part_tok = np.zeros(len(ext), dtype=np.int64)     # its first token among that one's
+        part_tok[members] = tok0[:len(members)] - group_tok0[group_of]
 
-        def add(b, tok0, n, k0, k1, pfx=-1, pfx_tok=0):
-            for row0 in range(0, n * group, unit):
-                items.append((b, tok0, n, row0, k0, k1, pfx, pfx_tok))
-
-        def add_tokens(b):
-            at = len(tokens)
-            tokens.extend((starts[b] + t, b, ext_lens[b] - 1 - t, 0) for t in range(ext_lens[b]))
-            return at
-
-        n_blocks = [-(-r // EXTEND_TILE_ROWS) for r in shared_rows]
-        self.n_stream, cuts = 0, []
+        self.n_stream = self.n_shared = self.n_pieces = 0
+        items, pieces, units = [], [], []
         if mfma:
-            steps = [(-(-n // KEYS_PER_STEP), r - EXTEND_TILE_ROWS * i)
-                     for (_, n), r, k in zip(groups, shared_rows, n_blocks)
-                     for i in range(k) for _ in range(n_kv)]
+            # Units: 256 rows of a group for a kv head each; pieces of their keys.
+            blocks = -(-shared_rows // EXTEND_TILE_ROWS)
+            g, hk = _ragged(np.arange(len(groups)), blocks * n_kv)
+            row0, hk = EXTEND_TILE_ROWS * (hk // n_kv), hk % n_kv
+            steps = -(-lengths[g] // KEYS_PER_STEP)
             if self.row_groups == 1:
-                self.n_stream = _stream_share(
-                    steps, [(-(-ext_lens[b] * group // 16), n) for b, n in own_keys.items()],
-                    n_kv, head_dim != 256, fp8, cus)
-            cuts = cut_units([k for k, _ in steps], cus - self.n_stream)
-        for (members, length), blocks in zip(groups, n_blocks):
-            tok0 = len(tokens)
-            for b in members:
-                front[b] = (len(units) if mfma else len(items), add_tokens(b) - tok0, length)
-            n = len(tokens) - tok0
-            if not mfma:
-                add(members[0], tok0, n, 0, length)
-                continue
-            steps = -(-length // KEYS_PER_STEP)
-            for block in range(blocks):
-                for hk in range(n_kv):
-                    parts = cuts[len(units)]
-                    units.append((len(pieces), parts))
-                    for i in range(parts):
-                        k0, k1 = (KEYS_PER_STEP * (steps * x // parts) for x in (i, i + 1))
-                        pieces.append((members[0], hk, EXTEND_TILE_ROWS * block, tok0, n, k0,
-                                       min(k1, length), len(pieces) + 1))
-        self.n_shared = len(items)
-        for b in range(len(ext_lens)):
-            if b not in long_:
-                pfx, pfx_tok, k0 = front.get(b, (-1, 0, 0))
-                add(b, add_tokens(b), ext_lens[b], k0, -1, pfx, pfx_tok)
+                self.n_stream = _stream_share(steps, shared_rows[g] - row0, -(-rows // 16),
+                                              own_keys, n_kv, head_dim != 256, fp8, cus)
+            cuts = cut_units(steps, cus - self.n_stream)
+            units = np.stack([np.cumsum(cuts) - cuts, cuts], axis=1)
+            u, i = _ragged(np.arange(len(g)), cuts)
+            g, k0, k1 = g[u], steps[u] * i // cuts[u], steps[u] * (i + 1) // cuts[u]
+            pieces = np.stack([first[g], hk[u], row0[u], group_tok0[g], n_toks[g],
+                               KEYS_PER_STEP * k0, np.minimum(KEYS_PER_STEP * k1, lengths[g]),
+                               np.arange(1, len(u) + 1)], axis=1)
+            self.n_pieces = len(pieces)
+            part[members] = ((np.cumsum(blocks) - blocks) * n_kv)[group_of]
+        elif self.shares:
+            n_units = -(-shared_rows // unit)
+            g, i = _ragged(np.arange(len(groups)), n_units)
+            items = _items(first[g], group_tok0[g], n_toks[g], unit * i, 0, lengths[g], -1, 0)
+            self.n_shared = len(items)
+            part[members] = (np.cumsum(n_units) - n_units)[group_of]
+        at, i = _ragged(np.arange(len(own)), -(-rows // unit))
+        b = own[at]
+        own_items = _items(b, tok0[len(members):][at], ext[b], unit * i, prefix[b], -1, part[b],
+                           part_tok[b])
+        items = np.concatenate([items, own_items]) if self.n_shared else own_items
         self.n_items = len(items)
-        work = np.zeros((0, 8), dtype=np.int32)
-        if long_:
+        work, self.route = [], None
+        if long_.any():
             work = plan_extend(ext_lens, n_q, n_kv, decode_to_decode_kernel=True)
-            work = work[np.isin(work[:, 0], list(long_))]
-        self.n_work, self.n_pieces = len(work), len(pieces)
-        long_lens = [ext_lens[b] for b in sorted(long_)]
-        self.route = Route(long_lens, sum(long_lens), n_q, n_kv, head_dim, kv_dtype, len(work),
-                           exact=True, max_len=max_len, cus=cus) if long_ else None
+            work = work[long_[work[:, 0]]]
+            long_lens = ext[long_].tolist()
+            self.route = Route(long_lens, sum(long_lens), n_q, n_kv, head_dim, kv_dtype, len(work),
+                               exact=True, max_len=max_len, cus=cus)
+        self.n_work = len(work)
         parts = [np.asarray(x, dtype=np.int32).reshape(-1)
                  for x in (items, work, pieces, tokens, units)]
         self._offsets = np.cumsum([0] + [4 * len(x) for x in parts])[:5].tolist()
