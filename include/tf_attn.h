@@ -312,8 +312,9 @@ int32_t tf_attn_rows(
  * tokens: device int32 [..][4] = {q row, request, tokens of the request that follow, 0}:
  * a token sees keys up to seq_lens[request] - 1 - that many.
  * slot_rows: the most rows that any item uses.
- * pieces (head_dim 256, or up to 128 with a bf16 pool; instead of shared items): device int32 [n_pieces][8] = {b, kv
- * head, row0, tok0, n_tok, k0, k1, slot + 1}: rows row0 .. row0 + 255 of the tokens over
+ * pieces (head_dim 256, or up to 128 with a bf16 pool; scale not negative; instead of
+ * shared items): device int32 [n_pieces][8] = {b, kv head, row0, tok0, n_tok, k0, k1,
+ * slot + 1}: rows row0 .. row0 + 255 of the tokens over
  * keys [k0, k1) of request b's table row; slots are 0 .. n_pieces - 1, a unit's (kv head
  * and 256 rows of a shared part) one behind the other, units = device int32 [..][2] =
  * {first slot, slots}, of a shared part's row block i and kv head h at pfx +

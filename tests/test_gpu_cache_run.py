@@ -1,6 +1,7 @@
 """The cache operators as a serving engine uses them, through the modules: a prompt is
 prefilled and scored, requests fork from it and decode on the shared prefix, their own
 tokens are scored and evicted, and decoding goes on with the shortened rows."""
+import threading
 from types import SimpleNamespace
 
 import pytest
@@ -8,7 +9,7 @@ import torch
 
 from tests.test_gpu_evict import expected
 from tokenfactory_amd import (ForwardBatch, FullAttention, FullAttnKVPool, SharedPrefixes,
-                              evict_tokens)
+                              evict_tokens, scored_attention)
 from tokenfactory_amd.req_to_token import DeviceReqToTokenTable
 
 pytestmark = pytest.mark.gpu
@@ -194,3 +195,49 @@ def test_decode_run_in_a_graph(gpu):
         want = [*run(), *state]
         for a, b in zip(got, want):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), step
+
+
+def test_threads_with_streams_of_their_own(gpu):
+    """Two threads, a stream each: one SharedPrefixes object and pool for both, scores and
+    tables of their own; every result is the one of a call alone."""
+    from tests.test_gpu_shared_prefix import call as shared_call
+    from tests.test_gpu_shared_prefix import shared_case
+
+    # a long prompt beside the parts: the second stream is the threads' common one
+    wl, members = shared_case([500, 0], [9, 1, 40, 3, 1500], [0, 0, 0, 0, 1],
+                              ext=[1, 1, 1, 1, 60], seed=31)
+    decode, _ = shared_case([500], [9, 1, 40, 3], [0] * 4, seed=32)
+    shared = SharedPrefixes(members)
+    table = decode.batch.req_to_token
+
+    def step():
+        out = shared_call(wl, shared)
+        scores = torch.zeros(table.shape, device=gpu)
+        own = table.clone()
+        scored = scored_attention(decode.q, decode.k_pool, decode.v_pool, decode.batch, scores)
+        lens, freed = evict_tokens(own, scores, decode.batch.req_pool_indices,
+                                   decode.batch.seq_lens, 300, max_seq_len=table.shape[1],
+                                   first=4, recent=16)
+        return out, scored, own, scores, lens, freed
+
+    want = step()
+    torch.cuda.synchronize()
+    failures = []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step()
+                    torch.cuda.current_stream().synchronize()
+                    failures.extend(i for i, (a, b) in enumerate(zip(got, want))
+                                    if not torch.equal(a, b))
+        except Exception as error:   # (a thread's own would be lost)
+            failures.append(error)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures

@@ -249,6 +249,28 @@ def test_slots_behind_2_gib(gpu):
     assert_scores(scores, before, wl, weights, True, what="far slots")
 
 
+@pytest.mark.parametrize("ext", [[1, 1], [7, 70]])
+@pytest.mark.parametrize("heads,d", [((24, 4), 256), ((32, 8), 128)])
+def test_slots_behind_4_gib(gpu, heads, d, ext):
+    wl = case([60, 90], ext, heads=heads, d=d, seed=17)
+    want, spread, weights = attention64(wl, 32)
+    n = wl.k_pool.shape[0]
+    slots = (1 << 32) // (2 * heads[1] * d) + 1 + n
+    k = torch.empty((slots, heads[1], d), dtype=torch.bfloat16, device=gpu)
+    v = torch.empty_like(k)
+    k[slots - n:], v[slots - n:] = wl.k_pool, wl.v_pool
+    table = wl.batch.req_to_token
+    table[table >= 0] += slots - n
+    small = (wl.k_pool, wl.v_pool)
+    wl.k_pool, wl.v_pool = k, v
+    scores = new_scores(wl)
+    before = scores.clone()
+    got = call(wl, scores)
+    wl.k_pool, wl.v_pool = small
+    assert_attention(got, want, spread, wl, f"far slots {heads} {ext}")
+    assert_scores(scores, before, wl, weights, True, window=32, what=f"far slots {heads} {ext}")
+
+
 def test_refusals(gpu):
     """Raised on the host before anything is launched: the scores stay."""
     wl = case([9, 30, 4], [1, 1, 1], seed=30)

@@ -271,6 +271,27 @@ def test_slots_behind_2_gib(gpu):
     assert_attention(got, want, spread, wl, "far slots")
 
 
+@pytest.mark.parametrize("heads,d,members", [((24, 4), 256, 3), ((32, 8), 128, 5),
+                                             ((16, 8), 128, 2), ((24, 4), 192, 3)])
+def test_slots_behind_4_gib(gpu, heads, d, members):
+    """Tiles of 256 and of 128 dims, and streamed parts, behind 2^32 bytes."""
+    wl, groups = shared_case([60], [5, 9, 1, 33, 2][:members], [0] * members, heads=heads, d=d,
+                             seed=18)
+    want, spread, _ = attention64(wl)
+    n = wl.k_pool.shape[0]
+    slots = (1 << 32) // (2 * heads[1] * d) + 1 + n
+    k = torch.empty((slots, heads[1], d), dtype=torch.bfloat16, device=gpu)
+    v = torch.empty_like(k)
+    k[slots - n:], v[slots - n:] = wl.k_pool, wl.v_pool
+    table = wl.batch.req_to_token
+    table[table >= 0] += slots - n
+    small = (wl.k_pool, wl.v_pool)
+    wl.k_pool, wl.v_pool = k, v
+    got = call(wl, SharedPrefixes(groups))
+    wl.k_pool, wl.v_pool = small
+    assert_attention(got, want, spread, wl, f"far slots {heads} D={d}")
+
+
 @pytest.mark.parametrize("d", [64, 192])
 def test_many_requests(gpu, d):
     """As many parts as one launch takes; at 192 dims, where the shared ones are parts too,

@@ -74,7 +74,9 @@ __device__ __forceinline__ Owners unit_owners(const PartArgs& a, int item, int h
 // rows from the partials, then of kWeightKeys keys at a time
 //   scores[row, k] (+)= sum over the heads of 2^(score - lse),
 // four keys a thread, a quarter of the threads for every fourth head, added in a fixed
-// order.  Bound by latency (of few keys) or by reading the scores.
+// order.  Bound by latency (of few keys) or by reading the scores: the whole launch takes
+// 6.9 us for one request of 900 keys and 20 for 64 of 1k to 8k (28 MB of scores; twice and
+// four times as many workgroups change nothing).
 constexpr int kMergeThreads = kMergeWaves * kWave;
 constexpr int kWeightHeads = kMergeThreads / 16;   // heads at a time
 constexpr int kWeightKeys = kMergeThreads;
@@ -310,8 +312,8 @@ struct PartPlan {
 };
 
 int make_part_plan(const char* fn, int32_t n_items, int32_t row_groups, int32_t slot_rows,
-                   int32_t n_pieces, int32_t n_stream, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype,
-                   PartPlan* p) {
+                   int32_t n_pieces, int32_t n_stream, int32_t num_q_heads,
+                   int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype, PartPlan* p) {
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
     return fail(TF_ERR_INVALID, "%s: num_q_heads=%d not a multiple of num_kv_heads=%d", fn,
                 num_q_heads, num_kv_heads);
@@ -469,6 +471,9 @@ extern "C" int32_t tf_attn_shared(
   if (n_shared < 0 || n_shared > n_items || (n_shared && n_pieces))
     return fail(TF_ERR_INVALID, "shared: %d of %d parts are shared, and %d pieces", n_shared,
                 n_items, n_pieces);
+  if (n_pieces && !(scale >= 0.f))
+    return fail(TF_ERR_UNSUPPORTED, "shared: scale=%g of pieces, whose rows follow their largest "
+                "product", (double)scale);
   if (n_items == n_shared) return TF_OK;
   rc = check_slot_call("shared", q, q_row_stride, k_pool, v_pool, pool_slots, kv_dtype, k_scale,
                        v_scale, req_to_token, rtt_rows, rtt_row_stride, rtt_cols,

@@ -11,7 +11,7 @@
 // parts, all of its 24 bits, smallest first, as in the streaming kernel at these head dims
 // (decode.hip): that triples the PV products, which these steps have to spare: they are
 // bound by their launch, their first loads and the partials (96 requests on 2000 keys, 32 /
-// 8 heads: 3.1 GFLOP).
+// 8 heads: 3.1 GFLOP, 38 us beside the streams of 700 own keys each at most, 113 MB).
 #include <math.h>
 
 #include "part_stream.h"
