@@ -155,7 +155,7 @@ def _items(*columns) -> np.ndarray:
 
 class _Plan:
     """The device lists of one step layout: parts of contexts and their tokens; the pieces of
-    long shared ones where MFMA tiles take them; and at head_dim 256 the extend kernel's
+    shared ones where MFMA tiles take them; and at head_dim 256 the extend kernel's
     entries of long prompts, which share nothing (MFMA-bound) and may be cut over their
     keys as in ``slot_based_attention``."""
 
