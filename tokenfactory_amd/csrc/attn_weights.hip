@@ -17,12 +17,16 @@
 // 2^(s - lse) summed per key over the rows, per kv head, in a fixed order; add_sums_kernel
 // adds the heads' sums (no atomics: results do not depend on timing) into the scores.
 //
-// Bound by the latency of a block's LDS round (two barriers per 32 rows): 4 prompts of 2048
-// new tokens on contexts of up to 10000, 24 / 4 heads of 256, window 32 (192 rows): 43 us of
-// statistics and 45 of sums, 15.7 GFLOP and 82 MB of K each, 5 for either small launch, where
-// the attention itself takes 1100.  Waves of 64 keys, half as many barriers per key, were no
-// faster (46 and 46 us: half as many workgroups).
+// Bound by latency.  4 prompts of 2048 new tokens on contexts of up to 10000, 24 / 4 heads of
+// 256, window 32 (192 rows): 43 us of statistics and 45 of sums, 11 GFLOP and 58 MB of K
+// each, 5 for either small launch, where the attention itself takes 1100; a workgroup takes
+// 1.6 us for its window, 4 to 7 for its keys and 2 per block of rows.  No faster: waves of
+// 64 keys, blocks of 64 rows, one barrier per block, three waves per SIMD in place of two.
+// Where keys are few, workgroups share a window's row blocks (3 prompts of 174 tokens on 190:
+// 14 and 16 us by one, 7 and 9.5 by six).
 #include <math.h>
+
+#include <algorithm>
 
 #include "tf_common.h"
 #include "tf_internal.h"
@@ -50,10 +54,11 @@ struct WeightArgs {
   int32_t batch, window, hkv, group, head_dim;
   int32_t cap;                  // keys that the workspace has room for (a multiple of 128)
   int32_t rows_cap;             // rows of a kv head it has room for
+  int32_t splits;               // workgroups that share the row blocks of 128 keys
   float scale_log2;
   float2* stats;                // [b][hk][row][cap / 128]
   float* lse;                   // [b][hk][row]
-  float* sums;                  // [b][hk][cap]
+  float* sums;                  // [b][hk][split][cap]
   float* scores;
   int64_t scores_stride;
   int32_t add;
@@ -85,6 +90,16 @@ __device__ Window window_of(const WeightArgs& a, int b, int64_t* red) {
   const int n = (int)max<int64_t>(0, min(min<int64_t>(ext, a.window),
                                          (int64_t)a.rows_cap / a.group));
   return Window{n, before + ext - n};
+}
+
+// The row blocks of a workgroup: its share of the window's.
+struct Blocks {
+  int first, end;
+};
+__device__ __forceinline__ Blocks blocks_of(const WeightArgs& a, const Window& win, int split) {
+  const int n = (win.n_tok * a.group + kBlock - 1) / kBlock;
+  const int each = (n + a.splits - 1) / a.splits;
+  return Blocks{min(n, split * each), min(n, (split + 1) * each)};
 }
 
 // One request's kv head against 128 keys, as the two passes share it.
@@ -169,12 +184,13 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(WeightArgs a) {
   __shared__ u32x4 qs[kBlock * T::kChunks];
   __shared__ float2 part[2][kWaves][kBlock];
   __shared__ int64_t red[kWaves];
-  const int b = blockIdx.y, hk = blockIdx.z;
+  const int b = blockIdx.y, hk = blockIdx.z / a.splits;
   const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 5, n = lane & 31;
   const int len = context_len(a, b);
   const Window win = window_of(a, b, red);
-  if (len == 0 || win.n_tok == 0) return;
-  const int n_rows = win.n_tok * a.group, n_blocks = (n_rows + kBlock - 1) / kBlock;
+  const int n_rows = win.n_tok * a.group;
+  const Blocks blocks = blocks_of(a, win, blockIdx.z % a.splits);
+  if (len == 0 || blocks.first >= blocks.end) return;
   const int64_t* rtt = a.rtt + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.rtt_stride;
   const float sl2 = a.scale_log2 * (FP8 ? a.k_scale[0] : 1.f);
   const int tiles = a.cap / kKeys;
@@ -184,13 +200,13 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(WeightArgs a) {
     const int key0 = tile * kKeys + 32 * w;
     T tl;
     u32x4 x[T::kLoads];
-    tl.fetch(a, win, hk, 0, x);
+    tl.fetch(a, win, hk, blocks.first, x);
     tl.load_keys(a, rtt, key0, len, hk, lane);
-    for (int i = 0; i < n_blocks; ++i) {
+    for (int i = blocks.first; i < blocks.end; ++i) {
       __syncthreads();   // the block before is read
       tl.stage(qs, x);
       __syncthreads();
-      if (i + 1 < n_blocks) tl.fetch(a, win, hk, i + 1, x);
+      if (i + 1 < blocks.end) tl.fetch(a, win, hk, i + 1, x);
       f32x16 s = tl.scores(qs, lane);
       const int seen = row_seen(a, win, i * kBlock + n, len, key0);
       float m = -INFINITY;
@@ -259,31 +275,35 @@ __global__ void __launch_bounds__(kThreads) key_sums_kernel(WeightArgs a) {
   using T = Tile<DP, FP8>;
   __shared__ u32x4 qs[kBlock * T::kChunks];
   __shared__ int64_t red[kWaves];
-  const int b = blockIdx.y, hk = blockIdx.z;
+  const int b = blockIdx.y, hk = blockIdx.z / a.splits;
   const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 5, n = lane & 31;
   const int len = context_len(a, b);
   const Window win = window_of(a, b, red);
-  if (len == 0 || win.n_tok == 0) return;
-  const int n_rows = win.n_tok * a.group, n_blocks = (n_rows + kBlock - 1) / kBlock;
+  const int n_rows = win.n_tok * a.group;
+  const Blocks blocks = blocks_of(a, win, blockIdx.z % a.splits);
+  if (len == 0) return;
   const int64_t* rtt = a.rtt + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.rtt_stride;
   const float sl2 = a.scale_log2 * (FP8 ? a.k_scale[0] : 1.f);
   const float* lse = a.lse + ((int64_t)b * a.hkv + hk) * a.rows_cap;
-  float* sums = a.sums + ((int64_t)b * a.hkv + hk) * a.cap;
+  // (a share without rows writes zeros)
+  float* sums = a.sums + ((int64_t)b * a.hkv * a.splits + blockIdx.z) * a.cap;
 
   for (int tile = blockIdx.x; tile * kKeys < len; tile += gridDim.x) {
     const int key0 = tile * kKeys + 32 * w;
     T tl;
     u32x4 x[T::kLoads];
-    tl.fetch(a, win, hk, 0, x);
-    tl.load_keys(a, rtt, key0, len, hk, lane);
+    if (blocks.first < blocks.end) {
+      tl.fetch(a, win, hk, blocks.first, x);
+      tl.load_keys(a, rtt, key0, len, hk, lane);
+    }
     f32x16 acc = {};
-    for (int i = 0; i < n_blocks; ++i) {
+    for (int i = blocks.first; i < blocks.end; ++i) {
       const int rho = i * kBlock + n;
       const float off = rho < n_rows ? lse[rho] : INFINITY;   // (repeats of the last row)
       __syncthreads();
       tl.stage(qs, x);
       __syncthreads();
-      if (i + 1 < n_blocks) tl.fetch(a, win, hk, i + 1, x);
+      if (i + 1 < blocks.end) tl.fetch(a, win, hk, i + 1, x);
       const f32x16 s = tl.scores(qs, lane);
       const int seen = rho < n_rows ? row_seen(a, win, rho, len, key0) : 0;
 #pragma unroll
@@ -291,32 +311,40 @@ __global__ void __launch_bounds__(kThreads) key_sums_kernel(WeightArgs a) {
         acc[r] += 8 * (r >> 2) + 4 * g + (r & 3) < seen ? fast_exp2(fmaf(s[r], sl2, -off)) : 0.f;
     }
     __syncthreads();
-    // Sums over the 32 rows; lane n keeps register n % 16 (its keys of this half).
+    // Sums over the 32 rows: lanes hand each other the half of their keys that they give up,
+    // until lane n is left with register n / 2.
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float v = acc[r];
+    for (int half = 8; half >= 1; half /= 2) {
+      const bool up = n & (2 * half);
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
-      if (n == r) sums[key0 + 8 * (r >> 2) + 4 * g + (r & 3)] = v;
+      for (int r = 0; r < half; ++r) {
+        const float kept = up ? acc[r + half] : acc[r], given = up ? acc[r] : acc[r + half];
+        acc[r] = kept + __shfl_xor(given, 2 * half, kWave);
+      }
     }
+    const float v = acc[0] + __shfl_xor(acc[0], 1, kWave);
+    const int r = n >> 1;
+    if (!(n & 1)) sums[key0 + 8 * (r >> 2) + 4 * g + (r & 3)] = v;
   }
 }
 
-// scores[row, k] (+)= the kv heads' sums, for the keys of each request.
+// scores[row, k] (+)= the sums of the kv heads and splits, for the keys of each request.
 __global__ void __launch_bounds__(kThreads) add_sums_kernel(WeightArgs a) {
   const int b = blockIdx.y;
   const int len = context_len(a, b);
   float* out = a.scores + clamp_i64(a.rpi[b], 0, a.rtt_rows - 1) * a.scores_stride;
-  const float* sums = a.sums + (int64_t)b * a.hkv * a.cap;
+  const int parts = a.hkv * a.splits;
+  const float* sums = a.sums + (int64_t)b * parts * a.cap;
   for (int k = blockIdx.x * kThreads + threadIdx.x; k < len; k += gridDim.x * kThreads) {
     float v = 0.f;
-    for (int h = 0; h < a.hkv; ++h) v += sums[(int64_t)h * a.cap + k];
+#pragma unroll 8
+    for (int h = 0; h < parts; ++h) v += sums[(int64_t)h * a.cap + k];
     out[k] = a.add ? out[k] + v : v;
   }
 }
 
 struct WeightPlan {
-  int32_t cap, rows_cap;
+  int32_t cap, rows_cap, splits;
   int64_t stats_bytes, lse_bytes, sums_bytes;
   int64_t total() const { return stats_bytes + lse_bytes + sums_bytes; }
 };
@@ -340,15 +368,20 @@ int make_weight_plan(int32_t batch, int32_t window, int32_t max_len, int32_t num
   p->cap = (int32_t)cap;
   p->rows_cap = (int32_t)rows;
   const int64_t units = (int64_t)batch * num_kv_heads;
+  // Row blocks are shared by several workgroups where there are fewer than CUs without.
+  const int64_t wgs = std::max<int64_t>(1, units * (cap / kKeys));
+  p->splits = (int32_t)std::max<int64_t>(
+      1, std::min<int64_t>({(rows + kBlock - 1) / kBlock, device_cu_count() / wgs,
+                            65535 / num_kv_heads, 64}));
   p->stats_bytes = (units * rows * (cap / kKeys) * 8 + 255) / 256 * 256;
   p->lse_bytes = (units * rows * 4 + 255) / 256 * 256;
-  p->sums_bytes = units * cap * 4;
+  p->sums_bytes = units * p->splits * cap * 4;
   return TF_OK;
 }
 
 template <int DP, bool FP8>
 void launch_tiles(const WeightArgs& a, hipStream_t s) {
-  const dim3 tiles((unsigned)(a.cap / kKeys), (unsigned)a.batch, (unsigned)a.hkv);
+  const dim3 tiles((unsigned)(a.cap / kKeys), (unsigned)a.batch, (unsigned)(a.hkv * a.splits));
   constexpr int kRowsWg = 4;
   const dim3 rows((unsigned)((a.rows_cap + kRowsWg - 1) / kRowsWg), (unsigned)a.batch,
                   (unsigned)a.hkv);
@@ -426,6 +459,7 @@ extern "C" int32_t tf_attn_weights(
   a.head_dim = head_dim;
   a.cap = p.cap;
   a.rows_cap = p.rows_cap;
+  a.splits = p.splits;
   a.scale_log2 = scale * kLog2e;
   char* ws = static_cast<char*>(workspace);
   a.stats = reinterpret_cast<float2*>(ws);
