@@ -378,9 +378,9 @@ int64_t tf_attn_weights_workspace_bytes(int32_t batch_size, int32_t window, int3
 
 int32_t tf_attn_weights(
     const void* q, int64_t q_row_stride, int64_t q_rows, const void* k_pool, int64_t pool_slots,
-    int32_t kv_dtype, const float* k_scale, const int64_t* req_to_token, int64_t rtt_rows, int64_t rtt_row_stride,
-    int64_t rtt_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
-    int32_t seq_len_override, const int64_t* extend_lens, int32_t batch_size, int32_t window,
+    int32_t kv_dtype, const float* k_scale, const int64_t* req_to_token, int64_t rtt_rows,
+    int64_t rtt_row_stride, int64_t rtt_cols, const int64_t* req_pool_indices,
+    const int64_t* seq_lens, int32_t seq_len_override, const int64_t* extend_lens, int32_t batch_size, int32_t window,
     int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
     float* scores, int64_t scores_row_stride, int32_t add, void* workspace,
     int64_t workspace_bytes, tf_stream_t stream);

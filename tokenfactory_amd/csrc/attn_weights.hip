@@ -415,8 +415,8 @@ extern "C" int64_t tf_attn_weights_workspace_bytes(int32_t batch_size, int32_t w
 extern "C" int32_t tf_attn_weights(
     const void* q, int64_t q_row_stride, int64_t q_rows, const void* k_pool, int64_t pool_slots,
     int32_t kv_dtype, const float* k_scale, const int64_t* req_to_token, int64_t rtt_rows,
-    int64_t rtt_row_stride, int64_t rtt_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
-    int32_t seq_len_override, const int64_t* extend_lens, int32_t batch_size, int32_t window,
+    int64_t rtt_row_stride, int64_t rtt_cols, const int64_t* req_pool_indices,
+    const int64_t* seq_lens, int32_t seq_len_override, const int64_t* extend_lens, int32_t batch_size, int32_t window,
     int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
     float* scores, int64_t scores_row_stride, int32_t add, void* workspace,
     int64_t workspace_bytes, tf_stream_t stream) {
@@ -474,7 +474,7 @@ extern "C" int32_t tf_attn_weights(
   else
     launch_dims<false>(a, s);
   const int64_t blocks = ((int64_t)p.cap + kThreads - 1) / kThreads;
-  hipLaunchKernelGGL(add_sums_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)batch_size),
-                     dim3(kThreads), 0, s, a);
+  const dim3 grid((unsigned)std::min<int64_t>(blocks, 64), (unsigned)batch_size);
+  hipLaunchKernelGGL(add_sums_kernel, grid, dim3(kThreads), 0, s, a);
   return launch_status("tf_attn_weights launch");
 }

@@ -12,9 +12,9 @@
 // Shared parts go through MFMA tiles instead (but many parts of few rows, or where nearly all
 // keys are own ones: shared_prefix.py has the rule and its figures), cut over their keys so that
 // every CU has a piece: the extend kernel's at head_dim 256 (extend.hip, kPrefix),
-// prefix_tiles.hip's up to 128.  Where the requests' own rows fit units of 16, up to four each, its own part is streamed
-// by other workgroups of the same launch: the tiles are bound by MFMA, the streams by HBM,
-// which about half of the CUs saturate.
+// prefix_tiles.hip's up to 128.  Where the requests' own rows fit units of 16, up to four
+// each, own parts are streamed by other workgroups of the same launch: the tiles are bound
+// by MFMA, the streams by HBM, which about half of the CUs saturate.
 //
 // part_stream_kernel does the decode kernel's tile work (decode.hip) with waves that
 // work alone: a persistent wave owns an equal share of all units' tiles (unit = (item, kv

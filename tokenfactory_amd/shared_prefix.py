@@ -329,7 +329,8 @@ def shared_prefix_attention(
     plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, q.device)
     with _native.launching(q.device, stream):
         if not plan.shares or plan.n_items > MAX_PARTS \
-                or (scaling is not None and not scaling >= 0) or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
+                or (scaling is not None and not scaling >= 0) \
+                or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
             return slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, scaling=scaling,
                                         k_scale=k_scale, v_scale=v_scale, out=out, gate=gate,
                                         out_amax=out_amax)
