@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import _native
-from .attention import (SHORT_ROWS, SPLIT_KEYS, Route, _KV_DTYPES, _check_inputs, _cu_count,
+from .attention import (SHORT_ROWS, Route, _KV_DTYPES, _check_inputs, _cu_count,
                         _epilogue, _fork_join_events, _output, _plan_event, _pool_scales, _scratch,
                         _side_stream, _upload, _ws_lock, slot_based_attention)
 from .fp8_linear import _ptr
@@ -36,10 +36,13 @@ class SharedPrefixes:
     requests whose table rows hold the same slots in their first ``length`` entries.  A
     request is in one group at most.  The lengths may exceed what a request sees (its
     rows mask the rest), so that one object serves a step's layers and, while the
-    extend lengths stay the same, later steps too; ``seq_lens`` are read at launch.
+    extend lengths stay the same, later steps too; ``seq_lens`` are read at launch, and
+    lists are made again as ``max_seq_len`` grows (see ``planned_length``).
 
     A graph may capture calls once an eager call with the same layout has run (it
-    uploads the lists); lists that a graph reads stay allocated."""
+    uploads the lists; of several, those of the nearest ``max_seq_len`` are taken).  Its
+    replays follow ``seq_lens``, but share out the CUs as for that length; lists that a
+    graph reads stay allocated."""
 
     def __init__(self, groups: Iterable[Tuple[Sequence[int], int]]):
         self.groups: List[Tuple[List[int], int]] = []
@@ -54,15 +57,25 @@ class SharedPrefixes:
             if length and len(members) > 1:   # (nothing is shared otherwise)
                 self.groups.append((members, length))
         self._last = max(seen, default=-1)
+        self._longest = max((n for _, n in self.groups), default=0)
         self._lock = threading.Lock()
         self._plans: Dict[tuple, _Plan] = {}
 
     def _plan(self, batch, n_tok, n_q, n_kv, head_dim, kv_dtype, device) -> "_Plan":
+        max_len = planned_length(int(batch.max_seq_len), self._longest)
         key = (device.index, batch.batch_size, n_tok, n_q, n_kv, head_dim, kv_dtype,
-               batch.req_to_token.shape[1], tuple(batch.extend_lens),
-               batch.max_extend_len > 1 and batch.max_seq_len >= SPLIT_KEYS)
+               batch.req_to_token.shape[1], tuple(batch.extend_lens), max_len)
         plan = self._plans.get(key)
-        if plan is not None:
+        if plan is not None and plan.ready:
+            return plan
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            # (lists cannot be made here: those of the layout that were made nearest by)
+            with self._lock:
+                made = [(abs(k[-1] - max_len), p) for k, p in self._plans.items()
+                        if k[:-1] == key[:-1] and p.ready]
+            if made:
+                return min(made, key=lambda x: x[0])[1]
+        elif plan is not None:
             return plan
         ext_lens = [int(e) for e in batch.extend_lens]
         if len(ext_lens) != batch.batch_size or sum(ext_lens) != n_tok \
@@ -80,9 +93,28 @@ class SharedPrefixes:
                 if len(self._plans) >= MAX_LAYOUTS:   # (calls under way hold their own)
                     del self._plans[next(iter(self._plans))]
                 plan = self._plans[key] = _Plan(self.groups, ext_lens, n_q, n_kv, head_dim, device,
-                                                _cu_count(device), int(batch.max_seq_len),
-                                                kv_dtype)
+                                                _cu_count(device), max_len, kv_dtype)
             return plan
+
+
+def _step_middle(n: int) -> int:
+    """The middle of the step that holds n: steps of an eighth to a quarter of a length,
+    the first of 64."""
+    if n < 64:
+        return 32
+    shift = n.bit_length() - 3
+    return ((n >> shift) << shift) + (1 << shift) // 2
+
+
+def planned_length(max_len: int, longest: int) -> int:
+    """The longest context that a plan is made for: a plan holds as long as what lies
+    behind the longest shared part (or a context that does not reach its end) stays in one
+    step of _step_middle, since the split of the CUs follows from the lengths (64 requests on
+    8192 keys with 4096 of their own each: 211 us; 403 by the split of their first step,
+    331 unshared)."""
+    if max_len <= longest:
+        return min(longest, _step_middle(max_len))
+    return longest + _step_middle(max_len - longest)
 
 
 KEYS_PER_STEP = 32   # of the extend kernel
@@ -255,6 +287,11 @@ class _Plan:
         self._addresses: List[int] = []
         self._kept = False
 
+    @property
+    def ready(self) -> bool:
+        """Whether a captured call finds its lists (or needs none)."""
+        return self._lists is not None or not self.shares
+
     def lists(self, batch) -> List[int]:
         """Addresses of (items, work, pieces, tokens, units) for launches on the current
         stream."""
@@ -326,8 +363,8 @@ def shared_prefix_attention(
     if n_q % n_kv:
         raise ValueError(f"num_q_heads {n_q} is not a multiple of num_kv_heads {n_kv}")
     kv_dtype = _KV_DTYPES[layer_k_buffer.dtype]
-    plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, q.device)
     with _native.launching(q.device, stream):
+        plan = shared._plan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, q.device)
         if not plan.shares or plan.n_items > MAX_PARTS \
                 or (scaling is not None and not scaling >= 0) \
                 or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
