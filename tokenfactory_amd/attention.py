@@ -332,43 +332,14 @@ class Route:
                      batch.req_to_token.shape[1], self.key_bytes, stream.cuda_stream)
 
 
-class StepPlan:
-    """The work lists of one model step for one head layout: the extend work
-    entries and the decode items / rows of a ``ForwardBatch``, planned on the
-    device (``tf_attn_plan_device``, from ``extend_lens_tensor``, and
-    ``tf_attn_plan_blocks`` where the step's ``Route`` needs it) by the first
-    attention call of the step and read by every later one.
+class BatchLists:
+    """Device lists planned by the first call made with a batch, on its stream, and read by
+    the batch's later ones.  Calls on another stream than the planning one wait for the
+    plan (an event recorded on the planning stream).  Tensors: ``meta`` and ``lists``."""
 
-    A model step runs every full-attention layer over the same batch
-    (``decoder_layer.py:68-69`` calls the attention once per layer), so the
-    lists do not change between layers (nor with ``seq_lens``: a split entry's
-    pieces follow the lengths at launch); ``slot_based_attention`` keeps one
-    ``StepPlan`` per (device, T, q heads, kv heads, head dim, pool dtype) on the
-    batch object itself.  Calls on another stream than the planning one wait for
-    the plan (an event recorded on the planning stream)."""
-
-    def __init__(self, batch, n_tok: int, n_q: int, n_kv: int, head_dim: int, kv_dtype: int,
-                 device: torch.device):
-        bsz = batch.batch_size
-        ext_t = batch.extend_lens_tensor
-        if ext_t is None or ext_t.device != device or ext_t.dtype != torch.long \
-                or ext_t.numel() != bsz or not ext_t.is_contiguous():
-            raise ValueError("a device plan needs batch.extend_lens_tensor: contiguous int64 "
-                             "[batch_size] on q's device")
-        self.batch_size, self.n_q, self.n_kv = bsz, n_q, n_kv
-        self.head_dim, self.kv_dtype = head_dim, kv_dtype
-        self.ext_t = ext_t
-        self.n_work = _native.plan_device_capacity(n_tok, bsz, n_q, n_kv)
-        self.n_dec = bsz
-        self.route = Route(batch.extend_lens, n_tok, n_q, n_kv, head_dim, kv_dtype, self.n_work,
-                           exact=True, max_len=int(batch.max_seq_len), cus=_cu_count(device))
-        self.meta = torch.empty(self.n_work * 8 + 2 * bsz + 4, dtype=torch.int32, device=device)
-        self.lists = self.route.alloc(device) if self.route.planned else None
-        base = self.meta.data_ptr() + 4 * self.n_work * 8
-        self.items = _DevPtr(base)
-        self.rows = _DevPtr(base + 4 * bsz)
-        self.status = _DevPtr(base + 8 * bsz)
-        self.device = device
+    def __init__(self, device: torch.device, meta: Optional[torch.Tensor],
+                 lists: Optional[torch.Tensor]):
+        self.device, self.meta, self.lists = device, meta, lists
         self._lock = threading.Lock()
         self._users = {_native.current_stream(device)}   # streams that own or have used the lists
         self._planned_on: Optional[torch.cuda.Stream] = None
@@ -385,13 +356,7 @@ class StepPlan:
                     if t is not None:
                         t.record_stream(stream)
             if self._planned_on is None:
-                _native.call("tf_attn_plan_device", self.ext_t.data_ptr(), self.batch_size,
-                             self.n_q, self.n_kv, 1, self.meta.data_ptr(), self.n_work,
-                             self.items.data_ptr(), self.rows.data_ptr(), self.n_dec,
-                             self.status.data_ptr(), stream.cuda_stream)
-                if self.lists is not None:
-                    self.route.plan(self.lists, self.meta.data_ptr(), self.n_work, self.items,
-                                    self.rows, self.n_dec, self.n_q, self.n_kv, batch, stream)
+                self._launch(batch, stream)
                 with _ws_lock:
                     self._event = _plan_event(self.device, stream)
                     self._event.record(stream)
@@ -401,14 +366,15 @@ class StepPlan:
                 # event again: the wait then covers more than this plan)
                 stream.wait_event(self._event)
 
+    def _launch(self, batch, stream: torch.cuda.Stream) -> None:
+        raise NotImplementedError
+
 
 _STEP_PLANS = "_tf_attn_step_plans"
 
 
-def step_plan(batch, n_tok: int, n_q: int, n_kv: int, head_dim: int, kv_dtype: int,
-              device: torch.device) -> StepPlan:
-    """The ``StepPlan`` of ``batch`` for this head layout (made on first use)."""
-    key = (device.index, n_tok, n_q, n_kv, head_dim, kv_dtype)
+def batch_lists(batch, key, make) -> BatchLists:
+    """The lists that ``batch`` carries under ``key`` (``make()`` on first use)."""
     with _ws_lock:
         plans = getattr(batch, _STEP_PLANS, None)
         if plans is None:
@@ -416,9 +382,62 @@ def step_plan(batch, n_tok: int, n_q: int, n_kv: int, head_dim: int, kv_dtype: i
             setattr(batch, _STEP_PLANS, plans)
         plan = plans.get(key)
         if plan is None:
-            plan = StepPlan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, device)
-            plans[key] = plan
+            plan = plans[key] = make()
         return plan
+
+
+class StepPlan(BatchLists):
+    """The work lists of one model step for one head layout: the extend work
+    entries and the decode items / rows of a ``ForwardBatch``, planned on the
+    device (``tf_attn_plan_device``, from ``extend_lens_tensor``, and
+    ``tf_attn_plan_blocks`` where the step's ``Route`` needs it) by the first
+    attention call of the step and read by every later one.
+
+    A model step runs every full-attention layer over the same batch
+    (``decoder_layer.py:68-69`` calls the attention once per layer), so the
+    lists do not change between layers (nor with ``seq_lens``: a split entry's
+    pieces follow the lengths at launch); ``slot_based_attention`` keeps one
+    ``StepPlan`` per (device, T, q heads, kv heads, head dim, pool dtype) on the
+    batch object itself."""
+
+    def __init__(self, batch, n_tok: int, n_q: int, n_kv: int, head_dim: int, kv_dtype: int,
+                 device: torch.device):
+        bsz = batch.batch_size
+        ext_t = batch.extend_lens_tensor
+        if ext_t is None or ext_t.device != device or ext_t.dtype != torch.long \
+                or ext_t.numel() != bsz or not ext_t.is_contiguous():
+            raise ValueError("a device plan needs batch.extend_lens_tensor: contiguous int64 "
+                             "[batch_size] on q's device")
+        self.batch_size, self.n_q, self.n_kv = bsz, n_q, n_kv
+        self.head_dim, self.kv_dtype = head_dim, kv_dtype
+        self.ext_t = ext_t
+        self.n_work = _native.plan_device_capacity(n_tok, bsz, n_q, n_kv)
+        self.n_dec = bsz
+        self.route = Route(batch.extend_lens, n_tok, n_q, n_kv, head_dim, kv_dtype, self.n_work,
+                           exact=True, max_len=int(batch.max_seq_len), cus=_cu_count(device))
+        super().__init__(
+            device,
+            torch.empty(self.n_work * 8 + 2 * bsz + 4, dtype=torch.int32, device=device),
+            self.route.alloc(device) if self.route.planned else None)
+        base = self.meta.data_ptr() + 4 * self.n_work * 8
+        self.items = _DevPtr(base)
+        self.rows = _DevPtr(base + 4 * bsz)
+        self.status = _DevPtr(base + 8 * bsz)
+
+    def _launch(self, batch, stream: torch.cuda.Stream) -> None:
+        _native.call("tf_attn_plan_device", self.ext_t.data_ptr(), self.batch_size, self.n_q,
+                     self.n_kv, 1, self.meta.data_ptr(), self.n_work, self.items.data_ptr(),
+                     self.rows.data_ptr(), self.n_dec, self.status.data_ptr(), stream.cuda_stream)
+        if self.lists is not None:
+            self.route.plan(self.lists, self.meta.data_ptr(), self.n_work, self.items, self.rows,
+                            self.n_dec, self.n_q, self.n_kv, batch, stream)
+
+
+def step_plan(batch, n_tok: int, n_q: int, n_kv: int, head_dim: int, kv_dtype: int,
+              device: torch.device) -> StepPlan:
+    """The ``StepPlan`` of ``batch`` for this head layout (made on first use)."""
+    return batch_lists(batch, (device.index, n_tok, n_q, n_kv, head_dim, kv_dtype),
+                       lambda: StepPlan(batch, n_tok, n_q, n_kv, head_dim, kv_dtype, device))
 
 
 def _ptr(t) -> Optional[int]:

@@ -20,9 +20,9 @@ import numpy as np
 import torch
 
 from . import _native
-from .attention import (SHORT_ROWS, Route, _KV_DTYPES, _check_inputs, _cu_count,
+from .attention import (SHORT_ROWS, BatchLists, Route, _KV_DTYPES, _check_inputs, _cu_count,
                         _epilogue, _fork_join_events, _output, _plan_event, _pool_scales, _scratch,
-                        _side_stream, _upload, _ws_lock, slot_based_attention)
+                        _side_stream, _upload, _ws_lock, batch_lists, slot_based_attention)
 from .fp8_linear import _ptr
 from .planning import EXTEND_TILE_ROWS, plan_extend
 
@@ -281,7 +281,6 @@ class _Plan:
         self._host = np.concatenate(parts)
         self._lock = threading.Lock()
         self._lists: Optional[torch.Tensor] = None
-        self._split: Optional[torch.Tensor] = None   # pieces of the long prompts' entries
         self._users: set = set()
         self._event = None
         self._addresses: List[int] = []
@@ -292,7 +291,7 @@ class _Plan:
         """Whether a captured call finds its lists (or needs none)."""
         return self._lists is not None or not self.shares
 
-    def lists(self, batch) -> List[int]:
+    def lists(self) -> List[int]:
         """Addresses of (items, work, pieces, tokens, units) for launches on the current
         stream."""
         capturing = torch.cuda.is_current_stream_capturing()
@@ -305,29 +304,43 @@ class _Plan:
                     raise RuntimeError("shared prefixes cannot be planned in a graph capture: "
                                        "run the call once before it")
                 self._lists = _upload(self._host, self.device, stream)
-                addresses = [self._lists.data_ptr() + at for at in self._offsets]
-                if self.route is not None and self.route.split:
-                    # (shares by the lengths of now; right for any later ones)
-                    self._split = self.route.alloc(self.device)
-                    self.route.plan(self._split, addresses[1], self.n_work, None, None, 0,
-                                    self.n_q, self.n_kv, batch, stream)
-                    addresses[1] = self._split.data_ptr()
-                self._addresses = addresses
+                self._addresses = [self._lists.data_ptr() + at for at in self._offsets]
                 with _ws_lock:
                     self._event = _plan_event(self.device, stream)
                     self._event.record(stream)
                 self._users.add(stream.cuda_stream)
             elif stream.cuda_stream not in self._users and not capturing:
                 # (torch waits for the device before it captures)
-                for t in (self._lists, self._split):
-                    if t is not None:
-                        t.record_stream(stream)
+                self._lists.record_stream(stream)
                 stream.wait_event(self._event)
                 self._users.add(stream.cuda_stream)
             if capturing and not self._kept:
                 self._kept = True
-                _captured.append((self._lists, self._split))
+                _captured.append(self._lists)
         return self._addresses
+
+    def cut_prompts(self, batch, work: int) -> torch.Tensor:
+        """The long prompts' entries (at ``work``) cut over their keys, by the batch's lengths: the
+        batch keeps them for its other calls; a captured call cuts them in the graph."""
+        stream = torch.cuda.current_stream(self.device)
+        if torch.cuda.is_current_stream_capturing():
+            cut = _PromptPieces(self, work)
+            cut._launch(batch, stream)
+        else:
+            cut = batch_lists(batch, self, lambda: _PromptPieces(self, work))
+            cut.ensure(batch, stream)
+        return cut.lists
+
+
+class _PromptPieces(BatchLists):
+    def __init__(self, plan: _Plan, work: int):
+        super().__init__(plan.device, None, plan.route.alloc(plan.device))
+        self._plan, self._work = plan, work
+
+    def _launch(self, batch, stream: torch.cuda.Stream) -> None:
+        plan = self._plan
+        plan.route.plan(self.lists, self._work, plan.n_work, None, None, 0, plan.n_q, plan.n_kv,
+                        batch, stream)
 
 
 def shared_prefix_attention(
@@ -377,7 +390,7 @@ def shared_prefix_attention(
             q = q.contiguous()
         out = _output(q, out)
         epilogue = _epilogue(q, gate, out_amax)
-        items, work, pieces, tokens, units = plan.lists(batch)
+        items, work, pieces, tokens, units = plan.lists()
         rtt = batch.req_to_token
         pool = (layer_k_buffer.data_ptr(), layer_v_buffer.data_ptr(), n_slots, kv_dtype,
                 _ptr(k_scale), _ptr(v_scale), rtt.data_ptr(), rtt.shape[0], rtt.stride(0),
@@ -401,6 +414,8 @@ def shared_prefix_attention(
         fork, join = _fork_join_events(q.device, main)
         fork.record(main)
         if plan.route.split:
+            cut = plan.cut_prompts(batch, work)
+            work = cut.data_ptr()
             split_ws = torch.empty(_native.load().tf_attn_extend_split_workspace_bytes(),
                                    dtype=torch.uint8, device=q.device)
             _native.call("tf_attn_extend_split", q.data_ptr(), q.stride(0), *pool, 0, work,
