@@ -299,7 +299,8 @@ int32_t tf_attn_rows(
     int64_t gate_row_stride, int64_t gate_head_stride, uint32_t* out_amax, tf_stream_t stream);
 
 /* tf_attn_shared: attention over parts of contexts, joined (a step whose requests
- * share prefixes: their keys are read once for all of them).
+ * share prefixes: their keys are read once for all of them by pieces, once per 16
+ * row_groups rows by shared items).
  * items: device int32 [n_items][8] = {b, tok0, n_tok, row0, k0, k1, pfx, pfx_tok},
  * 16-byte aligned, at most 2048: rows row0 .. row0 + 16 row_groups - 1 of the n_tok * G
  * rows (row = t * G + h) of the tokens at tokens[tok0] over keys [k0, k1) of request

@@ -53,7 +53,7 @@ constexpr int kHalf = kHalfTiles * kTile;        // in two halves by turns
 __device__ __forceinline__ int unit_span(int tiles) { return tiles ? tiles + kUnitTiles : 0; }
 
 // Scores on their way to memory (SCORED) wait in LDS, as many tiles' as there is room for
-// (28 KB a wave: 72 tiles of 6 rows), since loads issued after a store are waited for
+// (28 KB a wave: 74 tiles of 6 rows), since loads issued after a store are waited for
 // behind it: stored at every tile, or at every 8 tiles, they took a fifth of the kernel's
 // time (64 requests of 1k to 8k keys 239 us, 201 without stores).
 template <class C> constexpr int kKeptFloats = C::DP == 128 ? 12 << 8 : 28 << 8;

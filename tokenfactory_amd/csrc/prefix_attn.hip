@@ -1,5 +1,6 @@
 // Attention over parts of contexts, joined: steps whose requests share a prefix
-// (tf_attn_shared), its keys read once for all of them.
+// (tf_attn_shared), its keys read once for all of them (at some head dims once per 32 of
+// their rows, see below).
 //
 // The softmax over a row's keys splits at any key: with m_i, l_i and o_i the maximum,
 // the sum of 2^(s - m_i) and the sum of 2^(s - m_i) V over part i,
@@ -12,9 +13,15 @@
 // Shared parts go through MFMA tiles instead (but many parts of few rows, or where nearly all
 // keys are own ones: shared_prefix.py has the rule and its figures), cut over their keys so that
 // every CU has a piece: the extend kernel's at head_dim 256 (extend.hip, kPrefix),
-// prefix_tiles.hip's up to 128.  Where the requests' own rows fit units of 16, up to four
-// each, own parts are streamed by other workgroups of the same launch: the tiles are bound
-// by MFMA, the streams by HBM, which about half of the CUs saturate.
+// prefix_tiles.hip's up to 128 of bf16 pools.  Where the requests' own rows fit units of 16,
+// up to four each, own parts are streamed by other workgroups of the same launch: the tiles
+// keep the MFMA units busy, the streams wait for their loads, and at 256 dims a tile
+// workgroup's LDS leaves no room for a stream's on its CU.
+//
+// At other head dims (fp8 pools up to 128, any from 129 to 255) shared parts are streamed in
+// units of 16 or 32 rows, each of which reads the part's keys for itself: 64 requests on 8192
+// keys, 32 / 8 heads of 128 in fp8, are 8 units, 172 us (unshared 483; in bf16 by tiles 58),
+// 16 / 4 heads of 192 in bf16 112 (307).
 //
 // part_stream_kernel does the decode kernel's tile work (decode.hip) with waves that
 // work alone: a persistent wave owns an equal share of all units' tiles (unit = (item, kv

@@ -33,9 +33,9 @@ MAX_KEPT_BYTES = 4 << 30       # scores kept between the two halves of a step
 
 def _one_pass(bsz, n_q, n_kv, head_dim, kv_dtype, span) -> bool:
     """Whether a decode step keeps the attention's own scores for the weights (tf_attn_scored)
-    instead of computing them again: 4 bytes per head and key, where K and V are 4 to 16
-    times that, unless the table is so wide that the longest context's room for every
-    request is too much."""
+    instead of computing them again: 4 bytes per head and key, where K and V are head_dim /
+    group times that (43 at 24 / 4 heads of 256, 32 at 32 / 8 of 128; half in fp8), unless
+    the table is so wide that the longest context's room for every request is too much."""
     if n_q % n_kv or (kv_dtype == _native.TF_DTYPE_FP8_E4M3 and head_dim % 16):
         return False
     return (bsz * -(-(n_q // n_kv) // 16) <= MAX_ITEMS

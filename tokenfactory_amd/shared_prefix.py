@@ -5,7 +5,9 @@ Requests that hit the same radix-cache node hold the same slots in front
 prompt, branches of a conversation.  ``slot_based_attention`` reads every request's
 whole context; ``shared_prefix_attention`` reads a group's shared keys and values once
 for all of its requests, and each request's own behind them, and joins the two by their
-softmax statistics.  Same inputs, output and semantics otherwise.
+softmax statistics.  Same inputs, output and semantics otherwise.  (Once for all at head_dim
+256, and up to 128 of bf16 pools, where MFMA tiles take the shared part; elsewhere once per
+32 query rows of a kv head, new tokens x query heads per kv head.)
 
 ``SharedPrefixes`` names the groups of a step.  It keeps the step's work lists on the
 device, so that the layers of a model share them, as ``ForwardBatch`` carries those of
@@ -118,7 +120,7 @@ def planned_length(max_len: int, longest: int) -> int:
 
 
 KEYS_PER_STEP = 32   # of the extend kernel
-MIN_STEPS = 2        # of a piece: 3 requests on 300 keys 13.7 us, with 8 17.1, with 16 20.7
+MIN_STEPS = 2        # of a piece: 3 requests on 300 keys 18.3 us, with 8 18.5, with 16 21.9
 
 
 def cut_units(steps: Sequence[int], cus: int) -> np.ndarray:
@@ -359,9 +361,14 @@ def shared_prefix_attention(
     stream: Optional[torch.cuda.Stream] = None,
 ) -> torch.Tensor:
     """``slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch)`` for a batch
-    whose ``shared`` groups' keys and values are read once per group; the first member's
-    table row is the one read.  Arguments and result as there (sums are joined in another
-    order, so bf16 results may differ in the last bit).
+    whose ``shared`` groups' keys and values are read once per group (head_dim 256, or up to
+    128 with a bf16 pool), or once per 32 query rows of a kv head (other head dims: 64
+    requests on 8192 keys, 32 / 8 heads of 128 in fp8, 172 us for 483 unshared; in bf16 58
+    for 321); the first member's table row is the one read.  Arguments and result as there
+    (sums are joined in another order, so bf16 results may differ in the last bit).
+
+    Worth it where the shared part is most of what a step reads.  A few requests with little
+    in common lose: 4 on 512 shared keys with up to 6000 of their own 37 us for 27.
 
     Steps in which nothing is shared run ``slot_based_attention`` itself: no group of two
     requests with few new tokens (prompts of more than 64 rows, new tokens x query heads
