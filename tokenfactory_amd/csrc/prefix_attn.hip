@@ -56,8 +56,9 @@ part_stream_kernel(PartArgs a) {
 // them in flight per wave, lane l dims 4 l .. 4 l + 3.  Bound by the latency of those
 // reads (and by their bytes where a prefix is cut into many pieces).  A row whose sum
 // is not finite is done again over the keys it sees: an MFMA multiplies V rows that a
-// row does not see by zero, which is NaN for an infinite or NaN value there.
-// A row without a visible key is zeros.
+// row does not see by zero, which is NaN for an infinite or NaN value there.  So is one
+// whose sum is zero: its keys all score -inf (or below the tiles' first reference maximum),
+// or it sees none, for which nothing is read again and zeros are written.
 constexpr int kMergeWaves = 8;
 constexpr int kAhead = 8;
 
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
   uint32_t om = 0;
   const float vscale = FP8 ? a.v_scale[0] : 1.f;
   __bf16* orow = a.out + (int64_t)tok.qrow * a.out_stride + (int64_t)hq * D;
-  if (write && __ballot(not_finite(acc))) {
+  if (write && (l == 0.f || __ballot(not_finite(acc)))) {
     const int row_bytes = FP8 ? D : 2 * D;
     const int seen = token_seen(a, tok);
     RowState rs;
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kMergeWaves * kWave) part_merge_kernel(PartArg
     write = false;
   }
   if (write && lane_out) {
-    const float inv = l > 0.f || l != l ? vscale / l : 0.f;
+    const float inv = vscale / l;
     u32x2 o = {pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
     if (a.gate) {
       o[0] = gate_pair(o[0], gv[0]);
