@@ -5,7 +5,7 @@ import dataclasses
 import pytest
 import torch
 
-from tests.part_oracle import assert_attention, attention64
+from tests.part_oracle import assert_attention, attention64, score_error
 from tests.test_gpu_shared_prefix import call, shared_case
 from tokenfactory_amd import SharedPrefixes, scored_attention
 
@@ -57,9 +57,31 @@ def test_padding_stays_zero(gpu):
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("d", [256, 128, 192])
 def test_scored_decodes(gpu, d, layout):
+    """Output, and the weights: NaN for a request with such a row, the others' as ever."""
     wl, members, finite = case(layout, [1] * 4, d)
     print(f"[scored] D={d} {layout}", flush=True)
-    want, spread, _ = attention64(wl)
+    want, spread, weights = attention64(wl)
     scores = torch.zeros(wl.batch.req_to_token.shape, device=gpu)
     got = scored_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, scores, scaling=wl.scale)
     check(got, want, spread, finite, f"{d} {layout}")
+    check_weights(wl, finite, scores, weights)
+
+
+@pytest.mark.parametrize("d", [256, 64])
+def test_scored_prompts(gpu, d):
+    wl, members, finite = case(LAYOUTS[0], [2, 1, 3, 9], d)
+    _, _, weights = attention64(wl)
+    scores = torch.zeros(wl.batch.req_to_token.shape, device=gpu)
+    scored_attention(wl.q, wl.k_pool, wl.v_pool, wl.batch, scores, scaling=wl.scale)
+    check_weights(wl, finite, scores, weights)
+
+
+def check_weights(wl, finite, scores, weights):
+    for row, n, w in zip(wl.rows, wl.seq_lens, weights):
+        got = scores[row, :n].double().cpu()
+        assert torch.equal(got.isnan(), w.isnan()), row
+        if not w.isnan().any():   # (the bound of tests/test_gpu_scored_attention.py)
+            terms = wl.num_q_heads * 32
+            rel = 2 * score_error(finite) + (n / 32 + 64) * 2.0 ** -22 + terms * 2.0 ** -24
+            assert ((got - w).abs() <= w * rel * 1.01 + 2.0 ** -100).all(), row
+        assert (scores[row, n:] == 0).all()

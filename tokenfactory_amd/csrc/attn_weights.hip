@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(WeightArgs a) {
   }
 }
 
-// One wave per row: lse over the tiles of 128 keys, +inf where the row sees none.
+// One wave per row: lse over the tiles of 128 keys (-inf where the row sees none).
 template <int kRowsWg>
 __global__ void __launch_bounds__(kRowsWg * kWave) row_lse_kernel(WeightArgs a) {
   __shared__ int64_t red[kRowsWg];
@@ -266,8 +266,9 @@ __global__ void __launch_bounds__(kRowsWg * kWave) row_lse_kernel(WeightArgs a) 
     l = l * fast_exp2(m - rf) + l2 * fast_exp2(m2 - rf);
     m = mn;
   }
-  // (NaN scores: a NaN sum, whose logarithm passes on to every weight of the row)
-  if (lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+  // (NaN scores: a NaN sum, whose logarithm passes on to every weight of the row; so does the
+  // -inf of a row whose keys all score -inf)
+  if (lane == 0) a.lse[at] = m + log2f(l);
 }
 
 template <int DP, bool FP8>

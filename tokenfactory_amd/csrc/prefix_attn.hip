@@ -127,8 +127,9 @@ __device__ void add_weights(const PartArgs& a, int block) {
 #pragma unroll
       for (int d = 8; d >= 1; d >>= 1)
         join(__shfl_xor(m, d, kWave), __shfl_xor(l, d, kWave));
-      // (a NaN sum makes every weight of its row NaN)
-      if ((lane & 15) == 0) lse[i] = l == 0.f ? INFINITY : m + log2f(l);
+      // (a NaN sum makes every weight of its row NaN, and so does -inf, of a row whose keys
+      // all score -inf: every row sees one)
+      if ((lane & 15) == 0) lse[i] = m + log2f(l);
     }
     const float* rows = a.row_scores + ((int64_t)b * hq + h0) * a.score_cap;
     for (int64_t k0 = first; k0 < len; k0 += (int64_t)a.weight_blocks * kWeightKeys) {
