@@ -9,7 +9,7 @@ Public surface (the reference's names and contracts, see each module):
 * ``slot_based_attention`` / ``write_kv`` / ``gather_kv`` /
   ``qk_norm_rope_kv_write`` - the kernels' Python entry points
 * ``shared_prefix_attention`` / ``SharedPrefixes`` - attention of a step whose requests
-  share prefixes, read once per group
+  share prefixes, read for a group together
 * ``scored_attention`` - attention that sums up the weight every cached token gets
 * ``evict_tokens`` - drops the cached tokens of the least weight
 * ``LinearAttention`` / ``gdn_decode_step`` - Gated DeltaNet decode step

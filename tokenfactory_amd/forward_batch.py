@@ -18,7 +18,7 @@ What the attention path reads:
 prefix is ``seq_lens - extend_lens``, as at ``qwen3_8/full_attention.py:267``).
 
 Additions, which ``FullAttention.forward`` picks up: ``shared_prefixes`` (a
-``SharedPrefixes``: requests whose rows begin with the same slots, read once per group)
+``SharedPrefixes``: requests whose rows begin with the same slots, read for a group together)
 and ``token_scores`` (fp32 of ``req_to_token``'s shape, to which every full-attention layer
 adds the weights that the last ``score_window`` new tokens of each request give its keys;
 zero a row when a request takes it).  A step with both is scored and reads every
